@@ -1,0 +1,245 @@
+// Shared pieces of the attention kernels with modified scores and masks (attn_mod_fwd.cu,
+// attn_mod_bwd.cu).
+//
+// Score of query i and key j of one sequence, in units of log2 (so that the softmax is a power of
+// two):  y = log2(e) * (cap(scale * q_i . k_j) - slope_h |i - j|),  cap(x) = c tanh(x / c).
+// Every mask these kernels take - causal, a prefix seen in both directions, a window |i - j| < w,
+// documents (runs of equal ids; negative ids are padding) - leaves query i an interval
+// [lo_i, hi_i) of keys, and both ends never decrease with i. So the first and last row of a query
+// tile give the key blocks it has to visit (the hull [lo_first, hi_last)) and those it can visit
+// without looking at the mask (inside [lo_last, hi_first)), and for a block of keys the query
+// tiles that see it are found by bisection. Padding rows get the empty interval [i, i).
+#pragma once
+#include "common.cuh"
+#include "gemm_common.cuh"
+#include "ops.h"
+
+namespace ql {
+
+constexpr int AM_T = 128;  // rows of a query tile and of a key block
+
+// Launch arguments of both directions (the public structs, checked and flattened).
+struct AttnModArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* out;
+  const void* dout;
+  const int32_t* cu_seqlens;
+  const float* slopes;       // [HQ] or null
+  const int32_t* prefix_len; // [B] or null
+  const int2* docs;          // [n] (first, end) of the token's document in its sequence, or null
+  float* lse;                // [HQ, n]
+  float* dvec;               // [HQ, n] rowsum(dout * out), backward only
+  void* out_w;               // forward: out
+  void* dq;
+  void* dk;
+  void* dv;
+  float* parts;              // backward: dk / dv per split of a head group, or null
+  int64_t ld_out, ld_dout;   // row strides (elements)
+  float scale, softcap;
+  int n, B, max_len, HQ, HKV, causal, window;
+  int splits;                // backward: CTAs that share a KV head's query heads
+};
+
+struct AttnSeq {
+  int start, len, prefix, causal, window;
+  const int2* docs;  // of this sequence's first token, or null
+};
+
+__device__ __forceinline__ AttnSeq attn_seq(const AttnModArgs& a, int b) {
+  AttnSeq s;
+  s.start = a.cu_seqlens[b];
+  s.len = a.cu_seqlens[b + 1] - s.start;
+  s.causal = a.causal;
+  s.window = a.window;
+  s.prefix = a.prefix_len != nullptr ? min(max(a.prefix_len[b], 0), s.len) : 0;
+  s.docs = a.docs != nullptr ? a.docs + s.start : nullptr;
+  return s;
+}
+
+// [lo, hi) of query row i (i < len)
+__device__ __forceinline__ int2 attn_row_range(const AttnSeq& s, int i) {
+  int lo = 0, hi = s.len;
+  if (s.causal) hi = max(i + 1, s.prefix);
+  if (s.window > 0) {
+    lo = max(0, i - s.window + 1);
+    hi = min(hi, i + s.window);
+  }
+  if (s.docs != nullptr) {
+    const int2 d = s.docs[i];
+    lo = max(lo, d.x);
+    hi = min(hi, d.y);
+  }
+  return make_int2(lo, hi);
+}
+
+// Key blocks of the query tile starting at row r0: visited [first, end), unmasked [ffirst, fend).
+struct AttnBlocks {
+  int first, end, ffirst, fend;
+};
+__device__ __forceinline__ AttnBlocks attn_tile_blocks(const AttnSeq& s, int r0) {
+  AttnBlocks t{0, 0, 0, 0};
+  if (r0 >= s.len) return t;
+  const int2 a = attn_row_range(s, r0), b = attn_row_range(s, min(r0 + AM_T, s.len) - 1);
+  if (b.y <= a.x) return t;
+  t.first = a.x / AM_T;
+  t.end = (b.y + AM_T - 1) / AM_T;
+  t.ffirst = (b.x + AM_T - 1) / AM_T;
+  t.fend = a.y / AM_T;
+  return t;
+}
+
+// ---- packed pairs of floats ------------------------------------------------------------------
+__device__ __forceinline__ uint64_t pk2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void up2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// exp2_fma (common.cuh) on a pair: 2^x on the FMA pipe, x clamped at -125 (so never for a masked
+// score, which has to give an exact 0).
+__device__ __forceinline__ uint64_t exp2_fma2(uint64_t x) {
+  float a, b;
+  up2(x, a, b);
+  x = pk2(fmaxf(a, -125.f), fmaxf(b, -125.f));
+  const uint64_t magic = pk2(12582912.f, 12582912.f);
+  const uint64_t t = add2(x, magic);
+  const uint64_t f = fma2(add2(t, pk2(-12582912.f, -12582912.f)), pk2(-1.f, -1.f), x);
+  uint64_t p = pk2(0.009569981135427952f, 0.009569981135427952f);
+  p = fma2(p, f, pk2(0.05591755360364914f, 0.05591755360364914f));
+  p = fma2(p, f, pk2(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, pk2(0.6931218504905701f, 0.6931218504905701f));
+  p = fma2(p, f, pk2(0.9999992847442627f, 0.9999992847442627f));
+  float ta, tb, pa, pb;
+  up2(t, ta, tb);
+  up2(p, pa, pb);
+  // adding the rounded integer (the low bits of t) into the exponent field; the magic constant's
+  // own bits vanish in the shift by 23
+  return pk2(__int_as_float(__float_as_int(pa) + (__float_as_int(ta) << 23)),
+             __int_as_float(__float_as_int(pb) + (__float_as_int(tb) << 23)));
+}
+
+// tanh(u) = u P(u^2) for |u| <= 0.75: coefficients of this library's own fit (reweighted least
+// squares in relative error; 2.9e-8, 1.6e-7 in fp32 Horner evaluation).
+constexpr float TANH_POLY_MAX = 0.75f;
+__device__ __forceinline__ uint64_t tanh_poly2(uint64_t u) {
+  const uint64_t w = mul2(u, u);
+  uint64_t p = pk2(-0.004716250579804182f, -0.004716250579804182f);
+  p = fma2(p, w, pk2(0.019582899287343025f, 0.019582899287343025f));
+  p = fma2(p, w, pk2(-0.053344424813985825f, -0.053344424813985825f));
+  p = fma2(p, w, pk2(0.1332540661096573f, 0.1332540661096573f));
+  p = fma2(p, w, pk2(-0.33332958817481995f, -0.33332958817481995f));
+  p = fma2(p, w, pk2(1.f, 1.f));
+  return mul2(p, u);
+}
+
+// ---- tensor core with A in tensor memory -----------------------------------------------------
+// D += A . B with the 16-bit A [128 x 16] in TMEM (row = lane, two elements per 32-bit column)
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Which of the 128 rows [j0, j0 + 128) of a tile hold no key or query of the sequence (past its
+// end, or padding), as bits: word u of lane l's result covers rows 32 u .. 32 u + 31 (every lane
+// gets the same words). Their tile rows are zeroed before a tensor-core product, because a
+// masked probability of 0 times a NaN or infinity left in such a row would not be 0.
+__device__ __forceinline__ bool attn_dead_rows(const AttnSeq& s, int j0, uint32_t bad[4]) {
+  if (j0 + AM_T <= s.len && s.docs == nullptr) return false;
+  const int lane = threadIdx.x & 31;
+  uint32_t any = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int r = j0 + u * 32 + lane;
+    bool dead = r >= s.len;
+    if (!dead && s.docs != nullptr) {
+      const int2 d = s.docs[r];
+      dead = d.x >= d.y;
+    }
+    bad[u] = __ballot_sync(0xffffffffu, dead);
+    any |= bad[u];
+  }
+  return any != 0;
+}
+// Zeroes those rows of a [boxes][128 rows][128 bytes] tile (whole rows, so the swizzle inside a
+// row does not matter), by one warp.
+template <int BOXES>
+__device__ __forceinline__ void attn_zero_rows(uint8_t* tile, const uint32_t bad[4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    uint32_t m = bad[u];
+    while (m != 0) {
+      const int r = u * 32 + __ffs(m) - 1;
+      m &= m - 1;
+      if (lane < 8 * BOXES)
+        *reinterpret_cast<uint4*>(tile + (lane >> 3) * (AM_T * 128) + r * 128 + (lane & 7) * 16) =
+            make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+}
+
+// A wait of a whole warp (bounded, see mbar_wait): every lane gets the same answer, so a warp whose
+// wait ran out leaves together.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+}
+
+// Host: raises a kernel's dynamic shared-memory limit on the current device, once per device.
+inline int attn_smem_limit(const void* kernel, int bytes, unsigned long long* done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return QL_STATUS_CUDA;
+  if (dev < 64 && ((*done >> dev) & 1)) return QL_STATUS_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return QL_STATUS_CUDA;
+  if (dev < 64) *done |= 1ull << dev;
+  return QL_STATUS_OK;
+}
+
+// Host: a [n, heads * D] 16-bit matrix with row stride ld as boxes of 128 rows of one head.
+inline int attn_head_map(CUtensorMap* map, const void* ptr, int64_t n, int heads, int D, int64_t ld,
+                         bool bf16) {
+  return encode_chunked_map(map, ptr, n, (int64_t)heads * D, ld, AM_T, D / 64, bf16);
+}
+
+// Writes (first, end) of each token's document in its sequence (attn_mod_fwd.cu).
+int attn_doc_ranges(const int32_t* doc_ids, const int32_t* cu_seqlens, int B, int n, int2* ranges,
+                    cudaStream_t s);
+// The mode bits of the score: 1 capped, 2 distance bias.
+inline int attn_mode(const AttnModArgs& a) { return (a.softcap > 0.f ? 1 : 0) | (a.slopes != nullptr ? 2 : 0); }
+
+}  // namespace ql

@@ -1,0 +1,513 @@
+// Attention forward with modified scores and masks on the 5th-generation tensor cores (head dims
+// 64 and 128): see attn_mod.cuh for the score and the masks.
+//
+// One CTA takes two adjacent 128-query tiles of one head; both read the same K and V blocks of
+// 128 keys, so each block crosses from L2 once for 256 queries. Ten warps:
+//   warps 0-3, 4-7  softmax of tile 0 and of tile 1, one thread per query row (TMEM lane = row):
+//                   the row's 128 scores into registers, running maximum, P as 16-bit pairs back
+//                   into the score's TMEM columns, where the next product reads it as its A operand;
+//   warp 8          one thread issues the MMAs: for each block O_t += P_t V and then the next
+//                   block's S_t = Q_t K^T, tile 0 and tile 1 in turn, so the tensor core works on
+//                   one tile while the other tile's softmax runs;
+//   warp 9          TMA: Q tiles, then K and V blocks through a ring of tiles.
+// TMEM columns: S_0 [0, 128), S_1 [128, 256) (P_t in the first 64 of S_t), O_0 [256, 256 + D),
+// O_1 [384, 384 + D).
+// The running maximum moves only when it grows by more than 2^8; then the row's O is rescaled.
+// P is rounded to the input type for the product (half a step of 2^-8 or 2^-11 per probability,
+// averaged over the row's keys); the row sum adds the unrounded values in fp32.
+#include "attn_mod.cuh"
+#include "profile.h"
+
+namespace ql {
+
+namespace {
+
+template <int D>
+struct FwdCfg {
+  static constexpr int TILE = AM_T * D * 2;          // bytes of a 128-row tile
+  static constexpr int STAGES = D == 128 ? 5 : 8;    // ring of K / V tiles
+  static constexpr int OFF_KV = 2 * TILE;
+  static constexpr int OFF_BAR = OFF_KV + STAGES * TILE;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024 /*align*/;
+};
+constexpr int FWD_THREADS = 320;
+
+// What the score's modes need per kernel.
+struct ScoreConst {
+  float sl2;    // scale * log2(e): plain scores
+  float u;      // scale / cap
+  float cap2;   // cap * log2(e)
+};
+
+// Scores of one row and one key block, in place: raw products to log2 units (MODE 0 leaves them
+// raw: the scale rides in the exponent's FMA), masked ones to -inf. x: 128 values; dist0 = i - j0.
+template <int MODE, bool MASKED>
+__device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, float slope2,
+                                              float dist0, int rlo, int rhi) {
+  if constexpr ((MODE & 1) != 0) {
+    // the largest |u| of the warp's rows decides between the polynomial and tanhf
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < AM_T; i += 2)
+      mx = max3(mx, fabsf(__uint_as_float(x[i])), fabsf(__uint_as_float(x[i + 1])));
+    const bool poly = __all_sync(0xffffffffu, mx * c.u <= TANH_POLY_MAX);
+    if (poly) {
+      const uint64_t uu = pk2(c.u, c.u), cc = pk2(c.cap2, c.cap2);
+#pragma unroll
+      for (int i = 0; i < AM_T; i += 2) {
+        const uint64_t y = mul2(tanh_poly2(mul2(pk2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), uu)), cc);
+        float a, b;
+        up2(y, a, b);
+        x[i] = __float_as_uint(a);
+        x[i + 1] = __float_as_uint(b);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < AM_T; ++i)
+        x[i] = __float_as_uint(tanhf(__uint_as_float(x[i]) * c.u) * c.cap2);
+    }
+  }
+  if constexpr ((MODE & 2) != 0) {
+#pragma unroll
+    for (int i = 0; i < AM_T; ++i) {
+      const float y = (MODE & 1) != 0 ? __uint_as_float(x[i]) : __uint_as_float(x[i]) * c.sl2;
+      x[i] = __float_as_uint(y - fabsf(slope2 * (dist0 - (float)i)));
+    }
+  }
+  if constexpr (MASKED) {
+#pragma unroll
+    for (int i = 0; i < AM_T; ++i)
+      if (i < rlo || i >= rhi) x[i] = 0xff800000u;  // -inf
+  }
+}
+
+template <typename T, int D, int MODE>
+__global__ void __launch_bounds__(FWD_THREADS, 1)
+    attn_mod_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                        const __grid_constant__ CUtensorMap tv, const AttnModArgs a, int* err) {
+  using C = FwdCfg<D>;
+  constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int BOX = AM_T * 128;  // a 128-row x 64-column box
+  pdl_enter();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* q_full = bars;                      // [2]
+  uint64_t* s_full = bars + 2;                  // [2] score tile written; last: O complete
+  uint64_t* p_full = bars + 4;                  // [2] P written, O rescaled (128 threads)
+  uint64_t* kv_raw = bars + 6;                  // a V tile whose dead rows are zeroed first
+  uint64_t* drain = bars + 7;
+  uint64_t* kv_full = bars + 8;                 // [STAGES]
+  uint64_t* kv_empty = bars + 8 + C::STAGES;    // [STAGES]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8 + 2 * C::STAGES);
+
+  const int h = blockIdx.x % a.HQ, b = blockIdx.x / a.HQ;
+  const int q0 = (gridDim.y - 1 - blockIdx.y) * 2 * AM_T;  // the rows with the most keys first
+  const AttnSeq seq = attn_seq(a, b);
+  if (q0 >= seq.len) return;  // the whole CTA, before any barrier or TMEM is set up
+  const int kvh = h / (a.HQ / a.HKV);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AttnBlocks tb0 = attn_tile_blocks(seq, q0), tb1 = attn_tile_blocks(seq, q0 + AM_T);
+  int jb = tb0.first, je = tb0.end;  // blocks either tile visits
+  if (je <= jb) { jb = tb1.first; je = tb1.end; }
+  else if (tb1.end > tb1.first) { jb = min(jb, tb1.first); je = max(je, tb1.end); }
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 128);
+    }
+    mbar_init(kv_raw, 1);
+    mbar_init(drain, 1);
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    fence_barrier_init();
+    prefetch_tmap(&tq);
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+  }
+  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 9) {
+    // ---- loads ----
+    const int nblk = je - jb;
+    int issued = 0;   // ring slots filled
+    uint32_t raw = 0;
+    bool ok = true;
+    auto load_q = [&](int t) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&q_full[t], C::TILE);
+        tma_load_3d(smem + t * C::TILE, &tq, &q_full[t], 0, seq.start + q0 + t * AM_T, h * (D / 64));
+      }
+    };
+    if (nblk > 0) load_q(0);
+    for (int n = 0; ok && n < 2 * nblk; ++n) {
+      const int s = n % C::STAGES, row = (jb + (n >> 1)) * AM_T;
+      const bool is_v = n & 1;
+      uint32_t bad[4];
+      const bool dirty = is_v && attn_dead_rows(seq, row, bad);
+      if (n >= C::STAGES) ok = warp_wait(&kv_empty[s], (n / C::STAGES - 1) & 1, err);
+      if (!ok) break;
+      uint8_t* dst = smem + C::OFF_KV + s * C::TILE;
+      uint64_t* bar = dirty ? kv_raw : &kv_full[s];
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, C::TILE);
+        tma_load_3d(dst, is_v ? &tv : &tk, bar, 0, seq.start + row, kvh * (D / 64));
+      }
+      if (dirty) {
+        ok = warp_wait(kv_raw, raw, err);
+        if (!ok) break;
+        raw ^= 1;
+        attn_zero_rows<D / 64>(dst, bad);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[s]);
+      }
+      issued = n + 1;
+      if (n == 0) load_q(1);
+    }
+    if (!ok && lane == 0) {  // a wait ran out: let the copies in flight land before the CTA goes
+      mbar_wait(&q_full[0], 0, nullptr, 100000000ull);
+      mbar_wait(&q_full[1], 0, nullptr, 100000000ull);
+      for (int n = max(0, issued - C::STAGES); n < issued; ++n)
+        mbar_wait(&kv_full[n % C::STAGES], (n / C::STAGES) & 1, nullptr, 100000000ull);
+    }
+  } else if (warp == 8) {
+    // ---- MMA ----
+    if (lane == 0 && je > jb) {
+      constexpr uint32_t id_s = umma_idesc_f16(IS_BF16, 128, AM_T, false);
+      constexpr uint32_t id_o = umma_idesc_f16(IS_BF16, 128, D, true);  // V is MN-major
+      const uint32_t sq = smem_u32(smem), skv = smem_u32(smem + C::OFF_KV);
+      bool ok = mbar_wait(&q_full[0], 0, err) && mbar_wait(&q_full[1], 0, err);
+      for (int j = jb - 1; ok && j < je; ++j) {
+        const int nk = 2 * (j + 1 - jb), nv = 2 * (j - jb) + 1;  // ring positions of K_{j+1}, V_j
+        if (j + 1 < je) ok = mbar_wait(&kv_full[nk % C::STAGES], (nk / C::STAGES) & 1, err);
+        if (ok && j >= jb) ok = mbar_wait(&kv_full[nv % C::STAGES], (nv / C::STAGES) & 1, err);
+        if (!ok) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int first = t ? tb1.first : tb0.first, end = t ? tb1.end : tb0.end;
+          const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * 128;
+          if (j >= first && j < end) {  // O_t += P_t V_j
+            if (ok) ok = mbar_wait(&p_full[t], (j - first) & 1, err);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t bv = skv + (nv % C::STAGES) * C::TILE;
+#pragma unroll
+            for (int kk = 0; kk < AM_T / 16; ++kk)
+              umma_f16_ts(to, ts + kk * 8, umma_desc_mn_sw128(bv + kk * 2048, BOX, 1024), id_o,
+                          j > first || kk > 0);
+            if (j + 1 == end) umma_commit(&s_full[t]);
+          }
+          if (j + 1 >= first && j + 1 < end) {  // S_t = Q_t K_{j+1}^T (after P_t V_j in issue order)
+            tc_fence_after();
+            const uint32_t bk = skv + (nk % C::STAGES) * C::TILE, aq = sq + t * C::TILE;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * BOX + (kk & 3) * 32;
+              umma_f16(ts, umma_desc_k_sw128(aq + off), umma_desc_k_sw128(bk + off), id_s, kk > 0);
+            }
+            umma_commit(&s_full[t]);
+          }
+        }
+        if (!ok) break;
+        if (j >= jb) umma_commit(&kv_empty[nv % C::STAGES]);
+        if (j + 1 < je) umma_commit(&kv_empty[nk % C::STAGES]);
+      }
+      if (!ok) {  // a wait ran out: the products already issued finish before TMEM is freed
+        umma_commit(drain);
+        mbar_wait(drain, 0, nullptr, 100000000ull);
+      }
+    }
+  } else {
+    // ---- softmax ----
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int qi = q0 + t * AM_T + r;
+    const AttnBlocks tb = t ? tb1 : tb0;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t ts = lane_base + t * 128, to = lane_base + 256 + t * 128;
+    const int2 range = qi < seq.len ? attn_row_range(seq, qi) : make_int2(0, 0);
+    ScoreConst c;
+    c.sl2 = a.scale * 1.4426950408889634f;
+    c.u = (MODE & 1) != 0 ? a.scale / a.softcap : 0.f;
+    c.cap2 = a.softcap * 1.4426950408889634f;
+    const float slope2 = (MODE & 2) != 0 ? a.slopes[h] * 1.4426950408889634f : 0.f;
+    const float mul = MODE == 0 ? c.sl2 : 1.f;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    for (int j = tb.first; j < tb.end; ++j) {
+      const int n = j - tb.first;
+      ok = warp_wait(&s_full[t], n & 1, err);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t x[AM_T];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) tmem_ld32_nw(ts + u * 32, x + u * 32);
+      tmem_wait_ld();
+      const bool masked = j < tb.ffirst || j >= tb.fend;
+      const int j0 = j * AM_T;
+      if (masked) modify_scores<MODE, true>(x, c, slope2, (float)(qi - j0), range.x - j0, range.y - j0);
+      else modify_scores<MODE, false>(x, c, slope2, (float)(qi - j0), 0, 0);
+      float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < AM_T; i += 4) {
+        m0 = max3(m0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        m1 = max3(m1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+      }
+      const float ms = fmaxf(m0, m1) * mul;
+      float corr = 1.f;
+      if (ms > m_run + 8.f) {
+        corr = m_run == -INFINITY ? 0.f : ex2(m_run - ms);
+        m_run = ms;
+      }
+      const float mneg = m_run == -INFINITY ? 0.f : -m_run;
+      if (n > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+        // S_t of this block was committed after O_t += P_t V of the last one: O_t is complete
+#pragma unroll 1
+        for (int u = 0; u < D / 32; ++u) {
+          float ov[32];
+          tmem_ld32(to + u * 32, ov);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) ov[e] *= corr;
+          tmem_st32(to + u * 32, ov);
+        }
+      }
+      uint64_t sum0 = 0, sum1 = 0;  // pairs of +0.f
+      const uint64_t mul_2 = pk2(mul, mul), neg_2 = pk2(mneg, mneg);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        float w[32];  // 64 probabilities as 16-bit pairs
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const uint64_t y = fma2(pk2(__uint_as_float(x[g * 64 + 2 * i]), __uint_as_float(x[g * 64 + 2 * i + 1])), mul_2, neg_2);
+          float pa, pb;
+          up2(y, pa, pb);
+          pa = ex2(pa);
+          pb = ex2(pb);
+          const uint64_t p = pk2(pa, pb);
+          if (i & 1) sum1 = add2(sum1, p);
+          else sum0 = add2(sum0, p);
+          w[i] = __uint_as_float(pack_t2<T>(pa, pb));
+        }
+        tmem_st32(ts + g * 32, w);
+      }
+      float sa, sb, sc, sd;
+      up2(sum0, sa, sb);
+      up2(sum1, sc, sd);
+      l_run = l_run * corr + ((sa + sb) + (sc + sd));
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[t]);
+    }
+    if (tb.end > tb.first && ok) {
+      ok = warp_wait(&s_full[t], (tb.end - tb.first) & 1, err);
+      tc_fence_after();
+    }
+    if (ok) {
+      const float inv = l_run > 0.f ? 1.f / l_run : (l_run == 0.f ? 0.f : l_run);  // NaN stays
+      T* out = reinterpret_cast<T*>(a.out_w) + ((int64_t)(seq.start + qi) * a.HQ + h) * D;
+#pragma unroll 1
+      for (int u = 0; u < D / 32; ++u) {
+        float ov[32];
+        if (tb.end > tb.first) {
+          tmem_ld32(to + u * 32, ov);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) ov[e] = 0.f;
+        }
+        if (qi < seq.len) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            reinterpret_cast<uint4*>(out + u * 32)[v] =
+                make_uint4(pack_t2<T>(ov[8 * v] * inv, ov[8 * v + 1] * inv),
+                           pack_t2<T>(ov[8 * v + 2] * inv, ov[8 * v + 3] * inv),
+                           pack_t2<T>(ov[8 * v + 4] * inv, ov[8 * v + 5] * inv),
+                           pack_t2<T>(ov[8 * v + 6] * inv, ov[8 * v + 7] * inv));
+        }
+      }
+      if (qi < seq.len)
+        a.lse[(int64_t)h * a.n + seq.start + qi] = (m_run + log2f(l_run)) * 0.6931471805599453f;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Documents: (first, end) of the run of equal ids each token is in, within its sequence; a token
+// with a negative id gets the empty range (i, i). One CTA per sequence scans it in chunks of 4,096
+// tokens, forwards for the first tokens of the runs and backwards for their ends.
+constexpr int DOC_THREADS = 1024, DOC_PER = 4;
+
+template <bool REV>
+__device__ void doc_scan(const int32_t* ids, int len, int2* ranges, int* carry_smem) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int CH = DOC_THREADS * DOC_PER;
+  const int nch = (len + CH - 1) / CH;
+  int carry = REV ? len : 0;  // edge carried over from the chunks before
+  for (int ch = 0; ch < nch; ++ch) {
+    const int base = (REV ? nch - 1 - ch : ch) * CH + threadIdx.x * DOC_PER;
+    int id[DOC_PER + 1];  // with the neighbour before (REV: after) the thread's tokens
+#pragma unroll
+    for (int e = 0; e <= DOC_PER; ++e) {
+      const int i = base + e - (REV ? 0 : 1);
+      id[e] = i >= 0 && i < len ? ids[i] : -1;
+    }
+    // an edge: forwards the first token of a run (its index), backwards the last (index + 1);
+    // edge[e]: the nearest one at or before (REV: at or after) token e within the thread
+    int edge[DOC_PER], best = REV ? 0x7fffffff : -1;
+#pragma unroll
+    for (int k = 0; k < DOC_PER; ++k) {
+      const int e = REV ? DOC_PER - 1 - k : k, i = base + e;
+      const bool is = REV ? (i == len - 1 || id[e] != id[e + 1]) : (i == 0 || id[e] != id[e + 1]);
+      if (is && i < len) best = REV ? i + 1 : i;
+      edge[e] = best;
+    }
+    // exclusive scan over the threads (max forwards; min over the later threads backwards)
+    int v = best;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int w = REV ? __shfl_down_sync(0xffffffffu, v, o) : __shfl_up_sync(0xffffffffu, v, o);
+      if (REV ? lane + o < 32 : lane >= o) v = REV ? min(v, w) : max(v, w);
+    }
+    if (lane == (REV ? 0 : 31)) carry_smem[warp] = v;
+    int ex = REV ? __shfl_down_sync(0xffffffffu, v, 1) : __shfl_up_sync(0xffffffffu, v, 1);
+    if (lane == (REV ? 31 : 0)) ex = REV ? 0x7fffffff : -1;
+    __syncthreads();
+    int all = REV ? 0x7fffffff : -1;
+    for (int w = 0; w < DOC_THREADS / 32; ++w) {
+      const int x = carry_smem[w];
+      if (REV ? w > warp : w < warp) ex = REV ? min(ex, x) : max(ex, x);
+      all = REV ? min(all, x) : max(all, x);
+    }
+    if (REV) ex = ex == 0x7fffffff ? carry : ex;
+    else ex = ex == -1 ? carry : ex;
+#pragma unroll
+    for (int e = 0; e < DOC_PER; ++e) {
+      const int i = base + e;
+      if (i >= len) continue;
+      const int found = edge[e] == (REV ? 0x7fffffff : -1) ? ex : edge[e];
+      if (REV) ranges[i].y = id[e] < 0 ? i : found;
+      else ranges[i].x = id[e + 1] < 0 ? i : found;
+    }
+    if (REV ? all != 0x7fffffff : all != -1) carry = all;
+    __syncthreads();
+  }
+}
+
+__global__ void __launch_bounds__(DOC_THREADS) doc_ranges_kernel(const int32_t* ids,
+                                                                 const int32_t* cu, int2* ranges) {
+  pdl_enter();
+  __shared__ int sm[DOC_THREADS / 32];
+  const int start = cu[blockIdx.x], len = cu[blockIdx.x + 1] - start;
+  doc_scan<false>(ids + start, len, ranges + start, sm);
+  doc_scan<true>(ids + start, len, ranges + start, sm);
+}
+
+template <typename T, int D, int MODE>
+int launch_fwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mk,
+               const CUtensorMap& mv, cudaStream_t s) {
+  static unsigned long long done = 0;
+  auto kern = attn_mod_fwd_kernel<T, D, MODE>;
+  const int st = attn_smem_limit(reinterpret_cast<const void*>(kern), FwdCfg<D>::SMEM, &done);
+  if (st != QL_STATUS_OK) return st;
+  const dim3 grid((unsigned)(a.HQ * a.B), (unsigned)cdiv(a.max_len, 2 * AM_T));
+  launch_k(kern, grid, dim3(FWD_THREADS), FwdCfg<D>::SMEM, s, mq, mk, mv, a, status_word());
+  return launched(1);
+}
+
+template <typename T, int D>
+int dispatch_fwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mk,
+                 const CUtensorMap& mv, cudaStream_t s) {
+  switch (attn_mode(a)) {
+    case 0: return launch_fwd<T, D, 0>(a, mq, mk, mv, s);
+    case 1: return launch_fwd<T, D, 1>(a, mq, mk, mv, s);
+    case 2: return launch_fwd<T, D, 2>(a, mq, mk, mv, s);
+    default: return launch_fwd<T, D, 3>(a, mq, mk, mv, s);
+  }
+}
+
+}  // namespace
+
+int attn_doc_ranges(const int32_t* doc_ids, const int32_t* cu_seqlens, int B, int n, int2* ranges,
+                    cudaStream_t s) {
+  launch_k(doc_ranges_kernel, dim3((unsigned)B), dim3(DOC_THREADS), 0, s, doc_ids, cu_seqlens, ranges);
+  return launched(1);
+}
+
+// The checks both directions share.
+int attn_mod_check(const ql_attn_mod_args& m, AttnModArgs& a) {
+  if (m.D != 64 && m.D != 128) return QL_STATUS_UNSUPPORTED;
+  if (m.dtype != QL_F16 && m.dtype != QL_BF16) return QL_STATUS_BAD_ARG;
+  if (m.n < 0 || m.B < 0 || m.max_len < 0 || m.max_len > m.n || m.n > (1 << 29) || m.HKV <= 0 ||
+      m.HQ <= 0 || m.HQ % m.HKV != 0 || m.window < 0)
+    return QL_STATUS_BAD_ARG;
+  if ((int64_t)m.HQ * m.B > 0x7fffffff || cdiv(m.max_len, AM_T) > 65535) return QL_STATUS_UNSUPPORTED;
+  if (!(m.scale > 0.f && m.scale < INFINITY) || !(m.softcap >= 0.f && m.softcap < INFINITY))
+    return QL_STATUS_BAD_ARG;
+  if (m.n > 0 && m.B > 0 && (m.q == nullptr || m.k == nullptr || m.v == nullptr || m.out == nullptr ||
+                             m.lse == nullptr || m.cu_seqlens == nullptr))
+    return QL_STATUS_BAD_ARG;
+  if (m.doc_ids != nullptr && (m.ranges == nullptr || (reinterpret_cast<uintptr_t>(m.ranges) & 7)))
+    return QL_STATUS_BAD_ARG;
+  // TMA: 16-byte aligned bases and row strides
+  if (((reinterpret_cast<uintptr_t>(m.q) | reinterpret_cast<uintptr_t>(m.k) |
+        reinterpret_cast<uintptr_t>(m.v) | reinterpret_cast<uintptr_t>(m.out)) & 15) ||
+      ((m.ldq | m.ldk | m.ldv) & 7) || m.ldq < (int64_t)m.HQ * m.D ||
+      m.ldk < (int64_t)m.HKV * m.D || m.ldv < (int64_t)m.HKV * m.D)
+    return QL_STATUS_BAD_ARG;
+  a = AttnModArgs{};
+  a.q = m.q;
+  a.k = m.k;
+  a.v = m.v;
+  a.out = m.out;
+  a.out_w = m.out;
+  a.lse = m.lse;
+  a.cu_seqlens = m.cu_seqlens;
+  a.slopes = m.slopes;
+  a.prefix_len = m.prefix_len;
+  a.docs = m.doc_ids != nullptr ? reinterpret_cast<const int2*>(m.ranges) : nullptr;
+  a.scale = m.scale;
+  a.softcap = m.softcap;
+  a.n = m.n;
+  a.B = m.B;
+  a.max_len = m.max_len;
+  a.HQ = m.HQ;
+  a.HKV = m.HKV;
+  a.causal = m.causal;
+  a.window = m.window < (1 << 30) ? m.window : (1 << 30);
+  return QL_STATUS_OK;
+}
+
+int attn_mod_fwd(const ql_attn_mod_args& m, cudaStream_t s) {
+  AttnModArgs a;
+  int st = attn_mod_check(m, a);
+  if (st != QL_STATUS_OK) return st;
+  if (m.n == 0 || m.B == 0 || m.max_len == 0) return QL_STATUS_OK;
+  ProfScope prof(PK_ATTN_FWD, 0, 0, s);
+  if (m.doc_ids != nullptr) {
+    st = attn_doc_ranges(m.doc_ids, m.cu_seqlens, m.B, m.n, reinterpret_cast<int2*>(m.ranges), s);
+    if (st != QL_STATUS_OK) return st;
+  }
+  const bool bf = m.dtype == QL_BF16;
+  CUtensorMap mq, mk, mv;
+  if (attn_head_map(&mq, m.q, m.n, m.HQ, m.D, m.ldq, bf) != QL_STATUS_OK ||
+      attn_head_map(&mk, m.k, m.n, m.HKV, m.D, m.ldk, bf) != QL_STATUS_OK ||
+      attn_head_map(&mv, m.v, m.n, m.HKV, m.D, m.ldv, bf) != QL_STATUS_OK)
+    return QL_STATUS_CUDA;
+  if (m.D == 128) return bf ? dispatch_fwd<__nv_bfloat16, 128>(a, mq, mk, mv, s)
+                            : dispatch_fwd<__half, 128>(a, mq, mk, mv, s);
+  return bf ? dispatch_fwd<__nv_bfloat16, 64>(a, mq, mk, mv, s) : dispatch_fwd<__half, 64>(a, mq, mk, mv, s);
+}
+
+}  // namespace ql

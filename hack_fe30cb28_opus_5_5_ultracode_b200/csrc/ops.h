@@ -89,6 +89,7 @@ int attn_bwd_tc(const AttnBwdC& a, cudaStream_t s);  // D = 128 on tcgen05 (main
 void attn_set_impl(int impl);
 int exp2_fma_eval(const float* x, float* y, int64_t n, cudaStream_t s);
 int attn_bwd(const AttnBwdC& a, cudaStream_t s);
+int attn_mod_fwd(const ql_attn_mod_args& m, cudaStream_t s);
 }  // namespace ql
 
 namespace ql {

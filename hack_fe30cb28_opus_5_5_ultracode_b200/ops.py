@@ -481,6 +481,100 @@ def attn_bwd(dout, q, k, v, out, lse, cu_seqlens, max_len, scale, dq=None, dk=No
     return dq, dk, dv
 
 
+def _on_device(device):
+    """The device as the current one for a launch (nothing to switch in the usual case)."""
+    import contextlib
+
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _attn_mod_heads(t, name, n, heads, D, like):
+    if t.dim() != 3 or t.shape != (n, heads, D):
+        raise ValueError(f"{name} must be [{n}, {heads}, {D}], got {list(t.shape)}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must have q's dtype and device")
+    if t.numel() and (t.stride(2) != 1 or t.stride(1) != D):
+        raise ValueError(f"{name}'s heads must be contiguous within a row")
+    return t.stride(0) if n > 1 else heads * D
+
+
+def _attn_mod_vector(t, name, shape, dtype, like):
+    if t is None:
+        return
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() \
+            or t.device != like.device:
+        raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)} on q's device")
+
+
+def _attn_mod_fields(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes, window,
+                     doc_ids, prefix_len):
+    """The checked fields both directions of attn_mod share."""
+    _need_cuda(q, k, v, cu_seqlens, slopes, doc_ids, prefix_len)
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q and k must be [tokens, heads, D]")
+    n, HQ, D = q.shape
+    HKV = k.shape[1]
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"unsupported dtype {q.dtype}")
+    if D not in (64, 128):
+        raise ValueError(f"head size {D}: 64 or 128 are supported")
+    if HKV == 0 or HQ % HKV:
+        raise ValueError(f"{HQ} query heads over {HKV} key heads")
+    ldq = _attn_mod_heads(q, "q", n, HQ, D, q)
+    ldk = _attn_mod_heads(k, "k", n, HKV, D, q)
+    ldv = _attn_mod_heads(v, "v", n, HKV, D, q)
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must be int32 [sequences + 1]")
+    B = cu_seqlens.numel() - 1
+    _attn_mod_vector(cu_seqlens, "cu_seqlens", (B + 1,), torch.int32, q)
+    _attn_mod_vector(slopes, "slopes", (HQ,), torch.float32, q)
+    _attn_mod_vector(doc_ids, "doc_ids", (n,), torch.int32, q)
+    _attn_mod_vector(prefix_len, "prefix_len", (B,), torch.int32, q)
+    if prefix_len is not None and not causal:
+        raise ValueError("prefix_len needs causal=True (without it every key is seen already)")
+    if not 0 <= max_len <= n or window < 0 or not 0 < scale < float("inf") \
+            or not 0 <= softcap < float("inf"):
+        raise ValueError("needs 0 <= max_len <= tokens, window >= 0, 0 < scale < inf and "
+                         "0 <= softcap < inf")
+    ranges = torch.empty((n, 2), device=q.device, dtype=torch.int32) \
+        if doc_ids is not None else None
+    return dict(q=_ptr(q), k=_ptr(k), v=_ptr(v), cu_seqlens=_ptr(cu_seqlens), slopes=_ptr(slopes),
+                doc_ids=_ptr(doc_ids), prefix_len=_ptr(prefix_len), ranges=_ptr(ranges), ldq=ldq,
+                ldk=ldk, ldv=ldv, scale=float(scale), softcap=float(softcap), n=n, B=B,
+                max_len=int(max_len), HQ=HQ, HKV=HKV, D=D, dtype=dtype_code(q.dtype),
+                causal=int(bool(causal)), window=min(int(window), INT_MAX)), ranges
+
+
+def _attn_mod_like(t, name, shape, dtype, like):
+    if t is None:
+        return torch.empty(shape, device=like.device, dtype=dtype)
+    _attn_mod_vector(t, name, tuple(shape), dtype, like)
+    return t
+
+
+def attn_mod_fwd(q, k, v, cu_seqlens, max_len, scale, causal=True, softcap=0.0, slopes=None,
+                 window=0, doc_ids=None, prefix_len=None, out=None, lse=None):
+    """(out, lse) of varlen GQA attention with modified scores and masks (ql_attn_mod_fwd).
+
+    q [n, HQ, D], k / v [n, HKV, D] (fp16 or bf16, D 64 or 128; rows may be strided, e.g. slices of
+    a fused qkv), cu_seqlens int32 [B + 1], max_len at least the longest sequence. With positions
+    i, j within a sequence: s = cap(scale q_i . k_j) - slopes[h] |i - j|, cap(x) = softcap
+    tanh(x / softcap); a query sees key j if j <= i or j < prefix_len[b] (causal), |i - j| < window
+    (window > 0), and both are in the same run of equal doc_ids (negative ids: padding). slopes
+    fp32 [HQ], doc_ids int32 [n], prefix_len int32 [B]. out as q (contiguous), lse fp32 [HQ, n];
+    a query that sees nothing gets out 0 and lse -inf."""
+    f, ranges = _attn_mod_fields(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes,
+                                 window, doc_ids, prefix_len)
+    out = _attn_mod_like(out, "out", q.shape, q.dtype, q)
+    lse = _attn_mod_like(lse, "lse", (q.shape[1], q.shape[0]), torch.float32, q)
+    with _on_device(q.device):
+        args = _lib.struct("ql_attn_mod_args", out=_ptr(out), lse=_ptr(lse), **f)
+        call("ql_attn_mod_fwd", ctypes_ref(args), stream_ptr())
+    return out, lse
+
+
 def gather_rows(src, idx, out=None):
     n, H = idx.numel(), src.shape[1]
     out = out if out is not None else torch.empty((n, H), device=src.device, dtype=torch.float32)

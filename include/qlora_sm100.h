@@ -410,6 +410,47 @@ int ql_attn_set_deterministic(int on);
  * the reference). */
 int ql_exp2_fma_eval(const float* x, float* y, int64_t n, cudaStream_t stream);
 
+/* ---- varlen GQA attention with modified scores and masks -----------------------------------
+ * No counterpart in the reference (its attention is plain causal). Query i and key j of one
+ * sequence (positions within the sequence) score
+ *   s = cap(scale * q_i . k_j) - slopes[h] * |i - j|,   cap(x) = softcap * tanh(x / softcap)
+ * (softcap 0: cap(x) = x; slopes NULL: no distance bias), and i sees j if all of these hold:
+ *   causal:      j <= i, or j < prefix_len[b] (the sequence's prefix, seen in both directions);
+ *                causal = 0: every j;
+ *   window w:    |i - j| < w (0: no window);
+ *   documents:   i and j are in the same run of equal doc_ids (a document ends where the id
+ *                changes; a negative id is padding, which sees nothing and is seen by nothing).
+ * A query that sees no key gets out = 0, lse = -inf and zero gradients. Rows of q, k, v past the
+ * last sequence are not read into any result, and rows of the outputs there are left alone.
+ * q [n, HQ, D], k / v [n, HKV, D] of dtype with row strides ldq / ldk / ldv (elements, multiples of
+ * 8; the heads of a row contiguous), D = 64 or 128, 16-byte aligned; out, dout, dq, dk, dv
+ * contiguous in dtype; lse fp32 [HQ, n], natural log. scale > 0. max_len: at least the longest
+ * sequence. The gradients are summed in a fixed order (bit-identical from run to run); fp16
+ * gradients of small magnitude need a scaled loss, as everywhere in this library. */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;                  /* forward: written; backward: the forward's */
+  float* lse;
+  const int32_t* cu_seqlens;  /* [B + 1] */
+  const float* slopes;        /* [HQ] or NULL */
+  const int32_t* prefix_len;  /* [B] or NULL (needs causal) */
+  const int32_t* doc_ids;     /* [n] or NULL */
+  int32_t* ranges;            /* workspace [n][2], 8-byte aligned, with doc_ids */
+  const void* dout;           /* backward only, as the next five */
+  void* dq;
+  void* dk;
+  void* dv;
+  float* workspace;           /* ql_attn_mod_bwd_workspace(...) floats, 16-byte aligned */
+  int64_t workspace_floats;
+  int64_t ldq, ldk, ldv;
+  float scale, softcap;
+  int32_t n, B, max_len, HQ, HKV, D, dtype, causal, window;
+} ql_attn_mod_args;
+
+int ql_attn_mod_fwd(const ql_attn_mod_args* args, cudaStream_t stream);
+
 /* ---- head row order ----------------------------------------------------------------------
  * The head takes rows with a target first (solution/engine.py:731, 1364-1398):
  * gather: dst[i, :] = src[idx[i], :]; scatter: dst[idx[i], :] = src[i, :] * (*scale) (scale is a
