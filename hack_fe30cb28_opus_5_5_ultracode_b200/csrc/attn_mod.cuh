@@ -36,7 +36,6 @@ struct AttnModArgs {
   void* dk;
   void* dv;
   float* parts;              // backward: dk / dv per split of a head group, or null
-  int64_t ld_out, ld_dout;   // row strides (elements)
   float scale, softcap;
   int n, B, max_len, HQ, HKV, causal, window;
   int splits;                // backward: CTAs that share a KV head's query heads
@@ -74,20 +73,44 @@ __device__ __forceinline__ int2 attn_row_range(const AttnSeq& s, int i) {
   return make_int2(lo, hi);
 }
 
-// Key blocks of the query tile starting at row r0: visited [first, end), unmasked [ffirst, fend).
+// [lo, hi) of the query rows that see key j (j < len): the same conditions read from the key's
+// side; again both ends never decrease with j.
+__device__ __forceinline__ int2 attn_key_range(const AttnSeq& s, int j) {
+  int lo = 0, hi = s.len;
+  if (s.causal && j >= s.prefix) lo = j;
+  if (s.window > 0) {
+    lo = max(lo, j - s.window + 1);
+    hi = min(hi, j + s.window);
+  }
+  if (s.docs != nullptr) {
+    const int2 d = s.docs[j];
+    lo = max(lo, d.x);
+    hi = min(hi, d.y);
+  }
+  return make_int2(lo, hi);
+}
+
+// Blocks of 128 that the 128 rows from r0 on reach: visited [first, end), unmasked [ffirst, fend).
 struct AttnBlocks {
   int first, end, ffirst, fend;
 };
-__device__ __forceinline__ AttnBlocks attn_tile_blocks(const AttnSeq& s, int r0) {
+__device__ __forceinline__ AttnBlocks attn_blocks(int2 first_row, int2 last_row) {
   AttnBlocks t{0, 0, 0, 0};
-  if (r0 >= s.len) return t;
-  const int2 a = attn_row_range(s, r0), b = attn_row_range(s, min(r0 + AM_T, s.len) - 1);
-  if (b.y <= a.x) return t;
-  t.first = a.x / AM_T;
-  t.end = (b.y + AM_T - 1) / AM_T;
-  t.ffirst = (b.x + AM_T - 1) / AM_T;
-  t.fend = a.y / AM_T;
+  if (last_row.y <= first_row.x) return t;
+  t.first = first_row.x / AM_T;
+  t.end = (last_row.y + AM_T - 1) / AM_T;
+  t.ffirst = (last_row.x + AM_T - 1) / AM_T;
+  t.fend = first_row.y / AM_T;
   return t;
+}
+// Key blocks of a query tile, and query tiles of a key block.
+__device__ __forceinline__ AttnBlocks attn_tile_blocks(const AttnSeq& s, int r0) {
+  if (r0 >= s.len) return AttnBlocks{0, 0, 0, 0};
+  return attn_blocks(attn_row_range(s, r0), attn_row_range(s, min(r0 + AM_T, s.len) - 1));
+}
+__device__ __forceinline__ AttnBlocks attn_key_blocks(const AttnSeq& s, int r0) {
+  if (r0 >= s.len) return AttnBlocks{0, 0, 0, 0};
+  return attn_blocks(attn_key_range(s, r0), attn_key_range(s, min(r0 + AM_T, s.len) - 1));
 }
 
 // ---- packed pairs of floats ------------------------------------------------------------------
@@ -239,6 +262,8 @@ inline int attn_head_map(CUtensorMap* map, const void* ptr, int64_t n, int heads
 // Writes (first, end) of each token's document in its sequence (attn_mod_fwd.cu).
 int attn_doc_ranges(const int32_t* doc_ids, const int32_t* cu_seqlens, int B, int n, int2* ranges,
                     cudaStream_t s);
+// Checks the public arguments (both directions) and flattens them.
+int attn_mod_check(const ql_attn_mod_args& m, AttnModArgs& a);
 // The mode bits of the score: 1 capped, 2 distance bias.
 inline int attn_mode(const AttnModArgs& a) { return (a.softcap > 0.f ? 1 : 0) | (a.slopes != nullptr ? 2 : 0); }
 

@@ -391,6 +391,15 @@ int ql_attn_mod_fwd(const ql_attn_mod_args* args, cudaStream_t stream) {
   return done(ql::attn_mod_fwd(*args, stream), "ql_attn_mod_fwd");
 }
 
+int ql_attn_mod_bwd(const ql_attn_mod_args* args, cudaStream_t stream) {
+  if (args == nullptr) return fail(QL_STATUS_BAD_ARG, "ql_attn_mod_bwd");
+  return done(ql::attn_mod_bwd(*args, stream), "ql_attn_mod_bwd");
+}
+
+int64_t ql_attn_mod_bwd_workspace(const ql_attn_mod_args* args) {
+  return args == nullptr ? 0 : ql::attn_mod_bwd_workspace(*args);
+}
+
 int64_t ql_attn_bwd_partials_floats(int32_t n, int32_t max_len, int32_t HQ, int32_t HKV) {
   if (n <= 0 || max_len <= 0 || HKV <= 0 || HQ % HKV != 0) return 0;
   ql_attn_bwd_args a{};

@@ -90,6 +90,8 @@ void attn_set_impl(int impl);
 int exp2_fma_eval(const float* x, float* y, int64_t n, cudaStream_t s);
 int attn_bwd(const AttnBwdC& a, cudaStream_t s);
 int attn_mod_fwd(const ql_attn_mod_args& m, cudaStream_t s);
+int attn_mod_bwd(const ql_attn_mod_args& m, cudaStream_t s);
+int64_t attn_mod_bwd_workspace(const ql_attn_mod_args& m);
 }  // namespace ql
 
 namespace ql {

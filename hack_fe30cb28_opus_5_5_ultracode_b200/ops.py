@@ -575,6 +575,29 @@ def attn_mod_fwd(q, k, v, cu_seqlens, max_len, scale, causal=True, softcap=0.0, 
     return out, lse
 
 
+def attn_mod_bwd(dout, q, k, v, out, lse, cu_seqlens, max_len, scale, causal=True, softcap=0.0,
+                 slopes=None, window=0, doc_ids=None, prefix_len=None, dq=None, dk=None, dv=None):
+    """(dq, dk, dv) of attn_mod_fwd, in q's dtype, given its arguments, out and lse
+    (ql_attn_mod_bwd); dout [n, HQ, D] contiguous. Bit-identical from run to run."""
+    f, ranges = _attn_mod_fields(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes,
+                                 window, doc_ids, prefix_len)
+    _need_cuda(dout, out, lse)
+    _attn_mod_vector(dout, "dout", tuple(q.shape), q.dtype, q)
+    _attn_mod_vector(out, "out", tuple(q.shape), q.dtype, q)
+    _attn_mod_vector(lse, "lse", (q.shape[1], q.shape[0]), torch.float32, q)
+    dq = _attn_mod_like(dq, "dq", q.shape, q.dtype, q)
+    dk = _attn_mod_like(dk, "dk", k.shape, q.dtype, q)
+    dv = _attn_mod_like(dv, "dv", v.shape, q.dtype, q)
+    with _on_device(q.device):
+        args = _lib.struct("ql_attn_mod_args", out=_ptr(out), lse=_ptr(lse), dout=_ptr(dout),
+                           dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), **f)
+        need = int(_lib.lib().ql_attn_mod_bwd_workspace(ctypes_ref(args)))
+        ws = torch.empty(max(need, 4), device=q.device, dtype=torch.float32)
+        args.workspace, args.workspace_floats = _ptr(ws), ws.numel()
+        call("ql_attn_mod_bwd", ctypes_ref(args), stream_ptr())
+    return dq, dk, dv
+
+
 def gather_rows(src, idx, out=None):
     n, H = idx.numel(), src.shape[1]
     out = out if out is not None else torch.empty((n, H), device=src.device, dtype=torch.float32)

@@ -450,6 +450,10 @@ typedef struct {
 } ql_attn_mod_args;
 
 int ql_attn_mod_fwd(const ql_attn_mod_args* args, cudaStream_t stream);
+/* dq, dk, dv of every row of the sequences, given the forward's arguments, out and lse. */
+int ql_attn_mod_bwd(const ql_attn_mod_args* args, cudaStream_t stream);
+/* Floats of workspace the backward of these arguments needs (0 for arguments it refuses). */
+int64_t ql_attn_mod_bwd_workspace(const ql_attn_mod_args* args);
 
 /* ---- head row order ----------------------------------------------------------------------
  * The head takes rows with a target first (solution/engine.py:731, 1364-1398):

@@ -140,3 +140,24 @@ def test_forward_matches_the_formula(lengths, mode, heads, dtype):
     assert rel(out, want_out) < TOL[dtype]
     # lse in fp32: scores of a few units, rounded and exponentiated to ~1e-6 relative
     assert (lse.cpu().double()[~empty] - want_lse[~empty]).abs().max().item() < 2e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+@pytest.mark.parametrize("mode", MODES, ids=str)
+@pytest.mark.parametrize("heads,dtype", [((4, 2, 64), torch.bfloat16), ((6, 1, 128), torch.float16)],
+                         ids=["h4-2-64-bf16", "h6-1-128-fp16"])
+def test_backward_matches_the_formula(lengths, mode, heads, dtype):
+    q, k, v, dout, cu = batch(lengths, heads, dtype, seed=1)
+    scale = heads[2] ** -0.5
+    host, dev = mode_args(mode, lengths, heads[0])
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, max(lengths), scale, **dev)
+    got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, max(lengths), scale, **dev)
+    want = formula(q, k, v, lengths, scale, dout=dout, **host)[2:]
+    assert ops.device_status() == 0
+    for name, x, y in zip(("dq", "dk", "dv"), got, want):
+        assert x.dtype == dtype and torch.isfinite(x).all(), name
+        # a row whose probabilities are all 0 or 1 has a zero gradient in the formula, here at most
+        # the rounding of out inside dout . out: 2^-8 or 2^-11 of |dout| |out| ~ D
+        floor = TOL[dtype] * 0.02 * y.numel() ** 0.5
+        assert (x.double().cpu() - y).norm().item() < TOL[dtype] * y.norm().item() + floor, name
