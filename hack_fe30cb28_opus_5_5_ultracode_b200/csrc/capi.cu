@@ -233,6 +233,34 @@ int ql_rope_bwd(const ql_rope_bwd_args* args, cudaStream_t stream) {
   return done(ql::rope_bwd(*args, stream), "ql_rope_bwd");
 }
 
+int ql_mrope_fwd(const ql_mrope_args* args, cudaStream_t stream) {
+  if (args == nullptr) return fail(QL_STATUS_BAD_ARG, "ql_mrope_fwd");
+  return done(ql::mrope_fwd(*args, stream), "ql_mrope_fwd");
+}
+
+int ql_mrope_bwd(const ql_mrope_args* args, cudaStream_t stream) {
+  if (args == nullptr) return fail(QL_STATUS_BAD_ARG, "ql_mrope_bwd");
+  return done(ql::mrope_bwd(*args, stream), "ql_mrope_bwd");
+}
+
+int64_t ql_grad_norm_workspace(int count) { return count < 0 ? 0 : ql::grad_norm_workspace(count); }
+
+int ql_grad_norm(const ql_grad_tensor* tensors, int count, float inv_scale,
+                 const float* inv_scale_dev, float* norm, double* workspace,
+                 int64_t workspace_bytes, cudaStream_t stream) {
+  return done(ql::grad_norm(tensors, count, inv_scale, inv_scale_dev, norm, workspace,
+                            workspace_bytes, stream),
+              "ql_grad_norm");
+}
+
+int ql_clip_grads(const ql_grad_tensor* tensors, int count, float max_norm, float inv_scale,
+                  const float* inv_scale_dev, float* norm, double* workspace,
+                  int64_t workspace_bytes, cudaStream_t stream) {
+  return done(ql::clip_grads(tensors, count, max_norm, inv_scale, inv_scale_dev, norm, workspace,
+                             workspace_bytes, stream),
+              "ql_clip_grads");
+}
+
 int ql_glu_fwd(const void* gu, void* m, int64_t n, int I, int dtype, cudaStream_t stream) {
   return done(ql::glu_fwd(gu, m, n, I, dtype, stream), "ql_glu_fwd");
 }

@@ -1,0 +1,330 @@
+// Global 2-norm of a list of gradient tensors, and clipping by it.
+//
+// Two passes and no meeting of the CTAs inside a kernel: the first writes one sum of squares per
+// CTA; in the second every CTA adds those sums in the same order (fp64), so all arrive at the same
+// factor, and rescales its part. A gradient list that fits in L2 is read from HBM once; of a longer
+// one the second pass starts at the end, where the first pass left L2. Squares are summed in fp32 per
+// thread (four independent sums over at most a few thousand values), from there on in fp64.
+//
+// The tensors' addresses and sizes travel as kernel parameters (up to 1,024 tensors a launch), so a
+// call copies nothing to the device and can be captured. Work is cut into chunks of 32 KB of one
+// tensor, dealt to the CTAs in turn; a chunk whose addresses are 16-byte aligned moves 16 bytes per
+// thread, eight loads in flight, others element by element.
+//
+// Bound: HBM (one read for the norm; one read and one write for the rescale) for large lists, two
+// launch latencies for small ones.
+#include <algorithm>
+
+#include "common.cuh"
+#include "ops.h"
+#include "profile.h"
+
+namespace ql {
+
+namespace {
+
+constexpr int GC_THREADS = 256;
+constexpr int GC_CHUNK = 32768;      // bytes of gradient per chunk
+constexpr int GC_CTAS_PER_SM = 4;
+
+template <int MAX>
+struct GradList {
+  const void* grad[MAX];
+  void* out[MAX];
+  int64_t n[MAX];
+  int32_t first[MAX + 1];  // first chunk of each tensor; [count]: all chunks
+  uint8_t dtype[MAX], out_dtype[MAX];
+  int32_t count;
+};
+
+__device__ __forceinline__ int chunk_elems(int dtype) { return dtype == QL_F32 ? GC_CHUNK / 4 : GC_CHUNK / 2; }
+
+template <int MAX>
+__device__ __forceinline__ int tensor_of(const GradList<MAX>& l, int chunk) {
+  int lo = 0, hi = l.count;  // first[lo] <= chunk < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (l.first[mid] <= chunk) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void square16(const uint4& u, float* s) {
+  if constexpr (sizeof(T) == 4) {
+    const float* f = reinterpret_cast<const float*>(&u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = fmaf(f[e], f[e], s[e]);
+  } else {
+    const T* h = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = to_f<T>(h[e]);
+      s[e & 3] = fmaf(f, f, s[e & 3]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void chunk_squares(const T* p, int n, float* s) {
+  constexpr int V = 16 / sizeof(T);
+  int done = 0;
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    const uint4* v = reinterpret_cast<const uint4*>(p);
+    const int nv = n / V;
+    int i = threadIdx.x;
+    for (; i + 7 * GC_THREADS < nv; i += 8 * GC_THREADS) {
+      uint4 u[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[k] = v[i + k * GC_THREADS];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) square16<T>(u[k], s);
+    }
+    for (; i < nv; i += GC_THREADS) square16<T>(v[i], s);
+    done = nv * V;
+  }
+#pragma unroll 4
+  for (int i = done + threadIdx.x; i < n; i += GC_THREADS) {
+    const float f = to_f<T>(p[i]);
+    s[0] = fmaf(f, f, s[0]);
+  }
+}
+
+// Sum over the CTA in a fixed order; every thread gets it.
+__device__ __forceinline__ double cta_sum(double v) {
+  __shared__ double part[GC_THREADS / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double t = 0.0;
+#pragma unroll
+  for (int w = 0; w < GC_THREADS / 32; ++w) t += part[w];
+  return t;
+}
+
+template <int MAX>
+__global__ void __launch_bounds__(GC_THREADS) grad_squares_kernel(const __grid_constant__ GradList<MAX> l,
+                                                                  double* partial) {
+  pdl_enter();
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int c = blockIdx.x; c < l.first[l.count]; c += gridDim.x) {
+    const int t = tensor_of(l, c), dt = l.dtype[t], per = chunk_elems(dt);
+    const int64_t at = (int64_t)(c - l.first[t]) * per;
+    const int n = (int)min((int64_t)per, l.n[t] - at);
+    if (dt == QL_F32) chunk_squares(static_cast<const float*>(l.grad[t]) + at, n, s);
+    else if (dt == QL_F16) chunk_squares(static_cast<const __half*>(l.grad[t]) + at, n, s);
+    else chunk_squares(static_cast<const __nv_bfloat16*>(l.grad[t]) + at, n, s);
+  }
+  const double sum = cta_sum(((double)s[0] + (double)s[1]) + ((double)s[2] + (double)s[3]));
+  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+// The norm from the partial sums (the same in every CTA).
+__device__ __forceinline__ float total_norm(const double* partial, int partials, float inv_scale) {
+  double v = 0.0;
+  for (int i = threadIdx.x; i < partials; i += GC_THREADS) v += partial[i];
+  return (float)(sqrt(cta_sum(v)) * (double)inv_scale);
+}
+
+__global__ void __launch_bounds__(GC_THREADS) grad_norm_kernel(const double* partial, int partials,
+                                                               float inv_scale, const float* inv_scale_dev,
+                                                               float* norm) {
+  pdl_enter();
+  const float n = total_norm(partial, partials, inv_scale_dev != nullptr ? *inv_scale_dev : inv_scale);
+  if (threadIdx.x == 0) *norm = n;
+}
+
+template <typename TO, int V>
+__device__ __forceinline__ void store_v(TO* p, const float* v) {
+  if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+    for (int e = 0; e < V; e += 4)
+      __stcs(reinterpret_cast<float4*>(p + e), make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]));
+  } else if constexpr (V == 8) {
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(pack_t2<TO>(v[0], v[1]), pack_t2<TO>(v[2], v[3]),
+                                                   pack_t2<TO>(v[4], v[5]), pack_t2<TO>(v[6], v[7])));
+  } else {
+    __stcs(reinterpret_cast<uint2*>(p), make_uint2(pack_t2<TO>(v[0], v[1]), pack_t2<TO>(v[2], v[3])));
+  }
+}
+
+template <typename T, typename TO>
+__device__ __forceinline__ void chunk_scale(const T* p, TO* o, int n, float factor) {
+  constexpr int V = 16 / sizeof(T);
+  int done = 0;
+  if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
+    const uint4* v = reinterpret_cast<const uint4*>(p);
+    const int nv = n / V;
+    auto put = [&](const uint4& u, int at) {
+      const T* h = reinterpret_cast<const T*>(&u);
+      float f[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = to_f<T>(h[e]) * factor;
+      store_v<TO, V>(o + at * V, f);
+    };
+    int i = threadIdx.x;
+    for (; i + 7 * GC_THREADS < nv; i += 8 * GC_THREADS) {
+      uint4 u[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[k] = __ldcs(v + i + k * GC_THREADS);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) put(u[k], i + k * GC_THREADS);
+    }
+    for (; i < nv; i += GC_THREADS) put(__ldcs(v + i), i);
+    done = nv * V;
+  }
+#pragma unroll 4
+  for (int i = done + threadIdx.x; i < n; i += GC_THREADS) o[i] = from_f<TO>(to_f<T>(p[i]) * factor);
+}
+template <typename T>
+__device__ __forceinline__ void chunk_scale_to(const T* p, void* o, int out_dtype, int64_t at, int n, float factor) {
+  if (out_dtype == QL_F32) chunk_scale(p, static_cast<float*>(o) + at, n, factor);
+  else if (out_dtype == QL_F16) chunk_scale(p, static_cast<__half*>(o) + at, n, factor);
+  else chunk_scale(p, static_cast<__nv_bfloat16*>(o) + at, n, factor);
+}
+
+template <int MAX>
+__global__ void __launch_bounds__(GC_THREADS, GC_CTAS_PER_SM) grad_scale_kernel(const __grid_constant__ GradList<MAX> l,
+                                                                const double* partial, int partials,
+                                                                float max_norm, float inv_scale,
+                                                                const float* inv_scale_dev, float* norm,
+                                                                int in_place, int write_norm) {
+  pdl_enter();
+  if (inv_scale_dev != nullptr) inv_scale = *inv_scale_dev;
+  const float total = total_norm(partial, partials, inv_scale);
+  if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
+  const float ratio = max_norm / (total + 1e-6f);
+  const float factor = (ratio > 1.f ? 1.f : ratio) * inv_scale;  // a NaN stays one
+  if (in_place && factor == 1.f) return;                         // every gradient stays as it is
+  const int chunks = l.first[l.count];
+  for (int c = chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
+    const int t = tensor_of(l, c), dt = l.dtype[t], per = chunk_elems(dt);
+    const int64_t at = (int64_t)(c - l.first[t]) * per;
+    const int n = (int)min((int64_t)per, l.n[t] - at);
+    if (dt == QL_F32) chunk_scale_to(static_cast<const float*>(l.grad[t]) + at, l.out[t], l.out_dtype[t], at, n, factor);
+    else if (dt == QL_F16) chunk_scale_to(static_cast<const __half*>(l.grad[t]) + at, l.out[t], l.out_dtype[t], at, n, factor);
+    else chunk_scale_to(static_cast<const __nv_bfloat16*>(l.grad[t]) + at, l.out[t], l.out_dtype[t], at, n, factor);
+  }
+}
+
+constexpr int GC_SMALL = 128, GC_MAX = 1024;
+
+int elem_bytes(int dtype) { return dtype == QL_F32 ? 4 : 2; }
+bool dtype_ok(int dtype) { return dtype == QL_F16 || dtype == QL_BF16 || dtype == QL_F32; }
+
+// Tensors [begin, end) of the call as kernel parameters; false if there are too many chunks.
+template <int MAX>
+bool fill_list(const ql_grad_tensor* t, int begin, int end, GradList<MAX>& l) {
+  int64_t chunks = 0;
+  l.count = end - begin;
+  for (int i = begin; i < end; ++i) {
+    const int k = i - begin;
+    l.grad[k] = t[i].grad;
+    l.out[k] = t[i].out;
+    l.n[k] = t[i].n;
+    l.dtype[k] = (uint8_t)t[i].dtype;
+    l.out_dtype[k] = (uint8_t)t[i].out_dtype;
+    l.first[k] = (int32_t)chunks;
+    chunks += cdiv(t[i].n * elem_bytes(t[i].dtype), GC_CHUNK);
+    if (chunks > 0x3fffffff) return false;
+  }
+  l.first[l.count] = (int32_t)chunks;
+  return true;
+}
+
+int grid_of(int chunks) { return (int)std::max<int64_t>(1, std::min<int64_t>(chunks, (int64_t)sm_count() * GC_CTAS_PER_SM)); }
+
+struct ClipCall {
+  float max_norm, inv_scale;
+  const float* inv_scale_dev;
+  float* norm;
+  int in_place, partials;
+  double* partial;
+};
+
+template <int MAX>
+int squares(const ql_grad_tensor* t, int begin, int end, ClipCall& c, cudaStream_t s) {
+  GradList<MAX> l;
+  if (!fill_list(t, begin, end, l)) return QL_STATUS_UNSUPPORTED;
+  const int grid = grid_of(l.first[l.count]);
+  launch_k(grad_squares_kernel<MAX>, dim3(grid), dim3(GC_THREADS), 0, s, l, c.partial + c.partials);
+  c.partials += grid;
+  return launched(1);
+}
+template <int MAX>
+int rescale(const ql_grad_tensor* t, int begin, int end, const ClipCall& c, cudaStream_t s) {
+  GradList<MAX> l;
+  if (!fill_list(t, begin, end, l)) return QL_STATUS_UNSUPPORTED;
+  launch_k(grad_scale_kernel<MAX>, dim3(grid_of(l.first[l.count])), dim3(GC_THREADS), 0, s, l,
+           (const double*)c.partial, c.partials, c.max_norm, c.inv_scale, c.inv_scale_dev, c.norm,
+           c.in_place, begin == 0 ? 1 : 0);
+  return launched(1);
+}
+
+int clip_check(const ql_grad_tensor* t, int count, const float* norm, const double* ws, int64_t ws_bytes) {
+  if (count < 0 || (count > 0 && t == nullptr) || norm == nullptr || ws == nullptr ||
+      (reinterpret_cast<uintptr_t>(ws) & 7) || ws_bytes < grad_norm_workspace(count))
+    return QL_STATUS_BAD_ARG;
+  for (int i = 0; i < count; ++i)
+    if (t[i].n < 0 || t[i].n > (int64_t)1 << 40 || (t[i].n > 0 && t[i].grad == nullptr) || !dtype_ok(t[i].dtype) ||
+        (reinterpret_cast<uintptr_t>(t[i].grad) & (elem_bytes(t[i].dtype) - 1)))
+      return QL_STATUS_BAD_ARG;
+  return QL_STATUS_OK;
+}
+
+int all_squares(const ql_grad_tensor* t, int count, ClipCall& c, cudaStream_t s) {
+  for (int b = 0; b < count || b == 0; b += GC_MAX) {
+    const int e = std::min(count, b + GC_MAX);
+    const int st = e - b <= GC_SMALL ? squares<GC_SMALL>(t, b, e, c, s) : squares<GC_MAX>(t, b, e, c, s);
+    if (st != QL_STATUS_OK) return st;
+  }
+  return QL_STATUS_OK;
+}
+
+}  // namespace
+
+int64_t grad_norm_workspace(int count) {
+  return std::max<int64_t>(1, cdiv(count, GC_MAX)) * sm_count() * GC_CTAS_PER_SM * (int64_t)sizeof(double);
+}
+
+int grad_norm(const ql_grad_tensor* t, int count, float inv_scale, const float* inv_scale_dev, float* norm,
+              double* ws, int64_t ws_bytes, cudaStream_t s) {
+  int st = clip_check(t, count, norm, ws, ws_bytes);
+  if (st != QL_STATUS_OK) return st;
+  ProfScope prof(PK_OTHER, 0, 0, s);
+  ClipCall c{0.f, inv_scale, inv_scale_dev, norm, 0, 0, ws};
+  st = all_squares(t, count, c, s);
+  if (st != QL_STATUS_OK) return st;
+  launch_k(grad_norm_kernel, dim3(1), dim3(GC_THREADS), 0, s, (const double*)ws, c.partials, inv_scale,
+           inv_scale_dev, norm);
+  return launched(1);
+}
+
+int clip_grads(const ql_grad_tensor* t, int count, float max_norm, float inv_scale, const float* inv_scale_dev,
+               float* norm, double* ws, int64_t ws_bytes, cudaStream_t s) {
+  int st = clip_check(t, count, norm, ws, ws_bytes);
+  if (st != QL_STATUS_OK) return st;
+  if (!(max_norm >= 0.f)) return QL_STATUS_BAD_ARG;
+  int in_place = 1;
+  for (int i = 0; i < count; ++i) {
+    if (t[i].n == 0) continue;
+    if (t[i].out == nullptr || !dtype_ok(t[i].out_dtype) ||
+        (reinterpret_cast<uintptr_t>(t[i].out) & (elem_bytes(t[i].out_dtype) - 1)) ||
+        (t[i].out == t[i].grad && t[i].out_dtype != t[i].dtype))
+      return QL_STATUS_BAD_ARG;
+    in_place &= t[i].out == t[i].grad;
+  }
+  ProfScope prof(PK_OTHER, 0, 0, s);
+  ClipCall c{max_norm, inv_scale, inv_scale_dev, norm, in_place, 0, ws};
+  st = all_squares(t, count, c, s);
+  if (st != QL_STATUS_OK) return st;
+  for (int b = 0; b < count || b == 0; b += GC_MAX) {
+    const int e = std::min(count, b + GC_MAX);
+    st = e - b <= GC_SMALL ? rescale<GC_SMALL>(t, b, e, c, s) : rescale<GC_MAX>(t, b, e, c, s);
+    if (st != QL_STATUS_OK) return st;
+  }
+  return QL_STATUS_OK;
+}
+
+}  // namespace ql

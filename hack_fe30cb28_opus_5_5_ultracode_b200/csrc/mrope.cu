@@ -1,0 +1,494 @@
+// qkv + LoRA + rotary embedding with several position axes (time, height, width, ...), forward and
+// backward. Each of the D / 2 frequencies belongs to one axis; the angle of frequency f at token t
+// is the table's at row pos[axis(f)][t], so a text token (all positions equal) rotates as in
+// rope.cu and a picture's tokens by their row and column.
+//
+// A tile is 16 MT tokens. The tile's cosines and sines are gathered once into shared memory (a
+// gather of single floats where neighbouring frequencies belong to different axes) and serve every
+// head. Then each warp takes units of 32 columns of a head together with their 32 partners
+// D / 2 further on. The LoRA-B product of a unit is formed on the tensor cores in the layout the data
+// is moved in: the eight columns of an m16n8k16 step can be any eight outputs, and with output
+// 8 t + 2 j + e in column 2 t + e of step j, thread t of a row ends up with eight consecutive
+// columns after four steps - one 16-byte load and store. The product stays in fp32 (nothing is
+// rounded between the factors and the output). The backward uses the same ordering for the K
+// dimension of dx_lo = s g B, with g split into two 16-bit parts, so dx_lo is good to fp32.
+//
+// Bound: HBM for long batches (2 bytes read and 2 written per element in each direction), launch and
+// L2 latency for short ones.
+#include "common.cuh"
+#include "ops.h"
+#include "profile.h"
+
+namespace ql {
+
+namespace {
+
+constexpr int MR_RANK = 16;
+constexpr int MR_MAXHALF = 128;  // head sizes up to 256
+constexpr int MR_UNIT = 32;      // columns of a unit (and as many partners)
+
+struct MropeArgs {
+  const void* qkv;       // forward
+  const void* xq;
+  const void* xv;
+  const void* Bq;
+  const void* Bv;
+  void* q;
+  void* k;
+  void* v;
+  const void* dq;        // backward
+  const void* dk;
+  const void* dv;
+  void* dqkv;
+  float* dxlo_q;
+  float* dxlo_v;
+  const float* cos;
+  const float* sin;
+  const int32_t* pos;
+  int64_t ld_pos;
+  int32_t positions;
+  float lora_scale;
+  int n, HQ, HKV, D;
+  int* err;
+  uint8_t axis[MR_MAXHALF];
+};
+
+// cos / sin of the tile's tokens, [rows][half + 4] floats each
+__device__ __forceinline__ void stage_angles(const MropeArgs& a, float* sc, float* ss, int tok0, int rows) {
+  const int half = a.D / 2, pitch = half + 4;
+  for (int i = threadIdx.x; i < rows * half; i += blockDim.x) {
+    const int r = i / half, f = i % half, tok = tok0 + r;
+    float c = 0.f, s = 0.f;
+    if (tok < a.n) {
+      const int p = a.pos[a.axis[f] * a.ld_pos + tok];
+      if (p >= 0 && p < a.positions) {
+        c = __ldg(a.cos + (int64_t)p * half + f);
+        s = __ldg(a.sin + (int64_t)p * half + f);
+      } else {
+        raise_status(a.err, QL_STATUS_BAD_ARG);
+      }
+    }
+    sc[r * pitch + f] = c;
+    ss[r * pitch + f] = s;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* v) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+    const T* h = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f<T>(h[j]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* v) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_t2<T>(v[0], v[1]), pack_t2<T>(v[2], v[3]),
+                                            pack_t2<T>(v[4], v[5]), pack_t2<T>(v[6], v[7]));
+}
+
+// acc[m][rh][8] += x_lo . B^T for the 32 outputs from row o0 of B on: this thread's eight columns
+// 8 t .. 8 t + 7 of tokens g and g + 8 of each 16-token tile m
+template <typename T, int MT>
+__device__ __forceinline__ void lora_out(const uint32_t (*af)[4], const void* B, int64_t o0, float s,
+                                         float (*acc)[2][8]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t* base = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(B) +
+                         (o0 + (g >> 1) * 8 + (g & 1)) * MR_RANK);
+  uint32_t b0[4], b1[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {  // step j: column n of the step is output 8 (n / 2) + 2 j + n % 2
+    b0[j] = __ldg(base + j * MR_RANK + t);
+    b1[j] = __ldg(base + j * MR_RANK + 4 + t);
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      mma16816<T>(c, af[m], b0[j], b1[j]);
+      acc[m][0][2 * j] += c[0] * s;
+      acc[m][0][2 * j + 1] += c[1] * s;
+      acc[m][1][2 * j] += c[2] * s;
+      acc[m][1][2 * j + 1] += c[3] * s;
+    }
+}
+
+// A fragments of x_lo [n, 16] for the tile's tokens
+template <typename T, int MT>
+__device__ __forceinline__ void lora_in(const void* x, int tok0, int n, uint32_t (*af)[4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int rh = 0; rh < 2; ++rh) {
+      const int tok = tok0 + m * 16 + g + rh * 8;
+      uint32_t lo = 0, hi = 0;
+      if (tok < n) {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(x) + (int64_t)tok * MR_RANK);
+        lo = __ldg(p + t);
+        hi = __ldg(p + 4 + t);
+      }
+      af[m][rh] = lo;
+      af[m][2 + rh] = hi;
+    }
+}
+
+// ROWS tokens per tile: 8 (half of an m16 tile, for short batches) or 16 MT
+template <typename T, int MT, int ROWS>
+__global__ void __launch_bounds__(256) mrope_fwd_kernel(const __grid_constant__ MropeArgs a) {
+  pdl_enter();
+  extern __shared__ __align__(16) float angle_smem[];
+  const int half = a.D / 2, pitch = half + 4;
+  float* sc = angle_smem;
+  float* ss = angle_smem + ROWS * pitch;
+  const int tok0 = blockIdx.x * ROWS;
+  stage_angles(a, sc, ss, tok0, ROWS);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint32_t aq[MT][4], av[MT][4];
+  if (a.xq != nullptr) lora_in<T, MT>(a.xq, tok0, a.n, aq);
+  if (a.xv != nullptr) lora_in<T, MT>(a.xv, tok0, a.n, av);
+  __syncthreads();
+  const int per_head = half / MR_UNIT;
+  const int rot = (a.HQ + a.HKV) * per_head, units = rot + a.HKV * per_head;
+  const int64_t C = (int64_t)(a.HQ + 2 * a.HKV) * a.D;
+  const int step = gridDim.y * (blockDim.x >> 5);
+  for (int u = blockIdx.y * (blockDim.x >> 5) + warp; u < units; u += step) {
+    const bool is_rot = u < rot;
+    const int hh = is_rot ? u / per_head : a.HQ + a.HKV + (u - rot) / per_head;  // head of the qkv row
+    const int d0 = (u % per_head) * MR_UNIT, d = d0 + t * 8;
+    float x1[MT][2][8], x2[MT][2][8];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int rh = 0; rh < 2; ++rh) {
+        const int r = m * 16 + g + rh * 8, tok = tok0 + r;
+        if (r < ROWS && tok < a.n) {
+          const T* row = reinterpret_cast<const T*>(a.qkv) + tok * C + hh * a.D + d;
+          load8<T>(row, x1[m][rh]);
+          load8<T>(row + half, x2[m][rh]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x1[m][rh][e] = x2[m][rh][e] = 0.f;
+        }
+      }
+    const bool is_q = hh < a.HQ;
+    if (is_q ? a.xq != nullptr : (!is_rot && a.xv != nullptr)) {
+      const void* B = is_q ? a.Bq : a.Bv;
+      const int64_t o = (int64_t)(is_q ? hh : hh - a.HQ - a.HKV) * a.D + d0;
+      if (is_q) {
+        lora_out<T, MT>(aq, B, o, a.lora_scale, x1);
+        lora_out<T, MT>(aq, B, o + half, a.lora_scale, x2);
+      } else {
+        lora_out<T, MT>(av, B, o, a.lora_scale, x1);
+        lora_out<T, MT>(av, B, o + half, a.lora_scale, x2);
+      }
+    }
+    T* dst = is_q ? reinterpret_cast<T*>(a.q) + hh * a.D
+                  : is_rot ? reinterpret_cast<T*>(a.k) + (hh - a.HQ) * a.D
+                           : reinterpret_cast<T*>(a.v) + (hh - a.HQ - a.HKV) * a.D;
+    const int64_t ld = (int64_t)(is_q ? a.HQ : a.HKV) * a.D;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int rh = 0; rh < 2; ++rh) {
+        const int r = m * 16 + g + rh * 8, tok = tok0 + r;
+        if (r >= ROWS || tok >= a.n) continue;
+        float o1[8], o2[8];
+        if (is_rot) {
+          const float4* cp = reinterpret_cast<const float4*>(sc + r * pitch + d);
+          const float4* sp = reinterpret_cast<const float4*>(ss + r * pitch + d);
+          const float4 ca = cp[0], cb = cp[1], sa = sp[0], sb = sp[1];
+          const float c[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
+          const float s[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            o1[e] = x1[m][rh][e] * c[e] - x2[m][rh][e] * s[e];
+            o2[e] = x2[m][rh][e] * c[e] + x1[m][rh][e] * s[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            o1[e] = x1[m][rh][e];
+            o2[e] = x2[m][rh][e];
+          }
+        }
+        T* out = dst + tok * ld + d;
+        store8<T>(out, o1);
+        store8<T>(out + half, o2);
+      }
+  }
+}
+
+// c[2 tiles of N][4] += g . B for 32 columns of g (this thread: 8 t .. 8 t + 7 of tokens g and g + 8)
+// and the 32 rows of B from o0 on. Column n of N tile nt is rank 2 n + nt, so one 32-bit load of a
+// row of B serves both tiles; K index 2 t + e (8 + 2 t + e) of step s is row 8 t + 4 s + e (+ 2).
+template <typename T>
+__device__ __forceinline__ void lora_back(const float (*gv)[8], const void* B, int64_t o0, float (*c)[4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t* base = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(B) + (o0 + t * 8) * MR_RANK) + g;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = __ldg(base + (4 * s + e) * (MR_RANK / 2));
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int rh = 0; rh < 2; ++rh)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float p = gv[rh][4 * s + 2 * k], q = gv[rh][4 * s + 2 * k + 1];
+        const T ph = from_f<T>(p), qh = from_f<T>(q);
+        hi[rh + 2 * k] = pack_t2<T>(p, q);
+        lo[rh + 2 * k] = pack_t2<T>(p - to_f<T>(ph), q - to_f<T>(qh));
+      }
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      const uint32_t sel = nt == 0 ? 0x5410 : 0x7632;
+      const uint32_t b0 = __byte_perm(w[0], w[1], sel), b1 = __byte_perm(w[2], w[3], sel);
+      mma16816<T>(c[nt], hi, b0, b1);
+      mma16816<T>(c[nt], lo, b0, b1);
+    }
+  }
+}
+
+template <typename T, typename TG, int ROWS>
+__global__ void __launch_bounds__(256) mrope_bwd_kernel(const __grid_constant__ MropeArgs a) {
+  pdl_enter();
+  extern __shared__ __align__(16) float angle_smem[];
+  const int half = a.D / 2, pitch = half + 4;
+  float* sc = angle_smem;
+  float* ss = angle_smem + ROWS * pitch;
+  const int tok0 = blockIdx.x * ROWS;
+  stage_angles(a, sc, ss, tok0, ROWS);
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int warps = blockDim.x >> 5;
+  const int per_head = half / MR_UNIT;
+  const int rot = (a.HQ + a.HKV) * per_head, units = rot + a.HKV * per_head;
+  const int64_t C = (int64_t)(a.HQ + 2 * a.HKV) * a.D;
+  const bool lq = a.dxlo_q != nullptr, lv = a.dxlo_v != nullptr;
+  float cq[2][4] = {}, cv[2][4] = {};
+  for (int u = blockIdx.y * warps + warp; u < units; u += gridDim.y * warps) {
+    const bool is_rot = u < rot;
+    const int hh = is_rot ? u / per_head : a.HQ + a.HKV + (u - rot) / per_head;
+    const int d0 = (u % per_head) * MR_UNIT, d = d0 + t * 8;
+    const bool is_q = hh < a.HQ;
+    const TG* src = is_q ? reinterpret_cast<const TG*>(a.dq) + hh * a.D
+                         : is_rot ? reinterpret_cast<const TG*>(a.dk) + (hh - a.HQ) * a.D
+                                  : reinterpret_cast<const TG*>(a.dv) + (hh - a.HQ - a.HKV) * a.D;
+    const int64_t ld = (int64_t)(is_q ? a.HQ : a.HKV) * a.D;
+    float x1[2][8], x2[2][8];
+#pragma unroll
+    for (int rh = 0; rh < 2; ++rh) {
+      const int r = g + rh * 8, tok = tok0 + r;
+      if (r < ROWS && tok < a.n) {
+        load8<TG>(src + tok * ld + d, x1[rh]);
+        load8<TG>(src + tok * ld + d + half, x2[rh]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x1[rh][e] = x2[rh][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int rh = 0; rh < 2; ++rh) {
+      const int r = g + rh * 8, tok = tok0 + r;
+      if (r >= ROWS || tok >= a.n) continue;
+      if (is_rot) {
+        const float4* cp = reinterpret_cast<const float4*>(sc + r * pitch + d);
+        const float4* sp = reinterpret_cast<const float4*>(ss + r * pitch + d);
+        const float4 ca = cp[0], cb = cp[1], sa = sp[0], sb = sp[1];
+        const float c[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
+        const float s[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = x1[rh][e], q = x2[rh][e];
+          x1[rh][e] = p * c[e] + q * s[e];
+          x2[rh][e] = q * c[e] - p * s[e];
+        }
+      }
+      T* out = reinterpret_cast<T*>(a.dqkv) + tok * C + hh * a.D + d;
+      store8<T>(out, x1[rh]);
+      store8<T>(out + half, x2[rh]);
+    }
+    if (is_q ? lq : (!is_rot && lv)) {
+      const void* B = is_q ? a.Bq : a.Bv;
+      const int64_t o = (int64_t)(is_q ? hh : hh - a.HQ - a.HKV) * a.D + d0;
+      if (is_q) {
+        lora_back<T>(x1, B, o, cq);
+        lora_back<T>(x2, B, o + half, cq);
+      } else {
+        lora_back<T>(x1, B, o, cv);
+        lora_back<T>(x2, B, o + half, cv);
+      }
+    }
+  }
+  if (!lq && !lv) return;
+  // the warps' partial sums, added in warp order
+  float* red = angle_smem + 2 * ROWS * pitch;  // [warps][2][16 tokens][16]
+#pragma unroll
+  for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = g + (e >> 1) * 8, rank = 2 * (2 * t + (e & 1)) + nt;
+      red[((warp * 2 + 0) * 16 + r) * MR_RANK + rank] = cq[nt][e];
+      red[((warp * 2 + 1) * 16 + r) * MR_RANK + rank] = cv[nt][e];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * ROWS * MR_RANK; i += blockDim.x) {
+    const int ad = i / (ROWS * MR_RANK), r = (i / MR_RANK) % ROWS, rank = i % MR_RANK;
+    if (tok0 + r >= a.n || !(ad == 0 ? lq : lv)) continue;
+    float sum = 0.f;
+    for (int w = 0; w < warps; ++w) sum += red[((w * 2 + ad) * 16 + r) * MR_RANK + rank];
+    (ad == 0 ? a.dxlo_q : a.dxlo_v)[(int64_t)(tok0 + r) * MR_RANK + rank] = sum * a.lora_scale;
+  }
+}
+
+// The frequencies' axes: blocks of the sections, or dealt to the axes in turn while an axis has some
+// left. False if the sections do not make up D / 2.
+bool mrope_axes(const int32_t* sec, int axes, int interleaved, int half, uint8_t* axis) {
+  int64_t sum = 0;
+  for (int x = 0; x < axes; ++x) {
+    if (sec[x] < 0) return false;
+    sum += sec[x];
+  }
+  if (sum != half) return false;
+  int left[4] = {0, 0, 0, 0};
+  for (int x = 0; x < axes; ++x) left[x] = sec[x];
+  for (int f = 0, x = 0; f < half; ++f) {
+    if (interleaved) {
+      while (left[x] == 0) x = (x + 1) % axes;
+      axis[f] = (uint8_t)x;
+      --left[x];
+      x = (x + 1) % axes;
+    } else {
+      while (left[x] == 0) ++x;
+      axis[f] = (uint8_t)x;
+      --left[x];
+    }
+  }
+  return true;
+}
+
+int mrope_check(const ql_mrope_args& m, MropeArgs& a) {
+  if (m.n < 0 || m.HKV <= 0 || m.HQ <= 0 || m.D <= 0 || m.axes < 1 || m.axes > 4) return QL_STATUS_BAD_ARG;
+  if (m.D % 64 != 0 || m.D > 2 * MR_MAXHALF) return QL_STATUS_UNSUPPORTED;
+  if (m.dtype != QL_F16 && m.dtype != QL_BF16) return QL_STATUS_BAD_ARG;
+  a = MropeArgs{};
+  const int32_t sec[4] = {m.sec0, m.sec1, m.sec2, m.sec3};
+  if (!mrope_axes(sec, m.axes, m.interleaved, m.D / 2, a.axis)) return QL_STATUS_BAD_ARG;
+  if (m.n > 0 && (m.cos == nullptr || m.sin == nullptr || m.pos == nullptr || m.positions < 0 ||
+                  (m.axes > 1 && m.ld_pos < m.n)))
+    return QL_STATUS_BAD_ARG;
+  a.Bq = m.Bq;
+  a.Bv = m.Bv;
+  a.cos = m.cos;
+  a.sin = m.sin;
+  a.pos = m.pos;
+  a.ld_pos = m.ld_pos;
+  a.positions = m.positions;
+  a.lora_scale = m.lora_scale;
+  a.n = m.n;
+  a.HQ = m.HQ;
+  a.HKV = m.HKV;
+  a.D = m.D;
+  a.err = status_word();
+  return QL_STATUS_OK;
+}
+
+bool misaligned(std::initializer_list<const void*> ps, uintptr_t to) {
+  uintptr_t bits = 0;
+  for (const void* p : ps) bits |= reinterpret_cast<uintptr_t>(p);
+  return (bits & (to - 1)) != 0;
+}
+
+}  // namespace
+
+int mrope_fwd(const ql_mrope_args& m, cudaStream_t s) {
+  MropeArgs a;
+  const int st = mrope_check(m, a);
+  if (st != QL_STATUS_OK) return st;
+  if (m.n == 0) return QL_STATUS_OK;
+  if (m.qkv == nullptr || m.q == nullptr || m.k == nullptr || m.v == nullptr ||
+      (m.xq != nullptr && m.Bq == nullptr) || (m.xv != nullptr && m.Bv == nullptr) ||
+      misaligned({m.qkv, m.q, m.k, m.v}, 16) || misaligned({m.xq, m.xv, m.Bq, m.Bv}, 4))
+    return QL_STATUS_BAD_ARG;
+  a.qkv = m.qkv;
+  a.xq = m.xq;
+  a.xv = m.xv;
+  a.q = m.q;
+  a.k = m.k;
+  a.v = m.v;
+  const double elems = (double)m.n * (m.HQ + 2 * m.HKV) * m.D;
+  ProfScope prof(PK_ROPE_FWD, 0, elems * 4, s);
+  const int units = (m.HQ + 2 * m.HKV) * (m.D / 2 / MR_UNIT);
+  const int warps = units < 8 ? units : 8;
+#define QL_MROPEF(TT, MT, ROWS)                                                                   \
+  do {                                                                                            \
+    const int tiles = (int)cdiv(m.n, ROWS);                                                       \
+    int gy = (int)cdiv(2 * sm_count(), tiles); /* short batches: the columns over several CTAs */ \
+    const int most = (int)cdiv(units, warps);                                                     \
+    gy = gy < 1 ? 1 : gy > most ? most : gy;                                                      \
+    launch_k(mrope_fwd_kernel<TT, MT, ROWS>, dim3(tiles, gy), dim3(32 * warps),                   \
+             2 * ROWS * (m.D / 2 + 4) * 4, s, a);                                                 \
+  } while (0)
+  if (m.n > 32 * 4 * sm_count()) {
+    if (m.dtype == QL_F16) QL_MROPEF(__half, 2, 32); else QL_MROPEF(__nv_bfloat16, 2, 32);
+  } else {
+    if (m.dtype == QL_F16) QL_MROPEF(__half, 1, 16); else QL_MROPEF(__nv_bfloat16, 1, 16);
+  }
+#undef QL_MROPEF
+  return launched(1);
+}
+
+int mrope_bwd(const ql_mrope_args& m, cudaStream_t s) {
+  MropeArgs a;
+  const int st = mrope_check(m, a);
+  if (st != QL_STATUS_OK) return st;
+  if (m.grad_dtype != QL_F32 && m.grad_dtype != m.dtype) return QL_STATUS_BAD_ARG;
+  if (m.n == 0) return QL_STATUS_OK;
+  if (m.dq == nullptr || m.dk == nullptr || m.dv == nullptr || m.dqkv == nullptr ||
+      (m.dxlo_q != nullptr && m.Bq == nullptr) || (m.dxlo_v != nullptr && m.Bv == nullptr) ||
+      misaligned({m.dq, m.dk, m.dv, m.dqkv}, 16) || misaligned({m.Bq, m.Bv}, 4))
+    return QL_STATUS_BAD_ARG;
+  a.dq = m.dq;
+  a.dk = m.dk;
+  a.dv = m.dv;
+  a.dqkv = m.dqkv;
+  a.dxlo_q = m.dxlo_q;
+  a.dxlo_v = m.dxlo_v;
+  const bool lora = m.dxlo_q != nullptr || m.dxlo_v != nullptr;
+  const double elems = (double)m.n * (m.HQ + 2 * m.HKV) * m.D;
+  ProfScope prof(PK_ROPE_BWD, 0, elems * (m.grad_dtype == QL_F32 ? 6 : 4), s);
+  const int units = (m.HQ + 2 * m.HKV) * (m.D / 2 / MR_UNIT);
+  const int warps = units < 8 ? units : 8;
+#define QL_MROPEB(TT, TG, ROWS)                                                                   \
+  do {                                                                                            \
+    const int tiles = (int)cdiv(m.n, ROWS);                                                       \
+    int gy = lora ? 1 : (int)cdiv(2 * sm_count(), tiles);                                         \
+    const int most = (int)cdiv(units, warps);                                                     \
+    gy = gy < 1 ? 1 : gy > most ? most : gy;                                                      \
+    const int smem = 2 * ROWS * (m.D / 2 + 4) * 4 + (lora ? warps * 2 * 16 * MR_RANK * 4 : 0);    \
+    launch_k(mrope_bwd_kernel<TT, TG, ROWS>, dim3(tiles, gy), dim3(32 * warps), smem, s, a);      \
+  } while (0)
+#define QL_MROPEB2(ROWS)                                                                          \
+  do {                                                                                            \
+    if (m.dtype == QL_F16) {                                                                      \
+      if (m.grad_dtype == QL_F32) QL_MROPEB(__half, float, ROWS);                                 \
+      else QL_MROPEB(__half, __half, ROWS);                                                       \
+    } else {                                                                                      \
+      if (m.grad_dtype == QL_F32) QL_MROPEB(__nv_bfloat16, float, ROWS);                          \
+      else QL_MROPEB(__nv_bfloat16, __nv_bfloat16, ROWS);                                         \
+    }                                                                                             \
+  } while (0)
+  if (m.n > 16 * 2 * sm_count()) QL_MROPEB2(16); else QL_MROPEB2(8);
+#undef QL_MROPEB2
+#undef QL_MROPEB
+  return launched(1);
+}
+
+}  // namespace ql

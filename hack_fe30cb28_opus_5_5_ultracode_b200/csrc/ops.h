@@ -121,3 +121,13 @@ int profile_start(int capacity);
 int profile_stop();
 int profile_read(double* count, double* ms, double* flops, double* bytes);
 }  // namespace ql
+
+namespace ql {
+int mrope_fwd(const ql_mrope_args& m, cudaStream_t s);
+int mrope_bwd(const ql_mrope_args& m, cudaStream_t s);
+int64_t grad_norm_workspace(int count);
+int grad_norm(const ql_grad_tensor* t, int count, float inv_scale, const float* inv_scale_dev, float* norm,
+              double* ws, int64_t ws_bytes, cudaStream_t s);
+int clip_grads(const ql_grad_tensor* t, int count, float max_norm, float inv_scale, const float* inv_scale_dev,
+               float* norm, double* ws, int64_t ws_bytes, cudaStream_t s);
+}  // namespace ql

@@ -318,6 +318,192 @@ def rope_bwd(dq, dk, dv, cos, sin, pos, HQ, HKV, D, dtype=torch.float16, Bq=None
     return dqkv, dxlo_q, dxlo_v
 
 
+def _mrope_fields(cos, sin, pos, n, HQ, HKV, D, sections, interleaved, lora_scale, dtype, like):
+    """The checked fields both directions of mrope share."""
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"unsupported dtype {dtype}")
+    if HQ <= 0 or HKV <= 0 or D <= 0 or D % 64 or D > 256:
+        raise ValueError(f"heads ({HQ}, {HKV}, {D}): D must be 64, 128, 192 or 256")
+    axes = len(sections)
+    if not 1 <= axes <= 4 or any(x < 0 for x in sections) or sum(sections) != D // 2:
+        raise ValueError(f"sections {tuple(sections)} must be 1 to 4 counts that add to {D // 2}")
+    if pos.dim() != 2 or pos.shape != (axes, n) or pos.dtype != torch.int32 \
+            or (n > 1 and pos.stride(1) != 1):
+        raise ValueError(f"pos must be int32 [{axes}, {n}] with unit column stride")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dim() != 2 or t.shape != (cos.shape[0], D // 2) or t.dtype != torch.float32 \
+                or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous fp32 [positions, {D // 2}]")
+    if any(t.device != like.device for t in (cos, sin, pos)):
+        raise ValueError("cos, sin and pos must be on the input's device")
+    sec = [int(x) for x in sections] + [0] * (4 - axes)
+    return dict(cos=_ptr(cos), sin=_ptr(sin), pos=_ptr(pos), ld_pos=pos.stride(0) if axes > 1 else n,
+                lora_scale=float(lora_scale), n=n, HQ=HQ, HKV=HKV, D=D, dtype=dtype_code(dtype),
+                positions=cos.shape[0], axes=axes, sec0=sec[0], sec1=sec[1], sec2=sec[2],
+                sec3=sec[3], interleaved=int(bool(interleaved)))
+
+
+def _mrope_tensor(t, name, shape, dtype, like):
+    if t is None:
+        return
+    if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() \
+            or t.device != like.device:
+        raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)} on the input's device")
+
+
+def mrope_fwd(qkv, cos, sin, pos, HQ, HKV, D, sections, interleaved=False, lora_scale=1.0, xq=None,
+              xv=None, Bq=None, Bv=None, out=None):
+    """(q, k, v) of rope_fwd with several position axes (ql_mrope_fwd): pos int32 [axes, n],
+    sections = how many of the D / 2 frequencies each axis has, in blocks or (interleaved) dealt
+    to the axes in turn while an axis has some left; cos / sin the rotary table of one axis.
+    xq / Bq, xv / Bv: the LoRA-B products q += lora_scale xq Bq^T, added in fp32."""
+    _need_cuda(qkv, cos, sin, pos, xq, xv, Bq, Bv)
+    if qkv.dim() != 2:
+        raise ValueError("qkv must be [tokens, (HQ + 2 HKV) D]")
+    n, dt = qkv.shape[0], qkv.dtype
+    f = _mrope_fields(cos, sin, pos, n, HQ, HKV, D, sections, interleaved, lora_scale, dt, qkv)
+    _mrope_tensor(qkv, "qkv", (n, (HQ + 2 * HKV) * D), dt, qkv)
+    if (xq is None) != (Bq is None) or (xv is None) != (Bv is None):
+        raise ValueError("xq goes with Bq, and xv with Bv")
+    for name, t, shape in (("xq", xq, (n, 16)), ("xv", xv, (n, 16)), ("Bq", Bq, (HQ * D, 16)),
+                           ("Bv", Bv, (HKV * D, 16))):
+        _mrope_tensor(t, name, shape, dt, qkv)
+    if out is None:
+        q = torch.empty((n, HQ, D), device=qkv.device, dtype=dt)
+        k = torch.empty((n, HKV, D), device=qkv.device, dtype=dt)
+        v = torch.empty((n, HKV, D), device=qkv.device, dtype=dt)
+    else:
+        q, k, v = out
+        for name, t, heads in (("q", q, HQ), ("k", k, HKV), ("v", v, HKV)):
+            _mrope_tensor(t, name, (n, heads, D), dt, qkv)
+    with _on_device(qkv.device):
+        args = _lib.struct("ql_mrope_args", qkv=_ptr(qkv), xq=_ptr(xq), xv=_ptr(xv), Bq=_ptr(Bq),
+                           Bv=_ptr(Bv), q=_ptr(q), k=_ptr(k), v=_ptr(v), **f)
+        call("ql_mrope_fwd", ctypes_ref(args), stream_ptr())
+    return q, k, v
+
+
+def mrope_bwd(dq, dk, dv, cos, sin, pos, HQ, HKV, D, sections, interleaved=False,
+              dtype=torch.float16, Bq=None, Bv=None, lora_scale=1.0, out=None):
+    """(dqkv, dxlo_q, dxlo_v) of mrope_fwd (ql_mrope_bwd): the pre-rotary qkv gradient in `dtype`
+    from dq [n, HQ, D], dk / dv [n, HKV, D] (dtype or fp32), and with Bq / Bv the LoRA-A output
+    gradients lora_scale * (g . B), fp32 [n, 16]."""
+    _need_cuda(dq, dk, dv, cos, sin, pos, Bq, Bv)
+    if dq.dim() != 3:
+        raise ValueError("dq must be [tokens, HQ, D]")
+    n, dev = dq.shape[0], dq.device
+    f = _mrope_fields(cos, sin, pos, n, HQ, HKV, D, sections, interleaved, lora_scale, dtype, dq)
+    if dq.dtype not in (dtype, torch.float32):
+        raise ValueError(f"gradients must be {dtype} or fp32")
+    for name, t, heads in (("dq", dq, HQ), ("dk", dk, HKV), ("dv", dv, HKV)):
+        _mrope_tensor(t, name, (n, heads, D), dq.dtype, dq)
+    _mrope_tensor(Bq, "Bq", (HQ * D, 16), dtype, dq)
+    _mrope_tensor(Bv, "Bv", (HKV * D, 16), dtype, dq)
+    C = (HQ + 2 * HKV) * D
+    if out is not None:
+        _mrope_tensor(out, "out", (n, C), dtype, dq)
+    dqkv = out if out is not None else torch.empty((n, C), device=dev, dtype=dtype)
+    dxlo_q = torch.empty((n, 16), device=dev, dtype=torch.float32) if Bq is not None else None
+    dxlo_v = torch.empty((n, 16), device=dev, dtype=torch.float32) if Bv is not None else None
+    with _on_device(dev):
+        args = _lib.struct("ql_mrope_args", dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), dqkv=_ptr(dqkv),
+                           Bq=_ptr(Bq), Bv=_ptr(Bv), dxlo_q=_ptr(dxlo_q), dxlo_v=_ptr(dxlo_v),
+                           grad_dtype=dtype_code(dq.dtype), **f)
+        call("ql_mrope_bwd", ctypes_ref(args), stream_ptr())
+    return dqkv, dxlo_q, dxlo_v
+
+
+# ---------------------------------------------------------------------------------------------
+# gradient norm and clipping
+# ---------------------------------------------------------------------------------------------
+_GRAD_TENSOR = [("grad", "u8"), ("out", "u8"), ("n", "i8"), ("dtype", "i4"), ("out_dtype", "i4")]
+
+
+def _grad_list(tensors, name, device):
+    """(addresses, elements, dtype codes) of the tensors as numpy arrays, checked."""
+    import numpy as np
+
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError("CUDA tensors required (the library has no CPU path)")
+        if t.device != device:
+            raise ValueError(f"{name} must be on one device")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    return (np.array([t.data_ptr() for t in tensors], dtype=np.uint64),
+            np.array([t.numel() for t in tensors], dtype=np.int64),
+            np.array([dtype_code(t.dtype) for t in tensors], dtype=np.int32))
+
+
+def _overlap(addr, size, kind):
+    """Whether two of the tensors share memory."""
+    import numpy as np
+
+    end = addr + (size * np.where(kind == 2, 4, 2)).astype(np.uint64)
+    order = np.argsort(addr[size > 0], kind="stable")
+    a, e = addr[size > 0][order], end[size > 0][order]
+    return bool((a[1:] < e[:-1]).any())
+
+
+def _clip_call(grads, inv_scale, max_norm=None, out=None):
+    import numpy as np
+
+    grads = list(grads)
+    dev = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
+    addr, size, kind = _grad_list(grads, "gradients", dev)
+    arr = np.zeros(len(grads), dtype=_GRAD_TENSOR)
+    arr["grad"], arr["n"], arr["dtype"] = addr, size, kind
+    if max_norm is not None:
+        if _overlap(addr, size, kind):
+            raise ValueError("gradients share memory: each would be rescaled more than once")
+        if out is None:
+            arr["out"], arr["out_dtype"] = addr, kind
+        else:
+            out = list(out)
+            if len(out) != len(grads) or any(o.shape != g.shape for o, g in zip(out, grads)):
+                raise ValueError("out must hold a tensor of each gradient's shape")
+            o_addr, o_size, o_kind = _grad_list(out, "out", dev)
+            apart = (o_addr != addr) | (o_kind != kind)  # a gradient may be its own output
+            if _overlap(np.concatenate([addr, o_addr[apart]]),
+                        np.concatenate([size, o_size[apart]]),
+                        np.concatenate([kind, o_kind[apart]])):
+                raise ValueError("out shares memory with itself or with other gradients")
+            arr["out"], arr["out_dtype"] = o_addr, o_kind
+    scale_dev = None
+    if torch.is_tensor(inv_scale):
+        if inv_scale.numel() != 1 or inv_scale.dtype != torch.float32 or inv_scale.device != dev:
+            raise ValueError("inv_scale must be a number or an fp32 scalar on the gradients' device")
+        scale_dev, inv_scale = inv_scale, 1.0
+    norm = torch.empty((), device=dev, dtype=torch.float32)
+    with _on_device(dev):
+        ws = torch.empty(int(_lib.lib().ql_grad_norm_workspace(len(grads))), device=dev,
+                         dtype=torch.uint8)
+        tail = (float(inv_scale), _ptr(scale_dev), _ptr(norm), _ptr(ws), ws.numel(), stream_ptr())
+        if max_norm is None:
+            call("ql_grad_norm", arr.ctypes.data, len(grads), *tail)
+        else:
+            call("ql_clip_grads", arr.ctypes.data, len(grads), float(max_norm), *tail)
+    return norm
+
+
+def grad_norm(grads, inv_scale=1.0):
+    """The global 2-norm inv_scale * sqrt(sum of squares) of a list of gradient tensors (fp16, bf16
+    or fp32, contiguous, one device), as an fp32 scalar on the device (ql_grad_norm). inv_scale: a
+    number or a device scalar, e.g. one over a GradScaler's scale."""
+    return _clip_call(grads, inv_scale)
+
+
+def clip_grads(grads, max_norm, inv_scale=1.0, out=None):
+    """Rescales the gradients by inv_scale * min(1, max_norm / (norm + 1e-6)), in place or into the
+    tensors of `out` (same shapes, any of the three dtypes, e.g. fp32 master gradients), and returns
+    the norm before clipping as a device scalar (ql_clip_grads): torch.nn.utils.clip_grad_norm_ with
+    the unscaling folded in, in two kernels and with no host read. A norm that is not finite makes
+    every gradient not finite, as there."""
+    if not max_norm >= 0:
+        raise ValueError("max_norm must not be negative")
+    return _clip_call(grads, inv_scale, float(max_norm), out)
+
+
 # ---------------------------------------------------------------------------------------------
 # SwiGLU, LoRA weight gradients, embedding
 # ---------------------------------------------------------------------------------------------

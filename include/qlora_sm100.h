@@ -228,6 +228,41 @@ int ql_rope_fwd(const ql_rope_fwd_args* args, cudaStream_t stream);
  * solution/kernels.py:267-306) and dx_lo = s * (g @ B) (solution/engine.py:1322-1326). */
 int ql_rope_bwd(const ql_rope_bwd_args* args, cudaStream_t stream);
 
+/* ---- qkv + LoRA + RoPE with several position axes ------------------------------------------
+ * No counterpart in the reference (one position per token there). As ql_rope_fwd / ql_rope_bwd, but
+ * every one of the D / 2 frequencies belongs to one of `axes` (1 to 4) position axes and turns by
+ * its table entry at row pos[axis][token]. sec0 .. sec3: how many frequencies each axis has (their
+ * sum is D / 2), in blocks, or with `interleaved` dealt to the axes in turn while an axis has some
+ * left. D a multiple of 64, at most 256; rank 16; all tensors contiguous and 16-byte aligned
+ * (x*, B*: 4-byte). The LoRA-B product is added in fp32 without a rounding of its own, and dxlo is
+ * lora_scale * (g . B) of the unrounded gradient g, in fp32. A position outside [0, positions)
+ * records QL_STATUS_BAD_ARG in the device status word; its frequencies give 0. */
+typedef struct {
+  const void* qkv;      /* [n, (HQ + 2 HKV) D] */
+  const void* xq;       /* [n, 16] or NULL: q += lora_scale * xq . Bq^T */
+  const void* xv;
+  const void* Bq;       /* [HQ D, 16] */
+  const void* Bv;       /* [HKV D, 16] */
+  void* q;              /* [n, HQ, D] */
+  void* k;              /* [n, HKV, D] */
+  void* v;
+  const void* dq;       /* backward: [n, HQ, D] of grad_dtype (dtype or QL_F32) */
+  const void* dk;       /* [n, HKV, D] */
+  const void* dv;
+  void* dqkv;           /* [n, (HQ + 2 HKV) D] */
+  float* dxlo_q;        /* [n, 16] or NULL */
+  float* dxlo_v;
+  const float* cos;     /* [positions, D / 2] */
+  const float* sin;
+  const int32_t* pos;   /* [axes, n], row stride ld_pos */
+  int64_t ld_pos;
+  float lora_scale;
+  int32_t n, HQ, HKV, D, dtype, grad_dtype, positions, axes, sec0, sec1, sec2, sec3, interleaved;
+} ql_mrope_args;
+
+int ql_mrope_fwd(const ql_mrope_args* args, cudaStream_t stream);
+int ql_mrope_bwd(const ql_mrope_args* args, cudaStream_t stream);
+
 /* ---- SwiGLU ------------------------------------------------------------------------------ */
 /* Replaces _glu_fwd + glu_fwd_kernel (solution/engine.py:1012-1017, solution/kernels.py:312-321):
  * m[n, I] = silu(gu[:, :I]) * gu[:, I:]. I % 8 == 0. */
@@ -284,6 +319,31 @@ enum { QL_COLSUM_STATIC_FLOATS = 1048576 };
 int ql_lora_colsum_noalloc(const void* X, int64_t ldx, int x_dtype, const void* Y, int y_dtype,
                            int64_t n, int ncols, int rank, float scale, int transpose, float* out,
                            cudaStream_t stream);
+
+/* ---- global gradient norm and clipping ------------------------------------------------------
+ * No counterpart in the reference (HF Trainer clips through torch). norm = inv_scale *
+ * sqrt(sum of squares of every gradient); ql_clip_grads also writes
+ *   out = grad * inv_scale * min(1, max_norm / (norm + 1e-6))
+ * rounded once (out == grad: in place; nothing is written when that factor is 1). inv_scale undoes a
+ * loss scale; inv_scale_dev (a device float, or NULL) takes its place when given. A norm that is not
+ * finite makes the outputs not finite, as in torch. Gradients and outputs may differ in dtype from
+ * tensor to tensor (QL_F16, QL_BF16, QL_F32), must not overlap, and need only their own type's
+ * alignment (16 bytes is fastest). The tensor list is host memory, read during the call. The sums
+ * have a fixed order. workspace: ql_grad_norm_workspace(count) bytes, 8-byte aligned, of any
+ * content; calls that may overlap each need their own. */
+typedef struct {
+  const void* grad;
+  void* out;            /* ql_clip_grads only */
+  int64_t n;            /* elements */
+  int32_t dtype, out_dtype;
+} ql_grad_tensor;
+int64_t ql_grad_norm_workspace(int count);
+int ql_grad_norm(const ql_grad_tensor* tensors, int count, float inv_scale,
+                 const float* inv_scale_dev, float* norm, double* workspace,
+                 int64_t workspace_bytes, cudaStream_t stream);
+int ql_clip_grads(const ql_grad_tensor* tensors, int count, float max_norm, float inv_scale,
+                  const float* inv_scale_dev, float* norm, double* workspace,
+                  int64_t workspace_bytes, cudaStream_t stream);
 
 /* ---- embedding ---------------------------------------------------------------------------
  * Replaces the embedding lookup of FusedQwen2.step (solution/engine.py:1904-1907):

@@ -1,0 +1,197 @@
+"""The global gradient norm and clipping (ops.grad_norm / clip_grads) against 64-bit sums, and their
+refusals (CPU)."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from hack_fe30cb28_opus_5_5_ultracode_b200 import _lib, ops
+
+HALF_STEP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+def grads_of(sizes, dtypes, seed=0, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return [(torch.randn(n, generator=g) * std).to(dtypes[i % len(dtypes)]).cuda()
+            for i, n in enumerate(sizes)]
+
+
+def norm_of(grads):
+    return math.sqrt(sum(float(g.double().pow(2).sum()) for g in grads))
+
+
+def expected(grads, max_norm, inv_scale=1.0):
+    norm = norm_of(grads) * inv_scale
+    return norm, min(1.0, max_norm / (norm + 1e-6)) * inv_scale
+
+
+def check(outs, grads, factor):
+    for o, g in zip(outs, grads):
+        want = g.double() * factor
+        # one rounding of the result: half a step of the value, or of the smallest normal number
+        # for those below it; the fp32 factor is off by two roundings
+        step = want.abs().clamp(min=torch.finfo(o.dtype).tiny) * (HALF_STEP[o.dtype] + 3 * 2.0 ** -24)
+        assert ((o.double() - want).abs() <= step * 1.001).all()
+
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+LISTS = [([1], [F32]), ([0, 5, 0], [F16]), ([7, 8, 9, 4096, 8191, 8193, 16385, 1], [F32, BF16, F16]),
+         ([24576, 24576, 4096] * 37, [F32]), ([33] * 129, [BF16]), ([3, 50000] * 700, [F32, F16]),
+         ([10_000_001], [BF16]), ([3_000_000, 5], [F32])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes,dtypes", LISTS, ids=lambda x: str(x)[:30])
+@pytest.mark.parametrize("max_norm,inv_scale", [(1.0, 1.0), (0.5, 2.0 ** -7), (1e9, 1.0), (1e9, 0.5)])
+def test_norm_and_clip_match_64_bits(sizes, dtypes, max_norm, inv_scale):
+    grads = grads_of(sizes, dtypes)
+    norm, factor = expected(grads, max_norm, inv_scale)
+    got = ops.grad_norm(grads, inv_scale)
+    assert got.dtype == F32 and got.shape == ()
+    # squares and partial sums of at most a few thousand in fp32 (independent roundings), the
+    # rest in fp64, one rounding of the result
+    assert abs(got.item() - norm) <= 1e-6 * norm
+    outs = [torch.full_like(g, 7.0, dtype=F32) for g in grads]
+    keep = [g.clone() for g in grads]
+    assert torch.equal(ops.clip_grads(grads, max_norm, inv_scale, out=outs), got)
+    assert all(torch.equal(a, b) for a, b in zip(grads, keep))
+    check(outs, keep, factor)
+    assert torch.equal(ops.clip_grads(grads, max_norm, inv_scale), got)
+    check(grads, keep, factor)
+    if factor == 1.0:
+        assert all(torch.equal(a, b) for a, b in zip(grads, keep))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_views_at_any_alignment(offset):
+    for dtype in (F16, BF16, F32):
+        flat = grads_of([30011], [dtype])[0]
+        before = flat.clone()
+        views = [flat[offset:9000 + offset], flat[9000 + offset:9001 + offset], flat[12000 + offset:]]
+        norm, factor = expected([v.clone() for v in views], 1.0)
+        keep = [v.clone() for v in views]
+        assert abs(ops.clip_grads(views, 1.0).item() - norm) <= 1e-6 * norm
+        check(views, keep, factor)
+        assert torch.equal(flat[:offset], before[:offset])  # around and between the views
+        assert torch.equal(flat[9001 + offset:12000 + offset], before[9001 + offset:12000 + offset])
+
+
+@pytest.mark.gpu
+def test_the_scale_may_live_on_the_device():
+    grads = grads_of([1000, 3], [F32])
+    scale = torch.tensor(2.0 ** -5, device="cuda")
+    a, b = [g.clone() for g in grads], [g.clone() for g in grads]
+    assert torch.equal(ops.clip_grads(a, 0.1, scale), ops.clip_grads(b, 0.1, 2.0 ** -5))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_a_norm_that_is_not_finite_shows(bad):
+    grads = grads_of([1000, 3], [F32])
+    grads[1][2] = bad
+    want = [g.clone() for g in grads]
+    params = [torch.nn.Parameter(torch.zeros_like(g)) for g in want]
+    for p, g in zip(params, want):
+        p.grad = g
+    norm = torch.nn.utils.clip_grad_norm_(params, 1.0)
+    got = ops.clip_grads(grads, 1.0)
+    assert torch.equal(torch.isnan(got), torch.isnan(norm)) and not torch.isfinite(got)
+    for a, p in zip(grads, params):
+        assert torch.equal(torch.isfinite(a), torch.isfinite(p.grad))
+
+
+@pytest.mark.gpu
+def test_like_torch_on_an_adapter_sized_list():
+    grads = grads_of([24576, 4096] * 56, [F32], std=1e-3)
+    params = [torch.nn.Parameter(torch.zeros_like(g)) for g in grads]
+    for p, g in zip(params, grads):
+        p.grad = g.clone()
+    a = torch.nn.utils.clip_grad_norm_(params, 0.3)
+    b = ops.clip_grads(grads, 0.3)
+    assert abs(a.item() - b.item()) < 1e-6 * a.item()
+    for g, p in zip(grads, params):
+        assert torch.allclose(g, p.grad, rtol=1e-6, atol=0)
+
+
+@pytest.mark.gpu
+def test_an_empty_list_has_norm_zero():
+    assert ops.clip_grads([], 1.0).item() == 0.0
+    assert ops.grad_norm([]).item() == 0.0
+
+
+@pytest.mark.gpu
+def test_repeatable_and_capturable():
+    grads = grads_of([50001, 77, 8192] * 9, [BF16, F32])
+    outs = [torch.zeros_like(g) for g in grads]
+    want = ops.clip_grads(grads, 1.0, out=outs)
+    wanted = [o.clone() for o in outs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            norm = ops.clip_grads(grads, 1.0, out=outs)
+    for scale in (1.0, 3.0):
+        for g in grads:
+            g.mul_(scale)
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        if scale == 1.0:
+            assert torch.equal(norm, want) and all(torch.equal(a, b) for a, b in zip(outs, wanted))
+        else:
+            n, f = expected(grads, 1.0)
+            assert abs(norm.item() - n) < 1e-6 * n
+            check(outs, grads, f)
+
+
+@pytest.mark.gpu
+def test_bad_lists_are_refused():
+    a, b = grads_of([100, 50], [F32])
+    for bad, kw in (([a, a], {}), ([a, a[10:20]], {}), ([a[::2]], {}), ([a.int()], {}),
+                    ([a, b], dict(out=[a.clone()])), ([a, b], dict(out=[a.clone(), a.clone()])),
+                    ([a, b], dict(out=[b.new_zeros(100), a[:50]])), ([a], dict(out=[a[:].half()[:99]])),
+                    ([a], dict(inv_scale=torch.ones(2, device="cuda"))),
+                    ([a], dict(inv_scale=torch.ones((), device="cuda", dtype=torch.float64)))):
+        with pytest.raises(ValueError):
+            ops.clip_grads(bad, 1.0, **kw)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError):
+            ops.clip_grads([a], bad)
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.grad_norm([torch.ones(3)])
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.clip_grads([torch.ones(3)], 1.0)
+
+
+def test_the_overlap_check():
+    u8, i8, i4 = np.uint64, np.int64, np.int32
+    f = lambda a, n, k: ops._overlap(np.array(a, u8), np.array(n, i8), np.array(k, i4))  # noqa: E731
+    assert not f([400, 0], [10, 100], [2, 2])       # [400, 440) and [0, 400)
+    assert f([399, 0], [10, 100], [2, 2])
+    assert not f([200, 0], [10, 100], [2, 0])       # 16-bit: [0, 200)
+    assert not f([0, 0], [10, 0], [2, 2])           # an empty tensor shares nothing
+
+
+@pytest.mark.parametrize("change", [dict(dtype=3), dict(out_dtype=-1), dict(n=-1), dict(grad=0),
+                                    dict(out=0), dict(grad=(1 << 12) + 2), dict(out=(2 << 12) + 1),
+                                    dict(out=1 << 12, out_dtype=1), dict(max_norm=-1.0),
+                                    dict(max_norm=math.nan), dict(ws=0), dict(ws=4), dict(bytes=8)], ids=str)
+def test_the_library_refuses_before_any_launch(change):
+    arr = np.zeros(1, dtype=ops._GRAD_TENSOR)
+    f = dict(grad=1 << 12, out=2 << 12, n=10, dtype=2, out_dtype=2)
+    f.update({k: v for k, v in change.items() if k in f})
+    for k, v in f.items():
+        arr[k] = v
+    with pytest.raises(_lib.QLError) as e:
+        _lib.call("ql_clip_grads", arr.ctypes.data, 1, change.get("max_norm", 1.0), 1.0, None,
+                  3 << 12, change.get("ws", 4 << 12), change.get("bytes", 1 << 20), None)
+    assert e.value.status == 1

@@ -1,0 +1,212 @@
+"""qkv + LoRA + RoPE with several position axes (ops.mrope_fwd / mrope_bwd) against the formula in 64
+bits, and its refusals (CPU)."""
+
+import pytest
+import torch
+
+from hack_fe30cb28_opus_5_5_ultracode_b200 import _lib, ops
+
+
+def axes_of(sections, interleaved):
+    left, order = list(sections), []
+    if not interleaved:
+        return [x for x, c in enumerate(sections) for _ in range(c)]
+    while any(left):
+        for x in range(len(sections)):
+            if left[x]:
+                left[x] -= 1
+                order.append(x)
+    return order
+
+
+def rotate(x, cos, sin, back=False):
+    half = x.shape[-1] // 2
+    a, b = x[..., :half], x[..., half:]
+    s = -sin if back else sin
+    return torch.cat([a * cos - b * s, b * cos + a * s], -1)
+
+
+def angles(cos, sin, pos, sections, interleaved):
+    half = cos.shape[1]
+    ax = torch.tensor(axes_of(sections, interleaved))
+    row = pos.long()[ax].t()
+    f = torch.arange(half)
+    return cos.double()[row, f][:, None], sin.double()[row, f][:, None]
+
+
+def case(n, heads, dtype, sections, seed=0, positions=500):
+    HQ, HKV, D = heads
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    t = torch.outer(torch.arange(positions, dtype=torch.float64),
+                    1e4 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D))
+    return dict(qkv=r(n, (HQ + 2 * HKV) * D).to(dtype), cos=t.cos().float(), sin=t.sin().float(),
+                pos=torch.randint(0, positions, (len(sections), n), generator=g).int(),
+                xq=r(n, 16).to(dtype), xv=r(n, 16).to(dtype), Bq=(r(HQ * D, 16) * 0.2).to(dtype),
+                Bv=(r(HKV * D, 16) * 0.2).to(dtype), dq=r(n, HQ, D), dk=r(n, HKV, D),
+                dv=r(n, HKV, D))
+
+
+def cuda(c):
+    return {k: v.cuda() for k, v in c.items()}
+
+
+# one rounding of each output to the type: at most half a step, eps / 2, of the value (plus fp32
+# arithmetic, some 2^-21); in the 2-norm no more than that either
+HALF_STEP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def rel(x, y):
+    return ((x.double().cpu() - y).norm() / y.norm().clamp(min=1e-30)).item()
+
+
+SHAPES = [((4, 2, 64), (8, 12, 12), False), ((12, 2, 128), (16, 24, 24), True),
+          ((28, 4, 128), (64,), False), ((3, 3, 192), (50, 0, 16, 30), True),
+          ((5, 1, 256), (1, 127), True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 7, 8, 17, 300, 5001, 19001])
+@pytest.mark.parametrize("heads,sections,interleaved", SHAPES, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_forward_and_backward_match_the_formula(n, heads, sections, interleaved, dtype):
+    if n > 5000 and heads[0] > 12:
+        n = n // 4
+    HQ, HKV, D = heads
+    c, s = case(n, heads, dtype, sections), 1.75
+    d = cuda(c)
+    args = (d["cos"], d["sin"], d["pos"], HQ, HKV, D, sections)
+    cos, sin = angles(c["cos"], c["sin"], c["pos"], sections, interleaved)
+    x = c["qkv"].double().view(n, HQ + 2 * HKV, D)
+    for lora in (True, False):
+        kw = {k: d[k] for k in ("xq", "xv", "Bq", "Bv")} if lora else {}
+        got = ops.mrope_fwd(d["qkv"], *args, interleaved=interleaved, lora_scale=s, **kw)
+        q, k, v = x[:, :HQ], x[:, HQ:HQ + HKV], x[:, HQ + HKV:]
+        if lora:
+            q = q + s * (c["xq"].double() @ c["Bq"].double().t()).view(n, HQ, D)
+            v = v + s * (c["xv"].double() @ c["Bv"].double().t()).view(n, HKV, D)
+        for a, b in zip(got, (rotate(q, cos, sin), rotate(k, cos, sin), v)):
+            assert a.dtype == dtype and rel(a, b) < HALF_STEP[dtype] * 1.01 + 1e-6
+        for grads in (torch.float32, dtype):
+            gs = [c[k].to(grads) for k in ("dq", "dk", "dv")]
+            gd = [g.cuda() for g in gs]
+            kw = {k: d[k] for k in ("Bq", "Bv")} if lora else {}
+            dqkv, dxq, dxv = ops.mrope_bwd(*gd, *args, interleaved=interleaved, dtype=dtype,
+                                           lora_scale=s, **kw)
+            gq, gk = (rotate(g.double(), cos, sin, back=True) for g in gs[:2])
+            gv = gs[2].double()
+            want = torch.cat([gq, gk, gv], 1).view(n, -1)
+            assert dqkv.dtype == dtype and rel(dqkv, want) < HALF_STEP[dtype] * 1.01 + 1e-6
+            if not lora:
+                assert dxq is None and dxv is None
+                continue
+            # g in two 16-bit parts: what is left over is 2^-17 (bf16) of each term at most, and
+            # the fp32 sums of a few thousand terms add about as little
+            for a, b in ((dxq, s * gq.reshape(n, -1) @ c["Bq"].double()),
+                         (dxv, s * gv.reshape(n, -1) @ c["Bv"].double())):
+                assert a.dtype == torch.float32 and rel(a, b) < 2.0 ** -17 + 2e-6
+    assert ops.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_one_axis_equals_the_single_position_rope():
+    heads, n = (12, 2, 128), 700
+    c = cuda(case(n, heads, torch.float16, (64,)))
+    a = ops.rope_fwd(c["qkv"], c["cos"], c["sin"], c["pos"][0].contiguous(), *heads, 1.0)
+    b = ops.mrope_fwd(c["qkv"], c["cos"], c["sin"], c["pos"], *heads, (64,))
+    for x, y in zip(a, b):  # the same fp32 formula; contraction may differ by one rounding
+        assert rel(x, y.double().cpu()) < 2.0 ** -11
+
+
+@pytest.mark.gpu
+def test_strided_positions_and_given_outputs():
+    heads, n, sections = (4, 2, 64), 90, (8, 12, 12)
+    c = cuda(case(n, heads, torch.bfloat16, sections))
+    wide = torch.full((3, 200), -1, device="cuda", dtype=torch.int32)
+    wide[:, 10:10 + n] = c["pos"]
+    out = [torch.empty(n, h, 64, device="cuda", dtype=torch.bfloat16) for h in (4, 2, 2)]
+    got = ops.mrope_fwd(c["qkv"], c["cos"], c["sin"], wide[:, 10:10 + n], *heads, sections, out=out)
+    want = ops.mrope_fwd(c["qkv"], c["cos"], c["sin"], c["pos"], *heads, sections)
+    assert all(g is o and torch.equal(g, w) for g, o, w in zip(got, out, want))
+
+
+@pytest.mark.gpu
+def test_positions_off_the_table_are_reported_and_read_nothing():
+    heads, sections = (4, 2, 64), (8, 12, 12)
+    c = cuda(case(5, heads, torch.float16, sections))
+    c["pos"][1, 2], c["pos"][0, 4] = 500, -1
+    ops.device_status(clear=True)
+    q, _, v = ops.mrope_fwd(c["qkv"], c["cos"], c["sin"], c["pos"], *heads, sections)
+    assert ops.device_status(clear=True) == 1  # QL_STATUS_BAD_ARG
+    ax = torch.tensor(axes_of(sections, False) * 2)
+    assert not q[2, :, (ax == 1).cuda()].any() and not q[4, :, (ax == 0).cuda()].any()
+    assert q[2, :, (ax == 0).cuda()].all() and torch.isfinite(v).all()
+
+
+@pytest.mark.gpu
+def test_no_tokens():
+    c = cuda(case(0, (4, 2, 64), torch.float16, (8, 12, 12)))
+    q, k, v = ops.mrope_fwd(c["qkv"], c["cos"], c["sin"], c["pos"], 4, 2, 64, (8, 12, 12))
+    assert q.shape == (0, 4, 64) and k.shape == v.shape == (0, 2, 64)
+
+
+def test_cpu_tensors_are_refused():
+    c = case(3, (4, 2, 64), torch.float16, (8, 12, 12))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.mrope_fwd(c["qkv"], c["cos"], c["sin"], c["pos"], 4, 2, 64, (8, 12, 12))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.mrope_bwd(c["dq"], c["dk"], c["dv"], c["cos"], c["sin"], c["pos"], 4, 2, 64, (8, 12, 12))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("change", [dict(sections=(8, 12, 11)), dict(sections=(8, 12, 13, -1)),
+                                    dict(sections=(4,) * 8), dict(pos="long"), dict(pos="short"),
+                                    dict(cos="half"), dict(D=96), dict(qkv="strided"),
+                                    dict(xq="alone"), dict(Bq="dtype")], ids=str)
+def test_bad_arguments_are_refused(change):
+    c = cuda(case(6, (4, 2, 64), torch.float16, (8, 12, 12)))
+    kw = {k: c[k] for k in ("xq", "Bq")}
+    sections, D = change.get("sections", (8, 12, 12)), change.get("D", 64)
+    if change.get("pos") == "long":
+        c["pos"] = c["pos"].long()
+    if change.get("pos") == "short":
+        c["pos"] = c["pos"][:, :5]
+    if change.get("cos") == "half":
+        c["cos"] = c["cos"].half()
+    if change.get("qkv") == "strided":
+        c["qkv"] = torch.cat([c["qkv"], c["qkv"]], 1)[:, ::2]
+    if change.get("xq") == "alone":
+        del kw["Bq"]
+    if change.get("Bq") == "dtype":
+        kw["Bq"] = kw["Bq"].float()
+    with pytest.raises(ValueError):
+        ops.mrope_fwd(c["qkv"], c["cos"], c["sin"], c["pos"], 4, 2, D, sections, **kw)
+
+
+def fake_args(**change):
+    """Arguments the library checks before it launches anything (made-up, aligned addresses)."""
+    f = dict(qkv=1 << 12, q=2 << 12, k=3 << 12, v=4 << 12, dq=5 << 12, dk=6 << 12, dv=7 << 12,
+             dqkv=8 << 12, cos=9 << 12, sin=10 << 12, pos=11 << 12, ld_pos=5, lora_scale=1.0, n=5,
+             HQ=4, HKV=2, D=64, dtype=0, grad_dtype=0, positions=9, axes=3, sec0=8, sec1=12,
+             sec2=12, interleaved=0)
+    f.update(change)
+    return _lib.struct("ql_mrope_args", **f)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(axes=0), 1), (dict(axes=5), 1), (dict(sec0=9), 1), (dict(sec0=-8, sec1=28), 1),
+    (dict(D=32), 3), (dict(D=320), 3), (dict(dtype=2), 1), (dict(n=-1), 1), (dict(ld_pos=4), 1),
+    (dict(cos=None), 1), (dict(positions=-1), 1), (dict(HKV=0), 1)], ids=str)
+def test_the_library_refuses_before_any_launch(change, status):
+    for entry in ("ql_mrope_fwd", "ql_mrope_bwd"):
+        args = fake_args(**change)
+        with pytest.raises(_lib.QLError) as e:
+            _lib.call(entry, ops.ctypes_ref(args), None)
+        assert e.value.status == status
+    for entry, only in (("ql_mrope_fwd", dict(qkv=None)), ("ql_mrope_fwd", dict(q=8)),
+                        ("ql_mrope_fwd", dict(xq=1 << 16)), ("ql_mrope_bwd", dict(dqkv=None)),
+                        ("ql_mrope_bwd", dict(dxlo_q=1 << 16)), ("ql_mrope_bwd", dict(grad_dtype=1))):
+        args = fake_args(**only)
+        with pytest.raises(_lib.QLError) as e:
+            _lib.call(entry, ops.ctypes_ref(args), None)
+        assert e.value.status == 1
