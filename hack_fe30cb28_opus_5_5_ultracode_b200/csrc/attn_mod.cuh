@@ -185,16 +185,95 @@ __device__ __forceinline__ uint64_t tanh_poly2(uint64_t u) {
   return mul2(p, u);
 }
 
-// ---- tensor core with A in tensor memory -----------------------------------------------------
-// D += A . B with the 16-bit A [128 x 16] in TMEM (row = lane, two elements per 32-bit column)
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b,
-                                            uint32_t idesc, uint32_t accumulate) {
+// 16 consecutive fp32 columns of this thread's TMEM lane (with the wait), and into it (tmem_wait_st()
+// before they are read).
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+      : "memory");
+}
+
+// ---- whole products, issued by a converged warp -----------------------------------------------
+// The MMA warp runs its loop with all 32 lanes and elects the issuing one inside each instruction
+// sequence, and the operand descriptors differ from step to step by a constant in their low word. So
+// the compiler can keep descriptors and addresses in uniform registers: issued by `if (lane == 0)`
+// from descriptors built per step, the 16 MMAs of a tile and block took 1,400-2,000 cycles of this
+// warp, longer than the tensor core needs for them (8,192 causal tokens, 12 heads: 220 us,
+// and 194 us in this form).
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
+
+// High words of the operand descriptors (128-byte swizzle, version 1): stride 1024 B between groups of
+// 8 rows. Low words: start address / 16, and for MN-major operands the distance of 64-element chunks.
+constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo_k(uint32_t smem_addr) { return ((smem_addr >> 4) & 0x3FFFu) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_lo_mn(uint32_t smem_addr, uint32_t chunk) {
+  return ((smem_addr >> 4) & 0x3FFFu) | ((chunk >> 4) << 16);
+}
+
+// D (+)= A . B^T over a head of D_ elements, both operands K-major tiles of 64-column boxes
+#define QL_AM_SS(OFF)                                                                              \
+  "add.u32 x, %1, " OFF "; add.u32 y, %2, " OFF ";\n\t"                                            \
+  "mov.b64 a, {x, %4}; mov.b64 b, {y, %4};\n\t"                                                   \
+  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"                                  \
+  "setp.eq.u32 p, 0, 0;\n\t"
+template <int D_>
+__device__ __forceinline__ void umma_score(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+  static_assert(D_ == 64 || D_ == 128, "one or two 64-column boxes");
+  if constexpr (D_ == 64) {
+    asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 a, b;\n\t"
+                 "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, 0, 0;\n\t"
+                 QL_AM_SS("0") QL_AM_SS("2") QL_AM_SS("4") QL_AM_SS("6") "}"
+                 ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(DESC_HI) : "memory");
+  } else {  // the second box: 128 rows x 128 bytes further on
+    asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 a, b;\n\t"
+                 "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, 0, 0;\n\t"
+                 QL_AM_SS("0") QL_AM_SS("2") QL_AM_SS("4") QL_AM_SS("6")
+                 QL_AM_SS("1024") QL_AM_SS("1026") QL_AM_SS("1028") QL_AM_SS("1030") "}"
+                 ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(DESC_HI) : "memory");
+  }
+}
+#undef QL_AM_SS
+
+// D (+)= A . B over 128 rows of the MN-major tile B: A [128 x 128] 16-bit in TMEM, two elements per
+// 32-bit column, kept in parts of 16 PART columns whose starts are PART_STEP columns apart.
+#define QL_AM_TS(AOFF, BOFF)                                                                       \
+  "add.u32 x, %1, " AOFF "; add.u32 y, %2, " BOFF ";\n\t"                                          \
+  "mov.b64 b, {y, %4};\n\t"                                                                       \
+  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, p;\n\t"                                \
+  "setp.eq.u32 p, 0, 0;\n\t"
+// two parts of 32 columns, 64 apart (two softmax threads per row)
+__device__ __forceinline__ void umma_gather2(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t more) {
+  asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
+               "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+               QL_AM_TS("0", "0") QL_AM_TS("8", "128") QL_AM_TS("16", "256") QL_AM_TS("24", "384")
+               QL_AM_TS("64", "512") QL_AM_TS("72", "640") QL_AM_TS("80", "768") QL_AM_TS("88", "896") "}"
+               ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
+}
+// four parts of 16 columns, 32 apart (four softmax threads per row)
+__device__ __forceinline__ void umma_gather4(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t more) {
+  asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
+               "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+               QL_AM_TS("0", "0") QL_AM_TS("8", "128") QL_AM_TS("32", "256") QL_AM_TS("40", "384")
+               QL_AM_TS("64", "512") QL_AM_TS("72", "640") QL_AM_TS("96", "768") QL_AM_TS("104", "896") "}"
+               ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
+}
+#undef QL_AM_TS
+
+// umma_commit by the lane that issues the MMAs
+__device__ __forceinline__ void warp_commit(uint64_t* bar) {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+               "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+               ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Which of the 128 rows [j0, j0 + 128) of a tile hold no key or query of the sequence (past its
@@ -240,6 +319,14 @@ __device__ __forceinline__ void attn_zero_rows(uint8_t* tile, const uint32_t bad
 // wait ran out leaves together.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+}
+
+// One arrival for the warp, after every lane's work before it (TMEM loads and stores completed and
+// fenced by each lane). Arrivals of single lanes would be serialised on the barrier's word: 512 of them
+// a step held the backward's chain up by about a thousand cycles.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // Host: raises a kernel's dynamic shared-memory limit on the current device, once per device.

@@ -2,15 +2,16 @@
 // 64 and 128): see attn_mod.cuh for the score and the masks.
 //
 // One CTA takes two adjacent 128-query tiles of one head; both read the same K and V blocks of
-// 128 keys, so each block crosses from L2 once for 256 queries. Ten warps:
-//   warps 0-3, 4-7  softmax of tile 0 and of tile 1, one thread per query row (TMEM lane = row):
-//                   the row's 128 scores into registers, running maximum, P as 16-bit pairs back
-//                   into the score's TMEM columns, where the next product reads it as its A operand;
-//   warp 8          one thread issues the MMAs: for each block O_t += P_t V and then the next
+// 128 keys, so each block crosses from L2 once for 256 queries. Eighteen warps:
+//   warps 0-7, 8-15 softmax of tile 0 and of tile 1, two threads per query row (TMEM lane = row), 64
+//                   of the 128 keys each: scores into registers, the row's maximum (the two threads
+//                   exchange theirs through shared memory), P as 16-bit pairs back into the score's
+//                   TMEM columns, where the next product reads it as its A operand;
+//   warp 16         one thread issues the MMAs: for each block O_t += P_t V and then the next
 //                   block's S_t = Q_t K^T, tile 0 and tile 1 in turn, so the tensor core works on
 //                   one tile while the other tile's softmax runs;
-//   warp 9          TMA: Q tiles, then K and V blocks through a ring of tiles.
-// TMEM columns: S_0 [0, 128), S_1 [128, 256) (P_t in the first 64 of S_t), O_0 [256, 256 + D),
+//   warp 17         TMA: Q tiles, then K and V blocks through a ring of tiles.
+// TMEM columns: S_0 [0, 128), S_1 [128, 256) (P_t in the first 32 of each half of S_t), O_0 [256, 256 + D),
 // O_1 [384, 384 + D).
 // The running maximum moves only when it grows by more than 2^8; then the row's O is rescaled.
 // P is rounded to the input type for the product (half a step of 2^-8 or 2^-11 per probability,
@@ -27,10 +28,12 @@ struct FwdCfg {
   static constexpr int TILE = AM_T * D * 2;          // bytes of a 128-row tile
   static constexpr int STAGES = D == 128 ? 5 : 8;    // ring of K / V tiles
   static constexpr int OFF_KV = 2 * TILE;
-  static constexpr int OFF_BAR = OFF_KV + STAGES * TILE;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024 /*align*/;
+  static constexpr int OFF_M = OFF_KV + STAGES * TILE;  // [2 tiles][2 halves][128] fp32 exchange
+  static constexpr int OFF_BAR = OFF_M + 4 * AM_T * 4;
+  static constexpr int SMEM = OFF_BAR + 512;
 };
-constexpr int FWD_THREADS = 320;
+constexpr int FWD_THREADS = 576;
+constexpr int FWD_HC = 64;  // columns per softmax thread
 
 // What the score's modes need per kernel.
 struct ScoreConst {
@@ -40,7 +43,7 @@ struct ScoreConst {
 };
 
 // Scores of one row and one key block, in place: raw products to log2 units (MODE 0 leaves them
-// raw: the scale rides in the exponent's FMA), masked ones to -inf. x: 128 values; dist0 = i - j0.
+// raw: the scale rides in the exponent's FMA), masked ones to -inf. x: 64 values; dist0 = i - their first key.
 template <int MODE, bool MASKED>
 __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, float slope2,
                                               float dist0, int rlo, int rhi) {
@@ -48,13 +51,13 @@ __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, 
     // the largest |u| of the warp's rows decides between the polynomial and tanhf
     float mx = 0.f;
 #pragma unroll
-    for (int i = 0; i < AM_T; i += 2)
+    for (int i = 0; i < FWD_HC; i += 2)
       mx = max3(mx, fabsf(__uint_as_float(x[i])), fabsf(__uint_as_float(x[i + 1])));
     const bool poly = __all_sync(0xffffffffu, mx * c.u <= TANH_POLY_MAX);
     if (poly) {
       const uint64_t uu = pk2(c.u, c.u), cc = pk2(c.cap2, c.cap2);
 #pragma unroll
-      for (int i = 0; i < AM_T; i += 2) {
+      for (int i = 0; i < FWD_HC; i += 2) {
         const uint64_t y = mul2(tanh_poly2(mul2(pk2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), uu)), cc);
         float a, b;
         up2(y, a, b);
@@ -63,20 +66,20 @@ __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, 
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < AM_T; ++i)
+      for (int i = 0; i < FWD_HC; ++i)
         x[i] = __float_as_uint(tanhf(__uint_as_float(x[i]) * c.u) * c.cap2);
     }
   }
   if constexpr ((MODE & 2) != 0) {
 #pragma unroll
-    for (int i = 0; i < AM_T; ++i) {
+    for (int i = 0; i < FWD_HC; ++i) {
       const float y = (MODE & 1) != 0 ? __uint_as_float(x[i]) : __uint_as_float(x[i]) * c.sl2;
       x[i] = __float_as_uint(y - fabsf(slope2 * (dist0 - (float)i)));
     }
   }
   if constexpr (MASKED) {
 #pragma unroll
-    for (int i = 0; i < AM_T; ++i)
+    for (int i = 0; i < FWD_HC; ++i)
       if (i < rlo || i >= rhi) x[i] = 0xff800000u;  // -inf
   }
 }
@@ -89,24 +92,25 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int BOX = AM_T * 128;  // a 128-row x 64-column box
   pdl_enter();
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // no static shared memory: the base is aligned
+  float* sM = reinterpret_cast<float*>(smem + C::OFF_M);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* q_full = bars;                      // [2]
   uint64_t* s_full = bars + 2;                  // [2] score tile written; last: O complete
-  uint64_t* p_full = bars + 4;                  // [2] P written, O rescaled (128 threads)
+  uint64_t* p_full = bars + 4;                  // [2] P written, O rescaled (8 warps)
   uint64_t* kv_raw = bars + 6;                  // a V tile whose dead rows are zeroed first
   uint64_t* drain = bars + 7;
   uint64_t* kv_full = bars + 8;                 // [STAGES]
   uint64_t* kv_empty = bars + 8 + C::STAGES;    // [STAGES]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8 + 2 * C::STAGES);
+  uint64_t* row_max = bars + 8 + 2 * C::STAGES;  // [2][4] both halves of a tile's 32 rows (2 warps)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_max + 8);
 
   const int h = blockIdx.x % a.HQ, b = blockIdx.x / a.HQ;
   const int q0 = (gridDim.y - 1 - blockIdx.y) * 2 * AM_T;  // the rows with the most keys first
   const AttnSeq seq = attn_seq(a, b);
   if (q0 >= seq.len) return;  // the whole CTA, before any barrier or TMEM is set up
   const int kvh = h / (a.HQ / a.HKV);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const AttnBlocks tb0 = attn_tile_blocks(seq, q0), tb1 = attn_tile_blocks(seq, q0 + AM_T);
   int jb = tb0.first, je = tb0.end;  // blocks either tile visits
   if (je <= jb) { jb = tb1.first; je = tb1.end; }
@@ -116,7 +120,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 128);
+      mbar_init(&p_full[s], 8);
+      for (int w = 0; w < 4; ++w) mbar_init(&row_max[s * 4 + w], 2);
     }
     mbar_init(kv_raw, 1);
     mbar_init(drain, 1);
@@ -129,13 +134,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
   }
-  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (warp == 16) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-  if (warp == 9) {
+  if (warp == 17) {
     // ---- loads ----
     const int nblk = je - jb;
     int issued = 0;   // ring slots filled
@@ -179,60 +184,57 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       for (int n = max(0, issued - C::STAGES); n < issued; ++n)
         mbar_wait(&kv_full[n % C::STAGES], (n / C::STAGES) & 1, nullptr, 100000000ull);
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ---- MMA ----
-    if (lane == 0 && je > jb) {
+    if (je > jb) {
       constexpr uint32_t id_s = umma_idesc_f16(IS_BF16, 128, AM_T, false);
       constexpr uint32_t id_o = umma_idesc_f16(IS_BF16, 128, D, true);  // V is MN-major
-      const uint32_t sq = smem_u32(smem), skv = smem_u32(smem + C::OFF_KV);
-      bool ok = mbar_wait(&q_full[0], 0, err) && mbar_wait(&q_full[1], 0, err);
+      const uint32_t sq = desc_lo_k(smem_u32(smem));
+      const uint32_t sk = desc_lo_k(smem_u32(smem + C::OFF_KV));
+      const uint32_t sv = desc_lo_mn(smem_u32(smem + C::OFF_KV), BOX);
+      bool ok = warp_wait(&q_full[0], 0, err) && warp_wait(&q_full[1], 0, err);
       for (int j = jb - 1; ok && j < je; ++j) {
         const int nk = 2 * (j + 1 - jb), nv = 2 * (j - jb) + 1;  // ring positions of K_{j+1}, V_j
-        if (j + 1 < je) ok = mbar_wait(&kv_full[nk % C::STAGES], (nk / C::STAGES) & 1, err);
-        if (ok && j >= jb) ok = mbar_wait(&kv_full[nv % C::STAGES], (nv / C::STAGES) & 1, err);
+        if (j + 1 < je) ok = warp_wait(&kv_full[nk % C::STAGES], (nk / C::STAGES) & 1, err);
+        if (ok && j >= jb) ok = warp_wait(&kv_full[nv % C::STAGES], (nv / C::STAGES) & 1, err);
         if (!ok) break;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int first = t ? tb1.first : tb0.first, end = t ? tb1.end : tb0.end;
           const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * 128;
           if (j >= first && j < end) {  // O_t += P_t V_j
-            if (ok) ok = mbar_wait(&p_full[t], (j - first) & 1, err);
+            ok = warp_wait(&p_full[t], (j - first) & 1, err);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t bv = skv + (nv % C::STAGES) * C::TILE;
-#pragma unroll
-            for (int kk = 0; kk < AM_T / 16; ++kk)
-              umma_f16_ts(to, ts + kk * 8, umma_desc_mn_sw128(bv + kk * 2048, BOX, 1024), id_o,
-                          j > first || kk > 0);
-            if (j + 1 == end) umma_commit(&s_full[t]);
+            umma_gather2(to, ts, sv + (nv % C::STAGES) * (C::TILE >> 4), id_o, j > first);
+            if (j + 1 == end) warp_commit(&s_full[t]);
           }
           if (j + 1 >= first && j + 1 < end) {  // S_t = Q_t K_{j+1}^T (after P_t V_j in issue order)
             tc_fence_after();
-            const uint32_t bk = skv + (nk % C::STAGES) * C::TILE, aq = sq + t * C::TILE;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * BOX + (kk & 3) * 32;
-              umma_f16(ts, umma_desc_k_sw128(aq + off), umma_desc_k_sw128(bk + off), id_s, kk > 0);
-            }
-            umma_commit(&s_full[t]);
+            umma_score<D>(ts, sq + t * (C::TILE >> 4), sk + (nk % C::STAGES) * (C::TILE >> 4), id_s);
+            warp_commit(&s_full[t]);
           }
         }
         if (!ok) break;
-        if (j >= jb) umma_commit(&kv_empty[nv % C::STAGES]);
-        if (j + 1 < je) umma_commit(&kv_empty[nk % C::STAGES]);
+        if (j >= jb) warp_commit(&kv_empty[nv % C::STAGES]);
+        if (j + 1 < je) warp_commit(&kv_empty[nk % C::STAGES]);
       }
       if (!ok) {  // a wait ran out: the products already issued finish before TMEM is freed
-        umma_commit(drain);
-        mbar_wait(drain, 0, nullptr, 100000000ull);
+        warp_commit(drain);
+        if (lane == 0) mbar_wait(drain, 0, nullptr, 100000000ull);
+        __syncwarp();
       }
     }
   } else {
     // ---- softmax ----
-    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int t = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
     const int qi = q0 + t * AM_T + r;
     const AttnBlocks tb = t ? tb1 : tb0;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t ts = lane_base + t * 128, to = lane_base + 256 + t * 128;
+    const uint32_t ts = lane_base + t * 128 + half * FWD_HC, to = lane_base + 256 + t * 128 + half * (D / 2);
+    float* mine = sM + (2 * t + half) * AM_T + r;
+    const float* other = sM + (2 * t + (half ^ 1)) * AM_T + r;
+    uint64_t* pair = &row_max[t * 4 + (warp & 3)];
     const int2 range = qi < seq.len ? attn_row_range(seq, qi) : make_int2(0, 0);
     ScoreConst c;
     c.sl2 = a.scale * 1.4426950408889634f;
@@ -247,21 +249,27 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       ok = warp_wait(&s_full[t], n & 1, err);
       if (!ok) break;
       tc_fence_after();
-      uint32_t x[AM_T];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) tmem_ld32_nw(ts + u * 32, x + u * 32);
+      uint32_t x[FWD_HC];
+      tmem_ld32_nw(ts, x);
+      tmem_ld32_nw(ts + 32, x + 32);
       tmem_wait_ld();
       const bool masked = j < tb.ffirst || j >= tb.fend;
-      const int j0 = j * AM_T;
+      const int j0 = j * AM_T + half * FWD_HC;
       if (masked) modify_scores<MODE, true>(x, c, slope2, (float)(qi - j0), range.x - j0, range.y - j0);
       else modify_scores<MODE, false>(x, c, slope2, (float)(qi - j0), 0, 0);
       float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < AM_T; i += 4) {
+      for (int i = 0; i < FWD_HC; i += 4) {
         m0 = max3(m0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
         m1 = max3(m1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
       }
-      const float ms = fmaxf(m0, m1) * mul;
+      // the other half's maximum (its slot is written again only after P of this block is complete)
+      m0 = fmaxf(m0, m1);
+      *mine = m0;
+      warp_arrive(pair);
+      ok = warp_wait(pair, n & 1, err);
+      if (!ok) break;
+      const float ms = fmaxf(m0, *other) * mul;
       float corr = 1.f;
       if (ms > m_run + 8.f) {
         corr = m_run == -INFINITY ? 0.f : ex2(m_run - ms);
@@ -272,73 +280,91 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         // S_t of this block was committed after O_t += P_t V of the last one: O_t is complete
 #pragma unroll 1
         for (int u = 0; u < D / 32; ++u) {
-          float ov[32];
-          tmem_ld32(to + u * 32, ov);
+          float ov[16];
+          tmem_ld16(to + u * 16, ov);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) ov[e] *= corr;
-          tmem_st32(to + u * 32, ov);
+          for (int e = 0; e < 16; ++e) ov[e] *= corr;
+          tmem_st16(to + u * 16, ov);
         }
       }
       uint64_t sum0 = 0, sum1 = 0;  // pairs of +0.f
       const uint64_t mul_2 = pk2(mul, mul), neg_2 = pk2(mneg, mneg);
+      auto emit = [&](auto mix) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        float w[32];  // 64 probabilities as 16-bit pairs
+        for (int g = 0; g < 2; ++g) {
+          float w[16];  // 32 probabilities as 16-bit pairs
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const uint64_t y = fma2(pk2(__uint_as_float(x[g * 64 + 2 * i]), __uint_as_float(x[g * 64 + 2 * i + 1])), mul_2, neg_2);
-          float pa, pb;
-          up2(y, pa, pb);
-          pa = ex2(pa);
-          pb = ex2(pb);
-          const uint64_t p = pk2(pa, pb);
-          if (i & 1) sum1 = add2(sum1, p);
-          else sum0 = add2(sum0, p);
-          w[i] = __uint_as_float(pack_t2<T>(pa, pb));
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t y = fma2(pk2(__uint_as_float(x[g * 32 + 2 * i]), __uint_as_float(x[g * 32 + 2 * i + 1])), mul_2, neg_2);
+            uint64_t p;
+            if (decltype(mix)::value && (i & 3) == 3) {
+              p = exp2_fma2(y);
+            } else {
+              float pa, pb;
+              up2(y, pa, pb);
+              p = pk2(ex2(pa), ex2(pb));
+            }
+            if (i & 1) sum1 = add2(sum1, p);
+            else sum0 = add2(sum0, p);
+            float pa, pb;
+            up2(p, pa, pb);
+            w[i] = __uint_as_float(pack_t2<T>(pa, pb));
+          }
+          tmem_st16(ts + g * 16, w);
         }
-        tmem_st32(ts + g * 32, w);
-      }
+      };
+      // a quarter of the exponentials on the FMA pipe (exp2_fma2), whose results for masked scores
+      // would not be exact zeros: only in blocks without any
+      if (masked) emit(std::false_type{});
+      else emit(std::true_type{});
       float sa, sb, sc, sd;
       up2(sum0, sa, sb);
       up2(sum1, sc, sd);
       l_run = l_run * corr + ((sa + sb) + (sc + sd));
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&p_full[t]);
+      warp_arrive(&p_full[t]);
     }
     if (tb.end > tb.first && ok) {
       ok = warp_wait(&s_full[t], (tb.end - tb.first) & 1, err);
       tc_fence_after();
     }
+    // the row sum: both halves' sums, added in the same order in both threads
     if (ok) {
-      const float inv = l_run > 0.f ? 1.f / l_run : (l_run == 0.f ? 0.f : l_run);  // NaN stays
-      T* out = reinterpret_cast<T*>(a.out_w) + ((int64_t)(seq.start + qi) * a.HQ + h) * D;
+      *mine = l_run;
+      warp_arrive(pair);
+      ok = warp_wait(pair, (tb.end - tb.first) & 1, err);
+    }
+    if (ok) {
+      const float l_row = half ? *other + l_run : l_run + *other;
+      const float inv = l_row > 0.f ? 1.f / l_row : (l_row == 0.f ? 0.f : l_row);  // NaN stays
+      T* out = reinterpret_cast<T*>(a.out_w) + ((int64_t)(seq.start + qi) * a.HQ + h) * D + half * (D / 2);
 #pragma unroll 1
       for (int u = 0; u < D / 32; ++u) {
-        float ov[32];
+        float ov[16];
         if (tb.end > tb.first) {
-          tmem_ld32(to + u * 32, ov);
+          tmem_ld16(to + u * 16, ov);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) ov[e] = 0.f;
+          for (int e = 0; e < 16; ++e) ov[e] = 0.f;
         }
         if (qi < seq.len) {
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
-            reinterpret_cast<uint4*>(out + u * 32)[v] =
+          for (int v = 0; v < 2; ++v)
+            reinterpret_cast<uint4*>(out + u * 16)[v] =
                 make_uint4(pack_t2<T>(ov[8 * v] * inv, ov[8 * v + 1] * inv),
                            pack_t2<T>(ov[8 * v + 2] * inv, ov[8 * v + 3] * inv),
                            pack_t2<T>(ov[8 * v + 4] * inv, ov[8 * v + 5] * inv),
                            pack_t2<T>(ov[8 * v + 6] * inv, ov[8 * v + 7] * inv));
         }
       }
-      if (qi < seq.len)
-        a.lse[(int64_t)h * a.n + seq.start + qi] = (m_run + log2f(l_run)) * 0.6931471805599453f;
+      if (qi < seq.len && half == 0)
+        a.lse[(int64_t)h * a.n + seq.start + qi] = (m_run + log2f(l_row)) * 0.6931471805599453f;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
