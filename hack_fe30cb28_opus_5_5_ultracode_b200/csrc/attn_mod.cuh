@@ -148,41 +148,65 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return y;
 }
 
-// exp2_fma (common.cuh) on a pair: 2^x on the FMA pipe, x clamped at -125 (so never for a masked
-// score, which has to give an exact 0).
-__device__ __forceinline__ uint64_t exp2_fma2(uint64_t x) {
-  float a, b;
-  up2(x, a, b);
-  x = pk2(fmaxf(a, -125.f), fmaxf(b, -125.f));
-  const uint64_t magic = pk2(12582912.f, 12582912.f);
-  const uint64_t t = add2(x, magic);
-  const uint64_t f = fma2(add2(t, pk2(-12582912.f, -12582912.f)), pk2(-1.f, -1.f), x);
-  uint64_t p = pk2(0.009569981135427952f, 0.009569981135427952f);
-  p = fma2(p, f, pk2(0.05591755360364914f, 0.05591755360364914f));
-  p = fma2(p, f, pk2(0.240247443318367f, 0.240247443318367f));
-  p = fma2(p, f, pk2(0.6931218504905701f, 0.6931218504905701f));
-  p = fma2(p, f, pk2(0.9999992847442627f, 0.9999992847442627f));
-  float ta, tb, pa, pb;
-  up2(t, ta, tb);
-  up2(p, pa, pb);
-  // adding the rounded integer (the low bits of t) into the exponent field; the magic constant's
-  // own bits vanish in the shift by 23
-  return pk2(__int_as_float(__float_as_int(pa) + (__float_as_int(ta) << 23)),
-             __int_as_float(__float_as_int(pb) + (__float_as_int(tb) << 23)));
+// The arithmetic below runs on groups of independent pairs, one operation for the whole group before the
+// next: a softmax warp shares its scheduler with at most three others, so the distance between
+// dependent instructions has to come from the order they are written in.
+
+template <int N>
+__device__ __forceinline__ void ex2_2(uint64_t* x) {
+  float a[N], b[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) up2(x[i], a[i], b[i]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    a[i] = ex2(a[i]);
+    b[i] = ex2(b[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = pk2(a[i], b[i]);
 }
 
-// tanh(u) = u P(u^2) for |u| <= 0.75: coefficients of this library's own fit (reweighted least
+// tanh(u) = u P(u^2) for |u| <= 0.75, in place: coefficients of this library's own fit (reweighted least
 // squares in relative error; 2.9e-8, 1.6e-7 in fp32 Horner evaluation).
 constexpr float TANH_POLY_MAX = 0.75f;
-__device__ __forceinline__ uint64_t tanh_poly2(uint64_t u) {
-  const uint64_t w = mul2(u, u);
-  uint64_t p = pk2(-0.004716250579804182f, -0.004716250579804182f);
-  p = fma2(p, w, pk2(0.019582899287343025f, 0.019582899287343025f));
-  p = fma2(p, w, pk2(-0.053344424813985825f, -0.053344424813985825f));
-  p = fma2(p, w, pk2(0.1332540661096573f, 0.1332540661096573f));
-  p = fma2(p, w, pk2(-0.33332958817481995f, -0.33332958817481995f));
-  p = fma2(p, w, pk2(1.f, 1.f));
-  return mul2(p, u);
+template <int N>
+__device__ __forceinline__ void tanh_poly2(uint64_t* u) {
+  uint64_t w[N], p[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = mul2(u[i], u[i]);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    p[i] = fma2(w[i], pk2(-0.004716250579804182f, -0.004716250579804182f), pk2(0.019582899287343025f, 0.019582899287343025f));
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = fma2(p[i], w[i], pk2(-0.053344424813985825f, -0.053344424813985825f));
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = fma2(p[i], w[i], pk2(0.1332540661096573f, 0.1332540661096573f));
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = fma2(p[i], w[i], pk2(-0.33332958817481995f, -0.33332958817481995f));
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = fma2(p[i], w[i], pk2(1.f, 1.f));
+#pragma unroll
+  for (int i = 0; i < N; ++i) u[i] = mul2(p[i], u[i]);
+}
+// Largest |x| of N raw words.
+template <int N>
+__device__ __forceinline__ float abs_max(const uint32_t* x) {
+  float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; i += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      m[k] = max3(m[k], fabsf(__uint_as_float(x[i + 2 * k])), fabsf(__uint_as_float(x[i + 2 * k + 1])));
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+__device__ __forceinline__ uint64_t pair_of(const uint32_t* x) {
+  return pk2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ void unpair(uint64_t v, uint32_t* x) {
+  float a, b;
+  up2(v, a, b);
+  x[0] = __float_as_uint(a);
+  x[1] = __float_as_uint(b);
 }
 
 // 16 consecutive fp32 columns of this thread's TMEM lane (with the wait), and into it (tmem_wait_st()
@@ -193,6 +217,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
       : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
@@ -208,8 +239,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
 // sequence, and the operand descriptors differ from step to step by a constant in their low word. So
 // the compiler can keep descriptors and addresses in uniform registers: issued by `if (lane == 0)`
 // from descriptors built per step, the 16 MMAs of a tile and block took 1,400-2,000 cycles of this
-// warp, longer than the tensor core needs for them (8,192 causal tokens, 12 heads: 220 us,
-// and 194 us in this form).
+// warp, longer than the tensor core needs for them (8,192 causal tokens, 12 heads: 220 us
+// against 198 us in this form).
 __device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 
 // High words of the operand descriptors (128-byte swizzle, version 1): stride 1024 B between groups of
@@ -251,21 +282,35 @@ __device__ __forceinline__ void umma_score(uint32_t d, uint32_t a_lo, uint32_t b
   "mov.b64 b, {y, %4};\n\t"                                                                       \
   "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, p;\n\t"                                \
   "setp.eq.u32 p, 0, 0;\n\t"
-// two parts of 32 columns, 64 apart (two softmax threads per row)
+// two parts of 32 columns, 64 apart (two softmax threads per row); HALF 0: the first 32 rows of B's
+// first and of its second 64, HALF 1: the others
+template <int HALF>
 __device__ __forceinline__ void umma_gather2(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t more) {
-  asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
-               "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
-               QL_AM_TS("0", "0") QL_AM_TS("8", "128") QL_AM_TS("16", "256") QL_AM_TS("24", "384")
-               QL_AM_TS("64", "512") QL_AM_TS("72", "640") QL_AM_TS("80", "768") QL_AM_TS("88", "896") "}"
-               ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
+  if constexpr (HALF == 0)
+    asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
+                 "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+                 QL_AM_TS("0", "0") QL_AM_TS("8", "128") QL_AM_TS("64", "512") QL_AM_TS("72", "640") "}"
+                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
+                 "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+                 QL_AM_TS("16", "256") QL_AM_TS("24", "384") QL_AM_TS("80", "768") QL_AM_TS("88", "896") "}"
+                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
 }
-// four parts of 16 columns, 32 apart (four softmax threads per row)
+// four parts of 16 columns, 32 apart (four softmax threads per row); HALF 0: the first 16 rows of each
+// 32 of B's, HALF 1: the second
+template <int HALF>
 __device__ __forceinline__ void umma_gather4(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t more) {
-  asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
-               "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
-               QL_AM_TS("0", "0") QL_AM_TS("8", "128") QL_AM_TS("32", "256") QL_AM_TS("40", "384")
-               QL_AM_TS("64", "512") QL_AM_TS("72", "640") QL_AM_TS("96", "768") QL_AM_TS("104", "896") "}"
-               ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
+  if constexpr (HALF == 0)
+    asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
+                 "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+                 QL_AM_TS("0", "0") QL_AM_TS("32", "256") QL_AM_TS("64", "512") QL_AM_TS("96", "768") "}"
+                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
+                 "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+                 QL_AM_TS("8", "128") QL_AM_TS("40", "384") QL_AM_TS("72", "640") QL_AM_TS("104", "896") "}"
+                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
 }
 #undef QL_AM_TS
 

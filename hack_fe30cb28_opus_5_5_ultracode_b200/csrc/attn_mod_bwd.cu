@@ -41,76 +41,80 @@ struct BwdConst {
   float sl2, u, cap2, slope2;
 };
 
-// 32 raw scores of one TMEM lane into probabilities (16-bit pairs of what acc1 takes: p16) and into
-// the factors of dS (f, in place of x): probabilities times the cap's derivative. neg_lse: -lse2 by
-// column (PER_COL, from shared memory) or one value. Masked columns [0, lo) and [hi, 32) give 0.
-// dist0: row index minus the first column's, for the distance bias. p: plain probabilities where the
-// caller needs them beside f (a capped score of the dQ role).
+// 16 raw scores of one TMEM lane into probabilities (16-bit pairs of what acc1 takes: p16) and into
+// the factors of dS (f, in place of x): probabilities times the cap's derivative. poly: every |score|
+// of the warp is inside tanh_poly2's range. neg_lse: -lse2 by column (PER_COL, from shared memory) or
+// one value. Masked columns [0, lo) and [hi, 16) give 0. dist0: row index minus the first column's, for
+// the distance bias. p: plain probabilities where the caller needs them beside f (a capped score of
+// the dQ role).
 template <typename T, int MODE, bool MASKED, bool PER_COL>
-__device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, const BwdConst& c,
-                                          const float* neg_lse, float neg_lse_row, float dist0,
-                                          int lo, int hi) {
-  bool poly = true;
-  if constexpr ((MODE & 1) != 0) {
-    float mx = 0.f;
+__device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, const BwdConst& c, bool poly,
+                                          const float* neg_lse, float neg_lse_row, float dist0, int lo, int hi) {
+  uint64_t y[8], bend[8];
 #pragma unroll
-    for (int i = 0; i < HC; i += 2)
-      mx = max3(mx, fabsf(__uint_as_float(x[i])), fabsf(__uint_as_float(x[i + 1])));
-    poly = __all_sync(0xffffffffu, mx * c.u <= TANH_POLY_MAX);
-  }
-  const uint64_t row2 = pk2(neg_lse_row, neg_lse_row);
-#pragma unroll
-  for (int i = 0; i < HC; i += 4) {
-    uint64_t nl[2] = {row2, row2};
+  for (int e = 0; e < 8; e += 2) {
+    y[e] = y[e + 1] = pk2(neg_lse_row, neg_lse_row);
     if constexpr (PER_COL) {
-      const float4 l = *reinterpret_cast<const float4*>(neg_lse + i);
-      nl[0] = pk2(l.x, l.y);
-      nl[1] = pk2(l.z, l.w);
+      const float4 l = *reinterpret_cast<const float4*>(neg_lse + 2 * e);
+      y[e] = pk2(l.x, l.y);
+      y[e + 1] = pk2(l.z, l.w);
+    }
+  }
+  if constexpr ((MODE & 1) != 0) {
+    uint64_t th[8];
+    if (poly) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) th[e] = mul2(pair_of(x + 2 * e), pk2(c.u, c.u));
+      tanh_poly2<8>(th);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        th[e] = pk2(tanhf(__uint_as_float(x[2 * e]) * c.u), tanhf(__uint_as_float(x[2 * e + 1]) * c.u));
     }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int k = i + 2 * e;
-      const uint64_t raw = pk2(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-      uint64_t y, bend = 0;
-      if constexpr ((MODE & 1) != 0) {
-        uint64_t th;
-        if (poly) {
-          th = tanh_poly2(mul2(raw, pk2(c.u, c.u)));
-        } else {
-          th = pk2(tanhf(__uint_as_float(x[k]) * c.u), tanhf(__uint_as_float(x[k + 1]) * c.u));
-        }
-        bend = fma2(mul2(th, pk2(-1.f, -1.f)), th, pk2(1.f, 1.f));
-        y = fma2(th, pk2(c.cap2, c.cap2), nl[e]);
-      } else {
-        y = fma2(raw, pk2(c.sl2, c.sl2), nl[e]);
-      }
+    for (int e = 0; e < 8; ++e) y[e] = fma2(th[e], pk2(c.cap2, c.cap2), y[e]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bend[e] = mul2(th[e], pk2(-1.f, -1.f));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bend[e] = fma2(bend[e], th[e], pk2(1.f, 1.f));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = fma2(pair_of(x + 2 * e), pk2(c.sl2, c.sl2), y[e]);
+  }
+  if constexpr ((MODE & 2) != 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
       float ya, yb;
-      up2(y, ya, yb);
-      if constexpr ((MODE & 2) != 0) {
-        ya -= fabsf(c.slope2 * (dist0 - (float)k));
-        yb -= fabsf(c.slope2 * (dist0 - (float)(k + 1)));
-      }
-      float pa = ex2(ya), pb = ex2(yb);
-      if constexpr (MASKED) {
-        if (k < lo || k >= hi) pa = 0.f;
-        if (k + 1 < lo || k + 1 >= hi) pb = 0.f;
-      }
-      float fa = pa, fb = pb;
-      if constexpr ((MODE & 1) != 0) {
-        up2(mul2(pk2(pa, pb), bend), fa, fb);
-        // a masked score may be anything, infinities and NaN too: its factor is 0
-        if (MASKED && pa == 0.f) fa = 0.f;
-        if (MASKED && pb == 0.f) fb = 0.f;
-        if constexpr (!PER_COL) {
-          p[k] = pa;
-          p[k + 1] = pb;
-        }
-      }
-      x[k] = __float_as_uint(fa);
-      x[k + 1] = __float_as_uint(fb);
-      // acc1: dV takes P itself, the dQ role's correction what dS is made of
-      p16[k / 2] = __uint_as_float(PER_COL ? pack_t2<T>(pa, pb) : pack_t2<T>(fa, fb));
+      up2(y[e], ya, yb);
+      y[e] = pk2(ya - fabsf(c.slope2 * (dist0 - (float)(2 * e))), yb - fabsf(c.slope2 * (dist0 - (float)(2 * e + 1))));
     }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int k = 2 * e;
+    ex2_2<1>(y + e);
+    float pa, pb, fa, fb;
+    up2(y[e], pa, pb);
+    if constexpr (MASKED) {
+      if (k < lo || k >= hi) pa = 0.f;
+      if (k + 1 < lo || k + 1 >= hi) pb = 0.f;
+    }
+    fa = pa;
+    fb = pb;
+    if constexpr ((MODE & 1) != 0) {
+      up2(mul2(pk2(pa, pb), bend[e]), fa, fb);
+      // a masked score may be anything, infinities and NaN too: its factor is 0
+      if (MASKED && pa == 0.f) fa = 0.f;
+      if (MASKED && pb == 0.f) fb = 0.f;
+      if constexpr (!PER_COL) {
+        p[k] = pa;
+        p[k + 1] = pb;
+      }
+    }
+    x[k] = __float_as_uint(fa);
+    x[k + 1] = __float_as_uint(fb);
+    // acc1: dV takes P itself, the dQ role's correction what dS is made of
+    p16[e] = __uint_as_float(PER_COL ? pack_t2<T>(pa, pb) : pack_t2<T>(fa, fb));
   }
 }
 
@@ -120,37 +124,49 @@ template <typename T, int MODE, bool MASKED, bool PER_COL>
 __device__ __forceinline__ float bwd_ds(const uint32_t* f, const float* p, const uint32_t* dp, float* ds16,
                                         float dscale, const float* neg_d, float neg_d_row, int lo, int hi) {
   const uint64_t row2 = pk2(neg_d_row, neg_d_row), ds2 = pk2(dscale, dscale);
-  uint64_t sum = 0;  // a pair of +0.f
+  uint64_t sum[2] = {0, 0};  // pairs of +0.f
 #pragma unroll
-  for (int i = 0; i < HC; i += 4) {
-    uint64_t nd[2] = {row2, row2};
-    if constexpr (PER_COL) {
-      const float4 l = *reinterpret_cast<const float4*>(neg_d + i);
-      nd[0] = pk2(l.x, l.y);
-      nd[1] = pk2(l.z, l.w);
+  for (int i = 0; i < HC; i += 16) {
+    uint64_t g[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      uint64_t nd[2] = {row2, row2};
+      if constexpr (PER_COL) {
+        const float4 l = *reinterpret_cast<const float4*>(neg_d + i + 2 * e);
+        nd[0] = pk2(l.x, l.y);
+        nd[1] = pk2(l.z, l.w);
+      }
+      g[e] = fma2(pair_of(dp + i + 2 * e), ds2, nd[0]);
+      g[e + 1] = fma2(pair_of(dp + i + 2 * e + 2), ds2, nd[1]);
+    }
+    if constexpr (MASKED) {  // 0 times whatever a masked place holds
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int k = i + 2 * e;
+        float a, b;
+        up2(g[e], a, b);
+        g[e] = pk2(k < lo || k >= hi ? 0.f : a, k + 1 < lo || k + 1 >= hi ? 0.f : b);
+      }
+    }
+    if constexpr (!PER_COL && (MODE & 1) != 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e & 1] = fma2(g[e], pk2(p[i + 2 * e], p[i + 2 * e + 1]), sum[e & 1]);
     }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int k = i + 2 * e;
-      uint64_t g = fma2(pk2(__uint_as_float(dp[k]), __uint_as_float(dp[k + 1])), ds2, nd[e]);
+    for (int e = 0; e < 8; ++e) g[e] = mul2(g[e], pair_of(f + i + 2 * e));
+    if constexpr (!PER_COL && (MODE & 1) == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e & 1] = add2(sum[e & 1], g[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
       float a, b;
-      if constexpr (MASKED) {  // 0 times whatever a masked place holds
-        up2(g, a, b);
-        if (k < lo || k >= hi) a = 0.f;
-        if (k + 1 < lo || k + 1 >= hi) b = 0.f;
-        g = pk2(a, b);
-      }
-      const uint64_t v = mul2(g, pk2(__uint_as_float(f[k]), __uint_as_float(f[k + 1])));
-      if constexpr (!PER_COL) {
-        if constexpr ((MODE & 1) != 0) sum = fma2(g, pk2(p[k], p[k + 1]), sum);
-        else sum = add2(sum, v);
-      }
-      up2(v, a, b);
-      ds16[k / 2] = __uint_as_float(pack_t2<T>(a, b));
+      up2(g[e], a, b);
+      ds16[i / 2 + e] = __uint_as_float(pack_t2<T>(a, b));
     }
   }
   float a, b;
-  up2(sum, a, b);
+  up2(add2(sum[0], sum[1]), a, b);
   return a + b;
 }
 
@@ -174,12 +190,14 @@ __device__ __forceinline__ void store_row8(T* dst, const float* v) {
 template <int D>
 struct BwdCfg {
   static constexpr int TILE = AM_T * D * 2;
-  static constexpr int ST = 2;                              // ring of (U, W) pairs
-  static constexpr int OFF_Y = TILE, OFF_RING = 2 * TILE;   // stage s: U at + 2 s TILE, W after it
-  static constexpr int OFF_L = OFF_RING + 2 * ST * TILE;    // [ST][2][128] fp32: -lse2, -Dvec by column
-  static constexpr int OFF_R = OFF_L + ST * 2 * AM_T * 4;   // [4][128] fp32: a row's four partial sums
-  static constexpr int OFF_BAR = OFF_R + 4 * AM_T * 4;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  // U is held from its step's S to its acc2, W (dO of the dK / dV role, V of the other) not as long:
+  // with pairs of stages a tile's copy left one step's time before its S was due, and S waited for it
+  static constexpr int UST = 3, WST = 2;
+  static constexpr int OFF_Y = TILE, OFF_U = 2 * TILE, OFF_W = OFF_U + UST * TILE;
+  static constexpr int OFF_L = OFF_W + WST * TILE;          // [2][2][128] fp32: -lse2, -Dvec by column;
+                                                            // dQ role: [4][128] a row's partial sums
+  static constexpr int OFF_BAR = OFF_L + 4 * AM_T * 4;
+  static constexpr int SMEM = OFF_BAR + 512;
 };
 
 // One CTA per (128-row tile, head, sequence): query tiles of every query head for dQ; for dK and dV key
@@ -196,23 +214,25 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr float P_SHIFT = !DKV || IS_BF16 ? 0.f : 8.f, P_BACK = !DKV || IS_BF16 ? 1.f : 1.f / 256.f;
   pdl_enter();
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // no static shared memory: the base is aligned
   float* sL = reinterpret_cast<float*>(smem + C::OFF_L);
-  float* sR = reinterpret_cast<float*>(smem + C::OFF_R);
+  float* sR = sL;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* xy_full = bars;
   uint64_t* s_full = bars + 1;
-  uint64_t* p_full = bars + 2;   // P written (all softmax warps)
-  uint64_t* dp_full = bars + 3;
-  uint64_t* ds_full = bars + 4;  // dS written (all softmax warps)
-  uint64_t* out_full = bars + 5;
-  uint64_t* raw = bars + 6;
-  uint64_t* drain = bars + 7;
-  uint64_t* u_full = bars + 8;            // [ST] U landed, -lse2 and -Dvec stored (1 + the warp)
-  uint64_t* w_full = bars + 8 + C::ST;    // [ST]
-  uint64_t* empty = bars + 8 + 2 * C::ST; // [ST] every product reading the stage completed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8 + 3 * C::ST);
+  uint64_t* dp_full = bars + 2;
+  uint64_t* ds_full = bars + 3;  // dS written (all softmax warps)
+  uint64_t* out_full = bars + 4;
+  uint64_t* raw = bars + 5;
+  uint64_t* drain = bars + 6;
+  uint64_t* p_full = bars + 7;   // [2] half of P written (all softmax warps)
+  uint64_t* l_full = bars + 9;   // [2] -lse2 and -Dvec of a step stored
+  uint64_t* l_empty = bars + 11; // [2] and read (all softmax warps)
+  uint64_t* u_full = bars + 13;  // [UST]
+  uint64_t* u_empty = u_full + C::UST;
+  uint64_t* w_full = u_empty + C::UST;  // [WST]
+  uint64_t* w_empty = w_full + C::WST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(w_empty + C::WST);
 
   const int group = a.HQ / a.HKV;
   const int per_seq = DKV ? a.HKV * a.splits : a.HQ;
@@ -232,16 +252,23 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   if (threadIdx.x == 0) {
     mbar_init(xy_full, 1);
     mbar_init(s_full, 1);
-    mbar_init(p_full, BWD_SOFTMAX / 32);
     mbar_init(dp_full, 1);
     mbar_init(ds_full, BWD_SOFTMAX / 32);
     mbar_init(out_full, 1);
     mbar_init(raw, 1);
     mbar_init(drain, 1);
-    for (int s = 0; s < C::ST; ++s) {
-      mbar_init(&u_full[s], 2);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&p_full[s], BWD_SOFTMAX / 32);
+      mbar_init(&l_full[s], 1);
+      mbar_init(&l_empty[s], BWD_SOFTMAX / 32);
+    }
+    for (int s = 0; s < C::UST; ++s) {
+      mbar_init(&u_full[s], 1);
+      mbar_init(&u_empty[s], 1);
+    }
+    for (int s = 0; s < C::WST; ++s) {
       mbar_init(&w_full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&w_empty[s], 1);
     }
     fence_barrier_init();
     prefetch_tmap(&tx);
@@ -258,7 +285,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   if (warp == 17) {
     // ---- loads ----
     bool ok = true;
-    int issued = 0;
+    int un = 0, wn = 0;
     uint32_t raw_phase = 0;
     const int zx = (DKV ? kvh : h0) * (D / 64);
     if (lane == 0 && steps > 0) {
@@ -267,59 +294,64 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       tma_load_3d(smem + C::OFF_Y, &ty, xy_full, 0, seq.start + r0, zx);
     }
     for (int n = 0; ok && n < steps; ++n) {
-      const int s = n % C::ST, row = (tb.first + (DKV ? n % ntile : n)) * AM_T;
+      const int row = (tb.first + (DKV ? n % ntile : n)) * AM_T;
       const int h = DKV ? h0 + n / ntile : 0, zu = (DKV ? h : kvh) * (D / 64);
       // rows of U and W that belong to no query or key are zeroed before any product reads them
       uint32_t bad[4];
       const bool dirty = attn_dead_rows(seq, row, bad);
-      if (n >= C::ST) ok = warp_wait(&empty[s], (n / C::ST - 1) & 1, err);
-      if (!ok) break;
-      uint8_t* su = smem + C::OFF_RING + 2 * s * C::TILE;
-      uint8_t* sw = su + C::TILE;
-      if (lane == 0) {
-        if (dirty) {
-          mbar_arrive_expect_tx(raw, 2 * C::TILE);
-        } else {
-          mbar_arrive_expect_tx(&u_full[s], C::TILE);
-          mbar_arrive_expect_tx(&w_full[s], C::TILE);
-        }
-        tma_load_3d(su, &tu, dirty ? raw : &u_full[s], 0, seq.start + row, zu);
-        tma_load_3d(sw, &tw, dirty ? raw : &w_full[s], 0, seq.start + row, zu);
-      }
+      float l[4], dv[4];
       if constexpr (DKV) {
         const int64_t at = (int64_t)h * a.n + seq.start + row;
-        float* l = sL + s * 2 * AM_T;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int t = u * 32 + lane;
-          const float lse = row + t < seq.len ? a.lse[at + t] : -INFINITY;
-          // a query that sees nothing (lse -inf) or lies past the end: probability 0
-          l[t] = lse == -INFINITY ? -INFINITY : fmaf(lse, -1.4426950408889634f, P_SHIFT);
-          l[AM_T + t] = row + t < seq.len ? a.dvec[at + t] * -P_BACK : 0.f;
+          l[u] = row + t < seq.len ? a.lse[at + t] : -INFINITY;
+          dv[u] = row + t < seq.len ? a.dvec[at + t] : 0.f;
         }
       }
-      if (dirty) {
-        ok = warp_wait(raw, raw_phase, err);
-        if (!ok) break;
-        raw_phase ^= 1;
-        attn_zero_rows<D / 64>(su, bad);
-        attn_zero_rows<D / 64>(sw, bad);
-        fence_proxy_async_smem();
-        __syncwarp();
+      auto load = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* full) {
+        uint64_t* bar = dirty ? raw : full;
         if (lane == 0) {
-          mbar_arrive(&u_full[s]);
-          mbar_arrive(&w_full[s]);
+          mbar_arrive_expect_tx(bar, C::TILE);
+          tma_load_3d(dst, map, bar, 0, seq.start + row, zu);
         }
+        if (!dirty) return true;
+        if (!warp_wait(raw, raw_phase, err)) return false;
+        raw_phase ^= 1;
+        attn_zero_rows<D / 64>(dst, bad);
+        fence_proxy_async_smem();
+        warp_arrive(full);
+        return true;
+      };
+      const int us = n % C::UST, ws = n % C::WST;
+      if (n >= C::UST) ok = warp_wait(&u_empty[us], (n / C::UST - 1) & 1, err);
+      if (ok) ok = load(&tu, smem + C::OFF_U + us * C::TILE, &u_full[us]);
+      if (!ok) break;
+      un = n + 1;
+      if (n >= C::WST) ok = warp_wait(&w_empty[ws], (n / C::WST - 1) & 1, err);
+      if (ok) ok = load(&tw, smem + C::OFF_W + ws * C::TILE, &w_full[ws]);
+      if (!ok) break;
+      wn = n + 1;
+      if constexpr (DKV) {
+        if (n >= 2) ok = warp_wait(&l_empty[n & 1], ((n >> 1) - 1) & 1, err);
+        if (!ok) break;
+        float* sl = sL + (n & 1) * 2 * AM_T;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int t = u * 32 + lane;
+          // a query that sees nothing (lse -inf) or lies past the end: probability 0
+          sl[t] = l[u] == -INFINITY ? -INFINITY : fmaf(l[u], -1.4426950408889634f, P_SHIFT);
+          sl[AM_T + t] = dv[u] * -P_BACK;
+        }
+        warp_arrive(&l_full[n & 1]);
       }
-      warp_arrive(&u_full[s]);
-      issued = n + 1;
     }
     if (!ok && lane == 0) {  // a wait ran out: let the copies in flight land before the CTA goes
       mbar_wait(xy_full, 0, nullptr, 100000000ull);
-      for (int n = max(0, issued - C::ST); n < issued; ++n) {
-        mbar_wait(&u_full[n % C::ST], (n / C::ST) & 1, nullptr, 100000000ull);
-        mbar_wait(&w_full[n % C::ST], (n / C::ST) & 1, nullptr, 100000000ull);
-      }
+      for (int n = max(0, un - C::UST); n < un; ++n)
+        mbar_wait(&u_full[n % C::UST], (n / C::UST) & 1, nullptr, 100000000ull);
+      for (int n = max(0, wn - C::WST); n < wn; ++n)
+        mbar_wait(&w_full[n % C::WST], (n / C::WST) & 1, nullptr, 100000000ull);
     }
   } else if (warp == 16) {
     // ---- MMA ----
@@ -328,48 +360,44 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       constexpr uint32_t id_o = umma_idesc_f16(IS_BF16, 128, D, true);
       constexpr uint32_t TILE16 = C::TILE >> 4;
       const uint32_t sx = desc_lo_k(smem_u32(smem)), sy = sx + TILE16;
-      const uint32_t rk = desc_lo_k(smem_u32(smem + C::OFF_RING));       // K-major: products over the head
-      const uint32_t rm = desc_lo_mn(smem_u32(smem + C::OFF_RING), BOX); // MN-major: sums over its rows
-      bool ok = warp_wait(xy_full, 0, err) && warp_wait(&u_full[0], 0, err);
-      if (ok) {
+      const uint32_t uk = desc_lo_k(smem_u32(smem + C::OFF_U)), um = desc_lo_mn(smem_u32(smem + C::OFF_U), BOX);
+      const uint32_t wk = desc_lo_k(smem_u32(smem + C::OFF_W)), wm = desc_lo_mn(smem_u32(smem + C::OFF_W), BOX);
+      auto score = [&](int n) {  // S = X U^T
+        if (!warp_wait(&u_full[n % C::UST], (n / C::UST) & 1, err)) return false;
         tc_fence_after();
-        umma_score<D>(tmem, sx, rk, id_s);
+        umma_score<D>(tmem, sx, uk + (n % C::UST) * TILE16, id_s);
         warp_commit(s_full);
-        ok = warp_wait(&w_full[0], 0, err);
-      }
-      if (ok) {
+        return true;
+      };
+      auto dprob = [&](int n) {  // dP = Y W^T
+        if (!warp_wait(&w_full[n % C::WST], (n / C::WST) & 1, err)) return false;
         tc_fence_after();
-        umma_score<D>(tmem + 128, sy, rk + TILE16, id_s);
+        umma_score<D>(tmem + 128, sy, wk + (n % C::WST) * TILE16, id_s);
         warp_commit(dp_full);
-      }
+        if (!DKV) warp_commit(&w_empty[n % C::WST]);
+        return true;
+      };
+      bool ok = warp_wait(xy_full, 0, err) && score(0) && dprob(0);
       for (int n = 0; ok && n < steps; ++n) {
-        const int s = n % C::ST, s1 = (n + 1) % C::ST;
-        const uint32_t ph1 = ((n + 1) / C::ST) & 1;
-        ok = warp_wait(p_full, n & 1, err);
+        const uint32_t u0 = um + (n % C::UST) * TILE16, w0 = wm + (n % C::WST) * TILE16;
+        ok = warp_wait(&p_full[0], n & 1, err);
         if (!ok) break;
         tc_fence_after();
-        umma_gather4(tmem + 256, tmem, rm + (2 * s + (DKV ? 1 : 0)) * TILE16, id_o, n > 0);
-        if (n + 1 < steps) {
-          ok = warp_wait(&u_full[s1], ph1, err);
-          if (!ok) break;
-          tc_fence_after();
-          umma_score<D>(tmem, sx, rk + 2 * s1 * TILE16, id_s);
-          warp_commit(s_full);
-        }
-        ok = warp_wait(ds_full, n & 1, err);
+        umma_gather4<0>(tmem + 256, tmem, DKV ? w0 : u0, id_o, n > 0);
+        ok = warp_wait(&p_full[1], n & 1, err);
         if (!ok) break;
         tc_fence_after();
-        umma_gather4(tmem + 384, tmem + 128, rm + 2 * s * TILE16, id_o, n > 0);
-        warp_commit(&empty[s]);
-        if (n + 1 < steps) {
-          ok = warp_wait(&w_full[s1], ph1, err);
-          if (!ok) break;
-          tc_fence_after();
-          umma_score<D>(tmem + 128, sy, rk + (2 * s1 + 1) * TILE16, id_s);
-          warp_commit(dp_full);
-        } else {
-          warp_commit(out_full);
-        }
+        umma_gather4<1>(tmem + 256, tmem, DKV ? w0 : u0, id_o, 1);
+        if (DKV) warp_commit(&w_empty[n % C::WST]);
+        if (n + 1 < steps) ok = score(n + 1);
+        if (ok) ok = warp_wait(ds_full, n & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        umma_gather4<0>(tmem + 384, tmem + 128, u0, id_o, n > 0);
+        umma_gather4<1>(tmem + 384, tmem + 128, u0, id_o, 1);
+        warp_commit(&u_empty[n % C::UST]);
+        if (n + 1 < steps) ok = dprob(n + 1);
+        else warp_commit(out_full);
       }
       if (!ok) {  // a wait ran out: the products already issued finish before TMEM is freed
         warp_commit(drain);
@@ -411,13 +439,13 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     bool ok = true;
     const uint32_t ts = lane_base + part * HC;
     for (int n = 0; n < steps; ++n) {
-      const int s = n % C::ST, j = tb.first + (DKV ? n % ntile : n), i0 = j * AM_T + part * HC;
+      const int s = n & 1, j = tb.first + (DKV ? n % ntile : n), i0 = j * AM_T + part * HC;
       if (DKV && (MODE & 2) != 0 && n > 0 && n % ntile == 0) c = bwd_const<MODE>(a, h0 + n / ntile);
       const bool masked = j < tb.ffirst || j >= tb.fend;
       const int lo = range.x - i0, hi = range.y - i0;
       const float dist0 = (float)(ri - i0);
       ok = warp_wait(s_full, n & 1, err);
-      if (DKV && ok) ok = warp_wait(&u_full[s], (n / C::ST) & 1, err);  // -lse2 and -Dvec are visible
+      if (DKV && ok) ok = warp_wait(&l_full[s], (n >> 1) & 1, err);  // -lse2 and -Dvec are visible
       if (!ok) break;
       tc_fence_after();
       const float* nl = sL + s * 2 * AM_T + part * HC;
@@ -425,12 +453,19 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       float w[HC / 2], p[(MODE & 1) != 0 && !DKV ? HC : 1];
       tmem_ld32_nw(ts, x);
       tmem_wait_ld();
-      if (masked) bwd_probs<T, MODE, true, DKV>(x, w, p, c, nl, neg_lse, dist0, lo, hi);
-      else bwd_probs<T, MODE, false, DKV>(x, w, p, c, nl, neg_lse, dist0, 0, 0);
-      tmem_st16(ts, w);
-      tmem_wait_st();
-      tc_fence_before();
-      warp_arrive(p_full);
+      bool poly = true;
+      if constexpr ((MODE & 1) != 0) poly = __all_sync(0xffffffffu, abs_max<HC>(x) * c.u <= TANH_POLY_MAX);
+      // half of the columns at a time: acc1 starts on the first while the second is formed
+#pragma unroll
+      for (int g = 0; g < HC; g += 16) {
+        float* pg = p + ((MODE & 1) != 0 && !DKV ? g : 0);
+        if (masked) bwd_probs<T, MODE, true, DKV>(x + g, w, pg, c, poly, nl + g, neg_lse, dist0 - g, lo - g, hi - g);
+        else bwd_probs<T, MODE, false, DKV>(x + g, w, pg, c, poly, nl + g, neg_lse, dist0 - g, 0, 0);
+        tmem_st8(ts + g / 2, w);
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(&p_full[g / 16]);
+      }
       ok = warp_wait(dp_full, n & 1, err);
       if (!ok) break;
       tc_fence_after();
@@ -438,6 +473,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       tmem_wait_ld();
       if (masked) rest += bwd_ds<T, MODE, true, DKV>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, lo, hi);
       else rest += bwd_ds<T, MODE, false, DKV>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, 0, 0);
+      if (DKV) warp_arrive(&l_empty[s]);
       tmem_st16(ts + 128, w);
       tmem_wait_st();
       tc_fence_before();

@@ -49,20 +49,17 @@ __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, 
                                               float dist0, int rlo, int rhi) {
   if constexpr ((MODE & 1) != 0) {
     // the largest |u| of the warp's rows decides between the polynomial and tanhf
-    float mx = 0.f;
-#pragma unroll
-    for (int i = 0; i < FWD_HC; i += 2)
-      mx = max3(mx, fabsf(__uint_as_float(x[i])), fabsf(__uint_as_float(x[i + 1])));
-    const bool poly = __all_sync(0xffffffffu, mx * c.u <= TANH_POLY_MAX);
+    const bool poly = __all_sync(0xffffffffu, abs_max<FWD_HC>(x) * c.u <= TANH_POLY_MAX);
     if (poly) {
       const uint64_t uu = pk2(c.u, c.u), cc = pk2(c.cap2, c.cap2);
 #pragma unroll
-      for (int i = 0; i < FWD_HC; i += 2) {
-        const uint64_t y = mul2(tanh_poly2(mul2(pk2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), uu)), cc);
-        float a, b;
-        up2(y, a, b);
-        x[i] = __float_as_uint(a);
-        x[i + 1] = __float_as_uint(b);
+      for (int i = 0; i < FWD_HC; i += 16) {
+        uint64_t u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = mul2(pair_of(x + i + 2 * e), uu);
+        tanh_poly2<8>(u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) unpair(mul2(u[e], cc), x + i + 2 * e);
       }
     } else {
 #pragma unroll
@@ -97,12 +94,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* q_full = bars;                      // [2]
   uint64_t* s_full = bars + 2;                  // [2] score tile written; last: O complete
-  uint64_t* p_full = bars + 4;                  // [2] P written, O rescaled (8 warps)
-  uint64_t* kv_raw = bars + 6;                  // a V tile whose dead rows are zeroed first
-  uint64_t* drain = bars + 7;
-  uint64_t* kv_full = bars + 8;                 // [STAGES]
-  uint64_t* kv_empty = bars + 8 + C::STAGES;    // [STAGES]
-  uint64_t* row_max = bars + 8 + 2 * C::STAGES;  // [2][4] both halves of a tile's 32 rows (2 warps)
+  uint64_t* p_full = bars + 4;                  // [2] half of P written, O rescaled (8 warps)
+  uint64_t* p_full2 = bars + 6;                 // [2] the other half of P written
+  uint64_t* kv_raw = bars + 8;                  // a V tile whose dead rows are zeroed first
+  uint64_t* drain = bars + 9;
+  uint64_t* kv_full = bars + 10;                // [STAGES]
+  uint64_t* kv_empty = bars + 10 + C::STAGES;   // [STAGES]
+  uint64_t* row_max = bars + 10 + 2 * C::STAGES;  // [2][4] both halves of a tile's 32 rows (2 warps)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_max + 8);
 
   const int h = blockIdx.x % a.HQ, b = blockIdx.x / a.HQ;
@@ -121,6 +119,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       mbar_init(&q_full[s], 1);
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 8);
+      mbar_init(&p_full2[s], 8);
       for (int w = 0; w < 4; ++w) mbar_init(&row_max[s * 4 + w], 2);
     }
     mbar_init(kv_raw, 1);
@@ -206,7 +205,11 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
             ok = warp_wait(&p_full[t], (j - first) & 1, err);
             if (!ok) break;
             tc_fence_after();
-            umma_gather2(to, ts, sv + (nv % C::STAGES) * (C::TILE >> 4), id_o, j > first);
+            umma_gather2<0>(to, ts, sv + (nv % C::STAGES) * (C::TILE >> 4), id_o, j > first);
+            ok = warp_wait(&p_full2[t], (j - first) & 1, err);
+            if (!ok) break;
+            tc_fence_after();
+            umma_gather2<1>(to, ts, sv + (nv % C::STAGES) * (C::TILE >> 4), id_o, 1);
             if (j + 1 == end) warp_commit(&s_full[t]);
           }
           if (j + 1 >= first && j + 1 < end) {  // S_t = Q_t K_{j+1}^T (after P_t V_j in issue order)
@@ -257,19 +260,19 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       const int j0 = j * AM_T + half * FWD_HC;
       if (masked) modify_scores<MODE, true>(x, c, slope2, (float)(qi - j0), range.x - j0, range.y - j0);
       else modify_scores<MODE, false>(x, c, slope2, (float)(qi - j0), 0, 0);
-      float m0 = -INFINITY, m1 = -INFINITY;
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < FWD_HC; i += 4) {
-        m0 = max3(m0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-        m1 = max3(m1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
-      }
+      for (int i = 0; i < FWD_HC; i += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          mx[e] = max3(mx[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
       // the other half's maximum (its slot is written again only after P of this block is complete)
-      m0 = fmaxf(m0, m1);
-      *mine = m0;
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      *mine = top;
       warp_arrive(pair);
       ok = warp_wait(pair, n & 1, err);
       if (!ok) break;
-      const float ms = fmaxf(m0, *other) * mul;
+      const float ms = fmaxf(top, *other) * mul;
       float corr = 1.f;
       if (ms > m_run + 8.f) {
         corr = m_run == -INFINITY ? 0.f : ex2(m_run - ms);
@@ -287,43 +290,28 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
           tmem_st16(to + u * 16, ov);
         }
       }
-      uint64_t sum0 = 0, sum1 = 0;  // pairs of +0.f
+      uint64_t sum[4] = {0, 0, 0, 0};  // pairs of +0.f
       const uint64_t mul_2 = pk2(mul, mul), neg_2 = pk2(mneg, mneg);
-      auto emit = [&](auto mix) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          float w[16];  // 32 probabilities as 16-bit pairs
+      for (int g = 0; g < FWD_HC; g += 32) {
+        float w[16];  // 32 probabilities as 16-bit pairs
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint64_t y = fma2(pk2(__uint_as_float(x[g * 32 + 2 * i]), __uint_as_float(x[g * 32 + 2 * i + 1])), mul_2, neg_2);
-            uint64_t p;
-            if (decltype(mix)::value && (i & 3) == 3) {
-              p = exp2_fma2(y);
-            } else {
-              float pa, pb;
-              up2(y, pa, pb);
-              p = pk2(ex2(pa), ex2(pb));
-            }
-            if (i & 1) sum1 = add2(sum1, p);
-            else sum0 = add2(sum0, p);
-            float pa, pb;
-            up2(p, pa, pb);
-            w[i] = __uint_as_float(pack_t2<T>(pa, pb));
-          }
-          tmem_st16(ts + g * 16, w);
+        for (int i = 0; i < 16; ++i) {
+          uint64_t y = fma2(pair_of(x + g + 2 * i), mul_2, neg_2);
+          ex2_2<1>(&y);
+          sum[i & 3] = add2(sum[i & 3], y);
+          float pa, pb;
+          up2(y, pa, pb);
+          w[i] = __uint_as_float(pack_t2<T>(pa, pb));
         }
-      };
-      // a quarter of the exponentials on the FMA pipe (exp2_fma2), whose results for masked scores
-      // would not be exact zeros: only in blocks without any
-      if (masked) emit(std::false_type{});
-      else emit(std::true_type{});
-      float sa, sb, sc, sd;
-      up2(sum0, sa, sb);
-      up2(sum1, sc, sd);
-      l_run = l_run * corr + ((sa + sb) + (sc + sd));
-      tmem_wait_st();
-      tc_fence_before();
-      warp_arrive(&p_full[t]);
+        tmem_st16(ts + g / 2, w);
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(g == 0 ? &p_full[t] : &p_full2[t]);
+      }
+      float sa, sb;
+      up2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), sa, sb);
+      l_run = l_run * corr + (sa + sb);
     }
     if (tb.end > tb.first && ok) {
       ok = warp_wait(&s_full[t], (tb.end - tb.first) & 1, err);
