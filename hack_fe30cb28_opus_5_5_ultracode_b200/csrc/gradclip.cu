@@ -3,8 +3,9 @@
 // Two passes and no meeting of the CTAs inside a kernel: the first writes one sum of squares per
 // CTA; in the second every CTA adds those sums in the same order (fp64), so all arrive at the same
 // factor, and rescales its part. A gradient list that fits in L2 is read from HBM once; of a longer
-// one the second pass starts at the end, where the first pass left L2. Squares are summed in fp32 per
-// thread (four independent sums over at most a few thousand values), from there on in fp64.
+// one the second pass starts at the end, where the first pass left L2. Squares are summed in fp32 within
+// a thread's part of one chunk (four sums of at most 16 to 32 values, which is why the chunk is not
+// longer: over thousands of them the norm was off by 1.5e-6), from there on in fp64.
 //
 // The tensors' addresses and sizes travel as kernel parameters (up to 1,024 tensors a launch), so a
 // call copies nothing to the device and can be captured. Work is cut into chunks of 32 KB of one
@@ -107,16 +108,18 @@ template <int MAX>
 __global__ void __launch_bounds__(GC_THREADS) grad_squares_kernel(const __grid_constant__ GradList<MAX> l,
                                                                   double* partial) {
   pdl_enter();
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  double all = 0.0;
   for (int c = blockIdx.x; c < l.first[l.count]; c += gridDim.x) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
     const int t = tensor_of(l, c), dt = l.dtype[t], per = chunk_elems(dt);
     const int64_t at = (int64_t)(c - l.first[t]) * per;
     const int n = (int)min((int64_t)per, l.n[t] - at);
     if (dt == QL_F32) chunk_squares(static_cast<const float*>(l.grad[t]) + at, n, s);
     else if (dt == QL_F16) chunk_squares(static_cast<const __half*>(l.grad[t]) + at, n, s);
     else chunk_squares(static_cast<const __nv_bfloat16*>(l.grad[t]) + at, n, s);
+    all += ((double)s[0] + (double)s[1]) + ((double)s[2] + (double)s[3]);
   }
-  const double sum = cta_sum(((double)s[0] + (double)s[1]) + ((double)s[2] + (double)s[3]));
+  const double sum = cta_sum(all);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 

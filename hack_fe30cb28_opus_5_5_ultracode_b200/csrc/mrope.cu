@@ -11,7 +11,7 @@
 // 8 t + 2 j + e in column 2 t + e of step j, thread t of a row ends up with eight consecutive
 // columns after four steps - one 16-byte load and store. The product stays in fp32 (nothing is
 // rounded between the factors and the output). The backward uses the same ordering for the K
-// dimension of dx_lo = s g B, with g split into two 16-bit parts, so dx_lo is good to fp32.
+// dimension of dx_lo = s g B, with g split into 16-bit parts, so dx_lo is good to fp32.
 //
 // Bound: HBM for long batches (2 bytes read and 2 written per element in each direction), launch and
 // L2 latency for short ones.
@@ -236,22 +236,31 @@ __device__ __forceinline__ void lora_back(const float (*gv)[8], const void* B, i
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = __ldg(base + (4 * s + e) * (MR_RANK / 2));
-    uint32_t hi[4], lo[4];
+    // g in PARTS 16-bit pieces, each the rounding of what the ones before left: 2^-24 (bf16) or
+    // 2^-22 (fp16) of g stays behind
+    constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
+    float left[2][4];
 #pragma unroll
     for (int rh = 0; rh < 2; ++rh)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float p = gv[rh][4 * s + 2 * k], q = gv[rh][4 * s + 2 * k + 1];
-        const T ph = from_f<T>(p), qh = from_f<T>(q);
-        hi[rh + 2 * k] = pack_t2<T>(p, q);
-        lo[rh + 2 * k] = pack_t2<T>(p - to_f<T>(ph), q - to_f<T>(qh));
-      }
+      for (int k = 0; k < 4; ++k) left[rh][k] = gv[rh][4 * s + k];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      const uint32_t sel = nt == 0 ? 0x5410 : 0x7632;
-      const uint32_t b0 = __byte_perm(w[0], w[1], sel), b1 = __byte_perm(w[2], w[3], sel);
-      mma16816<T>(c[nt], hi, b0, b1);
-      mma16816<T>(c[nt], lo, b0, b1);
+    for (int part = 0; part < PARTS; ++part) {
+      uint32_t af[4];
+#pragma unroll
+      for (int rh = 0; rh < 2; ++rh)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float p = left[rh][2 * k], q = left[rh][2 * k + 1];
+          af[rh + 2 * k] = pack_t2<T>(p, q);
+          left[rh][2 * k] = p - to_f<T>(from_f<T>(p));
+          left[rh][2 * k + 1] = q - to_f<T>(from_f<T>(q));
+        }
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const uint32_t sel = nt == 0 ? 0x5410 : 0x7632;
+        mma16816<T>(c[nt], af, __byte_perm(w[0], w[1], sel), __byte_perm(w[2], w[3], sel));
+      }
     }
   }
 }
