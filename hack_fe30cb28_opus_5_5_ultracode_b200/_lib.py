@@ -103,7 +103,11 @@ def lib():
 
 def call(name, *args):
     """Calls an entry point returning a status and raises QLError unless it is 0."""
-    status = getattr(lib(), name)(*args)
+    return check(name, getattr(lib(), name)(*args))
+
+
+def check(name, status):
+    """Raises QLError for the status of a call to `name` unless it is 0."""
     if status != 0:
         msg = lib().ql_last_error().decode(errors="replace")
         raise QLError(name, status, msg)
@@ -116,6 +120,25 @@ def struct(name, **fields):
     for k, v in fields.items():
         setattr(s, k, v)
     return s
+
+
+_PACK = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_longlong: "q", ctypes.c_int32: "i",
+         ctypes.c_int: "i", ctypes.c_uint32: "I", ctypes.c_float: "f", ctypes.c_double: "d"}
+
+
+def packer(name, order):
+    """A function of the fields' values, in the given order (which has to be the header's), to the
+    bytes of an argument struct: a third of struct()'s time for the structs with many fields.
+    Pointers are addresses (0 for NULL)."""
+    import struct as _struct
+
+    fields = STRUCTS[name]._fields_
+    if tuple(f for f, _ in fields) != tuple(order.split()):
+        raise ValueError(f"{name} has the fields {[f for f, _ in fields]}")
+    fmt = _struct.Struct("@" + "".join(_PACK[t] for _, t in fields) + "0P")
+    if fmt.size != ctypes.sizeof(STRUCTS[name]):
+        raise ValueError(f"{name} packs to {fmt.size} bytes")
+    return fmt.pack
 
 
 def exported_symbols():

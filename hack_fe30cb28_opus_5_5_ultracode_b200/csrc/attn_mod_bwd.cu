@@ -612,11 +612,17 @@ int64_t dvec_floats(const AttnModArgs& a) { return ((int64_t)a.HQ * a.n + 3) / 4
 
 }  // namespace
 
-int64_t attn_mod_bwd_workspace(const ql_attn_mod_args& m) {
-  AttnModArgs a;
-  if (attn_mod_check(m, a) != QL_STATUS_OK) return 0;
+int64_t attn_mod_bwd_workspace(int n, int max_len, int HQ, int HKV, int D, int causal, int window) {
+  if (n <= 0 || max_len < 0 || HQ <= 0 || HKV <= 0 || HQ % HKV != 0 || D <= 0) return 0;
+  AttnModArgs a{};
+  a.n = n;
+  a.max_len = max_len;
+  a.HQ = HQ;
+  a.HKV = HKV;
+  a.causal = causal;
+  a.window = window;
   const int splits = dkv_splits(a);
-  return dvec_floats(a) + (splits > 1 ? 2 * (int64_t)splits * a.n * a.HKV * m.D : 0);
+  return dvec_floats(a) + (splits > 1 ? 2 * (int64_t)splits * n * HKV * D : 0);
 }
 
 int attn_mod_bwd(const ql_attn_mod_args& m, cudaStream_t s) {
@@ -630,7 +636,9 @@ int attn_mod_bwd(const ql_attn_mod_args& m, cudaStream_t s) {
         reinterpret_cast<uintptr_t>(m.workspace)) & 15))
     return QL_STATUS_BAD_ARG;
   a.splits = dkv_splits(a);
-  if (m.workspace == nullptr || m.workspace_floats < attn_mod_bwd_workspace(m)) return QL_STATUS_BAD_ARG;
+  if (m.workspace == nullptr ||
+      m.workspace_floats < attn_mod_bwd_workspace(a.n, a.max_len, a.HQ, a.HKV, m.D, a.causal, a.window))
+    return QL_STATUS_BAD_ARG;
   a.dout = m.dout;
   a.dq = m.dq;
   a.dk = m.dk;

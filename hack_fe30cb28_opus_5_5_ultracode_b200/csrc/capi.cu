@@ -245,19 +245,20 @@ int ql_mrope_bwd(const ql_mrope_args* args, cudaStream_t stream) {
 
 int64_t ql_grad_norm_workspace(int count) { return count < 0 ? 0 : ql::grad_norm_workspace(count); }
 
-int ql_grad_norm(const ql_grad_tensor* tensors, int count, float inv_scale,
-                 const float* inv_scale_dev, float* norm, double* workspace,
+int ql_grad_norm(const uint64_t* grads, const int64_t* elements, const int32_t* dtypes, int count,
+                 float inv_scale, const float* inv_scale_dev, float* norm, double* workspace,
                  int64_t workspace_bytes, cudaStream_t stream) {
-  return done(ql::grad_norm(tensors, count, inv_scale, inv_scale_dev, norm, workspace,
-                            workspace_bytes, stream),
+  return done(ql::grad_norm({grads, nullptr, elements, dtypes, nullptr, count}, inv_scale, inv_scale_dev,
+                            norm, workspace, workspace_bytes, stream),
               "ql_grad_norm");
 }
 
-int ql_clip_grads(const ql_grad_tensor* tensors, int count, float max_norm, float inv_scale,
-                  const float* inv_scale_dev, float* norm, double* workspace,
+int ql_clip_grads(const uint64_t* grads, const uint64_t* outs, const int64_t* elements,
+                  const int32_t* dtypes, const int32_t* out_dtypes, int count, float max_norm,
+                  float inv_scale, const float* inv_scale_dev, float* norm, double* workspace,
                   int64_t workspace_bytes, cudaStream_t stream) {
-  return done(ql::clip_grads(tensors, count, max_norm, inv_scale, inv_scale_dev, norm, workspace,
-                             workspace_bytes, stream),
+  return done(ql::clip_grads({grads, outs, elements, dtypes, out_dtypes, count}, max_norm, inv_scale,
+                             inv_scale_dev, norm, workspace, workspace_bytes, stream),
               "ql_clip_grads");
 }
 
@@ -424,8 +425,9 @@ int ql_attn_mod_bwd(const ql_attn_mod_args* args, cudaStream_t stream) {
   return done(ql::attn_mod_bwd(*args, stream), "ql_attn_mod_bwd");
 }
 
-int64_t ql_attn_mod_bwd_workspace(const ql_attn_mod_args* args) {
-  return args == nullptr ? 0 : ql::attn_mod_bwd_workspace(*args);
+int64_t ql_attn_mod_bwd_workspace(int32_t n, int32_t max_len, int32_t HQ, int32_t HKV, int32_t D,
+                                  int32_t causal, int32_t window) {
+  return ql::attn_mod_bwd_workspace(n, max_len, HQ, HKV, D, causal, window);
 }
 
 int64_t ql_attn_bwd_partials_floats(int32_t n, int32_t max_len, int32_t HQ, int32_t HKV) {

@@ -15,6 +15,8 @@
 // Bound: HBM (one read for the norm; one read and one write for the rescale) for large lists, two
 // launch latencies for small ones.
 #include <algorithm>
+#include <utility>
+#include <vector>
 
 #include "common.cuh"
 #include "ops.h"
@@ -218,18 +220,18 @@ bool dtype_ok(int dtype) { return dtype == QL_F16 || dtype == QL_BF16 || dtype =
 
 // Tensors [begin, end) of the call as kernel parameters; false if there are too many chunks.
 template <int MAX>
-bool fill_list(const ql_grad_tensor* t, int begin, int end, GradList<MAX>& l) {
+bool fill_list(const GradTensors& t, int begin, int end, GradList<MAX>& l) {
   int64_t chunks = 0;
   l.count = end - begin;
   for (int i = begin; i < end; ++i) {
     const int k = i - begin;
-    l.grad[k] = t[i].grad;
-    l.out[k] = t[i].out;
-    l.n[k] = t[i].n;
-    l.dtype[k] = (uint8_t)t[i].dtype;
-    l.out_dtype[k] = (uint8_t)t[i].out_dtype;
+    l.grad[k] = reinterpret_cast<const void*>(t.grads[i]);
+    l.out[k] = t.outs != nullptr ? reinterpret_cast<void*>(t.outs[i]) : nullptr;
+    l.n[k] = t.elements[i];
+    l.dtype[k] = (uint8_t)t.dtypes[i];
+    l.out_dtype[k] = t.outs != nullptr ? (uint8_t)t.out_dtypes[i] : 0;
     l.first[k] = (int32_t)chunks;
-    chunks += cdiv(t[i].n * elem_bytes(t[i].dtype), GC_CHUNK);
+    chunks += cdiv(t.elements[i] * elem_bytes(t.dtypes[i]), GC_CHUNK);
     if (chunks > 0x3fffffff) return false;
   }
   l.first[l.count] = (int32_t)chunks;
@@ -247,7 +249,7 @@ struct ClipCall {
 };
 
 template <int MAX>
-int squares(const ql_grad_tensor* t, int begin, int end, ClipCall& c, cudaStream_t s) {
+int squares(const GradTensors& t, int begin, int end, ClipCall& c, cudaStream_t s) {
   GradList<MAX> l;
   if (!fill_list(t, begin, end, l)) return QL_STATUS_UNSUPPORTED;
   const int grid = grid_of(l.first[l.count]);
@@ -256,7 +258,7 @@ int squares(const ql_grad_tensor* t, int begin, int end, ClipCall& c, cudaStream
   return launched(1);
 }
 template <int MAX>
-int rescale(const ql_grad_tensor* t, int begin, int end, const ClipCall& c, cudaStream_t s) {
+int rescale(const GradTensors& t, int begin, int end, const ClipCall& c, cudaStream_t s) {
   GradList<MAX> l;
   if (!fill_list(t, begin, end, l)) return QL_STATUS_UNSUPPORTED;
   launch_k(grad_scale_kernel<MAX>, dim3(grid_of(l.first[l.count])), dim3(GC_THREADS), 0, s, l,
@@ -265,18 +267,37 @@ int rescale(const ql_grad_tensor* t, int begin, int end, const ClipCall& c, cuda
   return launched(1);
 }
 
-int clip_check(const ql_grad_tensor* t, int count, const float* norm, const double* ws, int64_t ws_bytes) {
-  if (count < 0 || (count > 0 && t == nullptr) || norm == nullptr || ws == nullptr ||
-      (reinterpret_cast<uintptr_t>(ws) & 7) || ws_bytes < grad_norm_workspace(count))
+int clip_check(const GradTensors& t, const float* norm, const double* ws, int64_t ws_bytes) {
+  if (t.count < 0 || (t.count > 0 && (t.grads == nullptr || t.elements == nullptr || t.dtypes == nullptr)) ||
+      norm == nullptr || ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 7) ||
+      ws_bytes < grad_norm_workspace(t.count))
     return QL_STATUS_BAD_ARG;
-  for (int i = 0; i < count; ++i)
-    if (t[i].n < 0 || t[i].n > (int64_t)1 << 40 || (t[i].n > 0 && t[i].grad == nullptr) || !dtype_ok(t[i].dtype) ||
-        (reinterpret_cast<uintptr_t>(t[i].grad) & (elem_bytes(t[i].dtype) - 1)))
+  for (int i = 0; i < t.count; ++i)
+    if (t.elements[i] < 0 || t.elements[i] > (int64_t)1 << 40 || (t.elements[i] > 0 && t.grads[i] == 0) ||
+        !dtype_ok(t.dtypes[i]) || (t.grads[i] & (elem_bytes(t.dtypes[i]) - 1)))
       return QL_STATUS_BAD_ARG;
   return QL_STATUS_OK;
 }
 
-int all_squares(const ql_grad_tensor* t, int count, ClipCall& c, cudaStream_t s) {
+// Whether any two of the tensors written (or read beside one that is) share memory; an output that is
+// its own gradient counts once.
+bool any_overlap(const GradTensors& t) {
+  std::vector<std::pair<uint64_t, uint64_t>> spans;  // [first byte, end)
+  spans.reserve(2 * (size_t)t.count);
+  for (int i = 0; i < t.count; ++i) {
+    if (t.elements[i] == 0) continue;
+    spans.emplace_back(t.grads[i], t.grads[i] + (uint64_t)t.elements[i] * elem_bytes(t.dtypes[i]));
+    if (t.outs[i] != t.grads[i])
+      spans.emplace_back(t.outs[i], t.outs[i] + (uint64_t)t.elements[i] * elem_bytes(t.out_dtypes[i]));
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t k = 1; k < spans.size(); ++k)
+    if (spans[k].first < spans[k - 1].second) return true;
+  return false;
+}
+
+int all_squares(const GradTensors& t, ClipCall& c, cudaStream_t s) {
+  const int count = t.count;
   for (int b = 0; b < count || b == 0; b += GC_MAX) {
     const int e = std::min(count, b + GC_MAX);
     const int st = e - b <= GC_SMALL ? squares<GC_SMALL>(t, b, e, c, s) : squares<GC_MAX>(t, b, e, c, s);
@@ -291,39 +312,40 @@ int64_t grad_norm_workspace(int count) {
   return std::max<int64_t>(1, cdiv(count, GC_MAX)) * sm_count() * GC_CTAS_PER_SM * (int64_t)sizeof(double);
 }
 
-int grad_norm(const ql_grad_tensor* t, int count, float inv_scale, const float* inv_scale_dev, float* norm,
-              double* ws, int64_t ws_bytes, cudaStream_t s) {
-  int st = clip_check(t, count, norm, ws, ws_bytes);
+int grad_norm(const GradTensors& t, float inv_scale, const float* inv_scale_dev, float* norm, double* ws,
+              int64_t ws_bytes, cudaStream_t s) {
+  int st = clip_check(t, norm, ws, ws_bytes);
   if (st != QL_STATUS_OK) return st;
   ProfScope prof(PK_OTHER, 0, 0, s);
   ClipCall c{0.f, inv_scale, inv_scale_dev, norm, 0, 0, ws};
-  st = all_squares(t, count, c, s);
+  st = all_squares(t, c, s);
   if (st != QL_STATUS_OK) return st;
   launch_k(grad_norm_kernel, dim3(1), dim3(GC_THREADS), 0, s, (const double*)ws, c.partials, inv_scale,
            inv_scale_dev, norm);
   return launched(1);
 }
 
-int clip_grads(const ql_grad_tensor* t, int count, float max_norm, float inv_scale, const float* inv_scale_dev,
-               float* norm, double* ws, int64_t ws_bytes, cudaStream_t s) {
-  int st = clip_check(t, count, norm, ws, ws_bytes);
+int clip_grads(const GradTensors& t, float max_norm, float inv_scale, const float* inv_scale_dev, float* norm,
+               double* ws, int64_t ws_bytes, cudaStream_t s) {
+  int st = clip_check(t, norm, ws, ws_bytes);
   if (st != QL_STATUS_OK) return st;
-  if (!(max_norm >= 0.f)) return QL_STATUS_BAD_ARG;
+  if (!(max_norm >= 0.f) || (t.count > 0 && (t.outs == nullptr || t.out_dtypes == nullptr)))
+    return QL_STATUS_BAD_ARG;
   int in_place = 1;
-  for (int i = 0; i < count; ++i) {
-    if (t[i].n == 0) continue;
-    if (t[i].out == nullptr || !dtype_ok(t[i].out_dtype) ||
-        (reinterpret_cast<uintptr_t>(t[i].out) & (elem_bytes(t[i].out_dtype) - 1)) ||
-        (t[i].out == t[i].grad && t[i].out_dtype != t[i].dtype))
+  for (int i = 0; i < t.count; ++i) {
+    if (t.elements[i] == 0) continue;
+    if (t.outs[i] == 0 || !dtype_ok(t.out_dtypes[i]) || (t.outs[i] & (elem_bytes(t.out_dtypes[i]) - 1)) ||
+        (t.outs[i] == t.grads[i] && t.out_dtypes[i] != t.dtypes[i]))
       return QL_STATUS_BAD_ARG;
-    in_place &= t[i].out == t[i].grad;
+    in_place &= t.outs[i] == t.grads[i];
   }
+  if (any_overlap(t)) return QL_STATUS_BAD_ARG;
   ProfScope prof(PK_OTHER, 0, 0, s);
   ClipCall c{max_norm, inv_scale, inv_scale_dev, norm, in_place, 0, ws};
-  st = all_squares(t, count, c, s);
+  st = all_squares(t, c, s);
   if (st != QL_STATUS_OK) return st;
-  for (int b = 0; b < count || b == 0; b += GC_MAX) {
-    const int e = std::min(count, b + GC_MAX);
+  for (int b = 0; b < t.count || b == 0; b += GC_MAX) {
+    const int e = std::min(t.count, b + GC_MAX);
     st = e - b <= GC_SMALL ? rescale<GC_SMALL>(t, b, e, c, s) : rescale<GC_MAX>(t, b, e, c, s);
     if (st != QL_STATUS_OK) return st;
   }

@@ -91,7 +91,7 @@ int exp2_fma_eval(const float* x, float* y, int64_t n, cudaStream_t s);
 int attn_bwd(const AttnBwdC& a, cudaStream_t s);
 int attn_mod_fwd(const ql_attn_mod_args& m, cudaStream_t s);
 int attn_mod_bwd(const ql_attn_mod_args& m, cudaStream_t s);
-int64_t attn_mod_bwd_workspace(const ql_attn_mod_args& m);
+int64_t attn_mod_bwd_workspace(int n, int max_len, int HQ, int HKV, int D, int causal, int window);
 }  // namespace ql
 
 namespace ql {
@@ -126,8 +126,17 @@ namespace ql {
 int mrope_fwd(const ql_mrope_args& m, cudaStream_t s);
 int mrope_bwd(const ql_mrope_args& m, cudaStream_t s);
 int64_t grad_norm_workspace(int count);
-int grad_norm(const ql_grad_tensor* t, int count, float inv_scale, const float* inv_scale_dev, float* norm,
-              double* ws, int64_t ws_bytes, cudaStream_t s);
-int clip_grads(const ql_grad_tensor* t, int count, float max_norm, float inv_scale, const float* inv_scale_dev,
-               float* norm, double* ws, int64_t ws_bytes, cudaStream_t s);
+// A list of gradients (host memory); outs / out_dtypes null for the norm alone.
+struct GradTensors {
+  const uint64_t* grads;
+  const uint64_t* outs;
+  const int64_t* elements;
+  const int32_t* dtypes;
+  const int32_t* out_dtypes;
+  int count;
+};
+int grad_norm(const GradTensors& t, float inv_scale, const float* inv_scale_dev, float* norm, double* ws,
+              int64_t ws_bytes, cudaStream_t s);
+int clip_grads(const GradTensors& t, float max_norm, float inv_scale, const float* inv_scale_dev, float* norm,
+               double* ws, int64_t ws_bytes, cudaStream_t s);
 }  // namespace ql

@@ -3,6 +3,8 @@ the current stream. Names follow the reference's launch wrappers (solution/engin
 947-1045) so the tests read like the reference's own.
 """
 
+from array import array
+
 import torch
 
 from . import _lib
@@ -10,6 +12,7 @@ from ._lib import call
 
 _DT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 INT_MAX = 2147483647
+STATUS_BAD_ARG = 1  # QL_STATUS_BAD_ARG of include/qlora_sm100.h: the library refuses the arguments
 STATUS_UNSUPPORTED = 3  # QL_STATUS_UNSUPPORTED of include/qlora_sm100.h: no kernel for this request
 STATUS_TIMEOUT = 4  # QL_STATUS_TIMEOUT of include/qlora_sm100.h: a kernel gave up a bounded wait
 
@@ -38,6 +41,62 @@ def _need_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise ValueError("CUDA tensors required (the library has no CPU path)")
+
+
+_INF = float("inf")
+
+
+def _index_of(first, *others):
+    """The CUDA device index the tensors (None: absent) share."""
+    dev = first.get_device()
+    if dev < 0:
+        raise ValueError("CUDA tensors required (the library has no CPU path)")
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            _need_cuda(t)
+            raise ValueError("the tensors must be on one device")
+    return dev
+
+
+def _exact(t, name, shape, dtype):
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)}, got {t.dtype} "
+                         f"{list(t.shape)}")
+
+
+def _given(t, name, shape, dtype, dev):
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be on the inputs' device")
+    _exact(t, name, shape, dtype)
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
+
+
+class _on_device:
+    """Makes a CUDA device the current one for a launch (its current stream is launched on); nothing
+    to switch in the usual case."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _launch(name, dev, args):
+    """Calls an entry point that takes one packed argument struct, on device dev's current stream."""
+    with _on_device(dev):
+        call(name, args, stream_ptr())
 
 
 # ---------------------------------------------------------------------------------------------
@@ -318,37 +377,28 @@ def rope_bwd(dq, dk, dv, cos, sin, pos, HQ, HKV, D, dtype=torch.float16, Bq=None
     return dqkv, dxlo_q, dxlo_v
 
 
-def _mrope_fields(cos, sin, pos, n, HQ, HKV, D, sections, interleaved, lora_scale, dtype, like):
-    """The checked fields both directions of mrope share."""
-    if dtype not in (torch.float16, torch.bfloat16):
+_MROPE = _lib.packer("ql_mrope_args", """qkv xq xv Bq Bv q k v dq dk dv dqkv dxlo_q dxlo_v cos sin
+    pos ld_pos lora_scale n HQ HKV D dtype grad_dtype positions axes sec0 sec1 sec2 sec3
+    interleaved""")
+
+
+def _mrope_inputs(cos, sin, pos, n, HQ, HKV, D, sections, dtype):
+    """The checked (pos row stride, table rows, axes, four section sizes) both directions of mrope
+    share."""
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise ValueError(f"unsupported dtype {dtype}")
     if HQ <= 0 or HKV <= 0 or D <= 0 or D % 64 or D > 256:
         raise ValueError(f"heads ({HQ}, {HKV}, {D}): D must be 64, 128, 192 or 256")
     axes = len(sections)
-    if not 1 <= axes <= 4 or any(x < 0 for x in sections) or sum(sections) != D // 2:
+    if not 1 <= axes <= 4 or min(sections) < 0 or sum(sections) != D // 2:
         raise ValueError(f"sections {tuple(sections)} must be 1 to 4 counts that add to {D // 2}")
-    if pos.dim() != 2 or pos.shape != (axes, n) or pos.dtype != torch.int32 \
-            or (n > 1 and pos.stride(1) != 1):
+    if pos.dim() != 2 or pos.shape != (axes, n) or pos.dtype is not torch.int32 \
+            or (n > 1 and pos.stride(1) != 1) or (axes > 1 and pos.stride(0) < n):
         raise ValueError(f"pos must be int32 [{axes}, {n}] with unit column stride")
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t.dim() != 2 or t.shape != (cos.shape[0], D // 2) or t.dtype != torch.float32 \
-                or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous fp32 [positions, {D // 2}]")
-    if any(t.device != like.device for t in (cos, sin, pos)):
-        raise ValueError("cos, sin and pos must be on the input's device")
-    sec = [int(x) for x in sections] + [0] * (4 - axes)
-    return dict(cos=_ptr(cos), sin=_ptr(sin), pos=_ptr(pos), ld_pos=pos.stride(0) if axes > 1 else n,
-                lora_scale=float(lora_scale), n=n, HQ=HQ, HKV=HKV, D=D, dtype=dtype_code(dtype),
-                positions=cos.shape[0], axes=axes, sec0=sec[0], sec1=sec[1], sec2=sec[2],
-                sec3=sec[3], interleaved=int(bool(interleaved)))
-
-
-def _mrope_tensor(t, name, shape, dtype, like):
-    if t is None:
-        return
-    if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() \
-            or t.device != like.device:
-        raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)} on the input's device")
+    rows = cos.shape[0]
+    _exact(cos, "cos", (rows, D // 2), torch.float32)
+    _exact(sin, "sin", (rows, D // 2), torch.float32)
+    return pos.stride(0) if axes > 1 else n, rows, axes, (*sections, 0, 0, 0)[:4]
 
 
 def mrope_fwd(qkv, cos, sin, pos, HQ, HKV, D, sections, interleaved=False, lora_scale=1.0, xq=None,
@@ -357,29 +407,29 @@ def mrope_fwd(qkv, cos, sin, pos, HQ, HKV, D, sections, interleaved=False, lora_
     sections = how many of the D / 2 frequencies each axis has, in blocks or (interleaved) dealt
     to the axes in turn while an axis has some left; cos / sin the rotary table of one axis.
     xq / Bq, xv / Bv: the LoRA-B products q += lora_scale xq Bq^T, added in fp32."""
-    _need_cuda(qkv, cos, sin, pos, xq, xv, Bq, Bv)
+    dev = _index_of(qkv, cos, sin, pos, xq, xv, Bq, Bv)
     if qkv.dim() != 2:
         raise ValueError("qkv must be [tokens, (HQ + 2 HKV) D]")
     n, dt = qkv.shape[0], qkv.dtype
-    f = _mrope_fields(cos, sin, pos, n, HQ, HKV, D, sections, interleaved, lora_scale, dt, qkv)
-    _mrope_tensor(qkv, "qkv", (n, (HQ + 2 * HKV) * D), dt, qkv)
-    if (xq is None) != (Bq is None) or (xv is None) != (Bv is None):
-        raise ValueError("xq goes with Bq, and xv with Bv")
-    for name, t, shape in (("xq", xq, (n, 16)), ("xv", xv, (n, 16)), ("Bq", Bq, (HQ * D, 16)),
-                           ("Bv", Bv, (HKV * D, 16))):
-        _mrope_tensor(t, name, shape, dt, qkv)
+    ld, rows, axes, sec = _mrope_inputs(cos, sin, pos, n, HQ, HKV, D, sections, dt)
+    _exact(qkv, "qkv", (n, (HQ + 2 * HKV) * D), dt)
+    for lo, B, name, heads in ((xq, Bq, "q", HQ), (xv, Bv, "v", HKV)):
+        if (lo is None) != (B is None):
+            raise ValueError(f"x{name} goes with B{name}")
+        if lo is not None:
+            _exact(lo, "x" + name, (n, 16), dt)
+            _exact(B, "B" + name, (heads * D, 16), dt)
     if out is None:
-        q = torch.empty((n, HQ, D), device=qkv.device, dtype=dt)
-        k = torch.empty((n, HKV, D), device=qkv.device, dtype=dt)
-        v = torch.empty((n, HKV, D), device=qkv.device, dtype=dt)
+        q, k, v = qkv.new_empty((n, HQ, D)), qkv.new_empty((n, HKV, D)), qkv.new_empty((n, HKV, D))
     else:
         q, k, v = out
         for name, t, heads in (("q", q, HQ), ("k", k, HKV), ("v", v, HKV)):
-            _mrope_tensor(t, name, (n, heads, D), dt, qkv)
-    with _on_device(qkv.device):
-        args = _lib.struct("ql_mrope_args", qkv=_ptr(qkv), xq=_ptr(xq), xv=_ptr(xv), Bq=_ptr(Bq),
-                           Bv=_ptr(Bv), q=_ptr(q), k=_ptr(k), v=_ptr(v), **f)
-        call("ql_mrope_fwd", ctypes_ref(args), stream_ptr())
+            _given(t, name, (n, heads, D), dt, dev)
+    args = _MROPE(qkv.data_ptr(), _address(xq), _address(xv), _address(Bq), _address(Bv),
+                  q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, 0, 0, cos.data_ptr(),
+                  sin.data_ptr(), pos.data_ptr(), ld, lora_scale, n, HQ, HKV, D, _DT[dt], 0, rows,
+                  axes, *sec, bool(interleaved))
+    _launch("ql_mrope_fwd", dev, args)
     return q, k, v
 
 
@@ -388,101 +438,90 @@ def mrope_bwd(dq, dk, dv, cos, sin, pos, HQ, HKV, D, sections, interleaved=False
     """(dqkv, dxlo_q, dxlo_v) of mrope_fwd (ql_mrope_bwd): the pre-rotary qkv gradient in `dtype`
     from dq [n, HQ, D], dk / dv [n, HKV, D] (dtype or fp32), and with Bq / Bv the LoRA-A output
     gradients lora_scale * (g . B), fp32 [n, 16]."""
-    _need_cuda(dq, dk, dv, cos, sin, pos, Bq, Bv)
+    dev = _index_of(dq, dk, dv, cos, sin, pos, Bq, Bv)
     if dq.dim() != 3:
         raise ValueError("dq must be [tokens, HQ, D]")
-    n, dev = dq.shape[0], dq.device
-    f = _mrope_fields(cos, sin, pos, n, HQ, HKV, D, sections, interleaved, lora_scale, dtype, dq)
-    if dq.dtype not in (dtype, torch.float32):
+    n, gt = dq.shape[0], dq.dtype
+    ld, rows, axes, sec = _mrope_inputs(cos, sin, pos, n, HQ, HKV, D, sections, dtype)
+    if gt is not dtype and gt is not torch.float32:
         raise ValueError(f"gradients must be {dtype} or fp32")
-    for name, t, heads in (("dq", dq, HQ), ("dk", dk, HKV), ("dv", dv, HKV)):
-        _mrope_tensor(t, name, (n, heads, D), dq.dtype, dq)
-    _mrope_tensor(Bq, "Bq", (HQ * D, 16), dtype, dq)
-    _mrope_tensor(Bv, "Bv", (HKV * D, 16), dtype, dq)
+    _exact(dq, "dq", (n, HQ, D), gt)
+    _exact(dk, "dk", (n, HKV, D), gt)
+    _exact(dv, "dv", (n, HKV, D), gt)
+    dxlo_q = dxlo_v = None
+    if Bq is not None:
+        _exact(Bq, "Bq", (HQ * D, 16), dtype)
+        dxlo_q = dq.new_empty((n, 16), dtype=torch.float32)
+    if Bv is not None:
+        _exact(Bv, "Bv", (HKV * D, 16), dtype)
+        dxlo_v = dq.new_empty((n, 16), dtype=torch.float32)
     C = (HQ + 2 * HKV) * D
-    if out is not None:
-        _mrope_tensor(out, "out", (n, C), dtype, dq)
-    dqkv = out if out is not None else torch.empty((n, C), device=dev, dtype=dtype)
-    dxlo_q = torch.empty((n, 16), device=dev, dtype=torch.float32) if Bq is not None else None
-    dxlo_v = torch.empty((n, 16), device=dev, dtype=torch.float32) if Bv is not None else None
-    with _on_device(dev):
-        args = _lib.struct("ql_mrope_args", dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), dqkv=_ptr(dqkv),
-                           Bq=_ptr(Bq), Bv=_ptr(Bv), dxlo_q=_ptr(dxlo_q), dxlo_v=_ptr(dxlo_v),
-                           grad_dtype=dtype_code(dq.dtype), **f)
-        call("ql_mrope_bwd", ctypes_ref(args), stream_ptr())
-    return dqkv, dxlo_q, dxlo_v
+    if out is None:
+        out = dq.new_empty((n, C), dtype=dtype)
+    else:
+        _given(out, "out", (n, C), dtype, dev)
+    args = _MROPE(0, 0, 0, _address(Bq), _address(Bv), 0, 0, 0, dq.data_ptr(), dk.data_ptr(),
+                  dv.data_ptr(), out.data_ptr(), _address(dxlo_q), _address(dxlo_v),
+                  cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), ld, lora_scale, n, HQ, HKV, D,
+                  _DT[dtype], _DT[gt], rows, axes, *sec, bool(interleaved))
+    _launch("ql_mrope_bwd", dev, args)
+    return out, dxlo_q, dxlo_v
 
 
 # ---------------------------------------------------------------------------------------------
 # gradient norm and clipping
 # ---------------------------------------------------------------------------------------------
-_GRAD_TENSOR = [("grad", "u8"), ("out", "u8"), ("n", "i8"), ("dtype", "i4"), ("out_dtype", "i4")]
+_ADDRESS, _NUMEL = torch.Tensor.data_ptr, torch.Tensor.numel
+_CONTIGUOUS, _INDEX = torch.Tensor.is_contiguous, torch.Tensor.get_device
 
 
-def _grad_list(tensors, name, device):
-    """(addresses, elements, dtype codes) of the tensors as numpy arrays, checked."""
-    import numpy as np
-
-    for t in tensors:
-        if not t.is_cuda:
-            raise ValueError("CUDA tensors required (the library has no CPU path)")
-        if t.device != device:
-            raise ValueError(f"{name} must be on one device")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-    return (np.array([t.data_ptr() for t in tensors], dtype=np.uint64),
-            np.array([t.numel() for t in tensors], dtype=np.int64),
-            np.array([dtype_code(t.dtype) for t in tensors], dtype=np.int32))
-
-
-def _overlap(addr, size, kind):
-    """Whether two of the tensors share memory."""
-    import numpy as np
-
-    end = addr + (size * np.where(kind == 2, 4, 2)).astype(np.uint64)
-    order = np.argsort(addr[size > 0], kind="stable")
-    a, e = addr[size > 0][order], end[size > 0][order]
-    return bool((a[1:] < e[:-1]).any())
+def _grad_list(tensors, name, dev):
+    """The tensors' addresses and dtype codes as arrays for the library, after their checks."""
+    if dev < 0 or set(map(_INDEX, tensors)) - {dev}:
+        _need_cuda(*tensors)
+        raise ValueError(f"{name} must be on one device")
+    if not all(map(_CONTIGUOUS, tensors)):
+        raise ValueError(f"{name} must be contiguous")
+    kinds = [t.dtype for t in tensors]
+    if len(set(kinds)) == 1:
+        codes = array("i", (dtype_code(kinds[0]),)) * len(kinds)
+    else:
+        codes = array("i", map(dtype_code, kinds))
+    return array("Q", map(_ADDRESS, tensors)), codes
 
 
 def _clip_call(grads, inv_scale, max_norm=None, out=None):
-    import numpy as np
-
     grads = list(grads)
-    dev = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
-    addr, size, kind = _grad_list(grads, "gradients", dev)
-    arr = np.zeros(len(grads), dtype=_GRAD_TENSOR)
-    arr["grad"], arr["n"], arr["dtype"] = addr, size, kind
-    if max_norm is not None:
-        if _overlap(addr, size, kind):
-            raise ValueError("gradients share memory: each would be rescaled more than once")
-        if out is None:
-            arr["out"], arr["out_dtype"] = addr, kind
-        else:
-            out = list(out)
-            if len(out) != len(grads) or any(o.shape != g.shape for o, g in zip(out, grads)):
-                raise ValueError("out must hold a tensor of each gradient's shape")
-            o_addr, o_size, o_kind = _grad_list(out, "out", dev)
-            apart = (o_addr != addr) | (o_kind != kind)  # a gradient may be its own output
-            if _overlap(np.concatenate([addr, o_addr[apart]]),
-                        np.concatenate([size, o_size[apart]]),
-                        np.concatenate([kind, o_kind[apart]])):
-                raise ValueError("out shares memory with itself or with other gradients")
-            arr["out"], arr["out_dtype"] = o_addr, o_kind
-    scale_dev = None
+    count = len(grads)
+    dev = grads[0].get_device() if grads else torch.cuda.current_device()
+    addr, kind = _grad_list(grads, "gradients", dev)
+    size = array("q", map(_NUMEL, grads))
+    o_addr, o_kind = addr, kind
+    if out is not None:
+        out = list(out)
+        if array("q", map(_NUMEL, out)) != size:
+            raise ValueError("out must hold a tensor of as many elements for each gradient")
+        o_addr, o_kind = _grad_list(out, "out", dev)
+    scale_dev = 0
     if torch.is_tensor(inv_scale):
-        if inv_scale.numel() != 1 or inv_scale.dtype != torch.float32 or inv_scale.device != dev:
+        if inv_scale.numel() != 1 or inv_scale.dtype is not torch.float32 \
+                or inv_scale.get_device() != dev:
             raise ValueError("inv_scale must be a number or an fp32 scalar on the gradients' device")
-        scale_dev, inv_scale = inv_scale, 1.0
-    norm = torch.empty((), device=dev, dtype=torch.float32)
+        scale_dev, inv_scale = inv_scale.data_ptr(), 1.0
+    lib = _lib.lib()
+    addresses = [a.buffer_info()[0] for a in (addr, o_addr, size, kind, o_kind)]
     with _on_device(dev):
-        ws = torch.empty(int(_lib.lib().ql_grad_norm_workspace(len(grads))), device=dev,
-                         dtype=torch.uint8)
-        tail = (float(inv_scale), _ptr(scale_dev), _ptr(norm), _ptr(ws), ws.numel(), stream_ptr())
+        norm = torch.empty((), device="cuda", dtype=torch.float32)
+        ws = norm.new_empty(lib.ql_grad_norm_workspace(count) // 8, dtype=torch.float64)
+        tail = (inv_scale, scale_dev, norm.data_ptr(), ws.data_ptr(), ws.shape[0] * 8, stream_ptr())
         if max_norm is None:
-            call("ql_grad_norm", arr.ctypes.data, len(grads), *tail)
+            call("ql_grad_norm", addresses[0], addresses[2], addresses[3], count, *tail)
         else:
-            call("ql_clip_grads", arr.ctypes.data, len(grads), float(max_norm), *tail)
+            status = lib.ql_clip_grads(*addresses, count, max_norm, *tail)
+            if status == STATUS_BAD_ARG:
+                raise ValueError("gradients or outputs share memory with one another, or a gradient "
+                                 "is its own output in another dtype")
+            _lib.check("ql_clip_grads", status)
     return norm
 
 
@@ -495,7 +534,7 @@ def grad_norm(grads, inv_scale=1.0):
 
 def clip_grads(grads, max_norm, inv_scale=1.0, out=None):
     """Rescales the gradients by inv_scale * min(1, max_norm / (norm + 1e-6)), in place or into the
-    tensors of `out` (same shapes, any of the three dtypes, e.g. fp32 master gradients), and returns
+    tensors of `out` (as many elements each, any of the three dtypes, e.g. fp32 master gradients), and returns
     the norm before clipping as a device scalar (ql_clip_grads): torch.nn.utils.clip_grad_norm_ with
     the unscaling folded in, in two kernels and with no host read. A norm that is not finite makes
     every gradient not finite, as there."""
@@ -667,77 +706,52 @@ def attn_bwd(dout, q, k, v, out, lse, cu_seqlens, max_len, scale, dq=None, dk=No
     return dq, dk, dv
 
 
-def _on_device(device):
-    """The device as the current one for a launch (nothing to switch in the usual case)."""
-    import contextlib
-
-    if device.index is None or device.index == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_ATTN_MOD = _lib.packer("ql_attn_mod_args", """q k v out lse cu_seqlens slopes prefix_len doc_ids
+    ranges dout dq dk dv workspace workspace_floats ldq ldk ldv scale softcap n B max_len HQ HKV D
+    dtype causal window""")
 
 
-def _attn_mod_heads(t, name, n, heads, D, like):
-    if t.dim() != 3 or t.shape != (n, heads, D):
-        raise ValueError(f"{name} must be [{n}, {heads}, {D}], got {list(t.shape)}")
-    if t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must have q's dtype and device")
-    if t.numel() and (t.stride(2) != 1 or t.stride(1) != D):
-        raise ValueError(f"{name}'s heads must be contiguous within a row")
-    return t.stride(0) if n > 1 else heads * D
-
-
-def _attn_mod_vector(t, name, shape, dtype, like):
-    if t is None:
-        return
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() \
-            or t.device != like.device:
-        raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)} on q's device")
-
-
-def _attn_mod_fields(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes, window,
-                     doc_ids, prefix_len):
-    """The checked fields both directions of attn_mod share."""
-    _need_cuda(q, k, v, cu_seqlens, slopes, doc_ids, prefix_len)
+def _attn_mod_inputs(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes, window, doc_ids,
+                     prefix_len):
+    """The checked sizes both directions of attn_mod share: (n, HQ, HKV, D, B, row strides of q, k
+    and v, dtype code, device index, window as the library takes it)."""
+    dev = _index_of(q, k, v, cu_seqlens, slopes, doc_ids, prefix_len)
+    dt = q.dtype
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q and k must be [tokens, heads, D]")
     n, HQ, D = q.shape
     HKV = k.shape[1]
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"unsupported dtype {q.dtype}")
-    if D not in (64, 128):
+    if dt is not torch.float16 and dt is not torch.bfloat16:
+        raise ValueError(f"unsupported dtype {dt}")
+    if D != 64 and D != 128:
         raise ValueError(f"head size {D}: 64 or 128 are supported")
-    if HKV == 0 or HQ % HKV:
+    if HKV == 0 or HQ == 0 or HQ % HKV:
         raise ValueError(f"{HQ} query heads over {HKV} key heads")
-    ldq = _attn_mod_heads(q, "q", n, HQ, D, q)
-    ldk = _attn_mod_heads(k, "k", n, HKV, D, q)
-    ldv = _attn_mod_heads(v, "v", n, HKV, D, q)
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+    kv = (n, HKV, D)
+    strides = []
+    for name, t, shape, heads in (("q", q, q.shape, HQ), ("k", k, kv, HKV), ("v", v, kv, HKV)):
+        if t.shape != shape or t.dtype is not dt:
+            raise ValueError(f"{name} must be a {dt} {list(shape)}, got {t.dtype} {list(t.shape)}")
+        ld, inner, unit = t.stride()
+        if n and (unit != 1 or (inner != D and heads > 1)):
+            raise ValueError(f"{name}'s heads must be contiguous within a row")
+        strides.append(ld if n > 1 else heads * D)
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must be int32 [sequences + 1]")
-    B = cu_seqlens.numel() - 1
-    _attn_mod_vector(cu_seqlens, "cu_seqlens", (B + 1,), torch.int32, q)
-    _attn_mod_vector(slopes, "slopes", (HQ,), torch.float32, q)
-    _attn_mod_vector(doc_ids, "doc_ids", (n,), torch.int32, q)
-    _attn_mod_vector(prefix_len, "prefix_len", (B,), torch.int32, q)
-    if prefix_len is not None and not causal:
-        raise ValueError("prefix_len needs causal=True (without it every key is seen already)")
-    if not 0 <= max_len <= n or window < 0 or not 0 < scale < float("inf") \
-            or not 0 <= softcap < float("inf"):
+    B = cu_seqlens.shape[0] - 1
+    _exact(cu_seqlens, "cu_seqlens", (B + 1,), torch.int32)
+    if slopes is not None:
+        _exact(slopes, "slopes", (HQ,), torch.float32)
+    if doc_ids is not None:
+        _exact(doc_ids, "doc_ids", (n,), torch.int32)
+    if prefix_len is not None:
+        _exact(prefix_len, "prefix_len", (B,), torch.int32)
+        if not causal:
+            raise ValueError("prefix_len needs causal=True (without it every key is seen already)")
+    if not (0 <= max_len <= n and window >= 0 and 0 < scale < _INF and 0 <= softcap < _INF):
         raise ValueError("needs 0 <= max_len <= tokens, window >= 0, 0 < scale < inf and "
                          "0 <= softcap < inf")
-    ranges = torch.empty((n, 2), device=q.device, dtype=torch.int32) \
-        if doc_ids is not None else None
-    return dict(q=_ptr(q), k=_ptr(k), v=_ptr(v), cu_seqlens=_ptr(cu_seqlens), slopes=_ptr(slopes),
-                doc_ids=_ptr(doc_ids), prefix_len=_ptr(prefix_len), ranges=_ptr(ranges), ldq=ldq,
-                ldk=ldk, ldv=ldv, scale=float(scale), softcap=float(softcap), n=n, B=B,
-                max_len=int(max_len), HQ=HQ, HKV=HKV, D=D, dtype=dtype_code(q.dtype),
-                causal=int(bool(causal)), window=min(int(window), INT_MAX)), ranges
-
-
-def _attn_mod_like(t, name, shape, dtype, like):
-    if t is None:
-        return torch.empty(shape, device=like.device, dtype=dtype)
-    _attn_mod_vector(t, name, tuple(shape), dtype, like)
-    return t
+    return n, HQ, HKV, D, B, strides, _DT[dt], dev, min(window, INT_MAX)
 
 
 def attn_mod_fwd(q, k, v, cu_seqlens, max_len, scale, causal=True, softcap=0.0, slopes=None,
@@ -751,13 +765,22 @@ def attn_mod_fwd(q, k, v, cu_seqlens, max_len, scale, causal=True, softcap=0.0, 
     (window > 0), and both are in the same run of equal doc_ids (negative ids: padding). slopes
     fp32 [HQ], doc_ids int32 [n], prefix_len int32 [B]. out as q (contiguous), lse fp32 [HQ, n];
     a query that sees nothing gets out 0 and lse -inf."""
-    f, ranges = _attn_mod_fields(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes,
-                                 window, doc_ids, prefix_len)
-    out = _attn_mod_like(out, "out", q.shape, q.dtype, q)
-    lse = _attn_mod_like(lse, "lse", (q.shape[1], q.shape[0]), torch.float32, q)
-    with _on_device(q.device):
-        args = _lib.struct("ql_attn_mod_args", out=_ptr(out), lse=_ptr(lse), **f)
-        call("ql_attn_mod_fwd", ctypes_ref(args), stream_ptr())
+    n, HQ, HKV, D, B, ld, dt, dev, window = _attn_mod_inputs(
+        q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes, window, doc_ids, prefix_len)
+    if out is None:
+        out = q.new_empty((n, HQ, D))
+    else:
+        _given(out, "out", (n, HQ, D), q.dtype, dev)
+    if lse is None:
+        lse = q.new_empty((HQ, n), dtype=torch.float32)
+    else:
+        _given(lse, "lse", (HQ, n), torch.float32, dev)
+    ranges = q.new_empty((n, 2), dtype=torch.int32) if doc_ids is not None else None
+    args = _ATTN_MOD(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                     cu_seqlens.data_ptr(), _address(slopes), _address(prefix_len),
+                     _address(doc_ids), _address(ranges), 0, 0, 0, 0, 0, 0, *ld, scale, softcap, n,
+                     B, max_len, HQ, HKV, D, dt, bool(causal), window)
+    _launch("ql_attn_mod_fwd", dev, args)
     return out, lse
 
 
@@ -765,23 +788,31 @@ def attn_mod_bwd(dout, q, k, v, out, lse, cu_seqlens, max_len, scale, causal=Tru
                  slopes=None, window=0, doc_ids=None, prefix_len=None, dq=None, dk=None, dv=None):
     """(dq, dk, dv) of attn_mod_fwd, in q's dtype, given its arguments, out and lse
     (ql_attn_mod_bwd); dout [n, HQ, D] contiguous. Bit-identical from run to run."""
-    f, ranges = _attn_mod_fields(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes,
-                                 window, doc_ids, prefix_len)
-    _need_cuda(dout, out, lse)
-    _attn_mod_vector(dout, "dout", tuple(q.shape), q.dtype, q)
-    _attn_mod_vector(out, "out", tuple(q.shape), q.dtype, q)
-    _attn_mod_vector(lse, "lse", (q.shape[1], q.shape[0]), torch.float32, q)
-    dq = _attn_mod_like(dq, "dq", q.shape, q.dtype, q)
-    dk = _attn_mod_like(dk, "dk", k.shape, q.dtype, q)
-    dv = _attn_mod_like(dv, "dv", v.shape, q.dtype, q)
-    with _on_device(q.device):
-        args = _lib.struct("ql_attn_mod_args", out=_ptr(out), lse=_ptr(lse), dout=_ptr(dout),
-                           dq=_ptr(dq), dk=_ptr(dk), dv=_ptr(dv), **f)
-        need = int(_lib.lib().ql_attn_mod_bwd_workspace(ctypes_ref(args)))
-        ws = torch.empty(max(need, 4), device=q.device, dtype=torch.float32)
-        args.workspace, args.workspace_floats = _ptr(ws), ws.numel()
-        call("ql_attn_mod_bwd", ctypes_ref(args), stream_ptr())
-    return dq, dk, dv
+    n, HQ, HKV, D, B, ld, dt, dev, window = _attn_mod_inputs(
+        q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes, window, doc_ids, prefix_len)
+    dtype, shape, kv = q.dtype, (n, HQ, D), (n, HKV, D)
+    _given(dout, "dout", shape, dtype, dev)
+    _given(out, "out", shape, dtype, dev)
+    _given(lse, "lse", (HQ, n), torch.float32, dev)
+    grads = []
+    for name, t, want in (("dq", dq, shape), ("dk", dk, kv), ("dv", dv, kv)):
+        if t is None:
+            t = q.new_empty(want)
+        else:
+            _given(t, name, want, dtype, dev)
+        grads.append(t)
+    ranges = q.new_empty((n, 2), dtype=torch.int32) if doc_ids is not None else None
+    lib = _lib.lib()
+    with _on_device(dev):  # the workspace's size goes by the device's SMs
+        floats = lib.ql_attn_mod_bwd_workspace(n, max_len, HQ, HKV, D, bool(causal), window)
+    ws = q.new_empty(max(floats, 4), dtype=torch.float32)
+    args = _ATTN_MOD(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                     cu_seqlens.data_ptr(), _address(slopes), _address(prefix_len),
+                     _address(doc_ids), _address(ranges), dout.data_ptr(),
+                     *(t.data_ptr() for t in grads), ws.data_ptr(), ws.shape[0], *ld, scale,
+                     softcap, n, B, max_len, HQ, HKV, D, dt, bool(causal), window)
+    _launch("ql_attn_mod_bwd", dev, args)
+    return tuple(grads)
 
 
 def gather_rows(src, idx, out=None):

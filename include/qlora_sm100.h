@@ -326,23 +326,20 @@ int ql_lora_colsum_noalloc(const void* X, int64_t ldx, int x_dtype, const void* 
  *   out = grad * inv_scale * min(1, max_norm / (norm + 1e-6))
  * rounded once (out == grad: in place; nothing is written when that factor is 1). inv_scale undoes a
  * loss scale; inv_scale_dev (a device float, or NULL) takes its place when given. A norm that is not
- * finite makes the outputs not finite, as in torch. Gradients and outputs may differ in dtype from
- * tensor to tensor (QL_F16, QL_BF16, QL_F32), must not overlap, and need only their own type's
- * alignment (16 bytes is fastest). The tensor list is host memory, read during the call. The sums
- * have a fixed order. workspace: ql_grad_norm_workspace(count) bytes, 8-byte aligned, of any
- * content; calls that may overlap each need their own. */
-typedef struct {
-  const void* grad;
-  void* out;            /* ql_clip_grads only */
-  int64_t n;            /* elements */
-  int32_t dtype, out_dtype;
-} ql_grad_tensor;
+ * finite makes the outputs not finite, as in torch. The lists are host memory, read during the
+ * call: addresses, elements and dtypes (QL_F16, QL_BF16, QL_F32) of `count` gradients and, for
+ * ql_clip_grads, of their outputs. dtypes may differ from tensor to tensor; tensors need only their
+ * own type's alignment (16 bytes is fastest) and must not overlap, but for an output that is its own
+ * gradient (QL_STATUS_BAD_ARG). The sums have a fixed order. workspace:
+ * ql_grad_norm_workspace(count) bytes, 8-byte aligned, of any content; calls that may overlap each
+ * need their own. */
 int64_t ql_grad_norm_workspace(int count);
-int ql_grad_norm(const ql_grad_tensor* tensors, int count, float inv_scale,
-                 const float* inv_scale_dev, float* norm, double* workspace,
+int ql_grad_norm(const uint64_t* grads, const int64_t* elements, const int32_t* dtypes, int count,
+                 float inv_scale, const float* inv_scale_dev, float* norm, double* workspace,
                  int64_t workspace_bytes, cudaStream_t stream);
-int ql_clip_grads(const ql_grad_tensor* tensors, int count, float max_norm, float inv_scale,
-                  const float* inv_scale_dev, float* norm, double* workspace,
+int ql_clip_grads(const uint64_t* grads, const uint64_t* outs, const int64_t* elements,
+                  const int32_t* dtypes, const int32_t* out_dtypes, int count, float max_norm,
+                  float inv_scale, const float* inv_scale_dev, float* norm, double* workspace,
                   int64_t workspace_bytes, cudaStream_t stream);
 
 /* ---- embedding ---------------------------------------------------------------------------
@@ -512,8 +509,9 @@ typedef struct {
 int ql_attn_mod_fwd(const ql_attn_mod_args* args, cudaStream_t stream);
 /* dq, dk, dv of every row of the sequences, given the forward's arguments, out and lse. */
 int ql_attn_mod_bwd(const ql_attn_mod_args* args, cudaStream_t stream);
-/* Floats of workspace the backward of these arguments needs (0 for arguments it refuses). */
-int64_t ql_attn_mod_bwd_workspace(const ql_attn_mod_args* args);
+/* Floats of workspace the backward of a batch of these sizes needs. */
+int64_t ql_attn_mod_bwd_workspace(int32_t n, int32_t max_len, int32_t HQ, int32_t HKV, int32_t D,
+                                  int32_t causal, int32_t window);
 
 /* ---- head row order ----------------------------------------------------------------------
  * The head takes rows with a target first (solution/engine.py:731, 1364-1398):

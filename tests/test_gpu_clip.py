@@ -2,8 +2,8 @@
 refusals (CPU)."""
 
 import math
+from array import array
 
-import numpy as np
 import pytest
 import torch
 
@@ -172,26 +172,44 @@ def test_cpu_tensors_are_refused():
         ops.clip_grads([torch.ones(3)], 1.0)
 
 
-def test_the_overlap_check():
-    u8, i8, i4 = np.uint64, np.int64, np.int32
-    f = lambda a, n, k: ops._overlap(np.array(a, u8), np.array(n, i8), np.array(k, i4))  # noqa: E731
-    assert not f([400, 0], [10, 100], [2, 2])       # [400, 440) and [0, 400)
-    assert f([399, 0], [10, 100], [2, 2])
-    assert not f([200, 0], [10, 100], [2, 0])       # 16-bit: [0, 200)
-    assert not f([0, 0], [10, 0], [2, 2])           # an empty tensor shares nothing
+def lib_call(entry="ql_clip_grads", **change):
+    """A call with made-up addresses, for what the library checks before it launches anything."""
+    f = dict(grads=[1 << 20], outs=[2 << 20], n=[10], dtypes=[2], out_dtypes=[2], max_norm=1.0,
+             norm=3 << 20, ws=4 << 20, bytes=1 << 20)
+    f.update(change)
+    held = [array("Q", f["grads"]), array("Q", f["outs"]), array("q", f["n"]),
+            array("i", f["dtypes"]), array("i", f["out_dtypes"])]
+    at = [a.buffer_info()[0] for a in held]
+    tail = (1.0, None, f["norm"], f["ws"], f["bytes"], None)
+    if entry == "ql_grad_norm":
+        _lib.call(entry, at[0], at[2], at[3], len(held[0]), *tail)
+    else:
+        _lib.call(entry, *at, len(held[0]), f["max_norm"], *tail)
 
 
-@pytest.mark.parametrize("change", [dict(dtype=3), dict(out_dtype=-1), dict(n=-1), dict(grad=0),
-                                    dict(out=0), dict(grad=(1 << 12) + 2), dict(out=(2 << 12) + 1),
-                                    dict(out=1 << 12, out_dtype=1), dict(max_norm=-1.0),
-                                    dict(max_norm=math.nan), dict(ws=0), dict(ws=4), dict(bytes=8)], ids=str)
-def test_the_library_refuses_before_any_launch(change):
-    arr = np.zeros(1, dtype=ops._GRAD_TENSOR)
-    f = dict(grad=1 << 12, out=2 << 12, n=10, dtype=2, out_dtype=2)
-    f.update({k: v for k, v in change.items() if k in f})
-    for k, v in f.items():
-        arr[k] = v
+@pytest.mark.parametrize("change", [dict(dtypes=[3]), dict(n=[-1]), dict(grads=[0]),
+                                    dict(grads=[(1 << 20) + 2]), dict(norm=0), dict(ws=0),
+                                    dict(ws=(4 << 20) + 4), dict(bytes=8)], ids=str)
+def test_both_entries_refuse_before_any_launch(change):
+    for entry in ("ql_clip_grads", "ql_grad_norm"):
+        with pytest.raises(_lib.QLError) as e:
+            lib_call(entry, **change)
+        assert e.value.status == ops.STATUS_BAD_ARG
+
+
+TWO = dict(grads=[1 << 20, 2 << 20], outs=[1 << 20, 2 << 20], n=[100, 100], dtypes=[2, 2],
+           out_dtypes=[2, 2])
+
+
+@pytest.mark.parametrize("change", [
+    dict(out_dtypes=[-1]), dict(outs=[0]), dict(outs=[(2 << 20) + 1]), dict(max_norm=-1.0),
+    dict(max_norm=math.nan), dict(outs=[1 << 20], out_dtypes=[1]),
+    {**TWO, "grads": [1 << 20, 1 << 20], "outs": [1 << 20, 1 << 20]},       # the same tensor twice
+    {**TWO, "grads": [1 << 20, (1 << 20) + 396], "outs": [1 << 20, (1 << 20) + 396]},
+    {**TWO, "outs": [3 << 20, 3 << 20]},                                   # one output for two
+    {**TWO, "outs": [3 << 20, 1 << 20]},                                   # another's gradient
+    {**TWO, "dtypes": [1, 2], "outs": [(1 << 20) + 100, 3 << 20]}], ids=str)
+def test_clipping_refuses_before_any_launch(change):
     with pytest.raises(_lib.QLError) as e:
-        _lib.call("ql_clip_grads", arr.ctypes.data, 1, change.get("max_norm", 1.0), 1.0, None,
-                  3 << 12, change.get("ws", 4 << 12), change.get("bytes", 1 << 20), None)
-    assert e.value.status == 1
+        lib_call(**change)
+    assert e.value.status == ops.STATUS_BAD_ARG
