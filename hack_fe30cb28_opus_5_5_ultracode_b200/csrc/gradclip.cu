@@ -2,18 +2,19 @@
 //
 // Two passes and no meeting of the CTAs inside a kernel: the first writes one sum of squares per
 // CTA; in the second every CTA adds those sums in the same order (fp64), so all arrive at the same
-// factor, and rescales its part. A gradient list that fits in L2 is read from HBM once; of a longer
-// one the second pass starts at the end, where the first pass left L2. Squares are summed in fp32 within
-// a thread's part of one chunk (four sums of at most 16 to 32 values, which is why the chunk is not
-// longer: over thousands of them the norm was off by 1.5e-6), from there on in fp64.
+// factor, and rescales its part. A gradient list that fits in L2 is read from HBM once. Squares are
+// summed in fp32 over eight loads of a thread (four sums of 8 to 16 values; over thousands of them the
+// norm was off by 1.5e-6), from there on in fp64.
 //
 // The tensors' addresses and sizes travel as kernel parameters (up to 1,024 tensors a launch), so a
 // call copies nothing to the device and can be captured. Work is cut into chunks of 32 KB of one
-// tensor, dealt to the CTAs in turn; a chunk whose addresses are 16-byte aligned moves 16 bytes per
-// thread, eight loads in flight, others element by element.
+// tensor, and each CTA takes one stretch of them: it searches the list once and then walks it. Where
+// addresses are 16-byte aligned a thread moves up to 16 bytes at a time, eight loads in flight; other
+// spans go element by element.
 //
 // Bound: HBM (one read for the norm; one read and one write for the rescale) for large lists, two
-// launch latencies for small ones.
+// launch latencies for small ones. 0.9 G bf16 gradients: norm 256 us (7.0 TB/s), norm and rescale into
+// fp32 1,205 us (6.0 TB/s of the bytes both passes move).
 #include <algorithm>
 #include <utility>
 #include <vector>
@@ -68,28 +69,61 @@ __device__ __forceinline__ void square16(const uint4& u, float* s) {
   }
 }
 
+__device__ __forceinline__ double sum4(const float* s) {
+  return ((double)s[0] + (double)s[1]) + ((double)s[2] + (double)s[3]);
+}
+
 template <typename T>
-__device__ __forceinline__ void chunk_squares(const T* p, int n, float* s) {
+__device__ __forceinline__ double span_squares(const T* p, int64_t n) {
   constexpr int V = 16 / sizeof(T);
-  int done = 0;
+  double all = 0.0;
+  int64_t done = 0;
   if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
     const uint4* v = reinterpret_cast<const uint4*>(p);
-    const int nv = n / V;
-    int i = threadIdx.x;
+    const int64_t nv = n / V;
+    int64_t i = threadIdx.x;
     for (; i + 7 * GC_THREADS < nv; i += 8 * GC_THREADS) {
       uint4 u[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) u[k] = v[i + k * GC_THREADS];
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < 8; ++k) square16<T>(u[k], s);
+      all += sum4(s);
     }
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
     for (; i < nv; i += GC_THREADS) square16<T>(v[i], s);
+    all += sum4(s);
     done = nv * V;
   }
-#pragma unroll 4
-  for (int i = done + threadIdx.x; i < n; i += GC_THREADS) {
-    const float f = to_f<T>(p[i]);
-    s[0] = fmaf(f, f, s[0]);
+  // up to seven values of an aligned span, all of another one
+  for (int64_t i0 = done + threadIdx.x; i0 < n; i0 += 16 * GC_THREADS) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int64_t i = i0 + k * GC_THREADS;
+      const float f = i < n ? to_f<T>(p[i]) : 0.f;
+      s[k & 3] = fmaf(f, f, s[k & 3]);
+    }
+    all += sum4(s);
+  }
+  return all;
+}
+
+// The CTA's stretch of the list's chunks, cut at the tensors' ends: f(tensor, first element, elements).
+template <int MAX, typename F>
+__device__ __forceinline__ void walk(const GradList<MAX>& l, F f) {
+  const int64_t chunks = l.first[l.count];
+  const int c0 = (int)(chunks * blockIdx.x / gridDim.x), c1 = (int)(chunks * (blockIdx.x + 1) / gridDim.x);
+  if (c0 >= c1) return;
+  int t = tensor_of(l, c0);
+  for (int c = c0; c < c1; ++t) {
+    const int f0 = l.first[t], to = min(c1, l.first[t + 1]);
+    if (to > c) {
+      const int64_t per = chunk_elems(l.dtype[t]), at = (c - f0) * per;
+      f(t, at, min((to - c) * per, l.n[t] - at));
+      c = to;
+    }
   }
 }
 
@@ -111,16 +145,12 @@ __global__ void __launch_bounds__(GC_THREADS) grad_squares_kernel(const __grid_c
                                                                   double* partial) {
   pdl_enter();
   double all = 0.0;
-  for (int c = blockIdx.x; c < l.first[l.count]; c += gridDim.x) {
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    const int t = tensor_of(l, c), dt = l.dtype[t], per = chunk_elems(dt);
-    const int64_t at = (int64_t)(c - l.first[t]) * per;
-    const int n = (int)min((int64_t)per, l.n[t] - at);
-    if (dt == QL_F32) chunk_squares(static_cast<const float*>(l.grad[t]) + at, n, s);
-    else if (dt == QL_F16) chunk_squares(static_cast<const __half*>(l.grad[t]) + at, n, s);
-    else chunk_squares(static_cast<const __nv_bfloat16*>(l.grad[t]) + at, n, s);
-    all += ((double)s[0] + (double)s[1]) + ((double)s[2] + (double)s[3]);
-  }
+  walk(l, [&](int t, int64_t at, int64_t n) {
+    const int dt = l.dtype[t];
+    if (dt == QL_F32) all += span_squares(static_cast<const float*>(l.grad[t]) + at, n);
+    else if (dt == QL_F16) all += span_squares(static_cast<const __half*>(l.grad[t]) + at, n);
+    else all += span_squares(static_cast<const __nv_bfloat16*>(l.grad[t]) + at, n);
+  });
   const double sum = cta_sum(all);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
@@ -140,53 +170,47 @@ __global__ void __launch_bounds__(GC_THREADS) grad_norm_kernel(const double* par
   if (threadIdx.x == 0) *norm = n;
 }
 
-template <typename TO, int V>
-__device__ __forceinline__ void store_v(TO* p, const float* v) {
-  if constexpr (sizeof(TO) == 4) {
-#pragma unroll
-    for (int e = 0; e < V; e += 4)
-      __stcs(reinterpret_cast<float4*>(p + e), make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]));
-  } else if constexpr (V == 8) {
-    __stcs(reinterpret_cast<uint4*>(p), make_uint4(pack_t2<TO>(v[0], v[1]), pack_t2<TO>(v[2], v[3]),
-                                                   pack_t2<TO>(v[4], v[5]), pack_t2<TO>(v[6], v[7])));
-  } else {
-    __stcs(reinterpret_cast<uint2*>(p), make_uint2(pack_t2<TO>(v[0], v[1]), pack_t2<TO>(v[2], v[3])));
-  }
-}
+// V consecutive values as one access of 8 or 16 bytes
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Vec {
+  T e[V];
+};
 
 template <typename T, typename TO>
-__device__ __forceinline__ void chunk_scale(const T* p, TO* o, int n, float factor) {
-  constexpr int V = 16 / sizeof(T);
-  int done = 0;
+__device__ __forceinline__ void span_scale(const T* p, TO* o, int64_t n, float factor) {
+  // 16 bytes of the wider type per access, so that a warp's stores are whole lines: with 16 bytes of
+  // 16-bit gradients a thread's 32 bytes of fp32 went out as two half-filled sets of sectors
+  constexpr int V = 16 / (sizeof(T) > sizeof(TO) ? sizeof(T) : sizeof(TO));
+  int64_t done = 0;
   if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
-    const uint4* v = reinterpret_cast<const uint4*>(p);
-    const int nv = n / V;
-    auto put = [&](const uint4& u, int at) {
-      const T* h = reinterpret_cast<const T*>(&u);
-      float f[V];
+    const Vec<T, V>* v = reinterpret_cast<const Vec<T, V>*>(p);
+    Vec<TO, V>* w = reinterpret_cast<Vec<TO, V>*>(o);
+    const int64_t nv = n / V;
+    auto put = [&](const Vec<T, V>& u, int64_t at) {
+      Vec<TO, V> r;
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = to_f<T>(h[e]) * factor;
-      store_v<TO, V>(o + at * V, f);
+      for (int e = 0; e < V; ++e) r.e[e] = from_f<TO>(to_f<T>(u.e[e]) * factor);
+      w[at] = r;
     };
-    int i = threadIdx.x;
+    int64_t i = threadIdx.x;
     for (; i + 7 * GC_THREADS < nv; i += 8 * GC_THREADS) {
-      uint4 u[8];
+      Vec<T, V> u[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) u[k] = __ldcs(v + i + k * GC_THREADS);
+      for (int k = 0; k < 8; ++k) u[k] = v[i + k * GC_THREADS];
 #pragma unroll
       for (int k = 0; k < 8; ++k) put(u[k], i + k * GC_THREADS);
     }
-    for (; i < nv; i += GC_THREADS) put(__ldcs(v + i), i);
+    for (; i < nv; i += GC_THREADS) put(v[i], i);
     done = nv * V;
   }
-#pragma unroll 4
-  for (int i = done + threadIdx.x; i < n; i += GC_THREADS) o[i] = from_f<TO>(to_f<T>(p[i]) * factor);
+#pragma unroll 8
+  for (int64_t i = done + threadIdx.x; i < n; i += GC_THREADS) o[i] = from_f<TO>(to_f<T>(p[i]) * factor);
 }
 template <typename T>
-__device__ __forceinline__ void chunk_scale_to(const T* p, void* o, int out_dtype, int64_t at, int n, float factor) {
-  if (out_dtype == QL_F32) chunk_scale(p, static_cast<float*>(o) + at, n, factor);
-  else if (out_dtype == QL_F16) chunk_scale(p, static_cast<__half*>(o) + at, n, factor);
-  else chunk_scale(p, static_cast<__nv_bfloat16*>(o) + at, n, factor);
+__device__ __forceinline__ void span_scale_to(const T* p, void* o, int out_dtype, int64_t at, int64_t n, float factor) {
+  if (out_dtype == QL_F32) span_scale(p, static_cast<float*>(o) + at, n, factor);
+  else if (out_dtype == QL_F16) span_scale(p, static_cast<__half*>(o) + at, n, factor);
+  else span_scale(p, static_cast<__nv_bfloat16*>(o) + at, n, factor);
 }
 
 template <int MAX>
@@ -202,17 +226,13 @@ __global__ void __launch_bounds__(GC_THREADS, GC_CTAS_PER_SM) grad_scale_kernel(
   const float ratio = max_norm / (total + 1e-6f);
   const float factor = (ratio > 1.f ? 1.f : ratio) * inv_scale;  // a NaN stays one
   if (in_place && factor == 1.f) return;                         // every gradient stays as it is
-  const int chunks = l.first[l.count];
-  for (int c = chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
-    const int t = tensor_of(l, c), dt = l.dtype[t], per = chunk_elems(dt);
-    const int64_t at = (int64_t)(c - l.first[t]) * per;
-    const int n = (int)min((int64_t)per, l.n[t] - at);
-    if (dt == QL_F32) chunk_scale_to(static_cast<const float*>(l.grad[t]) + at, l.out[t], l.out_dtype[t], at, n, factor);
-    else if (dt == QL_F16) chunk_scale_to(static_cast<const __half*>(l.grad[t]) + at, l.out[t], l.out_dtype[t], at, n, factor);
-    else chunk_scale_to(static_cast<const __nv_bfloat16*>(l.grad[t]) + at, l.out[t], l.out_dtype[t], at, n, factor);
-  }
+  walk(l, [&](int t, int64_t at, int64_t n) {
+    const int dt = l.dtype[t], odt = l.out_dtype[t];
+    if (dt == QL_F32) span_scale_to(static_cast<const float*>(l.grad[t]) + at, l.out[t], odt, at, n, factor);
+    else if (dt == QL_F16) span_scale_to(static_cast<const __half*>(l.grad[t]) + at, l.out[t], odt, at, n, factor);
+    else span_scale_to(static_cast<const __nv_bfloat16*>(l.grad[t]) + at, l.out[t], odt, at, n, factor);
+  });
 }
-
 constexpr int GC_SMALL = 128, GC_MAX = 1024;
 
 int elem_bytes(int dtype) { return dtype == QL_F32 ? 4 : 2; }

@@ -3,7 +3,7 @@
 // is the table's at row pos[axis(f)][t], so a text token (all positions equal) rotates as in
 // rope.cu and a picture's tokens by their row and column.
 //
-// A tile is 16 MT tokens. The tile's cosines and sines are gathered once into shared memory (a
+// A tile is 16 tokens (8 in the backward of short batches). The tile's cosines and sines are gathered once into shared memory (a
 // gather of single floats where neighbouring frequencies belong to different axes) and serve every
 // head. Then each warp takes units of 32 columns of a head together with their 32 partners
 // D / 2 further on. The LoRA-B product of a unit is formed on the tensor cores in the layout the data
@@ -56,6 +56,7 @@ struct MropeArgs {
 // cos / sin of the tile's tokens, [rows][half + 4] floats each
 __device__ __forceinline__ void stage_angles(const MropeArgs& a, float* sc, float* ss, int tok0, int rows) {
   const int half = a.D / 2, pitch = half + 4;
+#pragma unroll 4
   for (int i = threadIdx.x; i < rows * half; i += blockDim.x) {
     const int r = i / half, f = i % half, tok = tok0 + r;
     float c = 0.f, s = 0.f;
@@ -73,16 +74,39 @@ __device__ __forceinline__ void stage_angles(const MropeArgs& a, float* sc, floa
   }
 }
 
+// 8 consecutive values of a row, as loaded and as floats
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* v) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
-    const T* h = reinterpret_cast<const T*>(&u);
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* p) {
+  Raw8<T> r;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f<T>(h[j]);
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t u) {
+  if constexpr (std::is_same<T, __half>::value) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+  } else {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void floats8(const Raw8<T>& r, float* v) {
+  const uint32_t* u = reinterpret_cast<const uint32_t*>(&r);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(u[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack2<T>(u[j]);
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
   }
 }
 template <typename T>
@@ -91,136 +115,125 @@ __device__ __forceinline__ void store8(T* p, const float* v) {
                                             pack_t2<T>(v[4], v[5]), pack_t2<T>(v[6], v[7]));
 }
 
-// acc[m][rh][8] += x_lo . B^T for the 32 outputs from row o0 of B on: this thread's eight columns
-// 8 t .. 8 t + 7 of tokens g and g + 8 of each 16-token tile m
-template <typename T, int MT>
-__device__ __forceinline__ void lora_out(const uint32_t (*af)[4], const void* B, int64_t o0, float s,
-                                         float (*acc)[2][8]) {
+// acc[rh][8] += s x_lo . B^T for the 32 outputs from row o0 of B on: this thread's eight columns
+// 8 t .. 8 t + 7 of tokens g and g + 8 of the tile
+template <typename T>
+__device__ __forceinline__ void lora_out(const uint32_t* af, const void* B, int64_t o0, float s, float (*acc)[8]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t* base = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(B) +
-                         (o0 + (g >> 1) * 8 + (g & 1)) * MR_RANK);
-  uint32_t b0[4], b1[4];
+  // step j: column n of the step is output 8 (n / 2) + 2 j + n % 2; the K indices of thread t
+  // (2 t, 2 t + 1, 2 t + 8, 2 t + 9) are ranks 4 t .. 4 t + 3, in both operands
+  const uint2* base = reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(B) +
+                      (o0 + (g >> 1) * 8 + (g & 1)) * MR_RANK) + t;
+  uint2 b[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {  // step j: column n of the step is output 8 (n / 2) + 2 j + n % 2
-    b0[j] = __ldg(base + j * MR_RANK + t);
-    b1[j] = __ldg(base + j * MR_RANK + 4 + t);
+  for (int j = 0; j < 4; ++j) b[j] = __ldg(base + j * (2 * MR_RANK / 4));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
+    mma16816<T>(c, af, b[j].x, b[j].y);
+    acc[0][2 * j] += c[0] * s;
+    acc[0][2 * j + 1] += c[1] * s;
+    acc[1][2 * j] += c[2] * s;
+    acc[1][2 * j + 1] += c[3] * s;
   }
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
-      mma16816<T>(c, af[m], b0[j], b1[j]);
-      acc[m][0][2 * j] += c[0] * s;
-      acc[m][0][2 * j + 1] += c[1] * s;
-      acc[m][1][2 * j] += c[2] * s;
-      acc[m][1][2 * j + 1] += c[3] * s;
-    }
 }
 
-// A fragments of x_lo [n, 16] for the tile's tokens
-template <typename T, int MT>
-__device__ __forceinline__ void lora_in(const void* x, int tok0, int n, uint32_t (*af)[4]) {
+// A fragment of x_lo [n, 16] for the tile's tokens
+template <typename T>
+__device__ __forceinline__ void lora_in(const void* x, int tok0, int rows, int n, uint32_t* af) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int rh = 0; rh < 2; ++rh) {
-      const int tok = tok0 + m * 16 + g + rh * 8;
-      uint32_t lo = 0, hi = 0;
-      if (tok < n) {
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(x) + (int64_t)tok * MR_RANK);
-        lo = __ldg(p + t);
-        hi = __ldg(p + 4 + t);
-      }
-      af[m][rh] = lo;
-      af[m][2 + rh] = hi;
-    }
+  for (int rh = 0; rh < 2; ++rh) {
+    const int r = g + rh * 8, tok = tok0 + r;
+    uint2 v = make_uint2(0u, 0u);
+    if (r < rows && tok < n)
+      v = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(x) + (int64_t)tok * MR_RANK) + t);
+    af[rh] = v.x;
+    af[2 + rh] = v.y;
+  }
 }
 
-// ROWS tokens per tile: 8 (half of an m16 tile, for short batches) or 16 MT
-template <typename T, int MT, int ROWS>
-__global__ void __launch_bounds__(256) mrope_fwd_kernel(const __grid_constant__ MropeArgs a) {
+// (o1, o2) = (x1 c -+ x2 s, x2 c +- x1 s) with the row's angles from shared memory; BACK: the inverse
+template <bool BACK>
+__device__ __forceinline__ void turn8(float* x1, float* x2, const float* cr, const float* sr) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const float4 c4 = reinterpret_cast<const float4*>(cr)[q], s4 = reinterpret_cast<const float4*>(sr)[q];
+    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p = x1[4 * q + e], r = x2[4 * q + e];
+      x1[4 * q + e] = BACK ? p * c[e] + r * s[e] : p * c[e] - r * s[e];
+      x2[4 * q + e] = BACK ? r * c[e] - p * s[e] : r * c[e] + p * s[e];
+    }
+  }
+}
+
+// A unit: 32 columns of one head and their 32 partners; v's heads come after the rotated ones.
+struct Unit {
+  int head, d0;  // head of the [q | k | v] row, first column
+};
+__device__ __forceinline__ Unit unit_of(int u, int per_head) { return {u / per_head, (u % per_head) * MR_UNIT}; }
+
+constexpr int MR_THREADS = 256, MR_CTAS = 3;  // 24 warps per SM at 80 registers (16 at 110: 136 us
+                                              // against 113 for 24 k tokens of 28 + 8 heads)
+
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(MR_THREADS, MR_CTAS) mrope_fwd_kernel(const __grid_constant__ MropeArgs a) {
   pdl_enter();
   extern __shared__ __align__(16) float angle_smem[];
   const int half = a.D / 2, pitch = half + 4;
   float* sc = angle_smem;
   float* ss = angle_smem + ROWS * pitch;
   const int tok0 = blockIdx.x * ROWS;
-  stage_angles(a, sc, ss, tok0, ROWS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint32_t aq[MT][4], av[MT][4];
-  if (a.xq != nullptr) lora_in<T, MT>(a.xq, tok0, a.n, aq);
-  if (a.xv != nullptr) lora_in<T, MT>(a.xv, tok0, a.n, av);
-  __syncthreads();
-  const int per_head = half / MR_UNIT;
-  const int rot = (a.HQ + a.HKV) * per_head, units = rot + a.HKV * per_head;
+  const int per_head = half / MR_UNIT, units = (a.HQ + 2 * a.HKV) * per_head;
   const int64_t C = (int64_t)(a.HQ + 2 * a.HKV) * a.D;
+  stage_angles(a, sc, ss, tok0, ROWS);
+  uint32_t aq[4], av[4];
+  if (a.xq != nullptr) lora_in<T>(a.xq, tok0, ROWS, a.n, aq);
+  if (a.xv != nullptr) lora_in<T>(a.xv, tok0, ROWS, a.n, av);
+  __syncthreads();
   const int step = gridDim.y * (blockDim.x >> 5);
   for (int u = blockIdx.y * (blockDim.x >> 5) + warp; u < units; u += step) {
-    const bool is_rot = u < rot;
-    const int hh = is_rot ? u / per_head : a.HQ + a.HKV + (u - rot) / per_head;  // head of the qkv row
-    const int d0 = (u % per_head) * MR_UNIT, d = d0 + t * 8;
-    float x1[MT][2][8], x2[MT][2][8];
+    const Unit un = unit_of(u, per_head);
+    const int d = un.d0 + t * 8;
+    const bool is_q = un.head < a.HQ, is_v = un.head >= a.HQ + a.HKV;
+    Raw8<T> raw[2][2];  // [row g / g + 8][first / partner]
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int rh = 0; rh < 2; ++rh) {
-        const int r = m * 16 + g + rh * 8, tok = tok0 + r;
-        if (r < ROWS && tok < a.n) {
-          const T* row = reinterpret_cast<const T*>(a.qkv) + tok * C + hh * a.D + d;
-          load8<T>(row, x1[m][rh]);
-          load8<T>(row + half, x2[m][rh]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x1[m][rh][e] = x2[m][rh][e] = 0.f;
-        }
-      }
-    const bool is_q = hh < a.HQ;
-    if (is_q ? a.xq != nullptr : (!is_rot && a.xv != nullptr)) {
-      const void* B = is_q ? a.Bq : a.Bv;
-      const int64_t o = (int64_t)(is_q ? hh : hh - a.HQ - a.HKV) * a.D + d0;
-      if (is_q) {
-        lora_out<T, MT>(aq, B, o, a.lora_scale, x1);
-        lora_out<T, MT>(aq, B, o + half, a.lora_scale, x2);
-      } else {
-        lora_out<T, MT>(av, B, o, a.lora_scale, x1);
-        lora_out<T, MT>(av, B, o + half, a.lora_scale, x2);
-      }
+    for (int rh = 0; rh < 2; ++rh) {
+      const int r = g + rh * 8, tok = tok0 + r;
+      const T* row = reinterpret_cast<const T*>(a.qkv) + tok * C + un.head * a.D + d;
+      raw[rh][0] = r < ROWS && tok < a.n ? load8<T>(row) : Raw8<T>{};
+      raw[rh][1] = r < ROWS && tok < a.n ? load8<T>(row + half) : Raw8<T>{};
     }
-    T* dst = is_q ? reinterpret_cast<T*>(a.q) + hh * a.D
-                  : is_rot ? reinterpret_cast<T*>(a.k) + (hh - a.HQ) * a.D
-                           : reinterpret_cast<T*>(a.v) + (hh - a.HQ - a.HKV) * a.D;
+    float x1[2][8], x2[2][8];
+#pragma unroll
+    for (int rh = 0; rh < 2; ++rh) {
+      floats8<T>(raw[rh][0], x1[rh]);
+      floats8<T>(raw[rh][1], x2[rh]);
+    }
+    if (is_q && a.xq != nullptr) {
+      const int64_t o = (int64_t)un.head * a.D + un.d0;
+      lora_out<T>(aq, a.Bq, o, a.lora_scale, x1);
+      lora_out<T>(aq, a.Bq, o + half, a.lora_scale, x2);
+    } else if (is_v && a.xv != nullptr) {
+      const int64_t o = (int64_t)(un.head - a.HQ - a.HKV) * a.D + un.d0;
+      lora_out<T>(av, a.Bv, o, a.lora_scale, x1);
+      lora_out<T>(av, a.Bv, o + half, a.lora_scale, x2);
+    }
+    T* dst = is_q ? reinterpret_cast<T*>(a.q) + un.head * a.D
+                  : is_v ? reinterpret_cast<T*>(a.v) + (un.head - a.HQ - a.HKV) * a.D
+                         : reinterpret_cast<T*>(a.k) + (un.head - a.HQ) * a.D;
     const int64_t ld = (int64_t)(is_q ? a.HQ : a.HKV) * a.D;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int rh = 0; rh < 2; ++rh) {
-        const int r = m * 16 + g + rh * 8, tok = tok0 + r;
-        if (r >= ROWS || tok >= a.n) continue;
-        float o1[8], o2[8];
-        if (is_rot) {
-          const float4* cp = reinterpret_cast<const float4*>(sc + r * pitch + d);
-          const float4* sp = reinterpret_cast<const float4*>(ss + r * pitch + d);
-          const float4 ca = cp[0], cb = cp[1], sa = sp[0], sb = sp[1];
-          const float c[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
-          const float s[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            o1[e] = x1[m][rh][e] * c[e] - x2[m][rh][e] * s[e];
-            o2[e] = x2[m][rh][e] * c[e] + x1[m][rh][e] * s[e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            o1[e] = x1[m][rh][e];
-            o2[e] = x2[m][rh][e];
-          }
-        }
-        T* out = dst + tok * ld + d;
-        store8<T>(out, o1);
-        store8<T>(out + half, o2);
-      }
+    for (int rh = 0; rh < 2; ++rh) {
+      const int r = g + rh * 8, tok = tok0 + r;
+      if (r >= ROWS || tok >= a.n) continue;
+      if (!is_v) turn8<false>(x1[rh], x2[rh], sc + r * pitch + d, ss + r * pitch + d);
+      store8<T>(dst + tok * ld + d, x1[rh]);
+      store8<T>(dst + tok * ld + d + half, x2[rh]);
+    }
   }
 }
 
@@ -251,10 +264,11 @@ __device__ __forceinline__ void lora_back(const float (*gv)[8], const void* B, i
       for (int rh = 0; rh < 2; ++rh)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float p = left[rh][2 * k], q = left[rh][2 * k + 1];
-          af[rh + 2 * k] = pack_t2<T>(p, q);
-          left[rh][2 * k] = p - to_f<T>(from_f<T>(p));
-          left[rh][2 * k + 1] = q - to_f<T>(from_f<T>(q));
+          const uint32_t h = pack_t2<T>(left[rh][2 * k], left[rh][2 * k + 1]);
+          const float2 f = unpack2<T>(h);
+          af[rh + 2 * k] = h;
+          left[rh][2 * k] -= f.x;
+          left[rh][2 * k + 1] -= f.y;
         }
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
@@ -266,74 +280,59 @@ __device__ __forceinline__ void lora_back(const float (*gv)[8], const void* B, i
 }
 
 template <typename T, typename TG, int ROWS>
-__global__ void __launch_bounds__(256) mrope_bwd_kernel(const __grid_constant__ MropeArgs a) {
+__global__ void __launch_bounds__(MR_THREADS, MR_CTAS) mrope_bwd_kernel(const __grid_constant__ MropeArgs a) {
   pdl_enter();
   extern __shared__ __align__(16) float angle_smem[];
   const int half = a.D / 2, pitch = half + 4;
   float* sc = angle_smem;
   float* ss = angle_smem + ROWS * pitch;
   const int tok0 = blockIdx.x * ROWS;
-  stage_angles(a, sc, ss, tok0, ROWS);
-  __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int warps = blockDim.x >> 5;
-  const int per_head = half / MR_UNIT;
-  const int rot = (a.HQ + a.HKV) * per_head, units = rot + a.HKV * per_head;
+  const int per_head = half / MR_UNIT, units = (a.HQ + 2 * a.HKV) * per_head;
   const int64_t C = (int64_t)(a.HQ + 2 * a.HKV) * a.D;
+  stage_angles(a, sc, ss, tok0, ROWS);
+  __syncthreads();
   const bool lq = a.dxlo_q != nullptr, lv = a.dxlo_v != nullptr;
   float cq[2][4] = {}, cv[2][4] = {};
   for (int u = blockIdx.y * warps + warp; u < units; u += gridDim.y * warps) {
-    const bool is_rot = u < rot;
-    const int hh = is_rot ? u / per_head : a.HQ + a.HKV + (u - rot) / per_head;
-    const int d0 = (u % per_head) * MR_UNIT, d = d0 + t * 8;
-    const bool is_q = hh < a.HQ;
-    const TG* src = is_q ? reinterpret_cast<const TG*>(a.dq) + hh * a.D
-                         : is_rot ? reinterpret_cast<const TG*>(a.dk) + (hh - a.HQ) * a.D
-                                  : reinterpret_cast<const TG*>(a.dv) + (hh - a.HQ - a.HKV) * a.D;
+    const Unit un = unit_of(u, per_head);
+    const int d = un.d0 + t * 8;
+    const bool is_q = un.head < a.HQ, is_v = un.head >= a.HQ + a.HKV;
+    const TG* src = is_q ? reinterpret_cast<const TG*>(a.dq) + un.head * a.D
+                         : is_v ? reinterpret_cast<const TG*>(a.dv) + (un.head - a.HQ - a.HKV) * a.D
+                                : reinterpret_cast<const TG*>(a.dk) + (un.head - a.HQ) * a.D;
     const int64_t ld = (int64_t)(is_q ? a.HQ : a.HKV) * a.D;
-    float x1[2][8], x2[2][8];
+    Raw8<TG> raw[2][2];
 #pragma unroll
     for (int rh = 0; rh < 2; ++rh) {
       const int r = g + rh * 8, tok = tok0 + r;
-      if (r < ROWS && tok < a.n) {
-        load8<TG>(src + tok * ld + d, x1[rh]);
-        load8<TG>(src + tok * ld + d + half, x2[rh]);
-      } else {
+      raw[rh][0] = r < ROWS && tok < a.n ? load8<TG>(src + tok * ld + d) : Raw8<TG>{};
+      raw[rh][1] = r < ROWS && tok < a.n ? load8<TG>(src + tok * ld + d + half) : Raw8<TG>{};
+    }
+    float x1[2][8], x2[2][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x1[rh][e] = x2[rh][e] = 0.f;
-      }
+    for (int rh = 0; rh < 2; ++rh) {
+      floats8<TG>(raw[rh][0], x1[rh]);
+      floats8<TG>(raw[rh][1], x2[rh]);
     }
 #pragma unroll
     for (int rh = 0; rh < 2; ++rh) {
       const int r = g + rh * 8, tok = tok0 + r;
       if (r >= ROWS || tok >= a.n) continue;
-      if (is_rot) {
-        const float4* cp = reinterpret_cast<const float4*>(sc + r * pitch + d);
-        const float4* sp = reinterpret_cast<const float4*>(ss + r * pitch + d);
-        const float4 ca = cp[0], cb = cp[1], sa = sp[0], sb = sp[1];
-        const float c[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
-        const float s[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = x1[rh][e], q = x2[rh][e];
-          x1[rh][e] = p * c[e] + q * s[e];
-          x2[rh][e] = q * c[e] - p * s[e];
-        }
-      }
-      T* out = reinterpret_cast<T*>(a.dqkv) + tok * C + hh * a.D + d;
+      if (!is_v) turn8<true>(x1[rh], x2[rh], sc + r * pitch + d, ss + r * pitch + d);
+      T* out = reinterpret_cast<T*>(a.dqkv) + tok * C + un.head * a.D + d;
       store8<T>(out, x1[rh]);
       store8<T>(out + half, x2[rh]);
     }
-    if (is_q ? lq : (!is_rot && lv)) {
-      const void* B = is_q ? a.Bq : a.Bv;
-      const int64_t o = (int64_t)(is_q ? hh : hh - a.HQ - a.HKV) * a.D + d0;
-      if (is_q) {
-        lora_back<T>(x1, B, o, cq);
-        lora_back<T>(x2, B, o + half, cq);
-      } else {
-        lora_back<T>(x1, B, o, cv);
-        lora_back<T>(x2, B, o + half, cv);
-      }
+    if (is_q && lq) {
+      const int64_t o = (int64_t)un.head * a.D + un.d0;
+      lora_back<T>(x1, a.Bq, o, cq);
+      lora_back<T>(x2, a.Bq, o + half, cq);
+    } else if (is_v && lv) {
+      const int64_t o = (int64_t)(un.head - a.HQ - a.HKV) * a.D + un.d0;
+      lora_back<T>(x1, a.Bv, o, cv);
+      lora_back<T>(x2, a.Bv, o + half, cv);
     }
   }
   if (!lq && !lv) return;
@@ -424,7 +423,7 @@ int mrope_fwd(const ql_mrope_args& m, cudaStream_t s) {
   if (m.n == 0) return QL_STATUS_OK;
   if (m.qkv == nullptr || m.q == nullptr || m.k == nullptr || m.v == nullptr ||
       (m.xq != nullptr && m.Bq == nullptr) || (m.xv != nullptr && m.Bv == nullptr) ||
-      misaligned({m.qkv, m.q, m.k, m.v}, 16) || misaligned({m.xq, m.xv, m.Bq, m.Bv}, 4))
+      misaligned({m.qkv, m.q, m.k, m.v}, 16) || misaligned({m.xq, m.xv, m.Bq, m.Bv}, 8))
     return QL_STATUS_BAD_ARG;
   a.qkv = m.qkv;
   a.xq = m.xq;
@@ -435,21 +434,14 @@ int mrope_fwd(const ql_mrope_args& m, cudaStream_t s) {
   const double elems = (double)m.n * (m.HQ + 2 * m.HKV) * m.D;
   ProfScope prof(PK_ROPE_FWD, 0, elems * 4, s);
   const int units = (m.HQ + 2 * m.HKV) * (m.D / 2 / MR_UNIT);
-  const int warps = units < 8 ? units : 8;
-#define QL_MROPEF(TT, MT, ROWS)                                                                   \
-  do {                                                                                            \
-    const int tiles = (int)cdiv(m.n, ROWS);                                                       \
-    int gy = (int)cdiv(2 * sm_count(), tiles); /* short batches: the columns over several CTAs */ \
-    const int most = (int)cdiv(units, warps);                                                     \
-    gy = gy < 1 ? 1 : gy > most ? most : gy;                                                      \
-    launch_k(mrope_fwd_kernel<TT, MT, ROWS>, dim3(tiles, gy), dim3(32 * warps),                   \
-             2 * ROWS * (m.D / 2 + 4) * 4, s, a);                                                 \
-  } while (0)
-  if (m.n > 32 * 4 * sm_count()) {
-    if (m.dtype == QL_F16) QL_MROPEF(__half, 2, 32); else QL_MROPEF(__nv_bfloat16, 2, 32);
-  } else {
-    if (m.dtype == QL_F16) QL_MROPEF(__half, 1, 16); else QL_MROPEF(__nv_bfloat16, 1, 16);
-  }
+  const int warps = units < MR_THREADS / 32 ? units : MR_THREADS / 32;
+  const int tiles = (int)cdiv(m.n, 16);
+  const int most = (int)cdiv(units, warps);
+  int gy = (int)cdiv(2 * sm_count(), tiles);  // short batches: the columns over several CTAs
+  gy = gy > most ? most : gy;
+#define QL_MROPEF(TT)                                                                       \
+  launch_k(mrope_fwd_kernel<TT, 16>, dim3(tiles, gy), dim3(32 * warps), 2 * 16 * (m.D / 2 + 4) * 4, s, a)
+  if (m.dtype == QL_F16) QL_MROPEF(__half); else QL_MROPEF(__nv_bfloat16);
 #undef QL_MROPEF
   return launched(1);
 }
@@ -462,7 +454,7 @@ int mrope_bwd(const ql_mrope_args& m, cudaStream_t s) {
   if (m.n == 0) return QL_STATUS_OK;
   if (m.dq == nullptr || m.dk == nullptr || m.dv == nullptr || m.dqkv == nullptr ||
       (m.dxlo_q != nullptr && m.Bq == nullptr) || (m.dxlo_v != nullptr && m.Bv == nullptr) ||
-      misaligned({m.dq, m.dk, m.dv, m.dqkv}, 16) || misaligned({m.Bq, m.Bv}, 4))
+      misaligned({m.dq, m.dk, m.dv, m.dqkv}, 16) || misaligned({m.Bq, m.Bv}, 8))
     return QL_STATUS_BAD_ARG;
   a.dq = m.dq;
   a.dk = m.dk;
@@ -474,7 +466,7 @@ int mrope_bwd(const ql_mrope_args& m, cudaStream_t s) {
   const double elems = (double)m.n * (m.HQ + 2 * m.HKV) * m.D;
   ProfScope prof(PK_ROPE_BWD, 0, elems * (m.grad_dtype == QL_F32 ? 6 : 4), s);
   const int units = (m.HQ + 2 * m.HKV) * (m.D / 2 / MR_UNIT);
-  const int warps = units < 8 ? units : 8;
+  const int warps = units < MR_THREADS / 32 ? units : MR_THREADS / 32;
 #define QL_MROPEB(TT, TG, ROWS)                                                                   \
   do {                                                                                            \
     const int tiles = (int)cdiv(m.n, ROWS);                                                       \
