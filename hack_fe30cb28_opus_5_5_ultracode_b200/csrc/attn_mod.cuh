@@ -219,13 +219,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
-      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -297,20 +290,13 @@ __device__ __forceinline__ void umma_gather2(uint32_t d, uint32_t a, uint32_t b_
                  QL_AM_TS("16", "256") QL_AM_TS("24", "384") QL_AM_TS("80", "768") QL_AM_TS("88", "896") "}"
                  ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
 }
-// four parts of 16 columns, 32 apart (four softmax threads per row); HALF 0: the first 16 rows of each
-// 32 of B's, HALF 1: the second
-template <int HALF>
+// four parts of 16 columns, 32 apart (four softmax threads per row)
 __device__ __forceinline__ void umma_gather4(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t more) {
-  if constexpr (HALF == 0)
-    asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
-                 "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
-                 QL_AM_TS("0", "0") QL_AM_TS("32", "256") QL_AM_TS("64", "512") QL_AM_TS("96", "768") "}"
-                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
-  else
-    asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
-                 "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
-                 QL_AM_TS("8", "128") QL_AM_TS("40", "384") QL_AM_TS("72", "640") QL_AM_TS("104", "896") "}"
-                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
+  asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
+               "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+               QL_AM_TS("0", "0") QL_AM_TS("8", "128") QL_AM_TS("32", "256") QL_AM_TS("40", "384")
+               QL_AM_TS("64", "512") QL_AM_TS("72", "640") QL_AM_TS("96", "768") QL_AM_TS("104", "896") "}"
+               ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
 }
 #undef QL_AM_TS
 

@@ -13,11 +13,12 @@
 //             X    Y    U    W    S         dP          acc1        acc2
 //   dQ        Q    dO   K    V    Q K^T     dO V^T      P K         dS K
 //   dK, dV    K    V    Q    dO   K Q^T     V dO^T      P^T dO      dS^T Q
-// While the softmax warps form P the tensor core does the last step's acc2 and this one's dP; while
-// they form dS it does acc1 and the next step's S. P and dS go back into the tensor-memory columns
-// their scores came from, as 16-bit values, and are the A operand of the next product. Sixteen softmax
-// warps, four threads per TMEM lane with 32 of the 128 columns each (no row reduction: the forward's
-// lse is known); with eight warps of 64 columns the SMs issued in 17-23 % of the cycles.
+// S is read into registers at once, so the next step's S is formed while this one's P is; P and dS go,
+// as 16-bit values, into the tensor-memory columns that dP leaves when it has been read (each thread
+// 16 + 16 of its own 32 columns) and are the A operand of acc1 and acc2. The tensor core's acc1, acc2
+// and next dP then run beside the next step's P. (With P in S's columns the next S had to wait for
+// acc1: 650 us instead of BWD_AFTER for 8,192 causal tokens of 12 + 2 heads.) Sixteen softmax warps, four
+// threads per TMEM lane with 32 of the 128 columns each (no row reduction: the forward's lse is known).
 //
 // Why the dQ role needs P K: Dvec from the forward's 16-bit output is off by the output's rounding,
 // and that error enters a whole row of dS with one sign - dQ was up to 1.9 times as far from the
@@ -41,8 +42,9 @@ struct BwdConst {
   float sl2, u, cap2, slope2;
 };
 
-// 16 raw scores of one TMEM lane into probabilities (16-bit pairs of what acc1 takes: p16) and into
-// the factors of dS (f, in place of x): probabilities times the cap's derivative. poly: every |score|
+// 16 raw scores of one TMEM lane into the factors of dS (f, in place of x): probabilities times the
+// cap's derivative. p16: the probabilities themselves as 16-bit pairs, where they are not f (a capped
+// score of the dK / dV role). poly: every |score|
 // of the warp is inside tanh_poly2's range. neg_lse: -lse2 by column (PER_COL, from shared memory) or
 // one value. Masked columns [0, lo) and [hi, 16) give 0. dist0: row index minus the first column's, for
 // the distance bias. p: plain probabilities where the caller needs them beside f (a capped score of
@@ -106,15 +108,15 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
       // a masked score may be anything, infinities and NaN too: its factor is 0
       if (MASKED && pa == 0.f) fa = 0.f;
       if (MASKED && pb == 0.f) fb = 0.f;
-      if constexpr (!PER_COL) {
+      if constexpr (PER_COL) {
+        p16[e] = __uint_as_float(pack_t2<T>(pa, pb));
+      } else {
         p[k] = pa;
         p[k + 1] = pb;
       }
     }
     x[k] = __float_as_uint(fa);
     x[k + 1] = __float_as_uint(fb);
-    // acc1: dV takes P itself, the dQ role's correction what dS is made of
-    p16[e] = __uint_as_float(PER_COL ? pack_t2<T>(pa, pb) : pack_t2<T>(fa, fb));
   }
 }
 
@@ -204,7 +206,7 @@ struct BwdCfg {
 // blocks of every KV head, times a.splits CTAs that share its query heads.
 // fp16, dK / dV: P is kept as 2^8 P (at most 2^8 where P is 1), so that the small probabilities of
 // long rows stay normal numbers; dS and dV take the factor back in fp32.
-// TMEM: S [0, 128), dP [128, 256), acc1 [256, 256 + D), acc2 [384, 384 + D).
+// TMEM: S [0, 128), dP, then P and dS [128, 256), acc1 [256, 256 + D), acc2 [384, 384 + D).
 template <typename T, int D, int MODE, bool DKV>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
     attn_mod_bwd_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap ty,
@@ -225,7 +227,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   uint64_t* out_full = bars + 4;
   uint64_t* raw = bars + 5;
   uint64_t* drain = bars + 6;
-  uint64_t* p_full = bars + 7;   // [2] half of P written (all softmax warps)
+  uint64_t* p_full = bars + 7;   // P written, dP read (all softmax warps)
+  uint64_t* s_free = bars + 8;   // S read (all softmax warps)
   uint64_t* l_full = bars + 9;   // [2] -lse2 and -Dvec of a step stored
   uint64_t* l_empty = bars + 11; // [2] and read (all softmax warps)
   uint64_t* u_full = bars + 13;  // [UST]
@@ -239,8 +242,9 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   const int b = blockIdx.x / per_seq, part_of_seq = blockIdx.x % per_seq;
   const int kvh = DKV ? part_of_seq / a.splits : part_of_seq / group;
   const int split = DKV ? part_of_seq % a.splits : 0;
-  const int heads = DKV ? group / a.splits : 1;         // query heads this CTA runs through
-  const int h0 = DKV ? kvh * group + split * heads : part_of_seq;
+  const int g0 = DKV ? group * split / a.splits : 0;    // query heads this CTA runs through
+  const int heads = DKV ? group * (split + 1) / a.splits - g0 : 1;
+  const int h0 = DKV ? kvh * group + g0 : part_of_seq;
   // the tiles with the most work first (causal: the last queries, the first keys)
   const int r0 = (DKV ? blockIdx.y : gridDim.y - 1 - blockIdx.y) * AM_T;
   const AttnSeq seq = attn_seq(a, b);
@@ -254,11 +258,12 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     mbar_init(s_full, 1);
     mbar_init(dp_full, 1);
     mbar_init(ds_full, BWD_SOFTMAX / 32);
+    mbar_init(p_full, BWD_SOFTMAX / 32);
+    mbar_init(s_free, BWD_SOFTMAX / 32);
     mbar_init(out_full, 1);
     mbar_init(raw, 1);
     mbar_init(drain, 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&p_full[s], BWD_SOFTMAX / 32);
       mbar_init(&l_full[s], 1);
       mbar_init(&l_empty[s], BWD_SOFTMAX / 32);
     }
@@ -378,26 +383,22 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         return true;
       };
       bool ok = warp_wait(xy_full, 0, err) && score(0) && dprob(0);
+      if (ok && steps > 1) ok = warp_wait(s_free, 0, err) && score(1);
       for (int n = 0; ok && n < steps; ++n) {
         const uint32_t u0 = um + (n % C::UST) * TILE16, w0 = wm + (n % C::WST) * TILE16;
-        ok = warp_wait(&p_full[0], n & 1, err);
+        ok = warp_wait(p_full, n & 1, err);
         if (!ok) break;
         tc_fence_after();
-        umma_gather4<0>(tmem + 256, tmem, DKV ? w0 : u0, id_o, n > 0);
-        ok = warp_wait(&p_full[1], n & 1, err);
-        if (!ok) break;
-        tc_fence_after();
-        umma_gather4<1>(tmem + 256, tmem, DKV ? w0 : u0, id_o, 1);
+        umma_gather4(tmem + 256, tmem + 128, DKV ? w0 : u0, id_o, n > 0);
         if (DKV) warp_commit(&w_empty[n % C::WST]);
-        if (n + 1 < steps) ok = score(n + 1);
-        if (ok) ok = warp_wait(ds_full, n & 1, err);
+        ok = warp_wait(ds_full, n & 1, err);
         if (!ok) break;
         tc_fence_after();
-        umma_gather4<0>(tmem + 384, tmem + 128, u0, id_o, n > 0);
-        umma_gather4<1>(tmem + 384, tmem + 128, u0, id_o, 1);
+        umma_gather4(tmem + 384, tmem + 128 + HC / 2, u0, id_o, n > 0);
         warp_commit(&u_empty[n % C::UST]);
         if (n + 1 < steps) ok = dprob(n + 1);
         else warp_commit(out_full);
+        if (ok && n + 2 < steps) ok = warp_wait(s_free, (n + 1) & 1, err) && score(n + 2);
       }
       if (!ok) {  // a wait ran out: the products already issued finish before TMEM is freed
         warp_commit(drain);
@@ -453,28 +454,34 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       float w[HC / 2], p[(MODE & 1) != 0 && !DKV ? HC : 1];
       tmem_ld32_nw(ts, x);
       tmem_wait_ld();
+      tc_fence_before();
+      warp_arrive(s_free);
       bool poly = true;
       if constexpr ((MODE & 1) != 0) poly = __all_sync(0xffffffffu, abs_max<HC>(x) * c.u <= TANH_POLY_MAX);
-      // half of the columns at a time: acc1 starts on the first while the second is formed
 #pragma unroll
       for (int g = 0; g < HC; g += 16) {
         float* pg = p + ((MODE & 1) != 0 && !DKV ? g : 0);
-        if (masked) bwd_probs<T, MODE, true, DKV>(x + g, w, pg, c, poly, nl + g, neg_lse, dist0 - g, lo - g, hi - g);
-        else bwd_probs<T, MODE, false, DKV>(x + g, w, pg, c, poly, nl + g, neg_lse, dist0 - g, 0, 0);
-        tmem_st8(ts + g / 2, w);
-        tmem_wait_st();
-        tc_fence_before();
-        warp_arrive(&p_full[g / 16]);
+        if (masked) bwd_probs<T, MODE, true, DKV>(x + g, w + g / 2, pg, c, poly, nl + g, neg_lse, dist0 - g, lo - g, hi - g);
+        else bwd_probs<T, MODE, false, DKV>(x + g, w + g / 2, pg, c, poly, nl + g, neg_lse, dist0 - g, 0, 0);
       }
       ok = warp_wait(dp_full, n & 1, err);
       if (!ok) break;
       tc_fence_after();
       tmem_ld32_nw(ts + 128, dp);
       tmem_wait_ld();
+      if constexpr (!DKV || (MODE & 1) == 0) {  // acc1 takes f itself
+#pragma unroll
+        for (int e = 0; e < HC / 2; ++e)
+          w[e] = __uint_as_float(pack_t2<T>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])));
+      }
+      tmem_st16(ts + 128, w);
+      tmem_wait_st();
+      tc_fence_before();
+      warp_arrive(p_full);
       if (masked) rest += bwd_ds<T, MODE, true, DKV>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, lo, hi);
       else rest += bwd_ds<T, MODE, false, DKV>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, 0, 0);
       if (DKV) warp_arrive(&l_empty[s]);
-      tmem_st16(ts + 128, w);
+      tmem_st16(ts + 128 + HC / 2, w);
       tmem_wait_st();
       tc_fence_before();
       warp_arrive(ds_full);
@@ -561,9 +568,11 @@ __global__ void __launch_bounds__(256) attn_mod_sum_kernel(const AttnModArgs a, 
 }
 
 // How many CTAs share a KV head's query heads: as few as keep the longest CTA (a key block that
-// every query tile sees) under half of an SM's share of all tiles, because each split costs a
-// write and a read of fp32 dk and dv; a divisor of the group. (8,192 tokens, 12 / 2 heads: 3 of the
-// 6 heads per CTA.)
+// every query tile sees) under SPLIT_SHARE of an SM's share of all tiles, because each split costs a
+// write and a read of fp32 dk and dv.
+#ifndef SPLIT_SHARE
+#define SPLIT_SHARE 0.8
+#endif
 int dkv_splits(const AttnModArgs& a) {
   const int group = a.HQ / a.HKV;
   const double tiles = (double)cdiv(a.max_len, AM_T);
@@ -572,7 +581,7 @@ int dkv_splits(const AttnModArgs& a) {
   const double mean = a.causal && longest == tiles ? tiles / 2 : longest;
   const double share = (double)cdiv(a.n, AM_T) * a.HQ * mean / sm_count();
   for (int s = 1; s < group; ++s)
-    if (group % s == 0 && (group / s) * longest <= 0.5 * share) return s;
+    if (cdiv(group, s) * longest <= SPLIT_SHARE * share) return s;
   return group;
 }
 
