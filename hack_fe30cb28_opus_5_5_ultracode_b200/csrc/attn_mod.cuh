@@ -188,6 +188,38 @@ __device__ __forceinline__ void tanh_poly2(uint64_t* u) {
 #pragma unroll
   for (int i = 0; i < N; ++i) u[i] = mul2(p[i], u[i]);
 }
+// c tanh(u x) = x (k0 + k1 x^2 + k2 x^4 + k3 x^6) for |u x| <= 0.4, in place: the fit with u and c in
+// its coefficients (1.0e-7 relative), five operations a pair where tanh_poly2 with its two
+// scalings takes nine. Scores of a model trained with a cap rarely leave this range.
+constexpr float TANH_SHORT_MAX = 0.4f;
+struct TanhShort {
+  float k[4];
+};
+__device__ __forceinline__ TanhShort tanh_short(float u, float c) {
+  const float t[4] = {0.9999998807907104f, -0.33331361413002014f, 0.13270977139472961f, -0.04755359888076782f};
+  TanhShort r;
+  float m = c * u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r.k[i] = m * t[i];
+    m *= u * u;
+  }
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void tanh_short2(uint64_t* x, const TanhShort& t) {
+  uint64_t w[N], p[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = mul2(x[i], x[i]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = fma2(w[i], pk2(t.k[3], t.k[3]), pk2(t.k[2], t.k[2]));
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = fma2(p[i], w[i], pk2(t.k[1], t.k[1]));
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = fma2(p[i], w[i], pk2(t.k[0], t.k[0]));
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = mul2(p[i], x[i]);
+}
 // Largest |x| of N raw words.
 template <int N>
 __device__ __forceinline__ float abs_max(const uint32_t* x) {
@@ -198,6 +230,13 @@ __device__ __forceinline__ float abs_max(const uint32_t* x) {
     for (int k = 0; k < 4; ++k)
       m[k] = max3(m[k], fabsf(__uint_as_float(x[i + 2 * k])), fabsf(__uint_as_float(x[i + 2 * k + 1])));
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+// Which form a warp's block of scores takes: 0 tanh_short2, 1 tanh_poly2, 2 tanhf.
+template <int N>
+__device__ __forceinline__ int tanh_form(const uint32_t* x, float u) {
+  const float m = abs_max<N>(x) * u;
+  if (__all_sync(0xffffffffu, m <= TANH_SHORT_MAX)) return 0;
+  return __all_sync(0xffffffffu, m <= TANH_POLY_MAX) ? 1 : 2;
 }
 __device__ __forceinline__ uint64_t pair_of(const uint32_t* x) {
   return pk2(__uint_as_float(x[0]), __uint_as_float(x[1]));

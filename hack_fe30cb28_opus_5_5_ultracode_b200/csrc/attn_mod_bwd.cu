@@ -17,7 +17,8 @@
 // as 16-bit values, into the tensor-memory columns that dP leaves when it has been read (each thread
 // 16 + 16 of its own 32 columns) and are the A operand of acc1 and acc2. The tensor core's acc1, acc2
 // and next dP then run beside the next step's P. (With P in S's columns the next S had to wait for
-// acc1: 650 us instead of BWD_AFTER for 8,192 causal tokens of 12 + 2 heads.) Sixteen softmax warps, four
+// acc1: 650 us
+// instead of 620 for 8,192 causal tokens of 12 + 2 heads.) Sixteen softmax warps, four
 // threads per TMEM lane with 32 of the 128 columns each (no row reduction: the forward's lse is known).
 //
 // Why the dQ role needs P K: Dvec from the forward's 16-bit output is off by the output's rounding,
@@ -40,17 +41,19 @@ constexpr int HC = 32;                        // columns per softmax thread
 
 struct BwdConst {
   float sl2, u, cap2, slope2;
+  TanhShort ts;
 };
 
 // 16 raw scores of one TMEM lane into the factors of dS (f, in place of x): probabilities times the
-// cap's derivative. p16: the probabilities themselves as 16-bit pairs, where they are not f (a capped
-// score of the dK / dV role). poly: every |score|
-// of the warp is inside tanh_poly2's range. neg_lse: -lse2 by column (PER_COL, from shared memory) or
+// cap's derivative, which comes as tanh^2 - 1: f of a capped score has the other sign until the
+// gradients' last scaling. p16: the probabilities themselves as 16-bit pairs, where they are not f (a capped
+// score of the dK / dV role). form: tanh_form of the warp's
+// scores. neg_lse: -lse2 by column (PER_COL, from shared memory) or
 // one value. Masked columns [0, lo) and [hi, 16) give 0. dist0: row index minus the first column's, for
 // the distance bias. p: plain probabilities where the caller needs them beside f (a capped score of
 // the dQ role).
 template <typename T, int MODE, bool MASKED, bool PER_COL>
-__device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, const BwdConst& c, bool poly,
+__device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, const BwdConst& c, int form,
                                           const float* neg_lse, float neg_lse_row, float dist0, int lo, int hi) {
   uint64_t y[8], bend[8];
 #pragma unroll
@@ -64,7 +67,11 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
   }
   if constexpr ((MODE & 1) != 0) {
     uint64_t th[8];
-    if (poly) {
+    if (form == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) th[e] = pair_of(x + 2 * e);
+      tanh_short2<8>(th, c.ts);
+    } else if (form == 1) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) th[e] = mul2(pair_of(x + 2 * e), pk2(c.u, c.u));
       tanh_poly2<8>(th);
@@ -76,9 +83,7 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = fma2(th[e], pk2(c.cap2, c.cap2), y[e]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) bend[e] = mul2(th[e], pk2(-1.f, -1.f));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) bend[e] = fma2(bend[e], th[e], pk2(1.f, 1.f));
+    for (int e = 0; e < 8; ++e) bend[e] = fma2(th[e], th[e], pk2(-1.f, -1.f));  // tanh^2 - 1: sign below
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = fma2(pair_of(x + 2 * e), pk2(c.sl2, c.sl2), y[e]);
@@ -122,13 +127,13 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
 
 // dS = f (dP dscale - Dvec') as 16-bit pairs; neg_d: -Dvec' by column or one value. The dQ role also
 // gets sum p (dP - Dvec) of its columns.
-template <typename T, int MODE, bool MASKED, bool PER_COL>
+template <typename T, int MODE, bool MASKED, bool PER_COL, int N>
 __device__ __forceinline__ float bwd_ds(const uint32_t* f, const float* p, const uint32_t* dp, float* ds16,
                                         float dscale, const float* neg_d, float neg_d_row, int lo, int hi) {
   const uint64_t row2 = pk2(neg_d_row, neg_d_row), ds2 = pk2(dscale, dscale);
   uint64_t sum[2] = {0, 0};  // pairs of +0.f
 #pragma unroll
-  for (int i = 0; i < HC; i += 16) {
+  for (int i = 0; i < N; i += 16) {
     uint64_t g[8];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
@@ -178,6 +183,7 @@ __device__ __forceinline__ BwdConst bwd_const(const AttnModArgs& a, int h) {
   c.sl2 = a.scale * 1.4426950408889634f;
   c.u = (MODE & 1) != 0 ? a.scale / a.softcap : 0.f;
   c.cap2 = a.softcap * 1.4426950408889634f;
+  if constexpr ((MODE & 1) != 0) c.ts = tanh_short(c.u, 1.f);
   c.slope2 = (MODE & 2) != 0 ? a.slopes[h] * 1.4426950408889634f : 0.f;
   return c;
 }
@@ -214,6 +220,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                         const AttnModArgs a, int* err) {
   using C = BwdCfg<D>;
   constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr float SIGN = (MODE & 1) != 0 ? -1.f : 1.f;  // of f, see bwd_probs
   constexpr float P_SHIFT = !DKV || IS_BF16 ? 0.f : 8.f, P_BACK = !DKV || IS_BF16 ? 1.f : 1.f / 256.f;
   pdl_enter();
   extern __shared__ __align__(1024) uint8_t smem[];  // no static shared memory: the base is aligned
@@ -450,40 +457,63 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       if (!ok) break;
       tc_fence_after();
       const float* nl = sL + s * 2 * AM_T + part * HC;
-      uint32_t x[HC], dp[HC];
+      uint32_t x[HC];
       float w[HC / 2], p[(MODE & 1) != 0 && !DKV ? HC : 1];
       tmem_ld32_nw(ts, x);
       tmem_wait_ld();
       tc_fence_before();
       warp_arrive(s_free);
-      bool poly = true;
-      if constexpr ((MODE & 1) != 0) poly = __all_sync(0xffffffffu, abs_max<HC>(x) * c.u <= TANH_POLY_MAX);
+      int form = 0;
+      if constexpr ((MODE & 1) != 0) form = tanh_form<HC>(x, c.u);
 #pragma unroll
       for (int g = 0; g < HC; g += 16) {
         float* pg = p + ((MODE & 1) != 0 && !DKV ? g : 0);
-        if (masked) bwd_probs<T, MODE, true, DKV>(x + g, w + g / 2, pg, c, poly, nl + g, neg_lse, dist0 - g, lo - g, hi - g);
-        else bwd_probs<T, MODE, false, DKV>(x + g, w + g / 2, pg, c, poly, nl + g, neg_lse, dist0 - g, 0, 0);
+        if (masked) bwd_probs<T, MODE, true, DKV>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, lo - g, hi - g);
+        else bwd_probs<T, MODE, false, DKV>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, 0, 0);
       }
       ok = warp_wait(dp_full, n & 1, err);
       if (!ok) break;
       tc_fence_after();
-      tmem_ld32_nw(ts + 128, dp);
-      tmem_wait_ld();
-      if constexpr (!DKV || (MODE & 1) == 0) {  // acc1 takes f itself
+      if constexpr ((MODE & 1) != 0 && !DKV) {
+        // f and p both live: dP in two halves, or the registers spill (the backward of 8,192 capped
+        // tokens then takes 945 us, not 724)
+        float ds[HC / 2];
 #pragma unroll
-        for (int e = 0; e < HC / 2; ++e)
-          w[e] = __uint_as_float(pack_t2<T>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])));
+        for (int g = 0; g < HC; g += 16) {
+          float dh[16];
+          tmem_ld16(ts + 128 + g, dh);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            w[g / 2 + e] = __uint_as_float(pack_t2<T>(__uint_as_float(x[g + 2 * e]), __uint_as_float(x[g + 2 * e + 1])));
+          const uint32_t* du = reinterpret_cast<const uint32_t*>(dh);
+          if (masked) rest += bwd_ds<T, MODE, true, DKV, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, lo - g, hi - g);
+          else rest += bwd_ds<T, MODE, false, DKV, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, 0, 0);
+        }
+        tmem_st16(ts + 128, w);
+        tmem_st16(ts + 128 + HC / 2, ds);
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(p_full);
+      } else {
+        uint32_t dp[HC];
+        tmem_ld32_nw(ts + 128, dp);
+        tmem_wait_ld();
+        if constexpr ((MODE & 1) == 0) {  // acc1 takes f itself
+#pragma unroll
+          for (int e = 0; e < HC / 2; ++e)
+            w[e] = __uint_as_float(pack_t2<T>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])));
+        }
+        tmem_st16(ts + 128, w);
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(p_full);
+        if (masked) rest += bwd_ds<T, MODE, true, DKV, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, lo, hi);
+        else rest += bwd_ds<T, MODE, false, DKV, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, 0, 0);
+        tmem_st16(ts + 128 + HC / 2, w);
+        tmem_wait_st();
+        tc_fence_before();
       }
-      tmem_st16(ts + 128, w);
-      tmem_wait_st();
-      tc_fence_before();
-      warp_arrive(p_full);
-      if (masked) rest += bwd_ds<T, MODE, true, DKV>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, lo, hi);
-      else rest += bwd_ds<T, MODE, false, DKV>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, 0, 0);
       if (DKV) warp_arrive(&l_empty[s]);
-      tmem_st16(ts + 128 + HC / 2, w);
-      tmem_wait_st();
-      tc_fence_before();
       warp_arrive(ds_full);
     }
     if (ok && steps > 0) {
@@ -506,7 +536,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             tmem_ld16(lane_base + 384 + col0 + u * 16, v);
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = steps > 0 ? (v[e] - rest * pk[e]) * a.scale : 0.f;
+          for (int e = 0; e < 16; ++e) v[e] = steps > 0 ? (v[e] - rest * pk[e]) * (SIGN * a.scale) : 0.f;
           if (live) {
             store_row8<T>(dst + u * 16, v);
             store_row8<T>(dst + u * 16 + 8, v + 8);
@@ -520,7 +550,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       for (int u = 0; u < D / 32; ++u) {  // dV's columns, then dK's
         const bool is_k = u >= D / 64;
         const int col = (is_k ? u - D / 64 : u) * 16;
-        const float sc = is_k ? a.scale : P_BACK;
+        const float sc = is_k ? SIGN * a.scale : P_BACK;
         float v[16];
         if (steps > 0) tmem_ld16(lane_base + (is_k ? 384 : 256) + col0 + col, v);
 #pragma unroll

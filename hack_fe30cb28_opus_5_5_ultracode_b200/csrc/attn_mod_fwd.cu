@@ -40,17 +40,28 @@ struct ScoreConst {
   float sl2;    // scale * log2(e): plain scores
   float u;      // scale / cap
   float cap2;   // cap * log2(e)
+  TanhShort ts;
 };
 
 // Scores of one row and one key block, in place: raw products to log2 units (MODE 0 leaves them
-// raw: the scale rides in the exponent's FMA), masked ones to -inf. x: 64 values; dist0 = i - their first key.
+// raw: the scale rides in the exponent's FMA), masked ones to -inf. x: 64 values; dist0 = i - their first key;
+// side: 1 (-1) if every key of the block comes before (after) every query of the tile, else 0.
 template <int MODE, bool MASKED>
 __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, float slope2,
-                                              float dist0, int rlo, int rhi) {
+                                              float dist0, float side, int rlo, int rhi) {
   if constexpr ((MODE & 1) != 0) {
-    // the largest |u| of the warp's rows decides between the polynomial and tanhf
-    const bool poly = __all_sync(0xffffffffu, abs_max<FWD_HC>(x) * c.u <= TANH_POLY_MAX);
-    if (poly) {
+    const int form = tanh_form<FWD_HC>(x, c.u);
+    if (form == 0) {
+#pragma unroll
+      for (int i = 0; i < FWD_HC; i += 16) {
+        uint64_t u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = pair_of(x + i + 2 * e);
+        tanh_short2<8>(u, c.ts);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) unpair(u[e], x + i + 2 * e);
+      }
+    } else if (form == 1) {
       const uint64_t uu = pk2(c.u, c.u), cc = pk2(c.cap2, c.cap2);
 #pragma unroll
       for (int i = 0; i < FWD_HC; i += 16) {
@@ -68,10 +79,16 @@ __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, 
     }
   }
   if constexpr ((MODE & 2) != 0) {
+    const uint64_t mul = pk2((MODE & 1) != 0 ? 1.f : c.sl2, (MODE & 1) != 0 ? 1.f : c.sl2);
+    if (side != 0.f) {  // every key on one side of every query: |i - j| = side (dist0 - column)
+      const float slope = side * slope2, base = -slope * dist0;
 #pragma unroll
-    for (int i = 0; i < FWD_HC; ++i) {
-      const float y = (MODE & 1) != 0 ? __uint_as_float(x[i]) : __uint_as_float(x[i]) * c.sl2;
-      x[i] = __float_as_uint(y - fabsf(slope2 * (dist0 - (float)i)));
+      for (int i = 0; i < FWD_HC; i += 2)
+        unpair(fma2(pair_of(x + i), mul, pk2(fmaf((float)i, slope, base), fmaf((float)(i + 1), slope, base))), x + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < FWD_HC; i += 2)
+        unpair(fma2(pair_of(x + i), mul, pk2(-fabsf(slope2 * (dist0 - (float)i)), -fabsf(slope2 * (dist0 - (float)(i + 1))))), x + i);
     }
   }
   if constexpr (MASKED) {
@@ -243,6 +260,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     c.sl2 = a.scale * 1.4426950408889634f;
     c.u = (MODE & 1) != 0 ? a.scale / a.softcap : 0.f;
     c.cap2 = a.softcap * 1.4426950408889634f;
+    if constexpr ((MODE & 1) != 0) c.ts = tanh_short(c.u, c.cap2);
     const float slope2 = (MODE & 2) != 0 ? a.slopes[h] * 1.4426950408889634f : 0.f;
     const float mul = MODE == 0 ? c.sl2 : 1.f;
     float m_run = -INFINITY, l_run = 0.f;
@@ -257,9 +275,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       tmem_ld32_nw(ts + 32, x + 32);
       tmem_wait_ld();
       const bool masked = j < tb.ffirst || j >= tb.fend;
-      const int j0 = j * AM_T + half * FWD_HC;
-      if (masked) modify_scores<MODE, true>(x, c, slope2, (float)(qi - j0), range.x - j0, range.y - j0);
-      else modify_scores<MODE, false>(x, c, slope2, (float)(qi - j0), 0, 0);
+      const int j0 = j * AM_T + half * FWD_HC, qt = q0 / AM_T + t;
+      const float side = j < qt ? 1.f : j > qt ? -1.f : 0.f;
+      if (masked) modify_scores<MODE, true>(x, c, slope2, (float)(qi - j0), side, range.x - j0, range.y - j0);
+      else modify_scores<MODE, false>(x, c, slope2, (float)(qi - j0), side, 0, 0);
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int i = 0; i < FWD_HC; i += 8)
