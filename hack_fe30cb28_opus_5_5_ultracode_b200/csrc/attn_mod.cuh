@@ -275,6 +275,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
 // against 198 us in this form).
 __device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 
+// A value every lane holds, as one the compiler knows to be the same (what comes from memory it takes to
+// differ, and then moves every descriptor from a vector register for every MMA).
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // High words of the operand descriptors (128-byte swizzle, version 1): stride 1024 B between groups of
 // 8 rows. Low words: start address / 16, and for MN-major operands the distance of 64-element chunks.
 constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
@@ -308,26 +312,19 @@ __device__ __forceinline__ void umma_score(uint32_t d, uint32_t a_lo, uint32_t b
 #undef QL_AM_SS
 
 // D (+)= A . B over 128 rows of the MN-major tile B: A [128 x 128] 16-bit in TMEM, two elements per
-// 32-bit column, kept in parts of 16 PART columns whose starts are PART_STEP columns apart.
+// 32-bit column.
 #define QL_AM_TS(AOFF, BOFF)                                                                       \
   "add.u32 x, %1, " AOFF "; add.u32 y, %2, " BOFF ";\n\t"                                          \
   "mov.b64 b, {y, %4};\n\t"                                                                       \
   "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, p;\n\t"                                \
   "setp.eq.u32 p, 0, 0;\n\t"
-// two parts of 32 columns, 64 apart (two softmax threads per row); HALF 0: the first 32 rows of B's
-// first and of its second 64, HALF 1: the others
-template <int HALF>
-__device__ __forceinline__ void umma_gather2(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t more) {
-  if constexpr (HALF == 0)
-    asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
-                 "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
-                 QL_AM_TS("0", "0") QL_AM_TS("8", "128") QL_AM_TS("64", "512") QL_AM_TS("72", "640") "}"
-                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
-  else
-    asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
-                 "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
-                 QL_AM_TS("16", "256") QL_AM_TS("24", "384") QL_AM_TS("80", "768") QL_AM_TS("88", "896") "}"
-                 ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
+// A's 64 columns in one piece
+__device__ __forceinline__ void umma_gather1(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t more) {
+  asm volatile("{\n\t.reg .pred p, e; .reg .b32 x, y; .reg .b64 b;\n\t"
+               "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+               QL_AM_TS("0", "0") QL_AM_TS("8", "128") QL_AM_TS("16", "256") QL_AM_TS("24", "384")
+               QL_AM_TS("32", "512") QL_AM_TS("40", "640") QL_AM_TS("48", "768") QL_AM_TS("56", "896") "}"
+               ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "n"(DESC_HI), "r"(more) : "memory");
 }
 // four parts of 16 columns, 32 apart (four softmax threads per row)
 __device__ __forceinline__ void umma_gather4(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t more) {

@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   if (r0 >= seq.len) return;  // the whole CTA, before any barrier or TMEM is set up
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const AttnBlocks tb = DKV ? attn_key_blocks(seq, r0) : attn_tile_blocks(seq, r0);
-  const int ntile = tb.end - tb.first, steps = ntile * heads;
+  const int ntile = tb.end - tb.first, steps = uniform(ntile * heads);
 
   if (threadIdx.x == 0) {
     mbar_init(xy_full, 1);

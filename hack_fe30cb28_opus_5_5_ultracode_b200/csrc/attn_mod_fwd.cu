@@ -2,17 +2,19 @@
 // 64 and 128): see attn_mod.cuh for the score and the masks.
 //
 // One CTA takes two adjacent 128-query tiles of one head; both read the same K and V blocks of
-// 128 keys, so each block crosses from L2 once for 256 queries. Eighteen warps:
+// 128 keys, so each block crosses from L2 once for 256 queries. Nineteen warps:
 //   warps 0-7, 8-15 softmax of tile 0 and of tile 1, two threads per query row (TMEM lane = row), 64
 //                   of the 128 keys each: scores into registers, the row's maximum (the two threads
-//                   exchange theirs through shared memory), P as 16-bit pairs back into the score's
-//                   TMEM columns, where the next product reads it as its A operand;
-//   warp 16         one thread issues the MMAs: for each block O_t += P_t V and then the next
-//                   block's S_t = Q_t K^T, tile 0 and tile 1 in turn, so the tensor core works on
-//                   one tile while the other tile's softmax runs;
-//   warp 17         TMA: Q tiles, then K and V blocks through a ring of tiles.
-// TMEM columns: S_0 [0, 128), S_1 [128, 256) (P_t in the first 32 of each half of S_t), O_0 [256, 256 + D),
-// O_1 [384, 384 + D).
+//                   exchange theirs through shared memory), P as 16-bit pairs into tensor memory,
+//                   where the next product reads it as its A operand;
+//   warps 16, 17    issue the MMAs of tile 0 and of tile 1: S_t = Q_t K^T into one score buffer that
+//                   goes from tile to tile as soon as it has been read, and O_t += P_t V when P_t is
+//                   there. So a tile's next scores are ready when its softmax warps are done with a
+//                   block. (Each instruction of such a warp waits its turn among those of four softmax
+//                   warps: one warp for both tiles took 1,800 cycles per tile and block, longer than
+//                   the softmax.)
+//   warp 18         TMA: Q tiles, then K and V blocks through a ring of tiles.
+// TMEM columns: S [0, 128), P_0 [128, 192), P_1 [192, 256), O_0 [256, 256 + D), O_1 [384, 384 + D).
 // The running maximum moves only when it grows by more than 2^8; then the row's O is rescaled.
 // P is rounded to the input type for the product (half a step of 2^-8 or 2^-11 per probability,
 // averaged over the row's keys); the row sum adds the unrounded values in fp32.
@@ -32,7 +34,7 @@ struct FwdCfg {
   static constexpr int OFF_BAR = OFF_M + 4 * AM_T * 4;
   static constexpr int SMEM = OFF_BAR + 512;
 };
-constexpr int FWD_THREADS = 576;
+constexpr int FWD_THREADS = 608;
 constexpr int FWD_HC = 64;  // columns per softmax thread
 
 // What the score's modes need per kernel.
@@ -109,16 +111,18 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem[];  // no static shared memory: the base is aligned
   float* sM = reinterpret_cast<float*>(smem + C::OFF_M);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* q_full = bars;                      // [2]
-  uint64_t* s_full = bars + 2;                  // [2] score tile written; last: O complete
-  uint64_t* p_full = bars + 4;                  // [2] half of P written, O rescaled (8 warps)
-  uint64_t* p_full2 = bars + 6;                 // [2] the other half of P written
-  uint64_t* kv_raw = bars + 8;                  // a V tile whose dead rows are zeroed first
-  uint64_t* drain = bars + 9;
-  uint64_t* kv_full = bars + 10;                // [STAGES]
-  uint64_t* kv_empty = bars + 10 + C::STAGES;   // [STAGES]
-  uint64_t* row_max = bars + 10 + 2 * C::STAGES;  // [2][4] both halves of a tile's 32 rows (2 warps)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_max + 8);
+  uint64_t* q_full = bars;                       // [2]
+  uint64_t* s_full = bars + 2;                   // [2] the tile's scores written
+  uint64_t* s_free = bars + 4;                   // [2] score buffer handed to the tile (8 warps)
+  uint64_t* p_full = bars + 6;                   // [2] P written, O rescaled (8 warps)
+  uint64_t* o_full = bars + 8;                   // [2] O += P V complete
+  uint64_t* kv_raw = bars + 10;                  // a V tile whose dead rows are zeroed first
+  uint64_t* drain = bars + 11;                   // [2]
+  uint64_t* kv_full = bars + 13;                 // [STAGES]
+  uint64_t* kv_empty = bars + 13 + C::STAGES;    // [STAGES] one arrival per tile
+  uint64_t* row_max = bars + 13 + 2 * C::STAGES; // [2][4] both halves of a tile's 32 rows (2 warps)
+  uint64_t* row_read = row_max + 8;              // [2][4] and read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_read + 8);
 
   const int h = blockIdx.x % a.HQ, b = blockIdx.x / a.HQ;
   const int q0 = (gridDim.y - 1 - blockIdx.y) * 2 * AM_T;  // the rows with the most keys first
@@ -126,24 +130,32 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   if (q0 >= seq.len) return;  // the whole CTA, before any barrier or TMEM is set up
   const int kvh = h / (a.HQ / a.HKV);
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const AttnBlocks tb0 = attn_tile_blocks(seq, q0), tb1 = attn_tile_blocks(seq, q0 + AM_T);
-  int jb = tb0.first, je = tb0.end;  // blocks either tile visits
-  if (je <= jb) { jb = tb1.first; je = tb1.end; }
-  else if (tb1.end > tb1.first) { jb = min(jb, tb1.first); je = max(je, tb1.end); }
+  AttnBlocks tb0 = attn_tile_blocks(seq, q0), tb1 = attn_tile_blocks(seq, q0 + AM_T);
+  tb0.first = uniform(tb0.first);
+  tb0.end = uniform(tb0.end);
+  tb1.first = uniform(tb1.first);
+  tb1.end = uniform(tb1.end);
+  // the blocks either tile visits: its own range, or the gap-free union where both have one
+  const bool any0 = tb0.end > tb0.first, any1 = tb1.end > tb1.first;
+  const int jb = !any1 || (any0 && tb0.first < tb1.first) ? tb0.first : tb1.first;
+  const int je = !any1 || (any0 && tb0.end > tb1.end) ? tb0.end : tb1.end;
+  auto visits = [&](int t, int j) { return t ? j >= tb1.first && j < tb1.end : j >= tb0.first && j < tb0.end; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&s_full[s], 1);
+      mbar_init(&s_free[s], 8);
       mbar_init(&p_full[s], 8);
-      mbar_init(&p_full2[s], 8);
-      for (int w = 0; w < 4; ++w) mbar_init(&row_max[s * 4 + w], 2);
+      mbar_init(&o_full[s], 1);
+      for (int w = 0; w < 8; ++w) mbar_init(&row_max[s * 8 + w], 2);  // row_max and row_read
     }
     mbar_init(kv_raw, 1);
-    mbar_init(drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], 2);
     }
     fence_barrier_init();
     prefetch_tmap(&tq);
@@ -156,10 +168,9 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-  if (warp == 17) {
+  if (warp == 18) {
     // ---- loads ----
-    const int nblk = je - jb;
-    int issued = 0;   // ring slots filled
+    int n = 0;  // ring positions filled
     uint32_t raw = 0;
     bool ok = true;
     auto load_q = [&](int t) {
@@ -168,80 +179,96 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         tma_load_3d(smem + t * C::TILE, &tq, &q_full[t], 0, seq.start + q0 + t * AM_T, h * (D / 64));
       }
     };
-    if (nblk > 0) load_q(0);
-    for (int n = 0; ok && n < 2 * nblk; ++n) {
-      const int s = n % C::STAGES, row = (jb + (n >> 1)) * AM_T;
-      const bool is_v = n & 1;
-      uint32_t bad[4];
-      const bool dirty = is_v && attn_dead_rows(seq, row, bad);
-      if (n >= C::STAGES) ok = warp_wait(&kv_empty[s], (n / C::STAGES - 1) & 1, err);
-      if (!ok) break;
-      uint8_t* dst = smem + C::OFF_KV + s * C::TILE;
-      uint64_t* bar = dirty ? kv_raw : &kv_full[s];
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar, C::TILE);
-        tma_load_3d(dst, is_v ? &tv : &tk, bar, 0, seq.start + row, kvh * (D / 64));
-      }
-      if (dirty) {
-        ok = warp_wait(kv_raw, raw, err);
+    if (je > jb) load_q(0);
+    for (int j = jb; ok && j < je; ++j) {
+      if (!visits(0, j) && !visits(1, j)) continue;
+      const int row = j * AM_T;
+#pragma unroll
+      for (int is_v = 0; is_v < 2; ++is_v, ++n) {
+        const int s = n % C::STAGES;
+        uint32_t bad[4];
+        const bool dirty = is_v && attn_dead_rows(seq, row, bad);
+        if (n >= C::STAGES) ok = warp_wait(&kv_empty[s], (n / C::STAGES - 1) & 1, err);
         if (!ok) break;
-        raw ^= 1;
-        attn_zero_rows<D / 64>(dst, bad);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[s]);
+        uint8_t* dst = smem + C::OFF_KV + s * C::TILE;
+        uint64_t* bar = dirty ? kv_raw : &kv_full[s];
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, C::TILE);
+          tma_load_3d(dst, is_v ? &tv : &tk, bar, 0, seq.start + row, kvh * (D / 64));
+        }
+        if (dirty) {
+          ok = warp_wait(kv_raw, raw, err);
+          if (!ok) break;
+          raw ^= 1;
+          attn_zero_rows<D / 64>(dst, bad);
+          fence_proxy_async_smem();
+          warp_arrive(&kv_full[s]);
+        }
+        if (n == 0) load_q(1);
       }
-      issued = n + 1;
-      if (n == 0) load_q(1);
     }
     if (!ok && lane == 0) {  // a wait ran out: let the copies in flight land before the CTA goes
       mbar_wait(&q_full[0], 0, nullptr, 100000000ull);
       mbar_wait(&q_full[1], 0, nullptr, 100000000ull);
-      for (int n = max(0, issued - C::STAGES); n < issued; ++n)
-        mbar_wait(&kv_full[n % C::STAGES], (n / C::STAGES) & 1, nullptr, 100000000ull);
+      for (int k = max(0, n - C::STAGES); k < n; ++k)
+        mbar_wait(&kv_full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, 100000000ull);
     }
-  } else if (warp == 16) {
-    // ---- MMA ----
+  } else if (warp == 16 || warp == 17) {
+    // ---- MMA of one tile ----
+    const int t = warp - 16;
     if (je > jb) {
       constexpr uint32_t id_s = umma_idesc_f16(IS_BF16, 128, AM_T, false);
       constexpr uint32_t id_o = umma_idesc_f16(IS_BF16, 128, D, true);  // V is MN-major
-      const uint32_t sq = desc_lo_k(smem_u32(smem));
+      const uint32_t sq = desc_lo_k(smem_u32(smem + t * C::TILE));
       const uint32_t sk = desc_lo_k(smem_u32(smem + C::OFF_KV));
       const uint32_t sv = desc_lo_mn(smem_u32(smem + C::OFF_KV), BOX);
-      bool ok = warp_wait(&q_full[0], 0, err) && warp_wait(&q_full[1], 0, err);
-      for (int j = jb - 1; ok && j < je; ++j) {
-        const int nk = 2 * (j + 1 - jb), nv = 2 * (j - jb) + 1;  // ring positions of K_{j+1}, V_j
-        if (j + 1 < je) ok = warp_wait(&kv_full[nk % C::STAGES], (nk / C::STAGES) & 1, err);
-        if (ok && j >= jb) ok = warp_wait(&kv_full[nv % C::STAGES], (nv / C::STAGES) & 1, err);
+      // The score buffer goes from item to item ((tile, block) pairs, block by block, tile 0 first): this
+      // tile's next scores are formed when the softmax warps that read the item before pass the buffer
+      // on to it (s_free). Blocks that only the other tile visits are handed back as they land, so that
+      // both warps see every turn of the ring.
+      const bool leads = t == 0 || !any0;  // has the first item
+      int ring = 0;                        // position of the block's K in the ring (V follows)
+      int n = 0, pend = -1;                // this tile's items so far; V of the product still to come
+      auto gather = [&]() {                // O += P V of item n - 1
+        const int s = pend % C::STAGES;
+        if (!warp_wait(&kv_full[s], (pend / C::STAGES) & 1, err) || !warp_wait(&p_full[t], (n - 1) & 1, err))
+          return false;
+        tc_fence_after();
+        umma_gather1(tmem + 256 + t * 128, tmem + 128 + t * 64, sv + s * (C::TILE >> 4), id_o, n > 1);
+        warp_commit(&o_full[t]);
+        warp_commit(&kv_empty[s]);
+        pend = -1;
+        return true;
+      };
+      bool ok = warp_wait(&q_full[t], 0, err);
+      for (int j = jb; ok && j < je; ++j) {
+        const bool mine = visits(t, j);
+        if (!mine && !visits(t ^ 1, j)) continue;  // not loaded
+        if (!mine && pend >= 0) ok = gather();
+        const int s = ring % C::STAGES, s1 = (ring + 1) % C::STAGES;
+        if (ok) ok = warp_wait(&kv_full[s], (ring / C::STAGES) & 1, err);
         if (!ok) break;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int first = t ? tb1.first : tb0.first, end = t ? tb1.end : tb0.end;
-          const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * 128;
-          if (j >= first && j < end) {  // O_t += P_t V_j
-            ok = warp_wait(&p_full[t], (j - first) & 1, err);
-            if (!ok) break;
-            tc_fence_after();
-            umma_gather2<0>(to, ts, sv + (nv % C::STAGES) * (C::TILE >> 4), id_o, j > first);
-            ok = warp_wait(&p_full2[t], (j - first) & 1, err);
-            if (!ok) break;
-            tc_fence_after();
-            umma_gather2<1>(to, ts, sv + (nv % C::STAGES) * (C::TILE >> 4), id_o, 1);
-            if (j + 1 == end) warp_commit(&s_full[t]);
-          }
-          if (j + 1 >= first && j + 1 < end) {  // S_t = Q_t K_{j+1}^T (after P_t V_j in issue order)
-            tc_fence_after();
-            umma_score<D>(ts, sq + t * (C::TILE >> 4), sk + (nk % C::STAGES) * (C::TILE >> 4), id_s);
-            warp_commit(&s_full[t]);
-          }
+        if (mine) {
+          if (n > 0 || !leads) ok = warp_wait(&s_free[t], (n - (leads ? 1 : 0)) & 1, err);
+          if (!ok) break;
+          tc_fence_after();
+          umma_score<D>(tmem, sq, sk + s * (C::TILE >> 4), id_s);
+          warp_commit(&s_full[t]);
+          warp_commit(&kv_empty[s]);
+          if (pend >= 0) ok = gather();
+          pend = ring + 1;
+          ++n;
+        } else {
+          warp_arrive(&kv_empty[s]);
+          ok = warp_wait(&kv_full[s1], ((ring + 1) / C::STAGES) & 1, err);
+          if (ok) warp_arrive(&kv_empty[s1]);
         }
-        if (!ok) break;
-        if (j >= jb) warp_commit(&kv_empty[nv % C::STAGES]);
-        if (j + 1 < je) warp_commit(&kv_empty[nk % C::STAGES]);
+        ring += 2;
       }
+      if (ok && pend >= 0) ok = gather();
       if (!ok) {  // a wait ran out: the products already issued finish before TMEM is freed
-        warp_commit(drain);
-        if (lane == 0) mbar_wait(drain, 0, nullptr, 100000000ull);
+        warp_commit(&drain[t]);
+        if (lane == 0) mbar_wait(&drain[t], 0, nullptr, 100000000ull);
         __syncwarp();
       }
     }
@@ -251,10 +278,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     const int qi = q0 + t * AM_T + r;
     const AttnBlocks tb = t ? tb1 : tb0;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t ts = lane_base + t * 128 + half * FWD_HC, to = lane_base + 256 + t * 128 + half * (D / 2);
+    const uint32_t ts = lane_base + half * FWD_HC, tp = lane_base + 128 + t * 64 + half * (FWD_HC / 2);
+    const uint32_t to = lane_base + 256 + t * 128 + half * (D / 2);
     float* mine = sM + (2 * t + half) * AM_T + r;
     const float* other = sM + (2 * t + (half ^ 1)) * AM_T + r;
     uint64_t* pair = &row_max[t * 4 + (warp & 3)];
+    uint64_t* pair_read = &row_read[t * 4 + (warp & 3)];
     const int2 range = qi < seq.len ? attn_row_range(seq, qi) : make_int2(0, 0);
     ScoreConst c;
     c.sl2 = a.scale * 1.4426950408889634f;
@@ -274,6 +303,11 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       tmem_ld32_nw(ts, x);
       tmem_ld32_nw(ts + 32, x + 32);
       tmem_wait_ld();
+      tc_fence_before();
+      // the buffer goes to tile 1 at this block, else to whichever tile visits the next one, or
+      // (tile 0's last block before a gap) to tile 1
+      const int heir = t == 0 && visits(1, j) ? 1 : visits(0, j + 1) ? 0 : visits(1, j + 1) || (t == 0 && any1) ? 1 : -1;
+      if (heir >= 0) warp_arrive(&s_free[heir]);
       const bool masked = j < tb.ffirst || j >= tb.fend;
       const int j0 = j * AM_T + half * FWD_HC, qt = q0 / AM_T + t;
       const float side = j < qt ? 1.f : j > qt ? -1.f : 0.f;
@@ -285,21 +319,28 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           mx[e] = max3(mx[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
-      // the other half's maximum (its slot is written again only after P of this block is complete)
+      // the other half's maximum
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      if (n > 0) ok = warp_wait(pair_read, (n - 1) & 1, err);  // the last block's has been read
+      if (!ok) break;
       *mine = top;
       warp_arrive(pair);
       ok = warp_wait(pair, n & 1, err);
       if (!ok) break;
       const float ms = fmaxf(top, *other) * mul;
+      warp_arrive(pair_read);
       float corr = 1.f;
       if (ms > m_run + 8.f) {
         corr = m_run == -INFINITY ? 0.f : ex2(m_run - ms);
         m_run = ms;
       }
       const float mneg = m_run == -INFINITY ? 0.f : -m_run;
+      if (n > 0) {  // O_t += P_t V of the last block is complete: P_t may be written, O_t rescaled
+        ok = warp_wait(&o_full[t], (n - 1) & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+      }
       if (n > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-        // S_t of this block was committed after O_t += P_t V of the last one: O_t is complete
 #pragma unroll 1
         for (int u = 0; u < D / 32; ++u) {
           float ov[16];
@@ -323,20 +364,21 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
           up2(y, pa, pb);
           w[i] = __uint_as_float(pack_t2<T>(pa, pb));
         }
-        tmem_st16(ts + g / 2, w);
-        tmem_wait_st();
-        tc_fence_before();
-        warp_arrive(g == 0 ? &p_full[t] : &p_full2[t]);
+        tmem_st16(tp + g / 2, w);
       }
+      tmem_wait_st();
+      tc_fence_before();
+      warp_arrive(&p_full[t]);
       float sa, sb;
       up2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), sa, sb);
       l_run = l_run * corr + (sa + sb);
     }
     if (tb.end > tb.first && ok) {
-      ok = warp_wait(&s_full[t], (tb.end - tb.first) & 1, err);
+      ok = warp_wait(&o_full[t], (tb.end - tb.first - 1) & 1, err);
       tc_fence_after();
     }
     // the row sum: both halves' sums, added in the same order in both threads
+    if (ok && tb.end > tb.first) ok = warp_wait(pair_read, (tb.end - tb.first - 1) & 1, err);
     if (ok) {
       *mine = l_run;
       warp_arrive(pair);
