@@ -396,6 +396,34 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
+// Columns c of 32 with lo <= c < hi, as bits.
+__device__ __forceinline__ uint32_t col_mask(int lo, int hi) {
+  const int a = max(lo, 0), b = min(hi, 32);
+  return b <= a ? 0u : (0xffffffffu >> (32 - (b - a))) << a;
+}
+
+// A warp's 32 result rows of W bytes (32, 64 or 128) through shared memory, so that they leave as whole
+// lines: one thread holds one row, and its 16-byte stores straight to global memory touched 32 lines
+// each (the epilogue of a 256-query CTA took 4,500 cycles). 16-byte chunk c of row r is kept at chunk
+// c ^ (r / rows per 128 bytes): eight neighbouring rows in eight different bank groups.
+template <int W>
+__device__ __forceinline__ uint8_t* stage_at(uint8_t* stage, int row, int chunk) {
+  return stage + row * W + ((chunk ^ ((row / (128 / W)) & (W / 16 - 1))) << 4);
+}
+// Rows [0, live) of the stage to dst, row pitch ld bytes.
+template <int W>
+__device__ __forceinline__ void stage_flush(uint8_t* stage, uint8_t* dst, int64_t ld, int live) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < W / 16; ++i) {
+    const int row = (i * 32 + lane) / (W / 16), chunk = lane % (W / 16);
+    if (row < live)
+      *reinterpret_cast<uint4*>(dst + row * ld + chunk * 16) = *reinterpret_cast<const uint4*>(stage_at<W>(stage, row, chunk));
+  }
+  __syncwarp();
+}
+
 // Host: raises a kernel's dynamic shared-memory limit on the current device, once per device.
 inline int attn_smem_limit(const void* kernel, int bytes, unsigned long long* done) {
   int dev = 0;

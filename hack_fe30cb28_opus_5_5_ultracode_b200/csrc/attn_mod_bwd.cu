@@ -49,12 +49,12 @@ struct BwdConst {
 // gradients' last scaling. p16: the probabilities themselves as 16-bit pairs, where they are not f (a capped
 // score of the dK / dV role). form: tanh_form of the warp's
 // scores. neg_lse: -lse2 by column (PER_COL, from shared memory) or
-// one value. Masked columns [0, lo) and [hi, 16) give 0. dist0: row index minus the first column's, for
+// one value. Columns whose bit in seen is 0 give 0. dist0: row index minus the first column's, for
 // the distance bias. p: plain probabilities where the caller needs them beside f (a capped score of
 // the dQ role).
 template <typename T, int MODE, bool MASKED, bool PER_COL>
 __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, const BwdConst& c, int form,
-                                          const float* neg_lse, float neg_lse_row, float dist0, int lo, int hi) {
+                                          const float* neg_lse, float neg_lse_row, float dist0, uint32_t seen) {
   uint64_t y[8], bend[8];
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
@@ -103,8 +103,8 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
     float pa, pb, fa, fb;
     up2(y[e], pa, pb);
     if constexpr (MASKED) {
-      if (k < lo || k >= hi) pa = 0.f;
-      if (k + 1 < lo || k + 1 >= hi) pb = 0.f;
+      if (!(seen >> k & 1)) pa = 0.f;
+      if (!(seen >> (k + 1) & 1)) pb = 0.f;
     }
     fa = pa;
     fb = pb;
@@ -129,7 +129,7 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
 // gets sum p (dP - Dvec) of its columns.
 template <typename T, int MODE, bool MASKED, bool PER_COL, int N>
 __device__ __forceinline__ float bwd_ds(const uint32_t* f, const float* p, const uint32_t* dp, float* ds16,
-                                        float dscale, const float* neg_d, float neg_d_row, int lo, int hi) {
+                                        float dscale, const float* neg_d, float neg_d_row, uint32_t seen) {
   const uint64_t row2 = pk2(neg_d_row, neg_d_row), ds2 = pk2(dscale, dscale);
   uint64_t sum[2] = {0, 0};  // pairs of +0.f
 #pragma unroll
@@ -152,7 +152,7 @@ __device__ __forceinline__ float bwd_ds(const uint32_t* f, const float* p, const
         const int k = i + 2 * e;
         float a, b;
         up2(g[e], a, b);
-        g[e] = pk2(k < lo || k >= hi ? 0.f : a, k + 1 < lo || k + 1 >= hi ? 0.f : b);
+        g[e] = pk2(seen >> k & 1 ? a : 0.f, seen >> (k + 1) & 1 ? b : 0.f);
       }
     }
     if constexpr (!PER_COL && (MODE & 1) != 0) {
@@ -188,11 +188,14 @@ __device__ __forceinline__ BwdConst bwd_const(const AttnModArgs& a, int h) {
   return c;
 }
 
-// 8 consecutive values of one row, rounded to the 16-bit type
-template <typename T>
-__device__ __forceinline__ void store_row8(T* dst, const float* v) {
-  *reinterpret_cast<uint4*>(dst) = make_uint4(pack_t2<T>(v[0], v[1]), pack_t2<T>(v[2], v[3]),
-                                              pack_t2<T>(v[4], v[5]), pack_t2<T>(v[6], v[7]));
+// 16 values as 16-bit chunks 2 u and 2 u + 1 of the row
+template <typename T, int W>
+__device__ __forceinline__ void stage16(uint8_t* stage, int row, int u, const float* v) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    *reinterpret_cast<uint4*>(stage_at<W>(stage, row, 2 * u + c)) =
+        make_uint4(pack_t2<T>(v[8 * c], v[8 * c + 1]), pack_t2<T>(v[8 * c + 2], v[8 * c + 3]),
+                   pack_t2<T>(v[8 * c + 4], v[8 * c + 5]), pack_t2<T>(v[8 * c + 6], v[8 * c + 7]));
 }
 
 template <int D>
@@ -257,10 +260,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   const AttnSeq seq = attn_seq(a, b);
   if (r0 >= seq.len) return;  // the whole CTA, before any barrier or TMEM is set up
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const AttnBlocks tb = DKV ? attn_key_blocks(seq, r0) : attn_tile_blocks(seq, r0);
-  const int ntile = tb.end - tb.first, steps = uniform(ntile * heads);
-
-  if (threadIdx.x == 0) {
+  // the loading warp sets the barriers up while the others allocate and look at the mask
+  if (warp == 17 && lane == 0) {
     mbar_init(xy_full, 1);
     mbar_init(s_full, 1);
     mbar_init(dp_full, 1);
@@ -283,12 +284,16 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       mbar_init(&w_empty[s], 1);
     }
     fence_barrier_init();
-    prefetch_tmap(&tx);
-    prefetch_tmap(&ty);
-    prefetch_tmap(&tu);
-    prefetch_tmap(&tw);
   }
   if (warp == 16) tmem_alloc(tmem_slot, 512);
+  const AttnBlocks tb = DKV ? attn_key_blocks(seq, r0) : attn_tile_blocks(seq, r0);
+  const int ntile = tb.end - tb.first, steps = uniform(ntile * heads);
+  if (warp == 17 && lane == 0 && steps > 0) {
+    const int zx = (DKV ? kvh : h0) * (D / 64);
+    mbar_arrive_expect_tx(xy_full, 2 * C::TILE);
+    tma_load_3d(smem, &tx, xy_full, 0, seq.start + r0, zx);
+    tma_load_3d(smem + C::OFF_Y, &ty, xy_full, 0, seq.start + r0, zx);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -299,12 +304,6 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     bool ok = true;
     int un = 0, wn = 0;
     uint32_t raw_phase = 0;
-    const int zx = (DKV ? kvh : h0) * (D / 64);
-    if (lane == 0 && steps > 0) {
-      mbar_arrive_expect_tx(xy_full, 2 * C::TILE);
-      tma_load_3d(smem, &tx, xy_full, 0, seq.start + r0, zx);
-      tma_load_3d(smem + C::OFF_Y, &ty, xy_full, 0, seq.start + r0, zx);
-    }
     for (int n = 0; ok && n < steps; ++n) {
       const int row = (tb.first + (DKV ? n % ntile : n)) * AM_T;
       const int h = DKV ? h0 + n / ntile : 0, zu = (DKV ? h : kvh) * (D / 64);
@@ -450,7 +449,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       const int s = n & 1, j = tb.first + (DKV ? n % ntile : n), i0 = j * AM_T + part * HC;
       if (DKV && (MODE & 2) != 0 && n > 0 && n % ntile == 0) c = bwd_const<MODE>(a, h0 + n / ntile);
       const bool masked = j < tb.ffirst || j >= tb.fend;
-      const int lo = range.x - i0, hi = range.y - i0;
+      const uint32_t seen = masked ? col_mask(range.x - i0, range.y - i0) : 0;
       const float dist0 = (float)(ri - i0);
       ok = warp_wait(s_full, n & 1, err);
       if (DKV && ok) ok = warp_wait(&l_full[s], (n >> 1) & 1, err);  // -lse2 and -Dvec are visible
@@ -468,8 +467,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 #pragma unroll
       for (int g = 0; g < HC; g += 16) {
         float* pg = p + ((MODE & 1) != 0 && !DKV ? g : 0);
-        if (masked) bwd_probs<T, MODE, true, DKV>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, lo - g, hi - g);
-        else bwd_probs<T, MODE, false, DKV>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, 0, 0);
+        if (masked) bwd_probs<T, MODE, true, DKV>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, seen >> g);
+        else bwd_probs<T, MODE, false, DKV>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, 0);
       }
       ok = warp_wait(dp_full, n & 1, err);
       if (!ok) break;
@@ -486,8 +485,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
           for (int e = 0; e < 8; ++e)
             w[g / 2 + e] = __uint_as_float(pack_t2<T>(__uint_as_float(x[g + 2 * e]), __uint_as_float(x[g + 2 * e + 1])));
           const uint32_t* du = reinterpret_cast<const uint32_t*>(dh);
-          if (masked) rest += bwd_ds<T, MODE, true, DKV, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, lo - g, hi - g);
-          else rest += bwd_ds<T, MODE, false, DKV, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, 0, 0);
+          if (masked) rest += bwd_ds<T, MODE, true, DKV, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, seen >> g);
+          else rest += bwd_ds<T, MODE, false, DKV, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, 0);
         }
         tmem_st16(ts + 128, w);
         tmem_st16(ts + 128 + HC / 2, ds);
@@ -507,8 +506,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(p_full);
-        if (masked) rest += bwd_ds<T, MODE, true, DKV, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, lo, hi);
-        else rest += bwd_ds<T, MODE, false, DKV, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, 0, 0);
+        if (masked) rest += bwd_ds<T, MODE, true, DKV, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, seen);
+        else rest += bwd_ds<T, MODE, false, DKV, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, 0);
         tmem_st16(ts + 128 + HC / 2, w);
         tmem_wait_st();
         tc_fence_before();
@@ -520,14 +519,17 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       ok = warp_wait(out_full, 0, err);
       tc_fence_after();
     }
-    const int col0 = part * (D / 4);  // this thread's columns of the results
+    // the results leave through X and Y, which every product has read
+    constexpr int W = D / 2;          // bytes of a quarter row of 16-bit values
+    const int col0 = part * (D / 4);  // this thread's columns
+    const int row0 = ri - lane;       // the warp's first row
+    uint8_t* stage = smem + warp * 32 * 2 * W;
     if constexpr (!DKV) {
       sR[part * AM_T + r] = rest;
       asm volatile("bar.sync 1, 512;" ::: "memory");
       rest = (sR[r] + sR[AM_T + r]) + (sR[2 * AM_T + r] + sR[3 * AM_T + r]);
       if (ok && live && part == 0) a.dvec[(int64_t)h0 * a.n + seq.start + ri] = rest - neg_d;
       if (ok) {
-        T* dst = reinterpret_cast<T*>(a.dq) + ((int64_t)(seq.start + ri) * a.HQ + h0) * D + col0;
 #pragma unroll
         for (int u = 0; u < D / 64; ++u) {
           float pk[16], v[16];
@@ -537,34 +539,38 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] = steps > 0 ? (v[e] - rest * pk[e]) * (SIGN * a.scale) : 0.f;
-          if (live) {
-            store_row8<T>(dst + u * 16, v);
-            store_row8<T>(dst + u * 16 + 8, v + 8);
-          }
+          stage16<T, W>(stage, lane, u, v);
         }
+        T* dst = reinterpret_cast<T*>(a.dq) + ((int64_t)(seq.start + row0) * a.HQ + h0) * D + col0;
+        stage_flush<W>(stage, reinterpret_cast<uint8_t*>(dst), (int64_t)a.HQ * D * 2, seq.len - row0);
       }
     } else if (ok) {
-      const int64_t at = ((int64_t)(seq.start + ri) * a.HKV + kvh) * D + col0;
+      const int64_t at = ((int64_t)(seq.start + row0) * a.HKV + kvh) * D + col0;
       const int64_t plane = (int64_t)a.n * a.HKV * D;
 #pragma unroll
-      for (int u = 0; u < D / 32; ++u) {  // dV's columns, then dK's
-        const bool is_k = u >= D / 64;
-        const int col = (is_k ? u - D / 64 : u) * 16;
+      for (int is_k = 0; is_k < 2; ++is_k) {
         const float sc = is_k ? SIGN * a.scale : P_BACK;
-        float v[16];
-        if (steps > 0) tmem_ld16(lane_base + (is_k ? 384 : 256) + col0 + col, v);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = steps > 0 ? v[e] * sc : 0.f;
-        if (!live) continue;
-        if (a.splits == 1) {
-          T* dst = reinterpret_cast<T*>(is_k ? a.dk : a.dv) + at + col;
-          store_row8<T>(dst, v);
-          store_row8<T>(dst + 8, v + 8);
-        } else {
-          float4* dst = reinterpret_cast<float4*>(a.parts + (2 * split + (is_k ? 0 : 1)) * plane + at + col);
+        for (int u = 0; u < D / 64; ++u) {
+          float v[16];
+          if (steps > 0) tmem_ld16(lane_base + (is_k ? 384 : 256) + col0 + u * 16, v);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) dst[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          for (int e = 0; e < 16; ++e) v[e] = steps > 0 ? v[e] * sc : 0.f;
+          if (a.splits == 1) {
+            stage16<T, W>(stage, lane, u, v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<float4*>(stage_at<2 * W>(stage, lane, 4 * u + e)) =
+                  make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          }
         }
+        if (a.splits == 1)
+          stage_flush<W>(stage, reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(is_k ? a.dk : a.dv) + at),
+                         (int64_t)a.HKV * D * 2, seq.len - row0);
+        else
+          stage_flush<2 * W>(stage, reinterpret_cast<uint8_t*>(a.parts + (2 * split + (is_k ? 0 : 1)) * plane + at),
+                             (int64_t)a.HKV * D * 4, seq.len - row0);
       }
     }
   }

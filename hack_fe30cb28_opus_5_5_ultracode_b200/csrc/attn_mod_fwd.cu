@@ -94,9 +94,10 @@ __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, 
     }
   }
   if constexpr (MASKED) {
+    const uint32_t m[2] = {col_mask(rlo, rhi), col_mask(rlo - 32, rhi - 32)};
 #pragma unroll
     for (int i = 0; i < FWD_HC; ++i)
-      if (i < rlo || i >= rhi) x[i] = 0xff800000u;  // -inf
+      if (!(m[i >> 5] >> (i & 31) & 1)) x[i] = 0xff800000u;  // -inf
   }
 }
 
@@ -130,18 +131,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   if (q0 >= seq.len) return;  // the whole CTA, before any barrier or TMEM is set up
   const int kvh = h / (a.HQ / a.HKV);
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  AttnBlocks tb0 = attn_tile_blocks(seq, q0), tb1 = attn_tile_blocks(seq, q0 + AM_T);
-  tb0.first = uniform(tb0.first);
-  tb0.end = uniform(tb0.end);
-  tb1.first = uniform(tb1.first);
-  tb1.end = uniform(tb1.end);
-  // the blocks either tile visits: its own range, or the gap-free union where both have one
-  const bool any0 = tb0.end > tb0.first, any1 = tb1.end > tb1.first;
-  const int jb = !any1 || (any0 && tb0.first < tb1.first) ? tb0.first : tb1.first;
-  const int je = !any1 || (any0 && tb0.end > tb1.end) ? tb0.end : tb1.end;
-  auto visits = [&](int t, int j) { return t ? j >= tb1.first && j < tb1.end : j >= tb0.first && j < tb0.end; };
-
-  if (threadIdx.x == 0) {
+  // the loading warp sets the barriers up and sends for Q while the others allocate and look at the mask
+  if (warp == 18 && lane == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&s_full[s], 1);
@@ -158,11 +149,26 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       mbar_init(&kv_empty[s], 2);
     }
     fence_barrier_init();
-    prefetch_tmap(&tq);
-    prefetch_tmap(&tk);
-    prefetch_tmap(&tv);
+    for (int t = 0; t < 2; ++t) {
+      mbar_arrive_expect_tx(&q_full[t], C::TILE);
+      tma_load_3d(smem + t * C::TILE, &tq, &q_full[t], 0, seq.start + q0 + t * AM_T, h * (D / 64));
+    }
   }
   if (warp == 16) tmem_alloc(tmem_slot, 512);
+  AttnBlocks tb0 = attn_tile_blocks(seq, q0), tb1 = attn_tile_blocks(seq, q0 + AM_T);
+  tb0.first = uniform(tb0.first);
+  tb0.end = uniform(tb0.end);
+  tb1.first = uniform(tb1.first);
+  tb1.end = uniform(tb1.end);
+  // the blocks either tile visits: its own range, or the gap-free union where both have one
+  const bool any0 = tb0.end > tb0.first, any1 = tb1.end > tb1.first;
+  const int jb = !any1 || (any0 && tb0.first < tb1.first) ? tb0.first : tb1.first;
+  const int je = !any1 || (any0 && tb0.end > tb1.end) ? tb0.end : tb1.end;
+  auto visits = [&](int t, int j) { return t ? j >= tb1.first && j < tb1.end : j >= tb0.first && j < tb0.end; };
+  if (warp == 18 && lane == 0 && je > jb) {  // the first K
+    mbar_arrive_expect_tx(&kv_full[0], C::TILE);
+    tma_load_3d(smem + C::OFF_KV, &tk, &kv_full[0], 0, seq.start + jb * AM_T, kvh * (D / 64));
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -173,18 +179,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     int n = 0;  // ring positions filled
     uint32_t raw = 0;
     bool ok = true;
-    auto load_q = [&](int t) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&q_full[t], C::TILE);
-        tma_load_3d(smem + t * C::TILE, &tq, &q_full[t], 0, seq.start + q0 + t * AM_T, h * (D / 64));
-      }
-    };
-    if (je > jb) load_q(0);
     for (int j = jb; ok && j < je; ++j) {
       if (!visits(0, j) && !visits(1, j)) continue;
       const int row = j * AM_T;
 #pragma unroll
       for (int is_v = 0; is_v < 2; ++is_v, ++n) {
+        if (n == 0) continue;  // sent for above
         const int s = n % C::STAGES;
         uint32_t bad[4];
         const bool dirty = is_v && attn_dead_rows(seq, row, bad);
@@ -204,7 +204,6 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
           fence_proxy_async_smem();
           warp_arrive(&kv_full[s]);
         }
-        if (n == 0) load_q(1);
       }
     }
     if (!ok && lane == 0) {  // a wait ran out: let the copies in flight land before the CTA goes
@@ -387,8 +386,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     if (ok) {
       const float l_row = half ? *other + l_run : l_run + *other;
       const float inv = l_row > 0.f ? 1.f / l_row : (l_row == 0.f ? 0.f : l_row);  // NaN stays
-      T* out = reinterpret_cast<T*>(a.out_w) + ((int64_t)(seq.start + qi) * a.HQ + h) * D + half * (D / 2);
-#pragma unroll 1
+      // Q's tile has been read for the last time (or, with no block, has landed by now): the rows leave
+      // through it
+      if (tb.end == tb.first) warp_wait(&q_full[t], 0, err);
+      constexpr int W = D;  // bytes of half a row
+      uint8_t* stage = smem + t * C::TILE + (warp & 7) * 32 * W;
+#pragma unroll
       for (int u = 0; u < D / 32; ++u) {
         float ov[16];
         if (tb.end > tb.first) {
@@ -397,16 +400,17 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 16; ++e) ov[e] = 0.f;
         }
-        if (qi < seq.len) {
 #pragma unroll
-          for (int v = 0; v < 2; ++v)
-            reinterpret_cast<uint4*>(out + u * 16)[v] =
-                make_uint4(pack_t2<T>(ov[8 * v] * inv, ov[8 * v + 1] * inv),
-                           pack_t2<T>(ov[8 * v + 2] * inv, ov[8 * v + 3] * inv),
-                           pack_t2<T>(ov[8 * v + 4] * inv, ov[8 * v + 5] * inv),
-                           pack_t2<T>(ov[8 * v + 6] * inv, ov[8 * v + 7] * inv));
-        }
+        for (int v = 0; v < 2; ++v)
+          *reinterpret_cast<uint4*>(stage_at<W>(stage, lane, 2 * u + v)) =
+              make_uint4(pack_t2<T>(ov[8 * v] * inv, ov[8 * v + 1] * inv),
+                         pack_t2<T>(ov[8 * v + 2] * inv, ov[8 * v + 3] * inv),
+                         pack_t2<T>(ov[8 * v + 4] * inv, ov[8 * v + 5] * inv),
+                         pack_t2<T>(ov[8 * v + 6] * inv, ov[8 * v + 7] * inv));
       }
+      const int row = qi - lane;  // the warp's first
+      T* out = reinterpret_cast<T*>(a.out_w) + ((int64_t)(seq.start + row) * a.HQ + h) * D + half * (D / 2);
+      stage_flush<W>(stage, reinterpret_cast<uint8_t*>(out), (int64_t)a.HQ * D * 2, seq.len - row);
       if (qi < seq.len && half == 0)
         a.lse[(int64_t)h * a.n + seq.start + qi] = (m_run + log2f(l_row)) * 0.6931471805599453f;
     }
