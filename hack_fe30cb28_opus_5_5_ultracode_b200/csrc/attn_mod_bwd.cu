@@ -373,38 +373,49 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       const uint32_t sx = desc_lo_k(smem_u32(smem)), sy = sx + TILE16;
       const uint32_t uk = desc_lo_k(smem_u32(smem + C::OFF_U)), um = desc_lo_mn(smem_u32(smem + C::OFF_U), BOX);
       const uint32_t wk = desc_lo_k(smem_u32(smem + C::OFF_W)), wm = desc_lo_mn(smem_u32(smem + C::OFF_W), BOX);
+      auto u_landed = [&](int n) { return warp_wait(&u_full[n % C::UST], (n / C::UST) & 1, err); };
+      auto w_landed = [&](int n) { return warp_wait(&w_full[n % C::WST], (n / C::WST) & 1, err); };
       auto score = [&](int n) {  // S = X U^T
-        if (!warp_wait(&u_full[n % C::UST], (n / C::UST) & 1, err)) return false;
         tc_fence_after();
         umma_score<D>(tmem, sx, uk + (n % C::UST) * TILE16, id_s);
         warp_commit(s_full);
-        return true;
       };
       auto dprob = [&](int n) {  // dP = Y W^T
-        if (!warp_wait(&w_full[n % C::WST], (n / C::WST) & 1, err)) return false;
         tc_fence_after();
         umma_score<D>(tmem + 128, sy, wk + (n % C::WST) * TILE16, id_s);
         warp_commit(dp_full);
         if (!DKV) warp_commit(&w_empty[n % C::WST]);
-        return true;
       };
-      bool ok = warp_wait(xy_full, 0, err) && score(0) && dprob(0);
-      if (ok && steps > 1) ok = warp_wait(s_free, 0, err) && score(1);
+      bool ok = warp_wait(xy_full, 0, err) && u_landed(0);
+      if (ok) score(0);
+      ok = ok && w_landed(0);
+      if (ok) dprob(0);
+      if (steps > 1) {
+        ok = ok && u_landed(1) && warp_wait(s_free, 0, err);
+        if (ok) score(1);
+      }
+      // Copies are waited for ahead of the softmax warps: every instruction of this warp takes its turn
+      // among those of four of them.
       for (int n = 0; ok && n < steps; ++n) {
         const uint32_t u0 = um + (n % C::UST) * TILE16, w0 = wm + (n % C::WST) * TILE16;
+        const bool more = n + 1 < steps;
         ok = warp_wait(p_full, n & 1, err);
         if (!ok) break;
         tc_fence_after();
         umma_gather4(tmem + 256, tmem + 128, DKV ? w0 : u0, id_o, n > 0);
         if (DKV) warp_commit(&w_empty[n % C::WST]);
-        ok = warp_wait(ds_full, n & 1, err);
+        if (more) ok = w_landed(n + 1);
+        ok = ok && warp_wait(ds_full, n & 1, err);
         if (!ok) break;
         tc_fence_after();
         umma_gather4(tmem + 384, tmem + 128 + HC / 2, u0, id_o, n > 0);
-        warp_commit(&u_empty[n % C::UST]);
-        if (n + 1 < steps) ok = dprob(n + 1);
+        if (more) dprob(n + 1);
         else warp_commit(out_full);
-        if (ok && n + 2 < steps) ok = warp_wait(s_free, (n + 1) & 1, err) && score(n + 2);
+        warp_commit(&u_empty[n % C::UST]);
+        if (n + 2 < steps) {
+          ok = u_landed(n + 2) && warp_wait(s_free, (n + 1) & 1, err);
+          if (ok) score(n + 2);
+        }
       }
       if (!ok) {  // a wait ran out: the products already issued finish before TMEM is freed
         warp_commit(drain);
