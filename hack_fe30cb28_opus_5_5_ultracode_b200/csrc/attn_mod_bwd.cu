@@ -207,7 +207,8 @@ struct BwdCfg {
   static constexpr int OFF_Y = TILE, OFF_U = 2 * TILE, OFF_W = OFF_U + UST * TILE;
   static constexpr int OFF_L = OFF_W + WST * TILE;          // [2][2][128] fp32: -lse2, -Dvec by column;
                                                             // dQ role: [4][128] a row's partial sums
-  static constexpr int OFF_BAR = OFF_L + 4 * AM_T * 4;
+  static constexpr int OFF_D = OFF_L + 4 * AM_T * 4;        // dQ role: [128] Dvec of the 16-bit output
+  static constexpr int OFF_BAR = OFF_D + AM_T * 4;
   static constexpr int SMEM = OFF_BAR + 512;
 };
 
@@ -229,6 +230,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem[];  // no static shared memory: the base is aligned
   float* sL = reinterpret_cast<float*>(smem + C::OFF_L);
   float* sR = sL;
+  float* sD = reinterpret_cast<float*>(smem + C::OFF_D);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* xy_full = bars;
   uint64_t* s_full = bars + 1;
@@ -260,6 +262,22 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   const AttnSeq seq = attn_seq(a, b);
   if (r0 >= seq.len) return;  // the whole CTA, before any barrier or TMEM is set up
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  // dQ role: the tile's rows of O and dO for Dvec, eight rows a warp in whole lines (a thread per quarter
+  // row, as the softmax has them, took 12,000 cycles to read its way through 128 lines at a time)
+  constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes per row, rows per load
+  uint4 ov[8 / RPI], gv[8 / RPI];
+  if (!DKV && warp < 16) {
+#pragma unroll
+    for (int i = 0; i < 8 / RPI; ++i) {
+      const int row = r0 + warp * 8 + i * RPI + lane / LPR;
+      const int64_t at = ((int64_t)(seq.start + row) * a.HQ + h0) * D + (lane % LPR) * 8;
+      ov[i] = gv[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < seq.len) {
+        ov[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.out) + at);
+        gv[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.dout) + at);
+      }
+    }
+  }
   // the loading warp sets the barriers up while the others allocate and look at the mask
   if (warp == 17 && lane == 0) {
     mbar_init(xy_full, 1);
@@ -293,6 +311,19 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     mbar_arrive_expect_tx(xy_full, 2 * C::TILE);
     tma_load_3d(smem, &tx, xy_full, 0, seq.start + r0, zx);
     tma_load_3d(smem + C::OFF_Y, &ty, xy_full, 0, seq.start + r0, zx);
+  }
+  if (!DKV && warp < 16) {
+#pragma unroll
+    for (int i = 0; i < 8 / RPI; ++i) {
+      const T* ot = reinterpret_cast<const T*>(&ov[i]);
+      const T* gt = reinterpret_cast<const T*>(&gv[i]);
+      float dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dot = fmaf(to_f<T>(ot[e]), to_f<T>(gt[e]), dot);
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if (lane % LPR == 0) sD[warp * 8 + i * RPI + lane / LPR] = dot;
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -432,27 +463,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     BwdConst c = bwd_const<MODE>(a, h0);
     float neg_lse = -INFINITY, neg_d = 0.f, rest = 0.f;
     if constexpr (!DKV) {
-      // Dvec of the 16-bit output: each of the row's four threads takes a quarter of the head
-      const bool sees = range.y > range.x;
-      float dot = 0.f;
-      if (sees) {
-        const int64_t at = ((int64_t)(seq.start + ri) * a.HQ + h0) * D + part * (D / 4);
-        const uint4* o = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.out) + at);
-        const uint4* g = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.dout) + at);
-#pragma unroll
-        for (int u = 0; u < D / 32; ++u) {
-          const uint4 ov = o[u], gv = g[u];
-          const T* ot = reinterpret_cast<const T*>(&ov);
-          const T* gt = reinterpret_cast<const T*>(&gv);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) dot = fmaf(to_f<T>(ot[e]), to_f<T>(gt[e]), dot);
-        }
+      if (range.y > range.x) {  // a row that sees nothing keeps probability 0 and Dvec 0
         neg_lse = a.lse[(int64_t)h0 * a.n + seq.start + ri] * -1.4426950408889634f;
+        neg_d = -sD[r];
       }
-      sR[part * AM_T + r] = dot;
-      asm volatile("bar.sync 1, 512;" ::: "memory");
-      neg_d = -((sR[r] + sR[AM_T + r]) + (sR[2 * AM_T + r] + sR[3 * AM_T + r]));
-      asm volatile("bar.sync 1, 512;" ::: "memory");  // sR is written again at the end
     }
     bool ok = true;
     const uint32_t ts = lane_base + part * HC;
