@@ -271,8 +271,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
 // sequence, and the operand descriptors differ from step to step by a constant in their low word. So
 // the compiler can keep descriptors and addresses in uniform registers: issued by `if (lane == 0)`
 // from descriptors built per step, the 16 MMAs of a tile and block took 1,400-2,000 cycles of this
-// warp, longer than the tensor core needs for them (8,192 causal tokens, 12 heads: 220 us
-// against 198 us in this form).
+// warp, longer than the tensor core needs for them (forward of 8,192 causal tokens, 12 heads: 10%).
 __device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 
 // A value every lane holds, as one the compiler knows to be the same (what comes from memory it takes to

@@ -17,9 +17,11 @@
 // as 16-bit values, into the tensor-memory columns that dP leaves when it has been read (each thread
 // 16 + 16 of its own 32 columns) and are the A operand of acc1 and acc2. The tensor core's acc1, acc2
 // and next dP then run beside the next step's P. (With P in S's columns the next S had to wait for
-// acc1: 650 us
-// instead of 620 for 8,192 causal tokens of 12 + 2 heads.) Sixteen softmax warps, four
-// threads per TMEM lane with 32 of the 128 columns each (no row reduction: the forward's lse is known).
+// acc1, and 8,192 causal tokens of 12 + 2 heads took 5% longer.) Sixteen softmax warps, four threads
+// per TMEM lane with 32 of the 128 columns each (no row reduction: the forward's lse is known).
+//
+// That shape takes 601 us for both launches (forward: 162): eight products at 1,370 TFLOP/s, what the
+// tensor cores sustain under the board's power limit. Twice the softmax's exponentials ride along.
 //
 // Why the dQ role needs P K: Dvec from the forward's 16-bit output is off by the output's rounding,
 // and that error enters a whole row of dS with one sign - dQ was up to 1.9 times as far from the
@@ -93,7 +95,7 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
     for (int e = 0; e < 8; ++e) {
       float ya, yb;
       up2(y[e], ya, yb);
-      y[e] = pk2(ya - fabsf(c.slope2 * (dist0 - (float)(2 * e))), yb - fabsf(c.slope2 * (dist0 - (float)(2 * e + 1))));
+      y[e] = pk2(ya - c.slope2 * fabsf(dist0 - (float)(2 * e)), yb - c.slope2 * fabsf(dist0 - (float)(2 * e + 1)));
     }
   }
 #pragma unroll
@@ -629,11 +631,9 @@ __global__ void __launch_bounds__(256) attn_mod_sum_kernel(const AttnModArgs a, 
 }
 
 // How many CTAs share a KV head's query heads: as few as keep the longest CTA (a key block that
-// every query tile sees) under SPLIT_SHARE of an SM's share of all tiles, because each split costs a
-// write and a read of fp32 dk and dv.
-#ifndef SPLIT_SHARE
-#define SPLIT_SHARE 0.8
-#endif
+// every query tile sees) under this fraction of an SM's share of all tiles, because each split costs a
+// write and a read of fp32 dk and dv (8,192 causal tokens, 12 + 2 heads: 3% longer with 0.5 than with 0.8).
+constexpr double SPLIT_SHARE = 0.8;
 int dkv_splits(const AttnModArgs& a) {
   const int group = a.HQ / a.HKV;
   const double tiles = (double)cdiv(a.max_len, AM_T);

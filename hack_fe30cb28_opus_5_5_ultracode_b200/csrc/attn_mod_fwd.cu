@@ -37,6 +37,11 @@ struct FwdCfg {
 constexpr int FWD_THREADS = 608;
 constexpr int FWD_HC = 64;  // columns per softmax thread
 
+// fp16 probabilities are kept as 2^7 P (at most 2^15, as P is at most 2^8 under a maximum that lags),
+// so that the many small ones of a long row stay normal numbers; the row sum has the same factor.
+template <typename T>
+constexpr float FWD_P_SHIFT = std::is_same<T, __half>::value ? 7.f : 0.f;
+
 // What the score's modes need per kernel.
 struct ScoreConst {
   float sl2;    // scale * log2(e): plain scores
@@ -90,7 +95,7 @@ __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, 
     } else {
 #pragma unroll
       for (int i = 0; i < FWD_HC; i += 2)
-        unpair(fma2(pair_of(x + i), mul, pk2(-fabsf(slope2 * (dist0 - (float)i)), -fabsf(slope2 * (dist0 - (float)(i + 1))))), x + i);
+        unpair(fma2(pair_of(x + i), mul, pk2(-slope2 * fabsf(dist0 - (float)i), -slope2 * fabsf(dist0 - (float)(i + 1)))), x + i);
     }
   }
   if constexpr (MASKED) {
@@ -333,7 +338,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         corr = m_run == -INFINITY ? 0.f : ex2(m_run - ms);
         m_run = ms;
       }
-      const float mneg = m_run == -INFINITY ? 0.f : -m_run;
+      const float mneg = m_run == -INFINITY ? 0.f : FWD_P_SHIFT<T> - m_run;
       if (n > 0) {  // O_t += P_t V of the last block is complete: P_t may be written, O_t rescaled
         ok = warp_wait(&o_full[t], (n - 1) & 1, err);
         if (!ok) break;
@@ -412,7 +417,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       T* out = reinterpret_cast<T*>(a.out_w) + ((int64_t)(seq.start + row) * a.HQ + h) * D + half * (D / 2);
       stage_flush<W>(stage, reinterpret_cast<uint8_t*>(out), (int64_t)a.HQ * D * 2, seq.len - row);
       if (qi < seq.len && half == 0)
-        a.lse[(int64_t)h * a.n + seq.start + qi] = (m_run + log2f(l_row)) * 0.6931471805599453f;
+        a.lse[(int64_t)h * a.n + seq.start + qi] = (m_run - FWD_P_SHIFT<T> + log2f(l_row)) * 0.6931471805599453f;
     }
   }
   tc_fence_before();
@@ -534,6 +539,8 @@ int attn_mod_check(const ql_attn_mod_args& m, AttnModArgs& a) {
   if ((int64_t)m.HQ * m.B > 0x7fffffff || cdiv(m.max_len, AM_T) > 65535) return QL_STATUS_UNSUPPORTED;
   if (!(m.scale > 0.f && m.scale < INFINITY) || !(m.softcap >= 0.f && m.softcap < INFINITY))
     return QL_STATUS_BAD_ARG;
+  // tanh_short's coefficients hold (scale / softcap)^7: finite up to 10^4, a cap that bends every score
+  if (m.softcap > 0.f && m.softcap < 1e-4f * m.scale) return QL_STATUS_BAD_ARG;
   if (m.n > 0 && m.B > 0 && (m.q == nullptr || m.k == nullptr || m.v == nullptr || m.out == nullptr ||
                              m.lse == nullptr || m.cu_seqlens == nullptr))
     return QL_STATUS_BAD_ARG;

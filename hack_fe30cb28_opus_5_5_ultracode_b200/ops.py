@@ -735,7 +735,11 @@ def _attn_mod_inputs(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slope
         ld, inner, unit = t.stride()
         if n and (unit != 1 or (inner != D and heads > 1)):
             raise ValueError(f"{name}'s heads must be contiguous within a row")
-        strides.append(ld if n > 1 else heads * D)
+        if n < 2:
+            ld = heads * D
+        if ld < heads * D or ld & 7 or t.data_ptr() & 15:
+            raise ValueError(f"{name}'s rows must start at multiples of 16 bytes and not overlap")
+        strides.append(ld)
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must be int32 [sequences + 1]")
     B = cu_seqlens.shape[0] - 1
@@ -751,6 +755,8 @@ def _attn_mod_inputs(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slope
     if not (0 <= max_len <= n and window >= 0 and 0 < scale < _INF and 0 <= softcap < _INF):
         raise ValueError("needs 0 <= max_len <= tokens, window >= 0, 0 < scale < inf and "
                          "0 <= softcap < inf")
+    if 0 < softcap < 1e-4 * scale:
+        raise ValueError("a softcap below 1e-4 scale is not supported")
     return n, HQ, HKV, D, B, strides, _DT[dt], dev, min(window, INT_MAX)
 
 
@@ -764,7 +770,7 @@ def attn_mod_fwd(q, k, v, cu_seqlens, max_len, scale, causal=True, softcap=0.0, 
     tanh(x / softcap); a query sees key j if j <= i or j < prefix_len[b] (causal), |i - j| < window
     (window > 0), and both are in the same run of equal doc_ids (negative ids: padding). slopes
     fp32 [HQ], doc_ids int32 [n], prefix_len int32 [B]. out as q (contiguous), lse fp32 [HQ, n];
-    a query that sees nothing gets out 0 and lse -inf."""
+    a query that sees nothing gets out 0 and lse -inf. Rows behind the last sequence are not written."""
     n, HQ, HKV, D, B, ld, dt, dev, window = _attn_mod_inputs(
         q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes, window, doc_ids, prefix_len)
     if out is None:

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from hack_fe30cb28_opus_5_5_ultracode_b200 import ops
+from hack_fe30cb28_opus_5_5_ultracode_b200 import _lib, ops
 
 
 def allowed_keys(length, causal=True, window=0, prefix=0, ids=None):
@@ -161,3 +161,289 @@ def test_backward_matches_the_formula(lengths, mode, heads, dtype):
         # the rounding of out inside dout . out: 2^-8 or 2^-11 of |dout| |out| ~ D
         floor = TOL[dtype] * 0.02 * y.numel() ** 0.5
         assert (x.double().cpu() - y).norm().item() < TOL[dtype] * y.norm().item() + floor, name
+
+
+ALL = dict(docs=True, prefix=True, window=90, softcap=30.0, slopes=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(4, 4, 64), (2, 1, 128)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_slices_of_a_fused_row_with_nan_in_the_padding(heads, dtype):
+    """q, k and v as slices of one buffer; padding tokens and rows behind the last sequence hold NaN and
+    infinities, which reach nothing, and the outputs' rows behind the last sequence stay."""
+    HQ, HKV, D = heads
+    lengths, extra = [200, 0, 333], 61
+    n = sum(lengths) + extra
+    q, k, v, dout, cu = batch(lengths, heads, dtype, seed=2, extra=extra)
+    host, dev = mode_args(ALL, lengths, HQ, seed=3, extra=extra)
+    for a, b in ((0, 3), (120, 140), (195, 230), (400, 401)):
+        host["doc_ids"][a:b] = -1
+    dev["doc_ids"].copy_(host["doc_ids"])
+    bad = (host["doc_ids"] < 0).cuda()
+    bad[n - extra:] = True
+    fused = torch.cat([t.flatten(1) for t in (q, k, v)], 1)
+    fused[bad] = torch.tensor([math.nan, math.inf, -math.inf], dtype=dtype).cuda()[
+        torch.arange(int(bad.sum())).cuda() % 3][:, None]
+    dout[bad] = math.nan
+    s = [fused[:, a:b].unflatten(1, (-1, D)) for a, b in
+         ((0, HQ * D), (HQ * D, (HQ + HKV) * D), ((HQ + HKV) * D, (HQ + 2 * HKV) * D))]
+    mark = 7.0
+    out, lse = torch.full_like(q, mark), torch.full((HQ, n), mark, device="cuda")
+    grads = [torch.full_like(t, mark) for t in (q, k, v)]
+    ops.attn_mod_fwd(*s, cu, 333, D ** -0.5, out=out, lse=lse, **dev)
+    ops.attn_mod_bwd(dout, *s, out, lse, cu, 333, D ** -0.5, dq=grads[0], dk=grads[1], dv=grads[2],
+                     **dev)
+    assert ops.device_status() == 0
+    want = formula(q, k, v, lengths, D ** -0.5,
+                   dout=torch.where(bad[:, None, None], 0, dout), **host)
+    for x in (out, *grads):
+        assert (x[n - extra:] == mark).all()
+    assert (lse[:, n - extra:] == mark).all()
+    assert not any(x[bad][:-extra].any() for x in (out, *grads))
+    assert torch.isneginf(lse[:, bad][:, :-extra]).all()
+    for x, y in zip((out, *grads), (want[0], *want[2:])):
+        x, y = x.double().cpu()[:n - extra], y[:n - extra]
+        floor = TOL[dtype] * 0.02 * y.numel() ** 0.5  # see test_backward_matches_the_formula
+        assert (x - y).norm().item() < TOL[dtype] * y.norm().item() + floor
+
+
+@pytest.mark.gpu
+def test_repeats_other_streams_replays_and_two_graphs_agree_to_the_bit():
+    lengths, heads, scale = [700, 1, 450], (6, 2, 64), 0.125
+    q, k, v, dout, cu = batch(lengths, heads, torch.bfloat16, seed=4)
+    _, dev = mode_args(ALL, lengths, heads[0])
+
+    def run():
+        out, lse = ops.attn_mod_fwd(q, k, v, cu, 700, scale, **dev)
+        return (out, lse, *ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 700, scale, **dev))
+
+    first = run()
+    same = lambda got: all(torch.equal(a, b) for a, b in zip(first, got))  # noqa: E731
+    assert same(run())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, results = [], []
+    with torch.cuda.stream(side):
+        assert same(run())
+        for _ in range(2):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=side):
+                results.append(run())
+    both = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for t in (t for r in results for t in r):
+        t.zero_()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, g in zip(both, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(same(r) for r in results)
+    # new contents in the captured tensors are read anew
+    q.copy_(q.flip(0))
+    graphs[0].replay()
+    again = run()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(again, results[0])) and not same(again)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_len", [130, 131, 200, 277])
+def test_max_len_may_be_longer_than_the_sequences(max_len):
+    lengths, heads = [130, 17, 130], (4, 1, 64)
+    q, k, v, dout, cu = batch(lengths, heads, torch.float16, seed=5)
+    want = formula(q, k, v, lengths, 0.125, dout=dout)
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, max_len, 0.125)
+    got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, max_len, 0.125)
+    for x, y in zip((out, *got), (want[0], *want[2:])):
+        assert rel(x, y) < 1.5 * TOL[torch.float16]
+
+
+@pytest.mark.gpu
+def test_a_window_beyond_every_length_is_none():
+    q, k, v, dout, cu = batch([300, 5], (2, 2, 128), torch.bfloat16, seed=6)
+    for causal in (True, False):
+        want = ops.attn_mod_fwd(q, k, v, cu, 300, 0.1, causal=causal)
+        for window in (300, ops.INT_MAX, 1 << 40):
+            got = ops.attn_mod_fwd(q, k, v, cu, 300, 0.1, causal=causal, window=window)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            g = ops.attn_mod_bwd(dout, q, k, v, *got, cu, 300, 0.1, causal=causal, window=window)
+            assert torch.isfinite(torch.cat([x.flatten() for x in g])).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [dict(), dict(softcap=40.0), dict(slopes="negative")], ids=str)
+@pytest.mark.parametrize("dtype,std", [(torch.bfloat16, 6.0), (torch.float16, 0.05)], ids=str)
+def test_scores_of_hundreds_and_of_nearly_nothing(mode, dtype, std):
+    """std 6: scores up to ~150, rows that one key takes almost whole; a distance bias that grows with
+    the distance (negative slopes)."""
+    lengths, heads = [290, 129], (4, 2, 64)
+    q, k, v, dout, cu = batch(lengths, heads, dtype, seed=7, std=std)
+    mode = dict(mode)
+    if mode.get("slopes") == "negative":
+        mode["slopes"] = -torch.tensor([0.5, 0.25, 0.01, 0.002])
+    dev = {a: b.cuda() if torch.is_tensor(b) else b for a, b in mode.items()}
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, 290, 0.125, **dev)
+    got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 290, 0.125, **dev)
+    want = formula(q, k, v, lengths, 0.125, dout=dout, **mode)
+    assert rel(out, want[0]) < TOL[dtype]
+    # fp32 sums of 64 products |q k| of up to ~70, off by at most 64 x 2^-24 x their sum (~360)
+    assert (lse.double().cpu() - want[1]).abs().max().item() < 64 * 2.0 ** -24 * 360
+    for x, y in zip(got, want[2:]):
+        floor = TOL[dtype] * 0.02 * max(std, 1) * y.numel() ** 0.5
+        assert (x.double().cpu() - y).norm().item() < TOL[dtype] * y.norm().item() + floor
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [dict(), dict(window=5000, softcap=30.0), dict(slopes=True)], ids=str)
+def test_long_rows(mode):
+    """33,001 tokens, rows of the result checked in 64 bits: one key's score is 10 above the rest, whose
+    probabilities near 2^-15 together weigh as much as it."""
+    n, heads, dtype = 33001, (2, 1, 64), torch.float16
+    q, k, v, dout, cu = batch([n], heads, dtype, seed=8, std=0.5)
+    q[..., 0] = 4.0
+    k[..., 0] = 0.0
+    k[3, 0, 0] = 20.0   # 4 x 20 x 0.125 = 10 above
+    host, dev = mode_args(mode, [n], 2)
+    rows = torch.tensor([0, 1, 127, 128, 4095, 20000, 32895, 32896, 33000])
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, n, 0.125, **dev)
+    grads = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, n, 0.125, **dev)
+    assert ops.device_status() == 0
+    kk, vv = k[:, 0].double().cpu(), v[:, 0].double().cpu()
+    want, want_dq = torch.zeros(len(rows), 2, 64).double(), torch.zeros(len(rows), 2, 64).double()
+    for h in range(2):
+        x = q[rows, h].double().cpu() @ kk.t() * 0.125
+        bend = torch.ones_like(x)
+        if "softcap" in mode:
+            bend = 1 - torch.tanh(x / 30) ** 2
+            x = 30 * torch.tanh(x / 30)
+        away = rows[:, None] - torch.arange(n)[None]
+        if "slopes" in mode:
+            x = x - float(host["slopes"][h]) * away.abs()
+        ok = (away >= 0) & (away < mode.get("window", n))
+        p = torch.softmax(x.masked_fill(~ok, -math.inf), -1)
+        want[:, h] = p @ vv
+        go = dout[rows, h].double().cpu()
+        ds = p * (go @ vv.t() - (go * want[:, h]).sum(-1, keepdim=True)) * bend * 0.125
+        want_dq[:, h] = ds @ kk
+    assert rel(out[rows], want) < TOL[dtype]
+    # fp16 dS of 2^-15 |dP - Dvec| (|dP - Dvec| ~ 8): steps of 2^-24, off by at most 2^-13 of it more
+    assert rel(grads[0][rows], want_dq) < TOL[dtype] + 2.0 ** -13
+    assert all(torch.isfinite(x).all() for x in grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [dict(causal=False), ALL, dict(prefix=True, softcap=3.0)], ids=str)
+def test_gradients_against_differences(mode):
+    """The derivative along the gradient's own direction is its norm: the formula's output moved both
+    ways along it, in 64 bits (the differences' own error is 1e-6 of it)."""
+    lengths, heads, dtype = [150, 61], (4, 2, 64), torch.bfloat16
+    q, k, v, dout, cu = batch(lengths, heads, dtype, seed=9)
+    host, dev = mode_args(mode, lengths, 4)
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, 150, 0.125, **dev)
+    grads = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 150, 0.125, **dev)
+    for at in range(3):
+        step = grads[at].double().cpu()
+        size = step.norm()
+        step = step / size * 1e-3
+        sides = []
+        for sign in (1, -1):
+            x = [t.double().cpu() for t in (q, k, v)]
+            x[at] = x[at] + sign * step
+            sides.append((formula(*x, lengths, 0.125, **host)[0] * dout.double().cpu()).sum())
+        slope = (sides[0] - sides[1]) / 2e-3
+        assert abs(slope - size) < TOL[dtype] * size
+
+
+@pytest.mark.gpu
+def test_no_tokens_and_no_sequences():
+    for lengths in ([], [0, 0]):
+        q, k, v, dout, cu = batch(lengths, (4, 2, 64), torch.float16)
+        cu = torch.zeros(len(lengths) + 1, dtype=torch.int32, device="cuda")
+        out, lse = ops.attn_mod_fwd(q, k, v, cu, 0, 0.125)
+        got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 0, 0.125)
+        assert [t.shape for t in got] == [q.shape, k.shape, v.shape] and lse.shape == (4, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("change", [
+    dict(scale=0.0), dict(scale=math.inf), dict(scale=math.nan), dict(softcap=-1.0),
+    dict(softcap=math.nan), dict(softcap=1e-6), dict(window=-1), dict(max_len=-1), dict(max_len=11),
+    dict(k="heads"), dict(k="dtype"), dict(k="short"), dict(k="order"), dict(k="odd"),
+    dict(v="expand"), dict(cu="long"), dict(cu="none"), dict(slopes="short"), dict(slopes="half"),
+    dict(doc_ids="short"), dict(prefix_len="short"), dict(prefix_len="ok", causal=False),
+    dict(doc_ids="cpu"), dict(D=96), dict(dtype=torch.float32), dict(out="dtype"),
+    dict(lse="shape")], ids=str)
+def test_bad_arguments_are_refused(change):
+    D, dtype = change.get("D", 64), change.get("dtype", torch.float16)
+    q, k, v, dout, cu = batch([10], (4, 2, D), dtype)
+    kw = dict(causal=change.get("causal", True))
+    kw.update({x: change[x] for x in ("softcap", "window") if x in change})
+    kind = change.get("k")
+    k = {"heads": k[:, :1].repeat(1, 3, 1), "dtype": k.bfloat16(), "short": k[:9],
+         "order": k.transpose(0, 1).contiguous().transpose(0, 1),
+         "odd": torch.zeros(10 * 2 * D + 1, device="cuda", dtype=dtype)[1:].view(10, 2, D)}.get(kind, k)
+    if "v" in change:
+        v = v[:1].expand(10, 2, D)
+    cu = {"long": cu.long(), "none": cu[:0]}.get(change.get("cu"), cu)
+    extra = {"slopes": {"short": torch.ones(3), "half": torch.ones(4).half()},
+             "doc_ids": {"short": torch.zeros(9).int(), "cpu": torch.zeros(10).int()},
+             "prefix_len": {"short": torch.zeros(2).int(), "ok": torch.zeros(1).int()}}
+    for name, kinds in extra.items():
+        if name in change:
+            t = kinds[change[name]]
+            kw[name] = t if change[name] == "cpu" else t.cuda()
+    if "out" in change:
+        kw["out"] = q.float()
+    if "lse" in change:
+        kw["lse"] = torch.zeros(10, 4, device="cuda")
+    args = (cu, change.get("max_len", 10), change.get("scale", 0.125))
+    with pytest.raises(ValueError):
+        ops.attn_mod_fwd(q, k, v, *args, **kw)
+    out, lse = kw.pop("out", q), kw.pop("lse", torch.zeros(4, 10, device="cuda"))
+    with pytest.raises(ValueError):
+        ops.attn_mod_bwd(dout, q, k, v, out, lse, *args, **kw)
+
+
+def test_cpu_tensors_are_refused():
+    q, kv = torch.zeros(4, 2, 64).half(), torch.zeros(4, 1, 64).half()
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.attn_mod_fwd(q, kv, kv, cu, 4, 0.125)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.attn_mod_bwd(q, q, kv, kv, q, torch.zeros(2, 4), cu, 4, 0.125)
+
+
+def fake_args(**change):
+    """Arguments the library checks before it launches anything (made-up, aligned addresses)."""
+    f = dict(q=1 << 12, k=2 << 12, v=3 << 12, out=4 << 12, lse=5 << 12, cu_seqlens=6 << 12,
+             dout=7 << 12, dq=8 << 12, dk=9 << 12, dv=10 << 12, workspace=11 << 12,
+             workspace_floats=1 << 20, ldq=256, ldk=128, ldv=128, scale=0.125, softcap=0.0, n=10,
+             B=1, max_len=10, HQ=4, HKV=2, D=64, dtype=0, causal=1, window=0)
+    f.update(change)
+    return _lib.struct("ql_attn_mod_args", **f)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(D=96), 3), (dict(dtype=2), 1), (dict(n=-1), 1), (dict(max_len=11), 1), (dict(HKV=3), 1),
+    (dict(HKV=0), 1), (dict(window=-1), 1), (dict(scale=0.0), 1), (dict(scale=math.nan), 1),
+    (dict(softcap=-1.0), 1), (dict(softcap=1e-6), 1), (dict(q=None), 1), (dict(k=(2 << 12) + 8), 1),
+    (dict(ldk=130), 1), (dict(ldk=64), 1), (dict(cu_seqlens=None), 1), (dict(lse=None), 1),
+    (dict(doc_ids=1 << 16), 1), (dict(doc_ids=1 << 16, ranges=(1 << 17) + 4), 1),
+    (dict(B=1 << 30), 3), (dict(n=1 << 24, max_len=1 << 24), 3), (dict(n=1 << 30), 1)], ids=str)
+def test_the_library_refuses_before_any_launch(change, status):
+    for entry in ("ql_attn_mod_fwd", "ql_attn_mod_bwd"):
+        args = fake_args(**change)
+        with pytest.raises(_lib.QLError) as e:
+            _lib.call(entry, ops.ctypes_ref(args), None)
+        assert e.value.status == status
+
+
+@pytest.mark.parametrize("change", [dict(dout=None), dict(dk=None), dict(dv=(10 << 12) + 2),
+                                    dict(workspace=None)], ids=str)
+def test_the_backward_refuses_before_any_launch(change):
+    args = fake_args(**change)
+    with pytest.raises(_lib.QLError) as e:
+        _lib.call("ql_attn_mod_bwd", ops.ctypes_ref(args), None)
+    assert e.value.status == ops.STATUS_BAD_ARG
