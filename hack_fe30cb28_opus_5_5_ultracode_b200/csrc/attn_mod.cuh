@@ -343,41 +343,47 @@ __device__ __forceinline__ void warp_commit(uint64_t* bar) {
 }
 
 // Which of the 128 rows [j0, j0 + 128) of a tile hold no key or query of the sequence (past its
-// end, or padding), as bits: word u of lane l's result covers rows 32 u .. 32 u + 31 (every lane
-// gets the same words). Their tile rows are zeroed before a tensor-core product, because a
-// masked probability of 0 times a NaN or infinity left in such a row would not be 0.
-__device__ __forceinline__ bool attn_dead_rows(const AttnSeq& s, int j0, uint32_t bad[4]) {
-  if (j0 + AM_T <= s.len && s.docs == nullptr) return false;
+// end, or padding), as bits: word u covers rows 32 u .. 32 u + 31 (every lane gets the same words).
+// Their tile rows are zeroed before a tensor-core product, because a masked probability of 0 times a
+// NaN or infinity left in such a row would not be 0.
+struct DeadRows {
+  uint32_t w[4];
+  bool any;
+};
+__device__ __forceinline__ DeadRows attn_dead_rows(const AttnSeq& s, int j0) {
+  DeadRows d{{0u, 0u, 0u, 0u}, false};
+  if (j0 + AM_T <= s.len && s.docs == nullptr) return d;
   const int lane = threadIdx.x & 31;
-  uint32_t any = 0;
+  bool dead[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int r = j0 + u * 32 + lane;
-    bool dead = r >= s.len;
-    if (!dead && s.docs != nullptr) {
-      const int2 d = s.docs[r];
-      dead = d.x >= d.y;
+    dead[u] = r >= s.len;
+    if (!dead[u] && s.docs != nullptr) {
+      const int2 e = s.docs[r];
+      dead[u] = e.x >= e.y;
     }
-    bad[u] = __ballot_sync(0xffffffffu, dead);
-    any |= bad[u];
   }
-  return any != 0;
-}
-// Zeroes those rows of a [boxes][128 rows][128 bytes] tile (whole rows, so the swizzle inside a
-// row does not matter), by one warp.
-template <int BOXES>
-__device__ __forceinline__ void attn_zero_rows(uint8_t* tile, const uint32_t bad[4]) {
-  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    uint32_t m = bad[u];
-    while (m != 0) {
-      const int r = u * 32 + __ffs(m) - 1;
-      m &= m - 1;
-      if (lane < 8 * BOXES)
-        *reinterpret_cast<uint4*>(tile + (lane >> 3) * (AM_T * 128) + r * 128 + (lane & 7) * 16) =
-            make_uint4(0u, 0u, 0u, 0u);
-    }
+    d.w[u] = __ballot_sync(0xffffffffu, dead[u]);
+    d.any |= d.w[u] != 0;
+  }
+  return d;
+}
+// Zeroes those rows of a [boxes][128 rows][128 bytes] tile (whole rows, so the swizzle inside a
+// row does not matter), by one warp: two or four rows a store.
+template <int BOXES>
+__device__ __forceinline__ void attn_zero_rows(uint8_t* tile, const DeadRows& d) {
+  constexpr int ROWS = 4 / BOXES;
+  const int lane = threadIdx.x & 31, sub = lane / (8 * BOXES);
+  uint8_t* at = tile + (lane >> 3) % BOXES * (AM_T * 128) + sub * 128 + (lane & 7) * 16;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (d.w[u] == 0) continue;
+#pragma unroll
+    for (int i = 0; i < 32; i += ROWS)
+      if (d.w[u] >> (i + sub) & 1) *reinterpret_cast<uint4*>(at + (u * 32 + i) * 128) = make_uint4(0u, 0u, 0u, 0u);
   }
 }
 

@@ -239,7 +239,6 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   uint64_t* dp_full = bars + 2;
   uint64_t* ds_full = bars + 3;  // dS written (all softmax warps)
   uint64_t* out_full = bars + 4;
-  uint64_t* raw = bars + 5;
   uint64_t* drain = bars + 6;
   uint64_t* p_full = bars + 7;   // P written, dP read (all softmax warps)
   uint64_t* s_free = bars + 8;   // S read (all softmax warps)
@@ -249,7 +248,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   uint64_t* u_empty = u_full + C::UST;
   uint64_t* w_full = u_empty + C::UST;  // [WST]
   uint64_t* w_empty = w_full + C::WST;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(w_empty + C::WST);
+  uint64_t* raw = w_empty + C::WST;     // [UST + WST] copies whose dead rows are zeroed first
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw + C::UST + C::WST);
 
   const int group = a.HQ / a.HKV;
   const int per_seq = DKV ? a.HKV * a.splits : a.HQ;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     mbar_init(p_full, BWD_SOFTMAX / 32);
     mbar_init(s_free, BWD_SOFTMAX / 32);
     mbar_init(out_full, 1);
-    mbar_init(raw, 1);
+    for (int k = 0; k < C::UST + C::WST; ++k) mbar_init(&raw[k], 1);
     mbar_init(drain, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&l_full[s], 1);
@@ -334,18 +334,51 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 
   if (warp == 17) {
     // ---- loads ----
+    // U two steps ahead, W one. Tiles with rows that belong to no query or key land on a raw barrier and
+    // are handed on when those rows have been zeroed, before any product reads them; what the waits
+    // for room need is always handed on before them.
     bool ok = true;
-    int un = 0, wn = 0;
-    uint32_t raw_phase = 0;
+    int un = 0, wn = 0;        // tiles sent for
+    uint32_t raw_phase = 0;    // of raw[0 .. UST + WST)
+    auto row_of = [&](int n) { return (tb.first + (DKV ? n % ntile : n)) * AM_T; };
+    auto send = [&](int n, bool is_w, const DeadRows& d) {
+      const int s = is_w ? n % C::WST : n % C::UST;
+      const int z = (DKV ? h0 + n / ntile : kvh) * (D / 64);
+      uint64_t* bar = d.any ? &raw[is_w ? C::UST + s : s] : is_w ? &w_full[s] : &u_full[s];
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, C::TILE);
+        tma_load_3d(smem + (is_w ? C::OFF_W : C::OFF_U) + s * C::TILE, is_w ? &tw : &tu, bar, 0,
+                    seq.start + row_of(n), z);
+      }
+      if (is_w) wn = n + 1;
+      else un = n + 1;
+    };
+    auto clean = [&](int n, bool is_w, const DeadRows& d) {
+      if (!d.any) return true;
+      const int s = is_w ? n % C::WST : n % C::UST, k = is_w ? C::UST + s : s;
+      if (!warp_wait(&raw[k], (raw_phase >> k) & 1, err)) return false;
+      raw_phase ^= 1u << k;
+      attn_zero_rows<D / 64>(smem + (is_w ? C::OFF_W : C::OFF_U) + s * C::TILE, d);
+      fence_proxy_async_smem();
+      warp_arrive(is_w ? &w_full[s] : &u_full[s]);
+      return true;
+    };
+    DeadRows d0{{0u, 0u, 0u, 0u}, false}, d1 = d0, d2 = d0;  // of steps n, n + 1, n + 2
+    if (steps > 0) {
+      d0 = attn_dead_rows(seq, row_of(0));
+      send(0, false, d0);
+      send(0, true, d0);
+    }
+    if (steps > 1) {
+      d1 = attn_dead_rows(seq, row_of(1));
+      send(1, false, d1);
+      send(1, true, d1);
+    }
     for (int n = 0; ok && n < steps; ++n) {
-      const int row = (tb.first + (DKV ? n % ntile : n)) * AM_T;
-      const int h = DKV ? h0 + n / ntile : 0, zu = (DKV ? h : kvh) * (D / 64);
-      // rows of U and W that belong to no query or key are zeroed before any product reads them
-      uint32_t bad[4];
-      const bool dirty = attn_dead_rows(seq, row, bad);
       float l[4], dv[4];
       if constexpr (DKV) {
-        const int64_t at = (int64_t)h * a.n + seq.start + row;
+        const int row = row_of(n);
+        const int64_t at = (int64_t)(h0 + n / ntile) * a.n + seq.start + row;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int t = u * 32 + lane;
@@ -353,31 +386,9 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
           dv[u] = row + t < seq.len ? a.dvec[at + t] : 0.f;
         }
       }
-      auto load = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* full) {
-        uint64_t* bar = dirty ? raw : full;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar, C::TILE);
-          tma_load_3d(dst, map, bar, 0, seq.start + row, zu);
-        }
-        if (!dirty) return true;
-        if (!warp_wait(raw, raw_phase, err)) return false;
-        raw_phase ^= 1;
-        attn_zero_rows<D / 64>(dst, bad);
-        fence_proxy_async_smem();
-        warp_arrive(full);
-        return true;
-      };
-      const int us = n % C::UST, ws = n % C::WST;
-      if (n >= C::UST) ok = warp_wait(&u_empty[us], (n / C::UST - 1) & 1, err);
-      if (ok) ok = load(&tu, smem + C::OFF_U + us * C::TILE, &u_full[us]);
-      if (!ok) break;
-      un = n + 1;
-      if (n >= C::WST) ok = warp_wait(&w_empty[ws], (n / C::WST - 1) & 1, err);
-      if (ok) ok = load(&tw, smem + C::OFF_W + ws * C::TILE, &w_full[ws]);
-      if (!ok) break;
-      wn = n + 1;
+      ok = clean(n, false, d0) && clean(n, true, d0);
       if constexpr (DKV) {
-        if (n >= 2) ok = warp_wait(&l_empty[n & 1], ((n >> 1) - 1) & 1, err);
+        if (ok && n >= 2) ok = warp_wait(&l_empty[n & 1], ((n >> 1) - 1) & 1, err);
         if (!ok) break;
         float* sl = sL + (n & 1) * 2 * AM_T;
 #pragma unroll
@@ -389,13 +400,25 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         }
         warp_arrive(&l_full[n & 1]);
       }
+      if (n > 0 && n + 1 < steps) {
+        ok = ok && warp_wait(&w_empty[(n + 1) % C::WST], ((n + 1) / C::WST - 1) & 1, err);
+        if (ok) send(n + 1, true, d1);
+      }
+      if (n + 2 < steps) {
+        d2 = attn_dead_rows(seq, row_of(n + 2));
+        if (n + 2 >= C::UST) ok = ok && warp_wait(&u_empty[(n + 2) % C::UST], ((n + 2) / C::UST - 1) & 1, err);
+        if (ok) send(n + 2, false, d2);
+      }
+      d0 = d1;
+      d1 = d2;
     }
     if (!ok && lane == 0) {  // a wait ran out: let the copies in flight land before the CTA goes
       mbar_wait(xy_full, 0, nullptr, 100000000ull);
+      for (int k = 0; k < C::UST + C::WST; ++k) mbar_wait(&raw[k], (raw_phase >> k) & 1, nullptr, 10000000ull);
       for (int n = max(0, un - C::UST); n < un; ++n)
-        mbar_wait(&u_full[n % C::UST], (n / C::UST) & 1, nullptr, 100000000ull);
+        mbar_wait(&u_full[n % C::UST], (n / C::UST) & 1, nullptr, 10000000ull);
       for (int n = max(0, wn - C::WST); n < wn; ++n)
-        mbar_wait(&w_full[n % C::WST], (n / C::WST) & 1, nullptr, 100000000ull);
+        mbar_wait(&w_full[n % C::WST], (n / C::WST) & 1, nullptr, 10000000ull);
     }
   } else if (warp == 16) {
     // ---- MMA ----

@@ -181,9 +181,22 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 
   if (warp == 18) {
     // ---- loads ----
-    int n = 0;  // ring positions filled
+    // A V tile with dead rows lands on kv_raw and is handed on when they have been zeroed, after the next
+    // K has been sent for.
+    int n = 0, unclean = -1;  // ring positions filled; the one whose rows are still to be zeroed
     uint32_t raw = 0;
+    DeadRows dead;
     bool ok = true;
+    auto clean = [&]() {
+      if (unclean < 0) return true;
+      if (!warp_wait(kv_raw, raw, err)) return false;
+      raw ^= 1;
+      attn_zero_rows<D / 64>(smem + C::OFF_KV + unclean * C::TILE, dead);
+      fence_proxy_async_smem();
+      warp_arrive(&kv_full[unclean]);
+      unclean = -1;
+      return true;
+    };
     for (int j = jb; ok && j < je; ++j) {
       if (!visits(0, j) && !visits(1, j)) continue;
       const int row = j * AM_T;
@@ -191,31 +204,28 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       for (int is_v = 0; is_v < 2; ++is_v, ++n) {
         if (n == 0) continue;  // sent for above
         const int s = n % C::STAGES;
-        uint32_t bad[4];
-        const bool dirty = is_v && attn_dead_rows(seq, row, bad);
-        if (n >= C::STAGES) ok = warp_wait(&kv_empty[s], (n / C::STAGES - 1) & 1, err);
+        if (is_v) {
+          ok = clean();
+          dead = attn_dead_rows(seq, row);
+        }
+        if (ok && n >= C::STAGES) ok = warp_wait(&kv_empty[s], (n / C::STAGES - 1) & 1, err);
         if (!ok) break;
-        uint8_t* dst = smem + C::OFF_KV + s * C::TILE;
+        const bool dirty = is_v && dead.any;
         uint64_t* bar = dirty ? kv_raw : &kv_full[s];
         if (lane == 0) {
           mbar_arrive_expect_tx(bar, C::TILE);
-          tma_load_3d(dst, is_v ? &tv : &tk, bar, 0, seq.start + row, kvh * (D / 64));
+          tma_load_3d(smem + C::OFF_KV + s * C::TILE, is_v ? &tv : &tk, bar, 0, seq.start + row, kvh * (D / 64));
         }
-        if (dirty) {
-          ok = warp_wait(kv_raw, raw, err);
-          if (!ok) break;
-          raw ^= 1;
-          attn_zero_rows<D / 64>(dst, bad);
-          fence_proxy_async_smem();
-          warp_arrive(&kv_full[s]);
-        }
+        if (dirty) unclean = s;
       }
     }
+    if (ok) ok = clean();
     if (!ok && lane == 0) {  // a wait ran out: let the copies in flight land before the CTA goes
       mbar_wait(&q_full[0], 0, nullptr, 100000000ull);
       mbar_wait(&q_full[1], 0, nullptr, 100000000ull);
+      if (unclean >= 0) mbar_wait(kv_raw, raw, nullptr, 100000000ull);
       for (int k = max(0, n - C::STAGES); k < n; ++k)
-        mbar_wait(&kv_full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, 100000000ull);
+        if (k % C::STAGES != unclean) mbar_wait(&kv_full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, 100000000ull);
     }
   } else if (warp == 16 || warp == 17) {
     // ---- MMA of one tile ----
