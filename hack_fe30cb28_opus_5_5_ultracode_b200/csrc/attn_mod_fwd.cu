@@ -25,11 +25,12 @@ namespace ql {
 
 namespace {
 
-template <int D>
+template <int D, bool SPLIT>
 struct FwdCfg {
   static constexpr int TILE = AM_T * D * 2;          // bytes of a 128-row tile
-  static constexpr int STAGES = D == 128 ? 5 : 8;    // ring of K / V tiles
-  static constexpr int OFF_KV = 2 * TILE;
+  static constexpr int Q_TILES = SPLIT ? 1 : 2;
+  static constexpr int STAGES = D == 128 ? 7 - Q_TILES : 8;  // ring of K / V tiles
+  static constexpr int OFF_KV = Q_TILES * TILE;
   static constexpr int OFF_M = OFF_KV + STAGES * TILE;  // [2 tiles][2 halves][128] fp32 exchange
   static constexpr int OFF_BAR = OFF_M + 4 * AM_T * 4;
   static constexpr int SMEM = OFF_BAR + 512;
@@ -106,11 +107,11 @@ __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, 
   }
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D, int MODE, bool SPLIT>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
     attn_mod_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                         const __grid_constant__ CUtensorMap tv, const AttnModArgs a, int* err) {
-  using C = FwdCfg<D>;
+  using C = FwdCfg<D, SPLIT>;
   constexpr bool IS_BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int BOX = AM_T * 128;  // a 128-row x 64-column box
   pdl_enter();
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_read + 8);
 
   const int h = blockIdx.x % a.HQ, b = blockIdx.x / a.HQ;
-  const int q0 = (gridDim.y - 1 - blockIdx.y) * 2 * AM_T;  // the rows with the most keys first
+  const int q0 = (gridDim.y - 1 - blockIdx.y) * C::Q_TILES * AM_T;  // the rows with the most keys first
   const AttnSeq seq = attn_seq(a, b);
   if (q0 >= seq.len) return;  // the whole CTA, before any barrier or TMEM is set up
   const int kvh = h / (a.HQ / a.HKV);
@@ -154,22 +155,25 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       mbar_init(&kv_empty[s], 2);
     }
     fence_barrier_init();
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < C::Q_TILES; ++t) {
       mbar_arrive_expect_tx(&q_full[t], C::TILE);
       tma_load_3d(smem + t * C::TILE, &tq, &q_full[t], 0, seq.start + q0 + t * AM_T, h * (D / 64));
     }
   }
   if (warp == 16) tmem_alloc(tmem_slot, 512);
-  AttnBlocks tb0 = attn_tile_blocks(seq, q0), tb1 = attn_tile_blocks(seq, q0 + AM_T);
+  AttnBlocks tb0 = attn_tile_blocks(seq, q0), tb1 = SPLIT ? tb0 : attn_tile_blocks(seq, q0 + AM_T);
   tb0.first = uniform(tb0.first);
   tb0.end = uniform(tb0.end);
   tb1.first = uniform(tb1.first);
   tb1.end = uniform(tb1.end);
   // the blocks either tile visits: its own range, or the gap-free union where both have one
-  const bool any0 = tb0.end > tb0.first, any1 = tb1.end > tb1.first;
-  const int jb = !any1 || (any0 && tb0.first < tb1.first) ? tb0.first : tb1.first;
-  const int je = !any1 || (any0 && tb0.end > tb1.end) ? tb0.end : tb1.end;
-  auto visits = [&](int t, int j) { return t ? j >= tb1.first && j < tb1.end : j >= tb0.first && j < tb0.end; };
+  const bool any0 = tb0.end > tb0.first, any1 = tb1.end > tb1.first + (SPLIT ? 1 : 0);
+  const int jb = SPLIT || !any1 || (any0 && tb0.first < tb1.first) ? tb0.first : tb1.first;
+  const int je = SPLIT || !any1 || (any0 && tb0.end > tb1.end) ? tb0.end : tb1.end;
+  auto visits = [&](int t, int j) {
+    if (SPLIT) return j >= tb0.first && j < tb0.end && ((j - tb0.first) & 1) == t;
+    return t ? j >= tb1.first && j < tb1.end : j >= tb0.first && j < tb0.end;
+  };
   if (warp == 18 && lane == 0 && je > jb) {  // the first K
     mbar_arrive_expect_tx(&kv_full[0], C::TILE);
     tma_load_3d(smem + C::OFF_KV, &tk, &kv_full[0], 0, seq.start + jb * AM_T, kvh * (D / 64));
@@ -222,7 +226,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     if (ok) ok = clean();
     if (!ok && lane == 0) {  // a wait ran out: let the copies in flight land before the CTA goes
       mbar_wait(&q_full[0], 0, nullptr, 100000000ull);
-      mbar_wait(&q_full[1], 0, nullptr, 100000000ull);
+      if (!SPLIT) mbar_wait(&q_full[1], 0, nullptr, 100000000ull);
       if (unclean >= 0) mbar_wait(kv_raw, raw, nullptr, 100000000ull);
       for (int k = max(0, n - C::STAGES); k < n; ++k)
         if (k % C::STAGES != unclean) mbar_wait(&kv_full[k % C::STAGES], (k / C::STAGES) & 1, nullptr, 100000000ull);
@@ -233,7 +237,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     if (je > jb) {
       constexpr uint32_t id_s = umma_idesc_f16(IS_BF16, 128, AM_T, false);
       constexpr uint32_t id_o = umma_idesc_f16(IS_BF16, 128, D, true);  // V is MN-major
-      const uint32_t sq = desc_lo_k(smem_u32(smem + t * C::TILE));
+      const uint32_t sq = desc_lo_k(smem_u32(smem + (SPLIT ? 0 : t * C::TILE)));
       const uint32_t sk = desc_lo_k(smem_u32(smem + C::OFF_KV));
       const uint32_t sv = desc_lo_mn(smem_u32(smem + C::OFF_KV), BOX);
       // The score buffer goes from item to item ((tile, block) pairs, block by block, tile 0 first): this
@@ -254,11 +258,11 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         pend = -1;
         return true;
       };
-      bool ok = warp_wait(&q_full[t], 0, err);
+      bool ok = warp_wait(&q_full[SPLIT ? 0 : t], 0, err);
       for (int j = jb; ok && j < je; ++j) {
         const bool mine = visits(t, j);
         if (!mine && !visits(t ^ 1, j)) continue;  // not loaded
-        if (!mine && pend >= 0) ok = gather();
+        if (!SPLIT && !mine && pend >= 0) ok = gather();  // it may have been the tile's last
         const int s = ring % C::STAGES, s1 = (ring + 1) % C::STAGES;
         if (ok) ok = warp_wait(&kv_full[s], (ring / C::STAGES) & 1, err);
         if (!ok) break;
@@ -289,7 +293,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   } else {
     // ---- softmax ----
     const int t = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
-    const int qi = q0 + t * AM_T + r;
+    const int qi = q0 + (SPLIT ? 0 : t * AM_T) + r;
     const AttnBlocks tb = t ? tb1 : tb0;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t ts = lane_base + half * FWD_HC, tp = lane_base + 128 + t * 64 + half * (FWD_HC / 2);
@@ -308,8 +312,9 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     const float mul = MODE == 0 ? c.sl2 : 1.f;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
-    for (int j = tb.first; j < tb.end; ++j) {
-      const int n = j - tb.first;
+    constexpr int STEP = SPLIT ? 2 : 1;
+    for (int j = tb.first + (SPLIT ? t : 0); j < tb.end; j += STEP) {
+      const int n = (j - tb.first) / STEP;
       ok = warp_wait(&s_full[t], n & 1, err);
       if (!ok) break;
       tc_fence_after();
@@ -320,10 +325,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       tc_fence_before();
       // the buffer goes to tile 1 at this block, else to whichever tile visits the next one, or
       // (tile 0's last block before a gap) to tile 1
-      const int heir = t == 0 && visits(1, j) ? 1 : visits(0, j + 1) ? 0 : visits(1, j + 1) || (t == 0 && any1) ? 1 : -1;
+      const int heir = SPLIT ? (j + 1 < tb.end ? t ^ 1 : -1) : t == 0 && visits(1, j) ? 1 : visits(0, j + 1) ? 0 : visits(1, j + 1) || (t == 0 && any1) ? 1 : -1;
       if (heir >= 0) warp_arrive(&s_free[heir]);
       const bool masked = j < tb.ffirst || j >= tb.fend;
-      const int j0 = j * AM_T + half * FWD_HC, qt = q0 / AM_T + t;
+      const int j0 = j * AM_T + half * FWD_HC, qt = q0 / AM_T + (SPLIT ? 0 : t);
       const float side = j < qt ? 1.f : j > qt ? -1.f : 0.f;
       if (masked) modify_scores<MODE, true>(x, c, slope2, (float)(qi - j0), side, range.x - j0, range.y - j0);
       else modify_scores<MODE, false>(x, c, slope2, (float)(qi - j0), side, 0, 0);
@@ -387,30 +392,60 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       up2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), sa, sb);
       l_run = l_run * corr + (sa + sb);
     }
-    if (tb.end > tb.first && ok) {
-      ok = warp_wait(&o_full[t], (tb.end - tb.first - 1) & 1, err);
+    const int count = max(0, tb.end - tb.first + STEP - 1 - (SPLIT ? t : 0)) / STEP;  // blocks it has had
+    if (count > 0 && ok) {
+      ok = warp_wait(&o_full[t], (count - 1) & 1, err);
       tc_fence_after();
     }
     // the row sum: both halves' sums, added in the same order in both threads
-    if (ok && tb.end > tb.first) ok = warp_wait(pair_read, (tb.end - tb.first - 1) & 1, err);
+    if (ok && count > 0) ok = warp_wait(pair_read, (count - 1) & 1, err);
     if (ok) {
       *mine = l_run;
       warp_arrive(pair);
-      ok = warp_wait(pair, (tb.end - tb.first) & 1, err);
+      ok = warp_wait(pair, count & 1, err);
+    }
+    // O's columns [col0, col0 + COLS) of this thread's row: O_t / l, or with SPLIT both halves of the keys
+    // brought to one maximum
+    constexpr int COLS = D / 2 / STEP;
+    const int col0 = (SPLIT ? 2 * t + half : half) * COLS;
+    float l_row = half ? *other + l_run : l_run + *other, f0 = 1.f, f1 = 0.f;
+    int count1 = 0;
+    if constexpr (SPLIT) {
+      asm volatile("bar.sync 1, 512;" ::: "memory");  // every sum has been read
+      if (half == 0) {
+        sM[2 * t * AM_T + r] = m_run;
+        sM[(2 * t + 1) * AM_T + r] = l_row;
+        if (!ok) sM[2 * t * AM_T + r] = NAN;
+      }
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+      tc_fence_after();
+      const float m0 = sM[r], m1 = sM[2 * AM_T + r];
+      m_run = fmaxf(m0, m1);
+      f0 = m0 == -INFINITY ? 0.f : ex2(m0 - m_run);
+      f1 = m1 == -INFINITY ? 0.f : ex2(m1 - m_run);
+      l_row = f0 * sM[AM_T + r] + f1 * sM[3 * AM_T + r];
+      ok = __all_sync(0xffffffffu, ok && m0 == m0 && m1 == m1);
+      count1 = tb.end - tb.first > 1;
     }
     if (ok) {
-      const float l_row = half ? *other + l_run : l_run + *other;
       const float inv = l_row > 0.f ? 1.f / l_row : (l_row == 0.f ? 0.f : l_row);  // NaN stays
       // Q's tile has been read for the last time (or, with no block, has landed by now): the rows leave
       // through it
-      if (tb.end == tb.first) warp_wait(&q_full[t], 0, err);
-      constexpr int W = D;  // bytes of half a row
-      uint8_t* stage = smem + t * C::TILE + (warp & 7) * 32 * W;
+      if (tb.end == tb.first) warp_wait(&q_full[SPLIT ? 0 : t], 0, err);
+      constexpr int W = 2 * COLS;  // bytes
+      const uint32_t o_at = lane_base + 256 + (SPLIT ? 0 : t * 128) + col0;
+      uint8_t* stage = smem + (SPLIT ? warp * 32 * W : t * C::TILE + (warp & 7) * 32 * W);
 #pragma unroll
-      for (int u = 0; u < D / 32; ++u) {
+      for (int u = 0; u < COLS / 16; ++u) {
         float ov[16];
         if (tb.end > tb.first) {
-          tmem_ld16(to + u * 16, ov);
+          tmem_ld16(o_at + u * 16, ov);
+          if constexpr (SPLIT) {
+            float o1[16];
+            if (count1) tmem_ld16(o_at + 128 + u * 16, o1);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) ov[e] = count1 ? ov[e] * f0 + o1[e] * f1 : ov[e] * f0;
+          }
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) ov[e] = 0.f;
@@ -424,9 +459,9 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                          pack_t2<T>(ov[8 * v + 6] * inv, ov[8 * v + 7] * inv));
       }
       const int row = qi - lane;  // the warp's first
-      T* out = reinterpret_cast<T*>(a.out_w) + ((int64_t)(seq.start + row) * a.HQ + h) * D + half * (D / 2);
+      T* out = reinterpret_cast<T*>(a.out_w) + ((int64_t)(seq.start + row) * a.HQ + h) * D + col0;
       stage_flush<W>(stage, reinterpret_cast<uint8_t*>(out), (int64_t)a.HQ * D * 2, seq.len - row);
-      if (qi < seq.len && half == 0)
+      if (qi < seq.len && col0 == 0)
         a.lse[(int64_t)h * a.n + seq.start + qi] = (m_run - FWD_P_SHIFT<T> + log2f(l_row)) * 0.6931471805599453f;
     }
   }
@@ -508,26 +543,48 @@ __global__ void __launch_bounds__(DOC_THREADS) doc_ranges_kernel(const int32_t* 
   doc_scan<true>(ids + start, len, ranges + start, sm);
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D, int MODE, bool SPLIT>
 int launch_fwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mk,
                const CUtensorMap& mv, cudaStream_t s) {
+  using C = FwdCfg<D, SPLIT>;
   static unsigned long long done = 0;
-  auto kern = attn_mod_fwd_kernel<T, D, MODE>;
-  const int st = attn_smem_limit(reinterpret_cast<const void*>(kern), FwdCfg<D>::SMEM, &done);
+  auto kern = attn_mod_fwd_kernel<T, D, MODE, SPLIT>;
+  const int st = attn_smem_limit(reinterpret_cast<const void*>(kern), C::SMEM, &done);
   if (st != QL_STATUS_OK) return st;
-  const dim3 grid((unsigned)(a.HQ * a.B), (unsigned)cdiv(a.max_len, 2 * AM_T));
-  launch_k(kern, grid, dim3(FWD_THREADS), FwdCfg<D>::SMEM, s, mq, mk, mv, a, status_word());
+  const dim3 grid((unsigned)(a.HQ * a.B), (unsigned)cdiv(a.max_len, C::Q_TILES * AM_T));
+  launch_k(kern, grid, dim3(FWD_THREADS), C::SMEM, s, mq, mk, mv, a, status_word());
   return launched(1);
+}
+
+// Whether a CTA takes one query tile, and its two halves every second key block (SPLIT): the chain of
+// the longest CTA is halved, against twice as many CTAs and twice the loads. Compared in key blocks
+// per SM, as the longest CTA and as an SM's share of all, with 3 blocks' time for a CTA's set-up and
+// end. Pairs against single tiles, us: 2,048 causal tokens of 12 heads 31 / 20; 8 x 64-2,048 of 4
+// heads, capped 33 / 21; but 4 x 1,024 of 12 heads 23 / 28, 2,048 of 28 heads 40 / 52.
+bool fwd_split(const AttnModArgs& a) {
+  const double tiles = (double)cdiv(a.max_len, AM_T);
+  const double reach = a.window > 0 ? (a.causal ? 1.0 : 2.0) * a.window / AM_T + 1 : 1e30;
+  const double longest = tiles < reach ? tiles : reach;
+  const double mean = a.causal && longest == tiles ? (tiles + 1) / 2 : longest;
+  const double pairs = (double)cdiv(a.n, 2 * AM_T) * a.HQ / sm_count();
+  const double whole = fmax(longest + 3, pairs * (mean + 3)), split = fmax(longest / 2 + 3, pairs * (mean + 6));
+  return split < 0.85 * whole;
+}
+
+template <typename T, int D, int MODE>
+int pick_fwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+             cudaStream_t s) {
+  return fwd_split(a) ? launch_fwd<T, D, MODE, true>(a, mq, mk, mv, s) : launch_fwd<T, D, MODE, false>(a, mq, mk, mv, s);
 }
 
 template <typename T, int D>
 int dispatch_fwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mk,
                  const CUtensorMap& mv, cudaStream_t s) {
   switch (attn_mode(a)) {
-    case 0: return launch_fwd<T, D, 0>(a, mq, mk, mv, s);
-    case 1: return launch_fwd<T, D, 1>(a, mq, mk, mv, s);
-    case 2: return launch_fwd<T, D, 2>(a, mq, mk, mv, s);
-    default: return launch_fwd<T, D, 3>(a, mq, mk, mv, s);
+    case 0: return pick_fwd<T, D, 0>(a, mq, mk, mv, s);
+    case 1: return pick_fwd<T, D, 1>(a, mq, mk, mv, s);
+    case 2: return pick_fwd<T, D, 2>(a, mq, mk, mv, s);
+    default: return pick_fwd<T, D, 3>(a, mq, mk, mv, s);
   }
 }
 

@@ -119,11 +119,11 @@ def mode_args(mode, lengths, HQ, seed=0, extra=0):
     return m, {key: x.cuda() if torch.is_tensor(x) else x for key, x in m.items()}
 
 
-LENGTHS = [[1], [0, 3, 0], [127, 129, 1], [300, 257, 33, 0, 700], [1030]]
+LENGTHS = [[1], [0, 3, 0], [127, 129, 1], [300, 257, 33, 0, 700], [1030], [257, 130, 5] * 40]
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+@pytest.mark.parametrize("lengths", LENGTHS, ids=lambda x: str(x)[:24])
 @pytest.mark.parametrize("mode", MODES, ids=str)
 @pytest.mark.parametrize("heads,dtype", [((4, 2, 64), torch.float16), ((7, 1, 128), torch.bfloat16)],
                          ids=["h4-2-64-fp16", "h7-1-128-bf16"])
@@ -143,7 +143,7 @@ def test_forward_matches_the_formula(lengths, mode, heads, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+@pytest.mark.parametrize("lengths", LENGTHS, ids=lambda x: str(x)[:24])
 @pytest.mark.parametrize("mode", MODES, ids=str)
 @pytest.mark.parametrize("heads,dtype", [((4, 2, 64), torch.bfloat16), ((6, 1, 128), torch.float16)],
                          ids=["h4-2-64-bf16", "h6-1-128-fp16"])
