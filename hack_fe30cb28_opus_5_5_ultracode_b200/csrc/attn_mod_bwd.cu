@@ -632,25 +632,34 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   }
 }
 
-// dk / dv of every row of a sequence: the splits' partials added in split order, rounded once.
+// dk and dv of every row of a sequence: the splits' partials added in split order, those of two splits
+// on their way at a time, rounded once.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_mod_sum_kernel(const AttnModArgs a, int D) {
   pdl_enter();
   const int64_t plane = (int64_t)a.n * a.HKV * D;
-  const int64_t have = (int64_t)(a.cu_seqlens[a.B] - a.cu_seqlens[0]) * a.HKV * D;
-  const int64_t first = (int64_t)a.cu_seqlens[0] * a.HKV * D;
-  const int64_t i = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) * 4;
-  if (i >= have) return;
+  const int64_t first = (int64_t)a.cu_seqlens[0] * a.HKV * D, end = (int64_t)a.cu_seqlens[a.B] * a.HKV * D;
+  const int64_t i = first + (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) * 4;
+  if (i >= end) return;
+  float4 s[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};  // dk, dv
+  for (int p = 0; p < a.splits; p += 2) {
+    float4 v[2][2];
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p < a.splits; ++p) {
-      const float4 v = *reinterpret_cast<const float4*>(a.parts + (2 * p + which) * plane + first + i);
-      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-    }
-    T* dst = reinterpret_cast<T*>(which == 0 ? a.dk : a.dv) + first + i;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_t2<T>(s.x, s.y), pack_t2<T>(s.z, s.w));
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        v[k][w] = p + k < a.splits ? *reinterpret_cast<const float4*>(a.parts + (2 * (p + k) + w) * plane + i)
+                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        s[w].x += v[k][w].x, s[w].y += v[k][w].y, s[w].z += v[k][w].z, s[w].w += v[k][w].w;
   }
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(w == 0 ? a.dk : a.dv) + i) =
+        make_uint2(pack_t2<T>(s[w].x, s[w].y), pack_t2<T>(s[w].z, s[w].w));
 }
 
 // How many CTAs share a KV head's query heads: as few as keep the longest CTA (a key block that

@@ -474,8 +474,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 }
 
 // Documents: (first, end) of the run of equal ids each token is in, within its sequence; a token
-// with a negative id gets the empty range (i, i). One CTA per sequence scans it in chunks of 4,096
-// tokens, forwards for the first tokens of the runs and backwards for their ends.
+// with a negative id gets the empty range (i, i). Two CTAs per sequence scan it in chunks of 4,096
+// tokens, one forwards for the first tokens of the runs and one backwards for their ends.
 constexpr int DOC_THREADS = 1024, DOC_PER = 4;
 
 template <bool REV>
@@ -539,8 +539,8 @@ __global__ void __launch_bounds__(DOC_THREADS) doc_ranges_kernel(const int32_t* 
   pdl_enter();
   __shared__ int sm[DOC_THREADS / 32];
   const int start = cu[blockIdx.x], len = cu[blockIdx.x + 1] - start;
-  doc_scan<false>(ids + start, len, ranges + start, sm);
-  doc_scan<true>(ids + start, len, ranges + start, sm);
+  if (blockIdx.y == 0) doc_scan<false>(ids + start, len, ranges + start, sm);
+  else doc_scan<true>(ids + start, len, ranges + start, sm);
 }
 
 template <typename T, int D, int MODE, bool SPLIT>
@@ -592,7 +592,7 @@ int dispatch_fwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap&
 
 int attn_doc_ranges(const int32_t* doc_ids, const int32_t* cu_seqlens, int B, int n, int2* ranges,
                     cudaStream_t s) {
-  launch_k(doc_ranges_kernel, dim3((unsigned)B), dim3(DOC_THREADS), 0, s, doc_ids, cu_seqlens, ranges);
+  launch_k(doc_ranges_kernel, dim3((unsigned)B, 2), dim3(DOC_THREADS), 0, s, doc_ids, cu_seqlens, ranges);
   return launched(1);
 }
 

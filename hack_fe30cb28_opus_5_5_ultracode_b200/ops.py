@@ -807,15 +807,16 @@ def attn_mod_bwd(dout, q, k, v, out, lse, cu_seqlens, max_len, scale, causal=Tru
         else:
             _given(t, name, want, dtype, dev)
         grads.append(t)
-    ranges = q.new_empty((n, 2), dtype=torch.int32) if doc_ids is not None else None
     lib = _lib.lib()
     with _on_device(dev):  # the workspace's size goes by the device's SMs
         floats = lib.ql_attn_mod_bwd_workspace(n, max_len, HQ, HKV, D, bool(causal), window)
-    ws = q.new_empty(max(floats, 4), dtype=torch.float32)
+    # a multiple of four floats, and behind it the documents' ranges
+    ws = q.new_empty(floats + (0 if doc_ids is None else 2 * n) + 4, dtype=torch.float32)
+    work = ws.data_ptr()
     args = _ATTN_MOD(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
                      cu_seqlens.data_ptr(), _address(slopes), _address(prefix_len),
-                     _address(doc_ids), _address(ranges), dout.data_ptr(),
-                     *(t.data_ptr() for t in grads), ws.data_ptr(), ws.shape[0], *ld, scale,
+                     _address(doc_ids), 0 if doc_ids is None else work + 4 * floats,
+                     dout.data_ptr(), *(t.data_ptr() for t in grads), work, floats, *ld, scale,
                      softcap, n, B, max_len, HQ, HKV, D, dt, bool(causal), window)
     _launch("ql_attn_mod_bwd", dev, args)
     return tuple(grads)
