@@ -447,3 +447,40 @@ def test_the_backward_refuses_before_any_launch(change):
     with pytest.raises(_lib.QLError) as e:
         _lib.call("ql_attn_mod_bwd", ops.ctypes_ref(args), None)
     assert e.value.status == ops.STATUS_BAD_ARG
+
+
+@pytest.mark.gpu
+def test_prefixes_beyond_the_sequence_and_below_zero():
+    lengths, heads = [140, 37, 5], (2, 1, 64)
+    q, k, v, dout, cu = batch(lengths, heads, torch.float16, seed=14)
+    prefix = torch.tensor([1 << 30, -(1 << 30), 5], dtype=torch.int32)
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, 140, 0.125, prefix_len=prefix.cuda())
+    got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 140, 0.125, prefix_len=prefix.cuda())
+    want = formula(q, k, v, lengths, 0.125, dout=dout, prefix_len=prefix)
+    for x, y in zip((out, *got), (want[0], *want[2:])):
+        assert rel(x, y) < 1.5 * TOL[torch.float16]
+
+
+@pytest.mark.gpu
+def test_tensors_beyond_32_bit_offsets():
+    """The last sequence of a batch of 2.3 G elements gives what it gives alone."""
+    HQ, HKV, D, length, B, dtype = 128, 2, 128, 2000, 70, torch.bfloat16
+    n = length * B
+    assert n * HQ * D > 1 << 31
+    torch.manual_seed(15)
+    q, dout = (torch.empty(n, HQ, D, device="cuda", dtype=dtype) for _ in range(2))
+    k, v = (torch.randn(n, HKV, D, device="cuda").to(dtype) for _ in range(2))
+    last = slice(n - length, n)
+    for t in (q, dout):
+        t[:-length].fill_(0.25)
+        t[last] = torch.randn(length, HQ, D, device="cuda").to(dtype)
+    cu = torch.arange(0, n + 1, length, device="cuda", dtype=torch.int32)
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, length, 0.1, window=100)
+    got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, length, 0.1, window=100)
+    s = [t[last].clone() for t in (q, k, v)]
+    one_out, one_lse = ops.attn_mod_fwd(*s, cu[:2], length, 0.1, window=100)
+    one = ops.attn_mod_bwd(dout[last].clone(), *s, one_out, one_lse, cu[:2], length, 0.1, window=100)
+    assert ops.device_status() == 0
+    for x, y in zip((out, *got), (one_out, *one)):
+        assert (x[last].double() - y.double()).norm() < TOL[dtype] * y.double().norm()
+    assert torch.allclose(lse[:, last], one_lse, atol=2e-5, rtol=0)

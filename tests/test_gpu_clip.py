@@ -213,3 +213,26 @@ def test_clipping_refuses_before_any_launch(change):
     with pytest.raises(_lib.QLError) as e:
         lib_call(**change)
     assert e.value.status == ops.STATUS_BAD_ARG
+
+
+@pytest.mark.gpu
+def test_lists_of_thousands_and_empty_tensors():
+    grads = grads_of([0, 5, 0, 129] * 700, [F32, BF16, F16])
+    norm, factor = expected(grads, 0.5)
+    before = [g.clone() for g in grads]
+    got = ops.clip_grads(grads, 0.5)
+    assert abs(got.item() - norm) < 1e-6 * norm
+    check(grads, before, factor)
+
+
+@pytest.mark.gpu
+def test_a_tensor_beyond_32_bit_offsets():
+    n = (1 << 31) + 12345
+    g = torch.zeros(n, device="cuda", dtype=BF16)
+    g[-1000:] = 3.0
+    g[:1000] = 4.0
+    norm = ops.clip_grads([g], 50.0)
+    assert abs(norm.item() - 25000 ** 0.5) < 1e-3
+    want = torch.tensor([4.0, 3.0]) * (50.0 / (25000 ** 0.5 + 1e-6))
+    assert torch.equal(torch.stack([g[0], g[-1]]).cpu(), want.to(BF16))
+    assert g[1000:-1000].abs().max().item() == 0

@@ -210,3 +210,25 @@ def test_the_library_refuses_before_any_launch(change, status):
         with pytest.raises(_lib.QLError) as e:
             _lib.call(entry, ops.ctypes_ref(args), None)
         assert e.value.status == 1
+
+
+@pytest.mark.gpu
+def test_tensors_beyond_32_bit_offsets():
+    """The last rows of a batch of 2.2 G elements give what they give alone."""
+    heads, sections, n, few = (64, 8, 128), (16, 24, 24), 212000, 100
+    HQ, HKV, D = heads
+    C = (HQ + 2 * HKV) * D
+    assert n * C > 1 << 31
+    c = cuda(case(few, heads, torch.bfloat16, sections))
+    big = torch.zeros(n, C, device="cuda", dtype=torch.bfloat16)
+    big[-few:] = c["qkv"]
+    pos = torch.zeros(3, n, device="cuda", dtype=torch.int32)
+    pos[:, -few:] = c["pos"]
+    tables = (c["cos"], c["sin"])
+    one = ops.mrope_fwd(c["qkv"], *tables, c["pos"], *heads, sections)
+    many = ops.mrope_fwd(big, *tables, pos, *heads, sections)
+    assert all(torch.equal(x[-few:], y) for x, y in zip(many, one))
+    back = ops.mrope_bwd(*many, *tables, pos, *heads, sections, dtype=torch.bfloat16, Bq=c["Bq"])
+    alone = ops.mrope_bwd(*one, *tables, c["pos"], *heads, sections, dtype=torch.bfloat16, Bq=c["Bq"])
+    assert torch.equal(back[0][-few:], alone[0])
+    assert rel(back[1][-few:], alone[1].double().cpu()) < 2.0 ** -20
