@@ -89,10 +89,19 @@ __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, 
   if constexpr ((MODE & 2) != 0) {
     const uint64_t mul = pk2((MODE & 1) != 0 ? 1.f : c.sl2, (MODE & 1) != 0 ? 1.f : c.sl2);
     if (side != 0.f) {  // every key on one side of every query: |i - j| = side (dist0 - column)
+      // four pairs of biases, moved on by eight columns at a time
       const float slope = side * slope2, base = -slope * dist0;
+      const uint64_t next = pk2(8.f * slope, 8.f * slope);
+      uint64_t bias[4];
 #pragma unroll
-      for (int i = 0; i < FWD_HC; i += 2)
-        unpair(fma2(pair_of(x + i), mul, pk2(fmaf((float)i, slope, base), fmaf((float)(i + 1), slope, base))), x + i);
+      for (int e = 0; e < 4; ++e) bias[e] = pk2(fmaf((float)(2 * e), slope, base), fmaf((float)(2 * e + 1), slope, base));
+#pragma unroll
+      for (int i = 0; i < FWD_HC; i += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          unpair(fma2(pair_of(x + i + 2 * e), mul, bias[e]), x + i + 2 * e);
+          bias[e] = add2(bias[e], next);
+        }
     } else {
 #pragma unroll
       for (int i = 0; i < FWD_HC; i += 2)
@@ -127,9 +136,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
   uint64_t* drain = bars + 11;                   // [2]
   uint64_t* kv_full = bars + 13;                 // [STAGES]
   uint64_t* kv_empty = bars + 13 + C::STAGES;    // [STAGES] one arrival per tile
-  uint64_t* row_max = bars + 13 + 2 * C::STAGES; // [2][4] both halves of a tile's 32 rows (2 warps)
-  uint64_t* row_read = row_max + 8;              // [2][4] and read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_read + 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13 + 2 * C::STAGES);
 
   const int h = blockIdx.x % a.HQ, b = blockIdx.x / a.HQ;
   const int q0 = (gridDim.y - 1 - blockIdx.y) * C::Q_TILES * AM_T;  // the rows with the most keys first
@@ -145,7 +152,6 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       mbar_init(&s_free[s], 8);
       mbar_init(&p_full[s], 8);
       mbar_init(&o_full[s], 1);
-      for (int w = 0; w < 8; ++w) mbar_init(&row_max[s * 8 + w], 2);  // row_max and row_read
     }
     mbar_init(kv_raw, 1);
     mbar_init(&drain[0], 1);
@@ -300,8 +306,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     const uint32_t to = lane_base + 256 + t * 128 + half * (D / 2);
     float* mine = sM + (2 * t + half) * AM_T + r;
     const float* other = sM + (2 * t + (half ^ 1)) * AM_T + r;
-    uint64_t* pair = &row_max[t * 4 + (warp & 3)];
-    uint64_t* pair_read = &row_read[t * 4 + (warp & 3)];
+    // the two warps of a row meet in a named barrier once per block, also after a wait has run out: a
+    // handshake over two mbarriers took 600 of a block's 3,300 cycles
+    const int pair = 2 + t * 4 + (warp & 3);
+    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory"); };
     const int2 range = qi < seq.len ? attn_row_range(seq, qi) : make_int2(0, 0);
     ScoreConst c;
     c.sl2 = a.scale * 1.4426950408889634f;
@@ -315,8 +323,11 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     constexpr int STEP = SPLIT ? 2 : 1;
     for (int j = tb.first + (SPLIT ? t : 0); j < tb.end; j += STEP) {
       const int n = (j - tb.first) / STEP;
-      ok = warp_wait(&s_full[t], n & 1, err);
-      if (!ok) break;
+      ok = ok && warp_wait(&s_full[t], n & 1, err);
+      if (!ok) {
+        meet();
+        continue;
+      }
       tc_fence_after();
       uint32_t x[FWD_HC];
       tmem_ld32_nw(ts, x);
@@ -338,27 +349,21 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           mx[e] = max3(mx[e], __uint_as_float(x[i + 2 * e]), __uint_as_float(x[i + 2 * e + 1]));
-      // the other half's maximum
+      // O_t += P_t V of the last block is complete: P_t may be written, O_t rescaled, and the other half has
+      // read this thread's last maximum
+      if (n > 0) ok = warp_wait(&o_full[t], (n - 1) & 1, err);
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      if (n > 0) ok = warp_wait(pair_read, (n - 1) & 1, err);  // the last block's has been read
-      if (!ok) break;
       *mine = top;
-      warp_arrive(pair);
-      ok = warp_wait(pair, n & 1, err);
-      if (!ok) break;
+      meet();
+      if (!ok) continue;
+      tc_fence_after();
       const float ms = fmaxf(top, *other) * mul;
-      warp_arrive(pair_read);
       float corr = 1.f;
       if (ms > m_run + 8.f) {
         corr = m_run == -INFINITY ? 0.f : ex2(m_run - ms);
         m_run = ms;
       }
       const float mneg = m_run == -INFINITY ? 0.f : FWD_P_SHIFT<T> - m_run;
-      if (n > 0) {  // O_t += P_t V of the last block is complete: P_t may be written, O_t rescaled
-        ok = warp_wait(&o_full[t], (n - 1) & 1, err);
-        if (!ok) break;
-        tc_fence_after();
-      }
       if (n > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
 #pragma unroll 1
         for (int u = 0; u < D / 32; ++u) {
@@ -398,12 +403,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       tc_fence_after();
     }
     // the row sum: both halves' sums, added in the same order in both threads
-    if (ok && count > 0) ok = warp_wait(pair_read, (count - 1) & 1, err);
-    if (ok) {
-      *mine = l_run;
-      warp_arrive(pair);
-      ok = warp_wait(pair, count & 1, err);
-    }
+    *mine = l_run;
+    meet();
     // O's columns [col0, col0 + COLS) of this thread's row: O_t / l, or with SPLIT both halves of the keys
     // brought to one maximum
     constexpr int COLS = D / 2 / STEP;
