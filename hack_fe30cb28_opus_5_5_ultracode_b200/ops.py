@@ -711,7 +711,7 @@ _ATTN_MOD = _lib.packer("ql_attn_mod_args", """q k v out lse cu_seqlens slopes p
     dtype causal window""")
 
 
-def _attn_mod_inputs(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes, window, doc_ids,
+def _attn_mod_inputs(q, k, v, cu_seqlens, max_len, scale, softcap, slopes, window, doc_ids,
                      prefix_len):
     """The checked sizes both directions of attn_mod share: (n, HQ, HKV, D, B, row strides of q, k
     and v, dtype code, device index, window as the library takes it)."""
@@ -750,8 +750,6 @@ def _attn_mod_inputs(q, k, v, cu_seqlens, max_len, scale, causal, softcap, slope
         _exact(doc_ids, "doc_ids", (n,), torch.int32)
     if prefix_len is not None:
         _exact(prefix_len, "prefix_len", (B,), torch.int32)
-        if not causal:
-            raise ValueError("prefix_len needs causal=True (without it every key is seen already)")
     if not (0 <= max_len <= n and window >= 0 and 0 < scale < _INF and 0 <= softcap < _INF):
         raise ValueError("needs 0 <= max_len <= tokens, window >= 0, 0 < scale < inf and "
                          "0 <= softcap < inf")
@@ -767,12 +765,13 @@ def attn_mod_fwd(q, k, v, cu_seqlens, max_len, scale, causal=True, softcap=0.0, 
     q [n, HQ, D], k / v [n, HKV, D] (fp16 or bf16, D 64 or 128; rows may be strided, e.g. slices of
     a fused qkv), cu_seqlens int32 [B + 1], max_len at least the longest sequence. With positions
     i, j within a sequence: s = cap(scale q_i . k_j) - slopes[h] |i - j|, cap(x) = softcap
-    tanh(x / softcap); a query sees key j if j <= i or j < prefix_len[b] (causal), |i - j| < window
+    tanh(x / softcap); a query sees key j if j <= i or j < prefix_len[b] (causal;
+    without it prefix_len changes nothing), |i - j| < window
     (window > 0), and both are in the same run of equal doc_ids (negative ids: padding). slopes
     fp32 [HQ], doc_ids int32 [n], prefix_len int32 [B]. out as q (contiguous), lse fp32 [HQ, n];
     a query that sees nothing gets out 0 and lse -inf. Rows behind the last sequence are not written."""
     n, HQ, HKV, D, B, ld, dt, dev, window = _attn_mod_inputs(
-        q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes, window, doc_ids, prefix_len)
+        q, k, v, cu_seqlens, max_len, scale, softcap, slopes, window, doc_ids, prefix_len)
     if out is None:
         out = q.new_empty((n, HQ, D))
     else:
@@ -795,7 +794,7 @@ def attn_mod_bwd(dout, q, k, v, out, lse, cu_seqlens, max_len, scale, causal=Tru
     """(dq, dk, dv) of attn_mod_fwd, in q's dtype, given its arguments, out and lse
     (ql_attn_mod_bwd); dout [n, HQ, D] contiguous. Bit-identical from run to run."""
     n, HQ, HKV, D, B, ld, dt, dev, window = _attn_mod_inputs(
-        q, k, v, cu_seqlens, max_len, scale, causal, softcap, slopes, window, doc_ids, prefix_len)
+        q, k, v, cu_seqlens, max_len, scale, softcap, slopes, window, doc_ids, prefix_len)
     dtype, shape, kv = q.dtype, (n, HQ, D), (n, HKV, D)
     _given(dout, "dout", shape, dtype, dev)
     _given(out, "out", shape, dtype, dev)

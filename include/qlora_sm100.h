@@ -493,7 +493,7 @@ typedef struct {
   float* lse;
   const int32_t* cu_seqlens;  /* [B + 1] */
   const float* slopes;        /* [HQ] or NULL */
-  const int32_t* prefix_len;  /* [B] or NULL (needs causal) */
+  const int32_t* prefix_len;  /* [B] or NULL; no effect without causal */
   const int32_t* doc_ids;     /* [n] or NULL */
   int32_t* ranges;            /* workspace [n][2], 8-byte aligned, with doc_ids */
   const void* dout;           /* backward only, as the next five */

@@ -372,14 +372,13 @@ def test_no_tokens_and_no_sequences():
     dict(softcap=math.nan), dict(softcap=1e-6), dict(window=-1), dict(max_len=-1), dict(max_len=11),
     dict(k="heads"), dict(k="dtype"), dict(k="short"), dict(k="order"), dict(k="odd"),
     dict(v="expand"), dict(cu="long"), dict(cu="none"), dict(slopes="short"), dict(slopes="half"),
-    dict(doc_ids="short"), dict(prefix_len="short"), dict(prefix_len="ok", causal=False),
+    dict(doc_ids="short"), dict(prefix_len="short"),
     dict(doc_ids="cpu"), dict(D=96), dict(dtype=torch.float32), dict(out="dtype"),
     dict(lse="shape")], ids=str)
 def test_bad_arguments_are_refused(change):
     D, dtype = change.get("D", 64), change.get("dtype", torch.float16)
     q, k, v, dout, cu = batch([10], (4, 2, D), dtype)
-    kw = dict(causal=change.get("causal", True))
-    kw.update({x: change[x] for x in ("softcap", "window") if x in change})
+    kw = {x: change[x] for x in ("softcap", "window") if x in change}
     kind = change.get("k")
     k = {"heads": k[:, :1].repeat(1, 3, 1), "dtype": k.bfloat16(), "short": k[:9],
          "order": k.transpose(0, 1).contiguous().transpose(0, 1),
@@ -389,7 +388,7 @@ def test_bad_arguments_are_refused(change):
     cu = {"long": cu.long(), "none": cu[:0]}.get(change.get("cu"), cu)
     extra = {"slopes": {"short": torch.ones(3), "half": torch.ones(4).half()},
              "doc_ids": {"short": torch.zeros(9).int(), "cpu": torch.zeros(10).int()},
-             "prefix_len": {"short": torch.zeros(2).int(), "ok": torch.zeros(1).int()}}
+             "prefix_len": {"short": torch.zeros(2).int()}}
     for name, kinds in extra.items():
         if name in change:
             t = kinds[change[name]]
@@ -484,3 +483,15 @@ def test_tensors_beyond_32_bit_offsets():
     for x, y in zip((out, *got), (one_out, *one)):
         assert (x[last].double() - y.double()).norm() < TOL[dtype] * y.double().norm()
     assert torch.allclose(lse[:, last], one_lse, atol=2e-5, rtol=0)
+
+
+@pytest.mark.gpu
+def test_a_prefix_without_causal_changes_nothing():
+    q, k, v, dout, cu = batch([200, 90], (2, 1, 128), torch.bfloat16, seed=16)
+    prefix = torch.tensor([50, 90], dtype=torch.int32).cuda()
+    for mods in (dict(), dict(window=40)):
+        a = ops.attn_mod_fwd(q, k, v, cu, 200, 0.1, causal=False, **mods)
+        b = ops.attn_mod_fwd(q, k, v, cu, 200, 0.1, causal=False, prefix_len=prefix, **mods)
+        g = ops.attn_mod_bwd(dout, q, k, v, *a, cu, 200, 0.1, causal=False, **mods)
+        h = ops.attn_mod_bwd(dout, q, k, v, *b, cu, 200, 0.1, causal=False, prefix_len=prefix, **mods)
+        assert all(torch.equal(x, y) for x, y in zip((*a, *g), (*b, *h)))
