@@ -20,7 +20,7 @@
 // acc1, and 8,192 causal tokens of 12 + 2 heads took 5% longer.) Sixteen softmax warps, four threads
 // per TMEM lane with 32 of the 128 columns each (no row reduction: the forward's lse is known).
 //
-// That shape takes 601 us for both launches (forward: 162): eight products at 1,370 TFLOP/s, what the
+// That shape takes 601 us for both launches (forward: 160): eight products at 1,370 TFLOP/s, what the
 // tensor cores sustain under the board's power limit. Twice the softmax's exponentials ride along.
 //
 // Why the dQ role needs P K: Dvec from the forward's 16-bit output is off by the output's rounding,
@@ -41,6 +41,24 @@ constexpr int BWD_THREADS = BWD_SOFTMAX + 64;
 constexpr int BOX = AM_T * 128;               // a 128-row x 64-column box
 constexpr int HC = 32;                        // columns per softmax thread
 
+// Batches of up to so many tokens run each step twice (TWICE), with the 16-bit roundings of P and dS and
+// then with the roundings of what those left: with few tokens the errors of single roundings do not
+// average out, and one such batch in 12 had a dQ or dK more than 1.5 times as far from the 64-bit one
+// as its own rounding (in two parts none of 109). 1 to 4 x 100 tokens of 12 + 2 heads: both launches 20 -> 25 us; 64 x 60
+// would go from 103 to 132.
+constexpr int TWICE_TOKENS = 256;
+
+// Two values as 16-bit numbers: their roundings, or (lo) the roundings of what those leave
+template <typename T, bool TWICE>
+__device__ __forceinline__ float part_t2(float a, float b, bool lo) {
+  uint32_t h = pack_t2<T>(a, b);
+  if (TWICE && lo) {
+    const T* v = reinterpret_cast<const T*>(&h);
+    h = pack_t2<T>(a - to_f<T>(v[0]), b - to_f<T>(v[1]));
+  }
+  return __uint_as_float(h);
+}
+
 struct BwdConst {
   float sl2, u, cap2, slope2;
   TanhShort ts;
@@ -54,9 +72,9 @@ struct BwdConst {
 // one value. Columns whose bit in seen is 0 give 0. dist0: row index minus the first column's, for
 // the distance bias. p: plain probabilities where the caller needs them beside f (a capped score of
 // the dQ role).
-template <typename T, int MODE, bool MASKED, bool PER_COL>
+template <typename T, int MODE, bool MASKED, bool PER_COL, bool TWICE>
 __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, const BwdConst& c, int form,
-                                          const float* neg_lse, float neg_lse_row, float dist0, uint32_t seen) {
+                                          const float* neg_lse, float neg_lse_row, float dist0, uint32_t seen, bool lo) {
   uint64_t y[8], bend[8];
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
@@ -116,7 +134,7 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
       if (MASKED && pa == 0.f) fa = 0.f;
       if (MASKED && pb == 0.f) fb = 0.f;
       if constexpr (PER_COL) {
-        p16[e] = __uint_as_float(pack_t2<T>(pa, pb));
+        p16[e] = part_t2<T, TWICE>(pa, pb, lo);
       } else {
         p[k] = pa;
         p[k + 1] = pb;
@@ -129,9 +147,9 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
 
 // dS = f (dP dscale - Dvec') as 16-bit pairs; neg_d: -Dvec' by column or one value. The dQ role also
 // gets sum p (dP - Dvec) of its columns.
-template <typename T, int MODE, bool MASKED, bool PER_COL, int N>
+template <typename T, int MODE, bool MASKED, bool PER_COL, bool TWICE, int N>
 __device__ __forceinline__ float bwd_ds(const uint32_t* f, const float* p, const uint32_t* dp, float* ds16,
-                                        float dscale, const float* neg_d, float neg_d_row, uint32_t seen) {
+                                        float dscale, const float* neg_d, float neg_d_row, uint32_t seen, bool lo) {
   const uint64_t row2 = pk2(neg_d_row, neg_d_row), ds2 = pk2(dscale, dscale);
   uint64_t sum[2] = {0, 0};  // pairs of +0.f
 #pragma unroll
@@ -171,12 +189,12 @@ __device__ __forceinline__ float bwd_ds(const uint32_t* f, const float* p, const
     for (int e = 0; e < 8; ++e) {
       float a, b;
       up2(g[e], a, b);
-      ds16[i / 2 + e] = __uint_as_float(pack_t2<T>(a, b));
+      ds16[i / 2 + e] = part_t2<T, TWICE>(a, b, lo);
     }
   }
   float a, b;
   up2(add2(sum[0], sum[1]), a, b);
-  return a + b;
+  return TWICE && lo ? 0.f : a + b;
 }
 
 template <int MODE>
@@ -219,7 +237,7 @@ struct BwdCfg {
 // fp16, dK / dV: P is kept as 2^8 P (at most 2^8 where P is 1), so that the small probabilities of
 // long rows stay normal numbers; dS and dV take the factor back in fp32.
 // TMEM: S [0, 128), dP, then P and dS [128, 256), acc1 [256, 256 + D), acc2 [384, 384 + D).
-template <typename T, int D, int MODE, bool DKV>
+template <typename T, int D, int MODE, bool DKV, bool TWICE>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
     attn_mod_bwd_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap ty,
                         const __grid_constant__ CUtensorMap tu, const __grid_constant__ CUtensorMap tw,
@@ -307,7 +325,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   }
   if (warp == 16) tmem_alloc(tmem_slot, 512);
   const AttnBlocks tb = DKV ? attn_key_blocks(seq, r0) : attn_tile_blocks(seq, r0);
-  const int ntile = tb.end - tb.first, steps = uniform(ntile * heads);
+  const int ntile = tb.end - tb.first, steps = uniform(ntile * heads * (TWICE ? 2 : 1));
   if (warp == 17 && lane == 0 && steps > 0) {
     const int zx = (DKV ? kvh : h0) * (D / 64);
     mbar_arrive_expect_tx(xy_full, 2 * C::TILE);
@@ -340,10 +358,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     bool ok = true;
     int un = 0, wn = 0;        // tiles sent for
     uint32_t raw_phase = 0;    // of raw[0 .. UST + WST)
-    auto row_of = [&](int n) { return (tb.first + (DKV ? n % ntile : n)) * AM_T; };
+    auto row_of = [&](int n) { return (tb.first + (DKV ? (n >> TWICE) % ntile : n >> TWICE)) * AM_T; };
     auto send = [&](int n, bool is_w, const DeadRows& d) {
       const int s = is_w ? n % C::WST : n % C::UST;
-      const int z = (DKV ? h0 + n / ntile : kvh) * (D / 64);
+      const int z = (DKV ? h0 + (n >> TWICE) / ntile : kvh) * (D / 64);
       uint64_t* bar = d.any ? &raw[is_w ? C::UST + s : s] : is_w ? &w_full[s] : &u_full[s];
       if (lane == 0) {
         mbar_arrive_expect_tx(bar, C::TILE);
@@ -378,7 +396,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       float l[4], dv[4];
       if constexpr (DKV) {
         const int row = row_of(n);
-        const int64_t at = (int64_t)(h0 + n / ntile) * a.n + seq.start + row;
+        const int64_t at = (int64_t)(h0 + (n >> TWICE) / ntile) * a.n + seq.start + row;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int t = u * 32 + lane;
@@ -496,8 +514,9 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     bool ok = true;
     const uint32_t ts = lane_base + part * HC;
     for (int n = 0; n < steps; ++n) {
-      const int s = n & 1, j = tb.first + (DKV ? n % ntile : n), i0 = j * AM_T + part * HC;
-      if (DKV && (MODE & 2) != 0 && n > 0 && n % ntile == 0) c = bwd_const<MODE>(a, h0 + n / ntile);
+      const bool lo = TWICE && (n & 1) != 0;
+      const int m = n >> TWICE, s = n & 1, j = tb.first + (DKV ? m % ntile : m), i0 = j * AM_T + part * HC;
+      if (DKV && (MODE & 2) != 0 && m > 0 && m % ntile == 0) c = bwd_const<MODE>(a, h0 + m / ntile);
       const bool masked = j < tb.ffirst || j >= tb.fend;
       const uint32_t seen = masked ? col_mask(range.x - i0, range.y - i0) : 0;
       const float dist0 = (float)(ri - i0);
@@ -517,8 +536,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 #pragma unroll
       for (int g = 0; g < HC; g += 16) {
         float* pg = p + ((MODE & 1) != 0 && !DKV ? g : 0);
-        if (masked) bwd_probs<T, MODE, true, DKV>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, seen >> g);
-        else bwd_probs<T, MODE, false, DKV>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, 0);
+        if (masked) bwd_probs<T, MODE, true, DKV, TWICE>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, seen >> g, lo);
+        else bwd_probs<T, MODE, false, DKV, TWICE>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, 0, lo);
       }
       ok = warp_wait(dp_full, n & 1, err);
       if (!ok) break;
@@ -533,10 +552,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
           tmem_ld16(ts + 128 + g, dh);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            w[g / 2 + e] = __uint_as_float(pack_t2<T>(__uint_as_float(x[g + 2 * e]), __uint_as_float(x[g + 2 * e + 1])));
+            w[g / 2 + e] = part_t2<T, TWICE>(__uint_as_float(x[g + 2 * e]), __uint_as_float(x[g + 2 * e + 1]), lo);
           const uint32_t* du = reinterpret_cast<const uint32_t*>(dh);
-          if (masked) rest += bwd_ds<T, MODE, true, DKV, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, seen >> g);
-          else rest += bwd_ds<T, MODE, false, DKV, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, 0);
+          if (masked) rest += bwd_ds<T, MODE, true, DKV, TWICE, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, seen >> g, lo);
+          else rest += bwd_ds<T, MODE, false, DKV, TWICE, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, 0, lo);
         }
         tmem_st16(ts + 128, w);
         tmem_st16(ts + 128 + HC / 2, ds);
@@ -550,14 +569,14 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         if constexpr ((MODE & 1) == 0) {  // acc1 takes f itself
 #pragma unroll
           for (int e = 0; e < HC / 2; ++e)
-            w[e] = __uint_as_float(pack_t2<T>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])));
+            w[e] = part_t2<T, TWICE>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]), lo);
         }
         tmem_st16(ts + 128, w);
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(p_full);
-        if (masked) rest += bwd_ds<T, MODE, true, DKV, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, seen);
-        else rest += bwd_ds<T, MODE, false, DKV, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, 0);
+        if (masked) rest += bwd_ds<T, MODE, true, DKV, TWICE, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, seen, lo);
+        else rest += bwd_ds<T, MODE, false, DKV, TWICE, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, 0, lo);
         tmem_st16(ts + 128 + HC / 2, w);
         tmem_wait_st();
         tc_fence_before();
@@ -580,6 +599,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       rest = (sR[r] + sR[AM_T + r]) + (sR[2 * AM_T + r] + sR[3 * AM_T + r]);
       if (ok && live && part == 0) a.dvec[(int64_t)h0 * a.n + seq.start + ri] = rest - neg_d;
       if (ok) {
+        const float sc = range.y - range.x == 1 ? 0.f : SIGN * a.scale;  // one key: the softmax is constant
 #pragma unroll
         for (int u = 0; u < D / 64; ++u) {
           float pk[16], v[16];
@@ -588,7 +608,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             tmem_ld16(lane_base + 384 + col0 + u * 16, v);
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = steps > 0 ? (v[e] - rest * pk[e]) * (SIGN * a.scale) : 0.f;
+          for (int e = 0; e < 16; ++e) v[e] = steps > 0 ? (v[e] - rest * pk[e]) * sc : 0.f;
           stage16<T, W>(stage, lane, u, v);
         }
         T* dst = reinterpret_cast<T*>(a.dq) + ((int64_t)(seq.start + row0) * a.HQ + h0) * D + col0;
@@ -678,12 +698,12 @@ int dkv_splits(const AttnModArgs& a) {
   return group;
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D, int MODE, bool TWICE>
 int launch_bwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mdo,
                const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
   static unsigned long long done_q = 0, done_kv = 0;
-  auto kq = attn_mod_bwd_kernel<T, D, MODE, false>;
-  auto kkv = attn_mod_bwd_kernel<T, D, MODE, true>;
+  auto kq = attn_mod_bwd_kernel<T, D, MODE, false, TWICE>;
+  auto kkv = attn_mod_bwd_kernel<T, D, MODE, true, TWICE>;
   constexpr int smem = BwdCfg<D>::SMEM;
   int st = attn_smem_limit(reinterpret_cast<const void*>(kq), smem, &done_q);
   if (st == QL_STATUS_OK) st = attn_smem_limit(reinterpret_cast<const void*>(kkv), smem, &done_kv);
@@ -699,14 +719,21 @@ int launch_bwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& m
   return launched(a.splits > 1 ? 3 : 2);
 }
 
+template <typename T, int D, int MODE>
+int pick_bwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMap& mk,
+             const CUtensorMap& mv, cudaStream_t s) {
+  return a.n <= TWICE_TOKENS ? launch_bwd<T, D, MODE, true>(a, mq, mdo, mk, mv, s)
+                                : launch_bwd<T, D, MODE, false>(a, mq, mdo, mk, mv, s);
+}
+
 template <typename T, int D>
 int dispatch_bwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mdo,
                  const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
   switch (attn_mode(a)) {
-    case 0: return launch_bwd<T, D, 0>(a, mq, mdo, mk, mv, s);
-    case 1: return launch_bwd<T, D, 1>(a, mq, mdo, mk, mv, s);
-    case 2: return launch_bwd<T, D, 2>(a, mq, mdo, mk, mv, s);
-    default: return launch_bwd<T, D, 3>(a, mq, mdo, mk, mv, s);
+    case 0: return pick_bwd<T, D, 0>(a, mq, mdo, mk, mv, s);
+    case 1: return pick_bwd<T, D, 1>(a, mq, mdo, mk, mv, s);
+    case 2: return pick_bwd<T, D, 2>(a, mq, mdo, mk, mv, s);
+    default: return pick_bwd<T, D, 3>(a, mq, mdo, mk, mv, s);
   }
 }
 

@@ -495,3 +495,29 @@ def test_a_prefix_without_causal_changes_nothing():
         g = ops.attn_mod_bwd(dout, q, k, v, *a, cu, 200, 0.1, causal=False, **mods)
         h = ops.attn_mod_bwd(dout, q, k, v, *b, cu, 200, 0.1, causal=False, prefix_len=prefix, **mods)
         assert all(torch.equal(x, y) for x, y in zip((*a, *g), (*b, *h)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths", [[45, 27], [5, 3, 9, 2], [1, 2, 1], [200]], ids=str)
+@pytest.mark.parametrize("mode", [dict(), dict(softcap=30.0), dict(slopes=True, causal=False)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_gradients_of_few_tokens_carry_their_own_rounding_only(lengths, mode, dtype):
+    """P and dS in two 16-bit parts: what stays is half a step of each result (the parts' own rest is
+    below 2^-15 of it, fp32 sums likewise: a tenth of a half-step is left for them)."""
+    heads, scale = (6, 2, 64), 0.125
+    q, k, v, dout, cu = batch(lengths, heads, dtype, seed=17)
+    host, dev = mode_args(mode, lengths, heads[0])
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, max(lengths), scale, **dev)
+    got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, max(lengths), scale, **dev)
+    want = formula(q, k, v, lengths, scale, dout=dout, **host)[2:]
+    for name, x, y in zip(("dq", "dk", "dv"), got, want):
+        assert rel(x, y) < 1.1 * torch.finfo(dtype).eps / 2, name
+
+
+@pytest.mark.gpu
+def test_rows_of_one_key_have_no_gradient_in_q():
+    q, k, v, dout, cu = batch([1, 300, 1], (4, 2, 64), torch.bfloat16, seed=18)
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, 300, 0.125, window=1, softcap=20.0)
+    dq, dk, dv = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 300, 0.125, window=1, softcap=20.0)
+    assert not dq.any() and torch.equal(out, v.repeat_interleave(2, 1))
+    assert rel(dv, dout.double().cpu().unflatten(1, (2, 2)).sum(2)) < 2.0 ** -8
