@@ -792,7 +792,8 @@ def attn_mod_fwd(q, k, v, cu_seqlens, max_len, scale, causal=True, softcap=0.0, 
 def attn_mod_bwd(dout, q, k, v, out, lse, cu_seqlens, max_len, scale, causal=True, softcap=0.0,
                  slopes=None, window=0, doc_ids=None, prefix_len=None, dq=None, dk=None, dv=None):
     """(dq, dk, dv) of attn_mod_fwd, in q's dtype, given its arguments, out and lse
-    (ql_attn_mod_bwd); dout [n, HQ, D] contiguous. Bit-identical from run to run."""
+    (ql_attn_mod_bwd); dout [n, HQ, D] contiguous; the gradients must not share memory with the
+    inputs. Bit-identical from run to run."""
     n, HQ, HKV, D, B, ld, dt, dev, window = _attn_mod_inputs(
         q, k, v, cu_seqlens, max_len, scale, softcap, slopes, window, doc_ids, prefix_len)
     dtype, shape, kv = q.dtype, (n, HQ, D), (n, HKV, D)
