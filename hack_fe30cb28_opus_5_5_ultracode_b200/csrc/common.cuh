@@ -57,8 +57,9 @@ __device__ __forceinline__ unsigned long long global_ns() {
   return t;
 }
 
+// Records a status; the highest code stays, so a timeout is seen whatever was recorded before it.
 __device__ __forceinline__ void raise_status(int* err, int code) {
-  if (err != nullptr) atomicCAS(err, 0, code);
+  if (err != nullptr) atomicMax(err, code);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -100,7 +101,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 
 // Waits for the phase of the given parity to complete. Returns false (and records a timeout in
 // *err) if it has not after limit_ns (QL_WAIT_NS unless a caller passes less); the caller then
-// stops issuing work. A wait also gives up as soon as another role has recorded a status.
+// stops issuing work. A wait also gives up as soon as another role has recorded a timeout; other
+// statuses (a bad id or position among some call's data) are no reason to leave work undone.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err,
                                           unsigned long long limit_ns = QL_WAIT_NS) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -112,7 +114,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
         raise_status(err, QL_STATUS_TIMEOUT);
         return false;
       }
-      if (err != nullptr && *(volatile int*)err != 0) return false;  // another role gave up
+      if (err != nullptr && *(volatile int*)err == QL_STATUS_TIMEOUT) return false;  // another role gave up
     }
   }
   return true;

@@ -245,7 +245,8 @@ def launch_count():
 
 
 def device_status(clear=True):
-    """The library's device status word (QL_STATUS_TIMEOUT if a kernel gave up a wait)."""
+    """The library's device status word: QL_STATUS_TIMEOUT if a kernel gave up a wait, else
+    QL_STATUS_BAD_ARG if an id or position lay outside its table."""
     import ctypes
 
     v = ctypes.c_int(0)
@@ -406,7 +407,8 @@ def mrope_fwd(qkv, cos, sin, pos, HQ, HKV, D, sections, interleaved=False, lora_
     """(q, k, v) of rope_fwd with several position axes (ql_mrope_fwd): pos int32 [axes, n],
     sections = how many of the D / 2 frequencies each axis has, in blocks or (interleaved) dealt
     to the axes in turn while an axis has some left; cos / sin the rotary table of one axis.
-    xq / Bq, xv / Bv: the LoRA-B products q += lora_scale xq Bq^T, added in fp32."""
+    xq / Bq, xv / Bv: the LoRA-B products q += lora_scale xq Bq^T, added in fp32. A position outside the
+    table turns nothing (its frequencies give 0) and is recorded for device_status()."""
     dev = _index_of(qkv, cos, sin, pos, xq, xv, Bq, Bv)
     if qkv.dim() != 2:
         raise ValueError("qkv must be [tokens, (HQ + 2 HKV) D]")

@@ -34,8 +34,11 @@ enum { QL_F16 = 0, QL_BF16 = 1, QL_F32 = 2 };
 const char* ql_version(void);
 /* Message of the last failed call on this host thread ("" if none). */
 const char* ql_last_error(void);
-/* Reads (and with clear != 0 resets) the device status word of the current device. Synchronous
- * (a device-to-host copy on the legacy stream): for tests and error paths, not the step. */
+/* Reads (and with clear != 0 resets) the device status word of the current device: the highest
+ * status a kernel has recorded. QL_STATUS_BAD_ARG (an id or position outside its table) changes
+ * nothing in other calls; after QL_STATUS_TIMEOUT the kernels that have to wait for long give up
+ * too until it is cleared. Synchronous (a device-to-host copy on the legacy stream): for tests and
+ * error paths, not the step. */
 int ql_device_status(int* status_out, int clear);
 /* Device address of the status word, which kernels are given to record a timeout in. */
 int* ql_device_status_ptr(void);
@@ -236,7 +239,8 @@ int ql_rope_bwd(const ql_rope_bwd_args* args, cudaStream_t stream);
  * left. D a multiple of 64, at most 256; rank 16; all tensors contiguous and 16-byte aligned
  * (x*, B*: 8-byte). The LoRA-B product is added in fp32 without a rounding of its own, and dxlo is
  * lora_scale * (g . B) of the unrounded gradient g, in fp32. A position outside [0, positions)
- * records QL_STATUS_BAD_ARG in the device status word; its frequencies give 0. */
+ * records QL_STATUS_BAD_ARG in the device status word, where it stays until it is read with clear
+ * (or a timeout is recorded over it); its frequencies give 0. Other calls are not affected. */
 typedef struct {
   const void* qkv;      /* [n, (HQ + 2 HKV) D] */
   const void* xq;       /* [n, 16] or NULL: q += lora_scale * xq . Bq^T */

@@ -1,6 +1,8 @@
 """qkv + LoRA + RoPE with several position axes (ops.mrope_fwd / mrope_bwd) against the formula in 64
 bits, and its refusals (CPU)."""
 
+import time
+
 import pytest
 import torch
 
@@ -232,3 +234,26 @@ def test_tensors_beyond_32_bit_offsets():
     alone = ops.mrope_bwd(*one, *tables, c["pos"], *heads, sections, dtype=torch.bfloat16, Bq=c["Bq"])
     assert torch.equal(back[0][-few:], alone[0])
     assert rel(back[1][-few:], alone[1].double().cpu()) < 2.0 ** -20
+
+
+@pytest.mark.gpu
+def test_a_bad_position_leaves_the_waits_of_other_calls_alone():
+    """The status word keeps the bad argument, and a wait that runs out afterwards lasts as long as its
+    limit and is recorded over it; other kernels run as if nothing had been recorded."""
+    heads, sections = (4, 2, 64), (8, 12, 12)
+    c = cuda(case(5, heads, torch.float16, sections))
+    c["pos"][1, 2] = -1
+    ops.device_status(clear=True)
+    ops.mrope_fwd(c["qkv"], c["cos"], c["sin"], c["pos"], *heads, sections)
+    assert ops.device_status(clear=False) == ops.STATUS_BAD_ARG
+    a, b = torch.randn(4096, 2048, device="cuda").half(), torch.randn(4096, 2048, device="cuda").half()
+    want = a.float() @ b.float().t()
+    for _ in range(5):
+        assert rel(ops.gemm(a, b), want.double().cpu()) < 1e-3
+    assert ops.device_status(clear=False) == ops.STATUS_BAD_ARG
+    returned = torch.zeros(1, device="cuda", dtype=torch.int32)
+    t0 = time.perf_counter()
+    _lib.call("ql_wait_probe", int(50e6), returned.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert returned.item() == 2 and 0.04 < time.perf_counter() - t0 < 1.9
+    assert ops.device_status(clear=True) == ops.STATUS_TIMEOUT
