@@ -11,7 +11,8 @@
 // 8 t + 2 j + e in column 2 t + e of step j, thread t of a row ends up with eight consecutive
 // columns after four steps - one 16-byte load and store. The product stays in fp32 (nothing is
 // rounded between the factors and the output). The backward uses the same ordering for the K
-// dimension of dx_lo = s g B, with g split into 16-bit parts, so dx_lo is good to fp32.
+// dimension of dx_lo = s g B, with g split into 16-bit parts (fp16: brought to one size by a power of
+// two per token and unit first), so dx_lo is good to fp32 whatever the gradients' size.
 //
 // Bound: HBM for long batches (2 bytes read and 2 written per element in each direction), launch and
 // L2 latency for short ones.
@@ -237,26 +238,54 @@ __global__ void __launch_bounds__(MR_THREADS, MR_CTAS) mrope_fwd_kernel(const __
   }
 }
 
-// c[2 tiles of N][4] += g . B for 32 columns of g (this thread: 8 t .. 8 t + 7 of tokens g and g + 8)
+// The power of two that brings a token's largest of 32 gradients to [2^14, 2^15), and its inverse. fp16
+// has no number below 2^-24 and none above 65,504: unscaled, the second part of a gradient of 10^-3
+// lost all but 2^-16 of it (10^-5: 2^-9), and fp32 gradients above 65,504 had none. A token's scale is
+// its own, as sizes differ from token to token; 0 (and what fp32 holds as a subnormal), infinities and NaN
+// keep a scale of 1.
+struct TokenScale {
+  float up, down;
+};
+__device__ __forceinline__ TokenScale token_scale(const float* v) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  int e = __float_as_int(m) >> 23;           // biased exponent
+  if (e == 0 || e == 255) return {1.f, 1.f};
+  e = max(e, 15);
+  return {__int_as_float((268 - e) << 23), __int_as_float((e - 14) << 23)};
+}
+
+// acc[2 tiles of N][4] += g . B for 32 columns of g (this thread: 8 t .. 8 t + 7 of tokens g and g + 8)
 // and the 32 rows of B from o0 on. Column n of N tile nt is rank 2 n + nt, so one 32-bit load of a
 // row of B serves both tiles; K index 2 t + e (8 + 2 t + e) of step s is row 8 t + 4 s + e (+ 2).
 template <typename T>
-__device__ __forceinline__ void lora_back(const float (*gv)[8], const void* B, int64_t o0, float (*c)[4]) {
+__device__ __forceinline__ void lora_back(const float (*gv)[8], const void* B, int64_t o0, float (*acc)[4]) {
+  constexpr bool SCALED = std::is_same<T, __half>::value;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t* base = reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(B) + (o0 + t * 8) * MR_RANK) + g;
+  float own[2][4] = {};
+  float (*c)[4] = SCALED ? own : acc;
+  TokenScale sc[2];
+  if constexpr (SCALED) {
+    sc[0] = token_scale(gv[0]);
+    sc[1] = token_scale(gv[1]);
+  }
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = __ldg(base + (4 * s + e) * (MR_RANK / 2));
     // g in PARTS 16-bit pieces, each the rounding of what the ones before left: 2^-24 (bf16) or
-    // 2^-22 (fp16) of g stays behind
+    // 2^-22 (fp16) of g stays behind, or 2^-39 of the token's largest
     constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
     float left[2][4];
 #pragma unroll
     for (int rh = 0; rh < 2; ++rh)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) left[rh][k] = gv[rh][4 * s + k];
+      for (int k = 0; k < 4; ++k) left[rh][k] = SCALED ? gv[rh][4 * s + k] * sc[rh].up : gv[rh][4 * s + k];
 #pragma unroll
     for (int part = 0; part < PARTS; ++part) {
       uint32_t af[4];
@@ -276,6 +305,12 @@ __device__ __forceinline__ void lora_back(const float (*gv)[8], const void* B, i
         mma16816<T>(c[nt], af, __byte_perm(w[0], w[1], sel), __byte_perm(w[2], w[3], sel));
       }
     }
+  }
+  if constexpr (SCALED) {
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[nt][e] = fmaf(own[nt][e], sc[e >> 1].down, acc[nt][e]);
   }
 }
 

@@ -257,3 +257,57 @@ def test_a_bad_position_leaves_the_waits_of_other_calls_alone():
     torch.cuda.synchronize()
     assert returned.item() == 2 and 0.04 < time.perf_counter() - t0 < 1.9
     assert ops.device_status(clear=True) == ops.STATUS_TIMEOUT
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-6, 1e-3, 1.0, 3e4, 1e6])
+@pytest.mark.parametrize("dtype,grads", [(torch.float16, torch.float32), (torch.float16, torch.float16),
+                                         (torch.bfloat16, torch.float32)], ids=str)
+def test_dx_lo_is_good_to_fp32_for_gradients_of_any_size(size, dtype, grads):
+    """One gradient a token, not turned (position 0), beside tokens with gradients of other sizes: dx_lo is
+    the product of two numbers. The parts g is split into leave 2^-22 of it at most, their
+    products with B are exact in fp32, and their sum, the CTA's and the scaling by 1.5 round
+    at most five times, by up to 2^-23 each: below 2^-20 together."""
+    HQ, HKV, D = heads = (4, 2, 64)
+    if grads == torch.float16 and size > 3e4:
+        size = 6e4
+    n, sections = 40, (8, 12, 12)
+    c = case(n, heads, dtype, sections, seed=21)
+    c["pos"].zero_()
+    g = torch.Generator().manual_seed(22)
+    at = torch.randint(0, HQ * D, (n,), generator=g), torch.randint(0, HKV * D, (n,), generator=g)
+    sizes = torch.where(torch.arange(n) % 3 == 0, 1.0, size)  # every third token ordinary
+    dq, dv = torch.zeros(n, HQ * D), torch.zeros(n, HKV * D)
+    for x, col in ((dq, at[0]), (dv, at[1])):
+        x[torch.arange(n), col] = (torch.rand(n, generator=g) + 0.09) * sizes
+    dq, dv = dq.to(grads), dv.to(grads)
+    d = cuda(c)
+    _, dxq, dxv = ops.mrope_bwd(dq.cuda().view(n, HQ, D), torch.zeros(n, HKV, D, device="cuda", dtype=grads),
+                                dv.cuda().view(n, HKV, D), d["cos"], d["sin"], d["pos"], *heads, sections,
+                                dtype=dtype, Bq=d["Bq"], Bv=d["Bv"], lora_scale=1.5)
+    assert ops.device_status() == 0
+    for got, x, B in ((dxq, dq, c["Bq"]), (dxv, dv, c["Bv"])):
+        want = 1.5 * x.double() @ B.double()
+        assert ((got.double().cpu() - want).abs() <= 2.0 ** -20 * want.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [77, 5003])
+@pytest.mark.parametrize("size", [1e-5, 1e-3, 1e6])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_dx_lo_of_small_and_large_gradients(size, dtype, n):
+    """Dense fp32 gradients whose sizes differ from token to token. Against |g| |B| summed, an fp32 sum of
+    256 terms in 16-term steps rounds some 50 times (split parts included) by at most 2^-23."""
+    HQ, HKV, D = heads = (4, 2, 64)
+    c, sections = case(n, heads, dtype, (8, 12, 12), seed=23), (8, 12, 12)
+    by = size * 10.0 ** (torch.arange(n) % 4 - 2.0)[:, None, None]
+    for x in ("dq", "dk", "dv"):
+        c[x] = c[x] * by
+    d = cuda(c)
+    got = ops.mrope_bwd(d["dq"], d["dk"], d["dv"], d["cos"], d["sin"], d["pos"], *heads, sections, dtype=dtype,
+                        Bq=d["Bq"], Bv=d["Bv"])[1:]
+    cos, sin = angles(c["cos"], c["sin"], c["pos"], sections, False)
+    gq, gv = rotate(c["dq"].double(), cos, sin, back=True).view(n, -1), c["dv"].double().view(n, -1)
+    for a, g, B in zip(got, (gq, gv), (c["Bq"].double(), c["Bv"].double())):
+        assert ((a.double().cpu() - g @ B).abs() <= 50 * 2.0 ** -23 * (g.abs() @ B.abs())).all()
+    assert ops.device_status() == 0
