@@ -20,15 +20,16 @@
 // acc1, and 8,192 causal tokens of 12 + 2 heads took 5% longer.) Sixteen softmax warps, four threads
 // per TMEM lane with 32 of the 128 columns each (no row reduction: the forward's lse is known).
 //
-// That shape takes 601 us for both launches (forward: 160): eight products at 1,370 TFLOP/s, what the
-// tensor cores sustain under the board's power limit. Twice the softmax's exponentials ride along.
+// That shape takes 624 us for both launches (forward: 160): eight products at 1,320 TFLOP/s, near what
+// the tensor cores sustain under the board's power limit. Twice the softmax's exponentials ride along.
 //
 // Why the dQ role needs P K: Dvec from the forward's 16-bit output is off by the output's rounding,
 // and that error enters a whole row of dS with one sign - dQ was up to 1.9 times as far from the
 // 64-bit gradient as its own rounding, dK likewise. So the dQ role starts from that Dvec, sums the row
 // r = sum P (dP - Dvec) in fp32 (zero for an exact Dvec), and puts it right at the end:
 // dQ = scale (dS K - r P K); the second launch reads Dvec + r. P and dS are rounded to the input
-// type for the products; every sum is fp32.
+// type for the products, in two parts where few terms are summed (PARTS_ROWS); every sum is fp32. An fp16
+// dS above 65,504 is infinite, also where scale dS would not be.
 #include "attn_mod.cuh"
 #include "profile.h"
 
@@ -41,22 +42,35 @@ constexpr int BWD_THREADS = BWD_SOFTMAX + 64;
 constexpr int BOX = AM_T * 128;               // a 128-row x 64-column box
 constexpr int HC = 32;                        // columns per softmax thread
 
-// Batches of up to so many tokens run each step twice (TWICE), with the 16-bit roundings of P and dS and
-// then with the roundings of what those left: with few tokens the errors of single roundings do not
-// average out, and one such batch in 12 had a dQ or dK more than 1.5 times as far from the 64-bit one
-// as its own rounding (in two parts none of 109). 1 to 4 x 100 tokens of 12 + 2 heads: both launches 20 -> 25 us; 64 x 60
-// would go from 103 to 132.
-constexpr int TWICE_TOKENS = 256;
+// In a tile none of whose rows sees more than so many others, P and dS take part in the products as two
+// 16-bit numbers each (`parts`), their roundings and the roundings of what those leave: where few terms make
+// up a gradient the errors of single roundings do not average out, and one short batch in 12 had a dQ or
+// dK more than 1.5 times as far from the 64-bit one as its own rounding (in two parts none of 109). The
+// rule looks at the tile's own mask, so a sequence has the same gradients whatever it is packed with. The
+// second parts lie in S's columns, and the next S waits for their products. Both launches, single
+// against two parts, us: 64 x 60 tokens of 12 + 2 heads 101 / 113, 4 x 300 in documents of 90 28 / 33,
+// 8,192 with a window of 100 118 / 150, 24 k of 28 + 4 heads in documents of 90 610 / 785. Rows that do without
+// pay for the choice: 8,192 causal tokens 607 / 624 (the softmax warps have no register left).
+constexpr int PARTS_ROWS = 256;
 
-// Two values as 16-bit numbers: their roundings, or (lo) the roundings of what those leave
-template <typename T, bool TWICE>
-__device__ __forceinline__ float part_t2(float a, float b, bool lo) {
+// Two values as 16-bit numbers: their roundings, or (REST) the roundings of what those leave
+template <typename T, bool REST>
+__device__ __forceinline__ float part_t2(float a, float b) {
   uint32_t h = pack_t2<T>(a, b);
-  if (TWICE && lo) {
+  if constexpr (REST) {
     const T* v = reinterpret_cast<const T*>(&h);
     h = pack_t2<T>(a - to_f<T>(v[0]), b - to_f<T>(v[1]));
   }
   return __uint_as_float(h);
+}
+
+// The second parts of 32 values to 16 columns of tensor memory (tmem_wait_st() before they are read)
+template <typename T>
+__device__ __forceinline__ void store_second(const uint32_t* x, uint32_t taddr) {
+  float l[HC / 2];
+#pragma unroll
+  for (int e = 0; e < HC / 2; ++e) l[e] = part_t2<T, true>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+  tmem_st16(taddr, l);
 }
 
 struct BwdConst {
@@ -71,10 +85,11 @@ struct BwdConst {
 // scores. neg_lse: -lse2 by column (PER_COL, from shared memory) or
 // one value. Columns whose bit in seen is 0 give 0. dist0: row index minus the first column's, for
 // the distance bias. p: plain probabilities where the caller needs them beside f (a capped score of
-// the dQ role).
-template <typename T, int MODE, bool MASKED, bool PER_COL, bool TWICE>
+// the dQ role). With parts, p16's second part goes to the tensor-memory columns at rest.
+template <typename T, int MODE, bool MASKED, bool PER_COL>
 __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, const BwdConst& c, int form,
-                                          const float* neg_lse, float neg_lse_row, float dist0, uint32_t seen, bool lo) {
+                                          const float* neg_lse, float neg_lse_row, float dist0, uint32_t seen, uint32_t rest,
+                                          bool parts) {
   uint64_t y[8], bend[8];
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
@@ -134,7 +149,8 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
       if (MASKED && pa == 0.f) fa = 0.f;
       if (MASKED && pb == 0.f) fb = 0.f;
       if constexpr (PER_COL) {
-        p16[e] = part_t2<T, TWICE>(pa, pb, lo);
+        y[e] = pk2(pa, pb);
+        p16[e] = part_t2<T, false>(pa, pb);
       } else {
         p[k] = pa;
         p[k + 1] = pb;
@@ -143,13 +159,25 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
     x[k] = __float_as_uint(fa);
     x[k + 1] = __float_as_uint(fb);
   }
+  if constexpr ((MODE & 1) != 0 && PER_COL) {
+    if (parts) {
+      float l[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float pa, pb;
+        up2(y[e], pa, pb);
+        l[e] = part_t2<T, true>(pa, pb);
+      }
+      tmem_st8(rest, l);
+    }
+  }
 }
 
-// dS = f (dP dscale - Dvec') as 16-bit pairs; neg_d: -Dvec' by column or one value. The dQ role also
-// gets sum p (dP - Dvec) of its columns.
-template <typename T, int MODE, bool MASKED, bool PER_COL, bool TWICE, int N>
-__device__ __forceinline__ float bwd_ds(const uint32_t* f, const float* p, const uint32_t* dp, float* ds16,
-                                        float dscale, const float* neg_d, float neg_d_row, uint32_t seen, bool lo) {
+// dS = f (dP dscale - Dvec'), in place of f and as 16-bit pairs; neg_d: -Dvec' by column or one value. The dQ
+// role also gets sum p (dP - Dvec) of its columns.
+template <typename T, int MODE, bool MASKED, bool PER_COL, int N>
+__device__ __forceinline__ float bwd_ds(uint32_t* f, const float* p, const uint32_t* dp, float* ds16,
+                                        float dscale, const float* neg_d, float neg_d_row, uint32_t seen) {
   const uint64_t row2 = pk2(neg_d_row, neg_d_row), ds2 = pk2(dscale, dscale);
   uint64_t sum[2] = {0, 0};  // pairs of +0.f
 #pragma unroll
@@ -189,12 +217,13 @@ __device__ __forceinline__ float bwd_ds(const uint32_t* f, const float* p, const
     for (int e = 0; e < 8; ++e) {
       float a, b;
       up2(g[e], a, b);
-      ds16[i / 2 + e] = part_t2<T, TWICE>(a, b, lo);
+      unpair(g[e], f + i + 2 * e);
+      ds16[i / 2 + e] = part_t2<T, false>(a, b);
     }
   }
   float a, b;
   up2(add2(sum[0], sum[1]), a, b);
-  return TWICE && lo ? 0.f : a + b;
+  return a + b;
 }
 
 template <int MODE>
@@ -236,8 +265,9 @@ struct BwdCfg {
 // blocks of every KV head, times a.splits CTAs that share its query heads.
 // fp16, dK / dV: P is kept as 2^8 P (at most 2^8 where P is 1), so that the small probabilities of
 // long rows stay normal numbers; dS and dV take the factor back in fp32.
-// TMEM: S [0, 128), dP, then P and dS [128, 256), acc1 [256, 256 + D), acc2 [384, 384 + D).
-template <typename T, int D, int MODE, bool DKV, bool TWICE>
+// TMEM: S, then the second parts of P and dS [0, 128), dP, then P and dS [128, 256), acc1 [256, 256 + D),
+// acc2 [384, 384 + D).
+template <typename T, int D, int MODE, bool DKV>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
     attn_mod_bwd_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap ty,
                         const __grid_constant__ CUtensorMap tu, const __grid_constant__ CUtensorMap tw,
@@ -325,7 +355,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   }
   if (warp == 16) tmem_alloc(tmem_slot, 512);
   const AttnBlocks tb = DKV ? attn_key_blocks(seq, r0) : attn_tile_blocks(seq, r0);
-  const int ntile = tb.end - tb.first, steps = uniform(ntile * heads * (TWICE ? 2 : 1));
+  const int ntile = tb.end - tb.first, steps = uniform(ntile * heads);
   if (warp == 17 && lane == 0 && steps > 0) {
     const int zx = (DKV ? kvh : h0) * (D / 64);
     mbar_arrive_expect_tx(xy_full, 2 * C::TILE);
@@ -345,8 +375,13 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       if (lane % LPR == 0) sD[warp * 8 + i * RPI + lane / LPR] = dot;
     }
   }
+  int sees = 0;  // rows that row threadIdx.x of the tile sees
+  if (warp < 4 && r0 + (int)threadIdx.x < seq.len) {
+    const int2 range = DKV ? attn_key_range(seq, r0 + threadIdx.x) : attn_row_range(seq, r0 + threadIdx.x);
+    sees = range.y - range.x;
+  }
   tc_fence_before();
-  __syncthreads();
+  const bool parts = uniform(__syncthreads_or(sees > PARTS_ROWS)) == 0;
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
@@ -358,10 +393,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     bool ok = true;
     int un = 0, wn = 0;        // tiles sent for
     uint32_t raw_phase = 0;    // of raw[0 .. UST + WST)
-    auto row_of = [&](int n) { return (tb.first + (DKV ? (n >> TWICE) % ntile : n >> TWICE)) * AM_T; };
+    auto row_of = [&](int n) { return (tb.first + (DKV ? n % ntile : n)) * AM_T; };
     auto send = [&](int n, bool is_w, const DeadRows& d) {
       const int s = is_w ? n % C::WST : n % C::UST;
-      const int z = (DKV ? h0 + (n >> TWICE) / ntile : kvh) * (D / 64);
+      const int z = (DKV ? h0 + n / ntile : kvh) * (D / 64);
       uint64_t* bar = d.any ? &raw[is_w ? C::UST + s : s] : is_w ? &w_full[s] : &u_full[s];
       if (lane == 0) {
         mbar_arrive_expect_tx(bar, C::TILE);
@@ -396,7 +431,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       float l[4], dv[4];
       if constexpr (DKV) {
         const int row = row_of(n);
-        const int64_t at = (int64_t)(h0 + (n >> TWICE) / ntile) * a.n + seq.start + row;
+        const int64_t at = (int64_t)(h0 + n / ntile) * a.n + seq.start + row;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int t = u * 32 + lane;
@@ -464,7 +499,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       if (ok) score(0);
       ok = ok && w_landed(0);
       if (ok) dprob(0);
-      if (steps > 1) {
+      if (steps > 1 && !parts) {
         ok = ok && u_landed(1) && warp_wait(s_free, 0, err);
         if (ok) score(1);
       }
@@ -477,16 +512,25 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         if (!ok) break;
         tc_fence_after();
         umma_gather4(tmem + 256, tmem + 128, DKV ? w0 : u0, id_o, n > 0);
+        if (parts) umma_gather4(tmem + 256, tmem, DKV ? w0 : u0, id_o, 1);
         if (DKV) warp_commit(&w_empty[n % C::WST]);
         if (more) ok = w_landed(n + 1);
         ok = ok && warp_wait(ds_full, n & 1, err);
         if (!ok) break;
         tc_fence_after();
         umma_gather4(tmem + 384, tmem + 128 + HC / 2, u0, id_o, n > 0);
+        if (parts) {
+          umma_gather4(tmem + 384, tmem + HC / 2, u0, id_o, 1);
+          if (more) {
+            ok = u_landed(n + 1);
+            if (!ok) break;
+            score(n + 1);
+          }
+        }
         if (more) dprob(n + 1);
         else warp_commit(out_full);
         warp_commit(&u_empty[n % C::UST]);
-        if (n + 2 < steps) {
+        if (n + 2 < steps && !parts) {
           ok = u_landed(n + 2) && warp_wait(s_free, (n + 1) & 1, err);
           if (ok) score(n + 2);
         }
@@ -514,9 +558,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     bool ok = true;
     const uint32_t ts = lane_base + part * HC;
     for (int n = 0; n < steps; ++n) {
-      const bool lo = TWICE && (n & 1) != 0;
-      const int m = n >> TWICE, s = n & 1, j = tb.first + (DKV ? m % ntile : m), i0 = j * AM_T + part * HC;
-      if (DKV && (MODE & 2) != 0 && m > 0 && m % ntile == 0) c = bwd_const<MODE>(a, h0 + m / ntile);
+      const int s = n & 1, j = tb.first + (DKV ? n % ntile : n), i0 = j * AM_T + part * HC;
+      if (DKV && (MODE & 2) != 0 && n > 0 && n % ntile == 0) c = bwd_const<MODE>(a, h0 + n / ntile);
       const bool masked = j < tb.ffirst || j >= tb.fend;
       const uint32_t seen = masked ? col_mask(range.x - i0, range.y - i0) : 0;
       const float dist0 = (float)(ri - i0);
@@ -536,15 +579,18 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 #pragma unroll
       for (int g = 0; g < HC; g += 16) {
         float* pg = p + ((MODE & 1) != 0 && !DKV ? g : 0);
-        if (masked) bwd_probs<T, MODE, true, DKV, TWICE>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, seen >> g, lo);
-        else bwd_probs<T, MODE, false, DKV, TWICE>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, 0, lo);
+        if (masked) bwd_probs<T, MODE, true, DKV>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, seen >> g, ts + g / 2, parts);
+        else bwd_probs<T, MODE, false, DKV>(x + g, w + g / 2, pg, c, form, nl + g, neg_lse, dist0 - g, 0, ts + g / 2, parts);
+      }
+      if ((MODE & 1) == 0 || !DKV) {  // acc1 takes f itself
+        if (parts) store_second<T>(x, ts);
       }
       ok = warp_wait(dp_full, n & 1, err);
       if (!ok) break;
       tc_fence_after();
       if constexpr ((MODE & 1) != 0 && !DKV) {
         // f and p both live: dP in two halves, or the registers spill (the backward of 8,192 capped
-        // tokens then takes 945 us, not 724)
+        // tokens then took 945 us, not 724; now 765)
         float ds[HC / 2];
 #pragma unroll
         for (int g = 0; g < HC; g += 16) {
@@ -552,10 +598,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
           tmem_ld16(ts + 128 + g, dh);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            w[g / 2 + e] = part_t2<T, TWICE>(__uint_as_float(x[g + 2 * e]), __uint_as_float(x[g + 2 * e + 1]), lo);
+            w[g / 2 + e] = part_t2<T, false>(__uint_as_float(x[g + 2 * e]), __uint_as_float(x[g + 2 * e + 1]));
           const uint32_t* du = reinterpret_cast<const uint32_t*>(dh);
-          if (masked) rest += bwd_ds<T, MODE, true, DKV, TWICE, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, seen >> g, lo);
-          else rest += bwd_ds<T, MODE, false, DKV, TWICE, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, 0, lo);
+          if (masked) rest += bwd_ds<T, MODE, true, DKV, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, seen >> g);
+          else rest += bwd_ds<T, MODE, false, DKV, 16>(x + g, p + g, du, ds + g / 2, P_BACK, nl, neg_d, 0);
         }
         tmem_st16(ts + 128, w);
         tmem_st16(ts + 128 + HC / 2, ds);
@@ -566,21 +612,22 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         uint32_t dp[HC];
         tmem_ld32_nw(ts + 128, dp);
         tmem_wait_ld();
-        if constexpr ((MODE & 1) == 0) {  // acc1 takes f itself
+        if constexpr ((MODE & 1) == 0) {
 #pragma unroll
           for (int e = 0; e < HC / 2; ++e)
-            w[e] = part_t2<T, TWICE>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]), lo);
+            w[e] = part_t2<T, false>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
         }
         tmem_st16(ts + 128, w);
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(p_full);
-        if (masked) rest += bwd_ds<T, MODE, true, DKV, TWICE, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, seen, lo);
-        else rest += bwd_ds<T, MODE, false, DKV, TWICE, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, 0, lo);
+        if (masked) rest += bwd_ds<T, MODE, true, DKV, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, seen);
+        else rest += bwd_ds<T, MODE, false, DKV, HC>(x, p, dp, w, P_BACK, nl + AM_T, neg_d, 0);
         tmem_st16(ts + 128 + HC / 2, w);
-        tmem_wait_st();
-        tc_fence_before();
       }
+      if (parts) store_second<T>(x, ts + HC / 2);
+      tmem_wait_st();
+      tc_fence_before();
       if (DKV) warp_arrive(&l_empty[s]);
       warp_arrive(ds_full);
     }
@@ -698,12 +745,12 @@ int dkv_splits(const AttnModArgs& a) {
   return group;
 }
 
-template <typename T, int D, int MODE, bool TWICE>
+template <typename T, int D, int MODE>
 int launch_bwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mdo,
                const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
   static unsigned long long done_q = 0, done_kv = 0;
-  auto kq = attn_mod_bwd_kernel<T, D, MODE, false, TWICE>;
-  auto kkv = attn_mod_bwd_kernel<T, D, MODE, true, TWICE>;
+  auto kq = attn_mod_bwd_kernel<T, D, MODE, false>;
+  auto kkv = attn_mod_bwd_kernel<T, D, MODE, true>;
   constexpr int smem = BwdCfg<D>::SMEM;
   int st = attn_smem_limit(reinterpret_cast<const void*>(kq), smem, &done_q);
   if (st == QL_STATUS_OK) st = attn_smem_limit(reinterpret_cast<const void*>(kkv), smem, &done_kv);
@@ -719,21 +766,14 @@ int launch_bwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& m
   return launched(a.splits > 1 ? 3 : 2);
 }
 
-template <typename T, int D, int MODE>
-int pick_bwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mdo, const CUtensorMap& mk,
-             const CUtensorMap& mv, cudaStream_t s) {
-  return a.n <= TWICE_TOKENS ? launch_bwd<T, D, MODE, true>(a, mq, mdo, mk, mv, s)
-                                : launch_bwd<T, D, MODE, false>(a, mq, mdo, mk, mv, s);
-}
-
 template <typename T, int D>
 int dispatch_bwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mdo,
                  const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
   switch (attn_mode(a)) {
-    case 0: return pick_bwd<T, D, 0>(a, mq, mdo, mk, mv, s);
-    case 1: return pick_bwd<T, D, 1>(a, mq, mdo, mk, mv, s);
-    case 2: return pick_bwd<T, D, 2>(a, mq, mdo, mk, mv, s);
-    default: return pick_bwd<T, D, 3>(a, mq, mdo, mk, mv, s);
+    case 0: return launch_bwd<T, D, 0>(a, mq, mdo, mk, mv, s);
+    case 1: return launch_bwd<T, D, 1>(a, mq, mdo, mk, mv, s);
+    case 2: return launch_bwd<T, D, 2>(a, mq, mdo, mk, mv, s);
+    default: return launch_bwd<T, D, 3>(a, mq, mdo, mk, mv, s);
   }
 }
 

@@ -795,7 +795,9 @@ def attn_mod_bwd(dout, q, k, v, out, lse, cu_seqlens, max_len, scale, causal=Tru
                  slopes=None, window=0, doc_ids=None, prefix_len=None, dq=None, dk=None, dv=None):
     """(dq, dk, dv) of attn_mod_fwd, in q's dtype, given its arguments, out and lse
     (ql_attn_mod_bwd); dout [n, HQ, D] contiguous; the gradients must not share memory with the
-    inputs. Bit-identical from run to run."""
+    inputs. Bit-identical from run to run. Rows that see (keys that are seen by) at most 256 others, by tiles
+    of 128, get gradients off by their own rounding only; longer sums add one rounding of P and dS. In
+    fp16 a loss scale too large for dS = P (dP - Dvec) gives gradients that are not finite."""
     n, HQ, HKV, D, B, ld, dt, dev, window = _attn_mod_inputs(
         q, k, v, cu_seqlens, max_len, scale, softcap, slopes, window, doc_ids, prefix_len)
     dtype, shape, kv = q.dtype, (n, HQ, D), (n, HKV, D)

@@ -487,8 +487,12 @@ int ql_exp2_fma_eval(const float* x, float* y, int64_t n, cudaStream_t stream);
  * 8; the heads of a row contiguous), D = 64 or 128, 16-byte aligned; out, dout, dq, dk, dv
  * contiguous in dtype; lse fp32 [HQ, n], natural log. scale > 0; softcap 0 or at least 1e-4 scale; slopes
  * of any sign. max_len: at least the longest
- * sequence. The gradients are summed in a fixed order (bit-identical from run to run); fp16
- * gradients of small magnitude need a scaled loss, as everywhere in this library. */
+ * sequence. The gradients are summed in a fixed order (bit-identical from run to run). P and dS, the
+ * operands of their products, are rounded to dtype, in two parts (the rounding and the rounding of
+ * what it left) wherever no row of a 128-row tile sees more than 256 others: there a gradient is off
+ * by its own rounding only, elsewhere by about 1.4 times that. fp16: gradients of small magnitude
+ * need a scaled loss, as everywhere in this library, and a dS = P (dP - Dvec) above 65,504 makes its
+ * gradients not finite (a loss scale that is too large). */
 typedef struct {
   const void* q;
   const void* k;

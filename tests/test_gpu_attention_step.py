@@ -1,6 +1,8 @@
 """The operators of a LoRA attention block with several position axes run together, as a training step
 would: mrope_fwd, attn_mod_fwd, attn_mod_bwd, mrope_bwd, the LoRA gradients, clip_grads."""
 
+import sys
+
 import pytest
 import torch
 
@@ -124,3 +126,43 @@ def test_a_captured_step_follows_its_inputs():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(replayed, eager))
     assert ops.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_a_step_of_longer_rows(dtype, monkeypatch):
+    """The chain where tiles see up to six blocks of keys, so that the backward's products run in one part."""
+    here = sys.modules[__name__]
+    lengths = [750, 1, 290]
+    monkeypatch.setattr(here, "LENGTHS", lengths)
+    monkeypatch.setattr(here, "WINDOW", 600)
+    n = sum(lengths)
+    c = case(n, (HQ, HKV, D), dtype, SECTIONS, seed=31)
+    g = torch.Generator().manual_seed(32)
+    dout = torch.randn(n, HQ, D, generator=g).to(dtype)
+    ids, prefix = (torch.arange(n) >= 740).int(), torch.tensor([200, 1, 0], dtype=torch.int32)
+    ids[700:720] = -1
+    want_out, want = in_64_bits(c, dout, ids, prefix, True)
+    d = {x: t.cuda() for x, t in c.items()}
+    cu = torch.tensor([0] + lengths, dtype=torch.int32).cumsum(0, dtype=torch.int32).cuda()
+    rope = (d["cos"], d["sin"], d["pos"], HQ, HKV, D, SECTIONS)
+    mods = dict(softcap=CAP, window=600, doc_ids=ids.cuda(), prefix_len=prefix.cuda())
+    q, k, v = ops.mrope_fwd(d["qkv"], *rope, interleaved=True, lora_scale=LORA, xq=d["xq"], Bq=d["Bq"],
+                            xv=d["xv"], Bv=d["Bv"])
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, 750, SCALE, **mods)
+    grads = ops.attn_mod_bwd(dout.cuda(), q, k, v, out, lse, cu, 750, SCALE, **mods)
+    dqkv, dxq, dxv = ops.mrope_bwd(*grads, *rope, interleaved=True, dtype=dtype, Bq=d["Bq"], Bv=d["Bv"],
+                                   lora_scale=LORA)
+    dB = ops.lora_grads([(dqkv[:, :HQ * D], d["xq"], LORA, False),
+                         (dqkv[:, (HQ + HKV) * D:], d["xv"], LORA, False)])
+    got = [dqkv, *dB, dxq, dxv]
+    norm = ops.grad_norm(got)
+    assert ops.device_status() == 0
+    # as many roundings as in test_a_step_of_them_together
+    u = torch.finfo(dtype).eps / 2
+    rel = lambda x, y: ((x.double().cpu() - y).norm() / y.norm()).item()  # noqa: E731
+    assert rel(out, want_out) < 5 * u
+    for name, x, y in zip(("qkv", "Bq", "Bv", "xq", "xv"), got, want):
+        assert rel(x, y) < 9 * u, name
+    total = torch.stack([y.norm() for y in want]).norm()
+    assert abs(norm.item() - total.item()) < 9 * u * total.item()

@@ -521,3 +521,73 @@ def test_rows_of_one_key_have_no_gradient_in_q():
     dq, dk, dv = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 300, 0.125, window=1, softcap=20.0)
     assert not dq.any() and torch.equal(out, v.repeat_interleave(2, 1))
     assert rel(dv, dout.double().cpu().unflatten(1, (2, 2)).sum(2)) < 2.0 ** -8
+
+
+def own_rounding(x, y, dtype):
+    """Whether x is as far from y as y's rounding to the type, and a little: the operands' second parts
+    leave 2^-16 (bf16) or 2^-22 of each term, fp16 ones below 2^-14 some 2^-25 of terms near 2^-7."""
+    spare = 2.0 ** -13 if dtype == torch.bfloat16 else 2.0 ** -16
+    return rel(x, y) < 1.02 * rel(y.to(dtype), y) + spare
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [dict(), dict(softcap=30.0), dict(slopes=True, causal=False)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_a_short_sequence_has_the_same_gradients_alone_and_in_a_batch(mode, dtype):
+    lengths, heads, scale = [45, 700, 256, 3, 129], (6, 2, 64), 0.125
+    q, k, v, dout, cu = batch(lengths, heads, dtype, seed=24)
+    host, dev = mode_args(mode, lengths, heads[0])
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, 700, scale, **dev)
+    got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 700, scale, **dev)
+    want = formula(q, k, v, lengths, scale, dout=dout, **host)[2:]
+    assert ops.device_status() == 0
+    at = 0
+    for length in lengths:
+        s = slice(at, at + length)
+        at += length
+        if length > 256:
+            continue
+        one = [t[s].contiguous() for t in (dout, q, k, v, out)] + [lse[:, s].contiguous()]
+        alone = ops.attn_mod_bwd(*one, cu.new_tensor([0, length]), length, scale, **dev)
+        assert torch.equal(alone[0], got[0][s])  # dk and dv: another split of the heads may sum in another order
+        for name, x, y, z in zip(("dq", "dk", "dv"), got, want, alone):
+            assert own_rounding(x[s], y[s], dtype) and own_rounding(z, y[s], dtype), (name, length)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [dict(window=4), dict(window=100, causal=False), dict(ids=True)], ids=str)
+def test_short_reaches_in_long_rows_carry_their_own_rounding_only(mode):
+    """Windows and documents of few keys in 2,100 tokens: as exact as a batch of few tokens."""
+    n, heads, dtype = 2100, (4, 1, 128), torch.bfloat16
+    q, k, v, dout, cu = batch([n], heads, dtype, seed=25)
+    mode = dict(mode)
+    if mode.pop("ids", False):
+        mode["doc_ids"] = torch.arange(n, dtype=torch.int32) // 30
+    dev = {a: b.cuda() if torch.is_tensor(b) else b for a, b in mode.items()}
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, n, 0.1, **dev)
+    got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, n, 0.1, **dev)
+    want = formula(q, k, v, [n], 0.1, dout=dout, **mode)[2:]
+    for name, x, y in zip(("dq", "dk", "dv"), got, want):
+        assert own_rounding(x, y, dtype), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [dict(causal=False), dict(softcap=3.0), dict(slopes=True)], ids=str)
+def test_gradients_of_longer_rows_against_differences(mode):
+    """test_gradients_against_differences where every tile sees more than two blocks of keys."""
+    lengths, heads, dtype = [700, 390], (4, 2, 64), torch.bfloat16
+    q, k, v, dout, cu = batch(lengths, heads, dtype, seed=26)
+    host, dev = mode_args(mode, lengths, 4)
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, 700, 0.125, **dev)
+    grads = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 700, 0.125, **dev)
+    for at in range(3):
+        step = grads[at].double().cpu()
+        size = step.norm()
+        step = step / size * 1e-3
+        sides = []
+        for sign in (1, -1):
+            x = [t.double().cpu() for t in (q, k, v)]
+            x[at] = x[at] + sign * step
+            sides.append((formula(*x, lengths, 0.125, **host)[0] * dout.double().cpu()).sum())
+        slope = (sides[0] - sides[1]) / 2e-3
+        assert abs(slope - size) < TOL[dtype] * size
