@@ -74,7 +74,8 @@ __device__ __forceinline__ void store_second(const uint32_t* x, uint32_t taddr) 
 }
 
 struct BwdConst {
-  float sl2, u, cap2, slope2;
+  float sl2, u, cap2;
+  float slope;  // the distance bias's, in units of raw products, or (capped) of log2
   TanhShort ts;
 };
 
@@ -115,21 +116,27 @@ __device__ __forceinline__ void bwd_probs(uint32_t* x, float* p16, float* p, con
       for (int e = 0; e < 8; ++e)
         th[e] = pk2(tanhf(__uint_as_float(x[2 * e]) * c.u), tanhf(__uint_as_float(x[2 * e + 1]) * c.u));
     }
+    // the distance bias in the order of the forward's roundings, so that its lse fits
+    if constexpr ((MODE & 2) != 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = fma2(th[e], pk2(c.cap2, c.cap2), y[e]);
+      for (int e = 0; e < 8; ++e) {
+        float ta, tb;
+        up2(mul2(th[e], pk2(c.cap2, c.cap2)), ta, tb);
+        y[e] = add2(pk2(fmaf(fabsf(dist0 - (float)(2 * e)), -c.slope, ta), fmaf(fabsf(dist0 - (float)(2 * e + 1)), -c.slope, tb)), y[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = fma2(th[e], pk2(c.cap2, c.cap2), y[e]);
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) bend[e] = fma2(th[e], th[e], pk2(-1.f, -1.f));  // tanh^2 - 1: sign below
   } else {
+    if constexpr ((MODE & 2) != 0) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(fmaf(fabsf(dist0 - (float)k), -c.slope, __uint_as_float(x[k])));
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = fma2(pair_of(x + 2 * e), pk2(c.sl2, c.sl2), y[e]);
-  }
-  if constexpr ((MODE & 2) != 0) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float ya, yb;
-      up2(y[e], ya, yb);
-      y[e] = pk2(ya - c.slope2 * fabsf(dist0 - (float)(2 * e)), yb - c.slope2 * fabsf(dist0 - (float)(2 * e + 1)));
-    }
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -233,7 +240,7 @@ __device__ __forceinline__ BwdConst bwd_const(const AttnModArgs& a, int h) {
   c.u = (MODE & 1) != 0 ? a.scale / a.softcap : 0.f;
   c.cap2 = a.softcap * 1.4426950408889634f;
   if constexpr ((MODE & 1) != 0) c.ts = tanh_short(c.u, 1.f);
-  c.slope2 = (MODE & 2) != 0 ? a.slopes[h] * 1.4426950408889634f : 0.f;
+  c.slope = (MODE & 2) == 0 ? 0.f : (MODE & 1) != 0 ? a.slopes[h] * 1.4426950408889634f : a.slopes[h] / a.scale;
   return c;
 }
 

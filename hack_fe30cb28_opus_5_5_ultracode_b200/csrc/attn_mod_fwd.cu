@@ -51,11 +51,14 @@ struct ScoreConst {
   TanhShort ts;
 };
 
-// Scores of one row and one key block, in place: raw products to log2 units (MODE 0 leaves them
-// raw: the scale rides in the exponent's FMA), masked ones to -inf. x: 64 values; dist0 = i - their first key;
-// side: 1 (-1) if every key of the block comes before (after) every query of the tile, else 0.
+// Scores of one row and one key block, in place: raw products stay in their units unless they are capped (the
+// scale rides in the exponent's FMA), capped ones come in log2 units, masked ones are -inf. x: 64 values;
+// dist0 = i - their first key; slope: the distance bias's, in the same units; side: 1 (-1) if every key of
+// the block comes before (after) every query of the tile, else 0. A bias is one FMA of the score, the slope
+// and an exact distance: sums of biases, from column to column, were off by up to seven roundings of the
+// whole bias, which shows where far keys carry the weight (negative slopes).
 template <int MODE, bool MASKED>
-__device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, float slope2,
+__device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, float slope,
                                               float dist0, float side, int rlo, int rhi) {
   if constexpr ((MODE & 1) != 0) {
     const int form = tanh_form<FWD_HC>(x, c.u);
@@ -87,25 +90,25 @@ __device__ __forceinline__ void modify_scores(uint32_t* x, const ScoreConst& c, 
     }
   }
   if constexpr ((MODE & 2) != 0) {
-    const uint64_t mul = pk2((MODE & 1) != 0 ? 1.f : c.sl2, (MODE & 1) != 0 ? 1.f : c.sl2);
+    const uint64_t by = pk2(-slope, -slope);
     if (side != 0.f) {  // every key on one side of every query: |i - j| = side (dist0 - column)
-      // four pairs of biases, moved on by eight columns at a time
-      const float slope = side * slope2, base = -slope * dist0;
-      const uint64_t next = pk2(8.f * slope, 8.f * slope);
-      uint64_t bias[4];
+      // four pairs of distances, moved on by eight columns at a time
+      const float first = side * dist0;
+      const uint64_t next = pk2(-8.f * side, -8.f * side);
+      uint64_t away[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bias[e] = pk2(fmaf((float)(2 * e), slope, base), fmaf((float)(2 * e + 1), slope, base));
+      for (int e = 0; e < 4; ++e) away[e] = pk2(first - side * (float)(2 * e), first - side * (float)(2 * e + 1));
 #pragma unroll
       for (int i = 0; i < FWD_HC; i += 8)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          unpair(fma2(pair_of(x + i + 2 * e), mul, bias[e]), x + i + 2 * e);
-          bias[e] = add2(bias[e], next);
+          unpair(fma2(away[e], by, pair_of(x + i + 2 * e)), x + i + 2 * e);
+          away[e] = add2(away[e], next);
         }
     } else {
 #pragma unroll
-      for (int i = 0; i < FWD_HC; i += 2)
-        unpair(fma2(pair_of(x + i), mul, pk2(-slope2 * fabsf(dist0 - (float)i), -slope2 * fabsf(dist0 - (float)(i + 1)))), x + i);
+      for (int i = 0; i < FWD_HC; ++i)
+        x[i] = __float_as_uint(fmaf(fabsf(dist0 - (float)i), -slope, __uint_as_float(x[i])));
     }
   }
   if constexpr (MASKED) {
@@ -316,8 +319,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     c.u = (MODE & 1) != 0 ? a.scale / a.softcap : 0.f;
     c.cap2 = a.softcap * 1.4426950408889634f;
     if constexpr ((MODE & 1) != 0) c.ts = tanh_short(c.u, c.cap2);
-    const float slope2 = (MODE & 2) != 0 ? a.slopes[h] * 1.4426950408889634f : 0.f;
-    const float mul = MODE == 0 ? c.sl2 : 1.f;
+    const float slope = (MODE & 2) == 0 ? 0.f : (MODE & 1) != 0 ? a.slopes[h] * 1.4426950408889634f : a.slopes[h] / a.scale;
+    const float mul = (MODE & 1) == 0 ? c.sl2 : 1.f;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
     constexpr int STEP = SPLIT ? 2 : 1;
@@ -341,8 +344,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
       const bool masked = j < tb.ffirst || j >= tb.fend;
       const int j0 = j * AM_T + half * FWD_HC, qt = q0 / AM_T + (SPLIT ? 0 : t);
       const float side = j < qt ? 1.f : j > qt ? -1.f : 0.f;
-      if (masked) modify_scores<MODE, true>(x, c, slope2, (float)(qi - j0), side, range.x - j0, range.y - j0);
-      else modify_scores<MODE, false>(x, c, slope2, (float)(qi - j0), side, 0, 0);
+      if (masked) modify_scores<MODE, true>(x, c, slope, (float)(qi - j0), side, range.x - j0, range.y - j0);
+      else modify_scores<MODE, false>(x, c, slope, (float)(qi - j0), side, 0, 0);
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int i = 0; i < FWD_HC; i += 8)
@@ -607,6 +610,7 @@ int attn_mod_check(const ql_attn_mod_args& m, AttnModArgs& a) {
   if ((int64_t)m.HQ * m.B > 0x7fffffff || cdiv(m.max_len, AM_T) > 65535) return QL_STATUS_UNSUPPORTED;
   if (!(m.scale > 0.f && m.scale < INFINITY) || !(m.softcap >= 0.f && m.softcap < INFINITY))
     return QL_STATUS_BAD_ARG;
+  if (m.slopes != nullptr && m.scale < 1e-30f) return QL_STATUS_BAD_ARG;  // slope / scale has to stay finite
   // tanh_short's coefficients hold (scale / softcap)^7: finite up to 10^4, a cap that bends every score
   if (m.softcap > 0.f && m.softcap < 1e-4f * m.scale) return QL_STATUS_BAD_ARG;
   if (m.n > 0 && m.B > 0 && (m.q == nullptr || m.k == nullptr || m.v == nullptr || m.out == nullptr ||

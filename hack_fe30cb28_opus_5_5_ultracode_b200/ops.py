@@ -755,6 +755,8 @@ def _attn_mod_inputs(q, k, v, cu_seqlens, max_len, scale, softcap, slopes, windo
     if not (0 <= max_len <= n and window >= 0 and 0 < scale < _INF and 0 <= softcap < _INF):
         raise ValueError("needs 0 <= max_len <= tokens, window >= 0, 0 < scale < inf and "
                          "0 <= softcap < inf")
+    if slopes is not None and scale < 1e-30:
+        raise ValueError("slopes with a scale below 1e-30 are not supported")
     if 0 < softcap < 1e-4 * scale:
         raise ValueError("a softcap below 1e-4 scale is not supported")
     return n, HQ, HKV, D, B, strides, _DT[dt], dev, min(window, INT_MAX)

@@ -591,3 +591,48 @@ def test_gradients_of_longer_rows_against_differences(mode):
             sides.append((formula(*x, lengths, 0.125, **host)[0] * dout.double().cpu()).sum())
         slope = (sides[0] - sides[1]) / 2e-3
         assert abs(slope - size) < TOL[dtype] * size
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("slope", [-0.4375, -0.8125, -0.7071])
+def test_distance_biases_of_thousands(slope):
+    """Keys 16,000 tokens away carry the weight (negative slopes, a window), q = 0: row after row the same scores,
+    -slope |i - j|, at other places of their blocks. A bias is off by one rounding of its own size,
+    and not at all where slope / scale x distance has few bits, so that the rows' lse differ by the
+    last step of their logarithm and sum at most."""
+    n, window, heads, dtype = 16700, 16000, (2, 1, 64), torch.float16
+    q, k, v, dout, cu = batch([n], heads, dtype, seed=27)
+    q.zero_()
+    dout.fill_(1.0)
+    mods = dict(window=window, slopes=torch.tensor([slope, slope / 2]).cuda())
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, n, 0.125, **mods)
+    dq, dk, dv = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, n, 0.125, **mods)
+    assert ops.device_status() == 0
+    away, few = torch.arange(window, dtype=torch.float64), 200  # the rest weighs less than 1e-18
+    vv, most = v[:, 0].double().cpu(), 0.0
+    for h, s in enumerate(mods["slopes"].double().tolist()):
+        want = torch.logsumexp(-s * away, 0).item()
+        most = max(most, want)
+        row = lse[h, window:].double().cpu()
+        # roundings of scale log2(e), slope / scale, a bias, the row's maximum and of the two steps to
+        # the natural logarithm, each 2^-24 of a number no larger than lse
+        assert ((row - want).abs() <= 6 * 2.0 ** -24 * want).all()
+        if slope != -0.7071:
+            assert (row.max() - row.min()).item() <= 2 * 2.0 ** -23 * want
+        p = torch.exp(-s * away[-few:] - want).flip(0)  # of keys i - window + 1, ...
+        exact = (vv.unfold(0, few, 1)[1:1 + n - window] * p).sum(-1)
+        # the biases' roundings once more, P's and the result's, each of at most sum p |v|
+        bound = (3 * 2.0 ** -24 * want + 3 * 2.0 ** -11) * vv.abs().max()
+        assert ((out[window:, h].double().cpu() - exact).abs() <= bound).all()
+    # with dout = 1 a key's dv is the sum of its probabilities, 1 a head where every row that gives it weight
+    # sees a whole window; the forward's lse roundings, as many of the backward's, P's and dv's
+    whole = dv[150:600].double().cpu()
+    assert ((whole - 2).abs() <= 2 * (2 * 2.0 ** -11 + 12 * 2.0 ** -24 * most)).all()
+    assert torch.isfinite(dq).all() and torch.isfinite(dk).all()
+
+
+def test_slopes_over_a_scale_of_nothing_are_refused():
+    for entry in ("ql_attn_mod_fwd", "ql_attn_mod_bwd"):
+        with pytest.raises(_lib.QLError) as e:
+            _lib.call(entry, ops.ctypes_ref(fake_args(slopes=12 << 12, scale=1e-31)), None)
+        assert e.value.status == ops.STATUS_BAD_ARG
