@@ -236,3 +236,33 @@ def test_a_tensor_beyond_32_bit_offsets():
     want = torch.tensor([4.0, 3.0]) * (50.0 / (25000 ** 0.5 + 1e-6))
     assert torch.equal(torch.stack([g[0], g[-1]]).cpu(), want.to(BF16))
     assert g[1000:-1000].abs().max().item() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtypes", [[F32], [BF16], [F32, BF16, F16]], ids=str)
+@pytest.mark.parametrize("size", [1e-30, 1e-22, 1e-15, 1e18, 1e25, 1e33])
+def test_squares_outside_the_range_of_fp32(size, dtypes):
+    """Gradients whose squares overflow or vanish in fp32: the norm and the clipped values stay right (the
+    factor is off by a rounding of the norm, of the ratio and of the product: 2^-22)."""
+    sizes = [1, 7, 2048, 4099, 40000, 8]
+    grads = grads_of(sizes, [F32], seed=5)
+    grads = [(g * (1.0 if dtypes[i % len(dtypes)] == F16 else size)).to(dtypes[i % len(dtypes)])
+             for i, g in enumerate(grads)]
+    grads.append(torch.zeros(5000, device="cuda"))
+    views = [*grads, torch.cat([grads[4].float(), grads[4].float()])[3:40003]]  # one that is not aligned
+    norm, factor = expected(views, size * 0.01)
+    assert abs(ops.grad_norm(views).item() - norm) <= 1e-6 * norm
+    outs = [torch.empty_like(g, dtype=F32) for g in views]
+    assert abs(ops.clip_grads(views, size * 0.01, out=outs).item() - norm) <= 1e-6 * norm
+    if 1e-20 < size < 1e20:  # else 1e-6 or a subnormal ratio decides
+        for o, g in zip(outs, views):
+            want = g.double() * factor
+            assert ((o.double() - want).abs() <= 2.0 ** -21 * want.abs() + torch.finfo(F32).tiny).all()
+    assert all(torch.isfinite(o).all() for o in outs)
+
+
+@pytest.mark.gpu
+def test_a_norm_beyond_fp32_is_infinite():
+    g = torch.full((100,), 3e38, device="cuda")
+    assert ops.grad_norm([g]).item() == math.inf
+    assert ops.grad_norm([g], 0.01).item() == pytest.approx(3e37, rel=1e-6)
