@@ -538,8 +538,9 @@ def clip_grads(grads, max_norm, inv_scale=1.0, out=None):
     """Rescales the gradients by inv_scale * min(1, max_norm / (norm + 1e-6)), in place or into the
     tensors of `out` (as many elements each, any of the three dtypes, e.g. fp32 master gradients), and returns
     the norm before clipping as a device scalar (ql_clip_grads): torch.nn.utils.clip_grad_norm_ with
-    the unscaling folded in, in two kernels and with no host read. A norm that is not finite makes
-    every gradient not finite, as there."""
+    the unscaling folded in, in two kernels and with no host read. As there, a NaN makes the norm and
+    every gradient NaN, and an infinite norm makes finite gradients 0 and infinite ones NaN: look at
+    the norm, not at the gradients, for an overflow."""
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative")
     return _clip_call(grads, inv_scale, float(max_norm), out)

@@ -329,8 +329,10 @@ int ql_lora_colsum_noalloc(const void* X, int64_t ldx, int x_dtype, const void* 
  * sqrt(sum of squares of every gradient); ql_clip_grads also writes
  *   out = grad * inv_scale * min(1, max_norm / (norm + 1e-6))
  * rounded once (out == grad: in place; nothing is written when that factor is 1). inv_scale undoes a
- * loss scale; inv_scale_dev (a device float, or NULL) takes its place when given. A norm that is not
- * finite makes the outputs not finite, as in torch. The lists are host memory, read during the
+ * loss scale; inv_scale_dev (a device float, or NULL) takes its place when given. As in torch, a NaN
+ * among the gradients makes the norm and every output NaN; an infinite one, or a norm beyond fp32,
+ * makes the norm infinite and the factor 0: finite gradients become 0 and infinite ones NaN, so it is
+ * the norm that tells. The lists are host memory, read during the
  * call: addresses, elements and dtypes (QL_F16, QL_BF16, QL_F32) of `count` gradients and, for
  * ql_clip_grads, of their outputs. dtypes may differ from tensor to tensor; tensors need only their
  * own type's alignment (16 bytes is fastest) and must not overlap, but for an output that is its own

@@ -266,3 +266,21 @@ def test_a_norm_beyond_fp32_is_infinite():
     g = torch.full((100,), 3e38, device="cuda")
     assert ops.grad_norm([g]).item() == math.inf
     assert ops.grad_norm([g], 0.01).item() == pytest.approx(3e37, rel=1e-6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("place", [False, True])
+def test_what_an_infinite_norm_and_a_nan_do(place):
+    """An infinite norm: finite gradients become 0, infinite ones NaN. A NaN: all become NaN."""
+    for bad in (math.inf, -math.inf, math.nan):
+        grads = grads_of([1000, 3, 50], [F32, BF16], seed=6)
+        grads[1][2] = bad
+        outs = None if place else [torch.full_like(g, 7.0, dtype=F32) for g in grads]
+        norm = ops.clip_grads(grads, 1.0, out=outs)
+        got = grads if place else outs
+        if math.isnan(bad):
+            assert math.isnan(norm.item()) and all(torch.isnan(o).all() for o in got)
+            continue
+        assert norm.item() == math.inf and math.isnan(got[1][2].item())
+        got[1][2] = 0.0
+        assert not any(o.any() for o in got)
