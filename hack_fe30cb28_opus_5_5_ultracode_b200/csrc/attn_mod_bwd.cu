@@ -812,8 +812,25 @@ int attn_mod_bwd(const ql_attn_mod_args& m, cudaStream_t s) {
         reinterpret_cast<uintptr_t>(m.workspace)) & 15))
     return QL_STATUS_BAD_ARG;
   a.splits = dkv_splits(a);
-  if (m.workspace == nullptr ||
-      m.workspace_floats < attn_mod_bwd_workspace(a.n, a.max_len, a.HQ, a.HKV, m.D, a.causal, a.window))
+  const int64_t floats = attn_mod_bwd_workspace(a.n, a.max_len, a.HQ, a.HKV, m.D, a.causal, a.window);
+  if (m.workspace == nullptr || m.workspace_floats < floats) return QL_STATUS_BAD_ARG;
+  // the second launch reads the inputs when the first has written dq
+  const int64_t rows = m.n, row = (int64_t)m.HQ * m.D, kv_row = (int64_t)m.HKV * m.D;
+  if (outputs_overlap({{m.dq, rows * row * 2},
+                       {m.dk, rows * kv_row * 2},
+                       {m.dv, rows * kv_row * 2},
+                       {m.workspace, floats * 4},
+                       {m.doc_ids != nullptr ? m.ranges : nullptr, rows * 8}},
+                      {{m.q, ((rows - 1) * m.ldq + row) * 2},
+                       {m.k, ((rows - 1) * m.ldk + kv_row) * 2},
+                       {m.v, ((rows - 1) * m.ldv + kv_row) * 2},
+                       {m.out, rows * row * 2},
+                       {m.dout, rows * row * 2},
+                       {m.lse, rows * m.HQ * 4},
+                       {m.cu_seqlens, ((int64_t)m.B + 1) * 4},
+                       {m.slopes, (int64_t)m.HQ * 4},
+                       {m.prefix_len, (int64_t)m.B * 4},
+                       {m.doc_ids, rows * 4}}))
     return QL_STATUS_BAD_ARG;
   a.dout = m.dout;
   a.dq = m.dq;

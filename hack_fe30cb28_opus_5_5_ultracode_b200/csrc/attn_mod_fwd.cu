@@ -652,6 +652,18 @@ int attn_mod_fwd(const ql_attn_mod_args& m, cudaStream_t s) {
   int st = attn_mod_check(m, a);
   if (st != QL_STATUS_OK) return st;
   if (m.n == 0 || m.B == 0 || m.max_len == 0) return QL_STATUS_OK;
+  // out may take q's place: a CTA writes the rows and the head whose q it alone has read
+  const int64_t rows = m.n, row = (int64_t)m.HQ * m.D;
+  const bool in_place = m.out == m.q && m.ldq == row;
+  if (outputs_overlap({{m.out, rows * row * 2}, {m.lse, rows * m.HQ * 4}, {m.doc_ids != nullptr ? m.ranges : nullptr, rows * 8}},
+                      {{in_place ? nullptr : m.q, ((rows - 1) * m.ldq + row) * 2},
+                       {m.k, ((rows - 1) * m.ldk + (int64_t)m.HKV * m.D) * 2},
+                       {m.v, ((rows - 1) * m.ldv + (int64_t)m.HKV * m.D) * 2},
+                       {m.cu_seqlens, ((int64_t)m.B + 1) * 4},
+                       {m.slopes, (int64_t)m.HQ * 4},
+                       {m.prefix_len, (int64_t)m.B * 4},
+                       {m.doc_ids, rows * 4}}))
+    return QL_STATUS_BAD_ARG;
   ProfScope prof(PK_ATTN_FWD, 0, 0, s);
   if (m.doc_ids != nullptr) {
     st = attn_doc_ranges(m.doc_ids, m.cu_seqlens, m.B, m.n, reinterpret_cast<int2*>(m.ranges), s);

@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../include/qlora_sm100.h"
 
 namespace ql {
@@ -123,6 +125,24 @@ int profile_read(double* count, double* ms, double* flops, double* bytes);
 }  // namespace ql
 
 namespace ql {
+// Memory a call reads or writes, for the entries that refuse outputs sharing it.
+struct MemSpan {
+  uint64_t first, end;  // bytes; empty: no such argument
+  MemSpan(const void* p, int64_t bytes)
+      : first(reinterpret_cast<uint64_t>(p)), end(p != nullptr && bytes > 0 ? first + (uint64_t)bytes : first) {}
+  bool meets(const MemSpan& o) const { return first < o.end && o.first < end; }
+};
+// Whether anything written shares memory with what is read or with something else written.
+inline bool outputs_overlap(std::initializer_list<MemSpan> written, std::initializer_list<MemSpan> read) {
+  for (const MemSpan* w = written.begin(); w != written.end(); ++w) {
+    for (const MemSpan& r : read)
+      if (w->meets(r)) return true;
+    for (const MemSpan* o = written.begin(); o != w; ++o)
+      if (w->meets(*o)) return true;
+  }
+  return false;
+}
+
 int mrope_fwd(const ql_mrope_args& m, cudaStream_t s);
 int mrope_bwd(const ql_mrope_args& m, cudaStream_t s);
 int64_t grad_norm_workspace(int count);

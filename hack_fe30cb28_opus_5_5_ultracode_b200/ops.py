@@ -96,7 +96,11 @@ class _on_device:
 def _launch(name, dev, args):
     """Calls an entry point that takes one packed argument struct, on device dev's current stream."""
     with _on_device(dev):
-        call(name, args, stream_ptr())
+        status = getattr(_lib.lib(), name)(args, stream_ptr())
+    if status == STATUS_BAD_ARG:  # what is not checked before the call
+        raise ValueError("outputs that share memory with an input or one another, or that do not "
+                         "start at a multiple of 16 bytes")
+    _lib.check(name, status)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -774,7 +778,9 @@ def attn_mod_fwd(q, k, v, cu_seqlens, max_len, scale, causal=True, softcap=0.0, 
     without it prefix_len changes nothing), |i - j| < window
     (window > 0), and both are in the same run of equal doc_ids (negative ids: padding). slopes
     fp32 [HQ], doc_ids int32 [n], prefix_len int32 [B]. out as q (contiguous), lse fp32 [HQ, n];
-    a query that sees nothing gets out 0 and lse -inf. Rows behind the last sequence are not written."""
+    a query that sees nothing gets out 0 and lse -inf. Rows behind the last sequence are not written. out
+    may be a contiguous q itself; otherwise outputs that share memory with an input or one another are
+    refused."""
     n, HQ, HKV, D, B, ld, dt, dev, window = _attn_mod_inputs(
         q, k, v, cu_seqlens, max_len, scale, softcap, slopes, window, doc_ids, prefix_len)
     if out is None:
@@ -797,8 +803,8 @@ def attn_mod_fwd(q, k, v, cu_seqlens, max_len, scale, causal=True, softcap=0.0, 
 def attn_mod_bwd(dout, q, k, v, out, lse, cu_seqlens, max_len, scale, causal=True, softcap=0.0,
                  slopes=None, window=0, doc_ids=None, prefix_len=None, dq=None, dk=None, dv=None):
     """(dq, dk, dv) of attn_mod_fwd, in q's dtype, given its arguments, out and lse
-    (ql_attn_mod_bwd); dout [n, HQ, D] contiguous; the gradients must not share memory with the
-    inputs. Bit-identical from run to run. Rows that see (keys that are seen by) at most 256 others, by tiles
+    (ql_attn_mod_bwd); dout [n, HQ, D] contiguous; gradients that share memory with an input or one
+    another are refused. Bit-identical from run to run. Rows that see (keys that are seen by) at most 256 others, by tiles
     of 128, get gradients off by their own rounding only; longer sums add one rounding of P and dS. In
     fp16 a loss scale too large for dS = P (dP - Dvec) gives gradients that are not finite."""
     n, HQ, HKV, D, B, ld, dt, dev, window = _attn_mod_inputs(

@@ -484,7 +484,9 @@ int ql_exp2_fma_eval(const float* x, float* y, int64_t n, cudaStream_t stream);
  *   documents:   i and j are in the same run of equal doc_ids (a document ends where the id
  *                changes; a negative id is padding, which sees nothing and is seen by nothing).
  * A query that sees no key gets out = 0, lse = -inf and zero gradients. Rows of q, k, v past the
- * last sequence are not read into any result, and rows of the outputs there are left alone.
+ * last sequence are not read into any result, and rows of the outputs there are left alone. What is
+ * written must not share memory with what is read or with one another (QL_STATUS_BAD_ARG), but for a
+ * forward whose out is q itself, contiguous.
  * q [n, HQ, D], k / v [n, HKV, D] of dtype with row strides ldq / ldk / ldv (elements, multiples of
  * 8; the heads of a row contiguous), D = 64 or 128, 16-byte aligned; out, dout, dq, dk, dv
  * contiguous in dtype; lse fp32 [HQ, n], natural log. scale > 0 (with

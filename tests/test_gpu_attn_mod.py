@@ -633,6 +633,53 @@ def test_distance_biases_of_thousands(slope):
 
 def test_slopes_over_a_scale_of_nothing_are_refused():
     for entry in ("ql_attn_mod_fwd", "ql_attn_mod_bwd"):
+        args = fake_args(slopes=12 << 12, scale=1e-31)
         with pytest.raises(_lib.QLError) as e:
-            _lib.call(entry, ops.ctypes_ref(fake_args(slopes=12 << 12, scale=1e-31)), None)
+            _lib.call(entry, ops.ctypes_ref(args), None)
         assert e.value.status == ops.STATUS_BAD_ARG
+
+
+APART = {f: (i + 1) << 20 for i, f in enumerate(("q", "k", "v", "out", "lse", "cu_seqlens", "dout", "dq",
+                                                 "dk", "dv", "workspace", "slopes", "prefix_len",
+                                                 "doc_ids", "ranges"))}
+
+
+@pytest.mark.parametrize("entry,change", [
+    *(("ql_attn_mod_fwd", c) for c in (
+        dict(out="q", ldq=264), dict(out="k"), dict(out="v"), dict(lse="q"), dict(out="lse"), dict(lse="cu_seqlens"),
+        dict(out=APART["k"] - 16), dict(out=APART["q"] + 9 * 512 + 496), dict(ranges="v"),
+        dict(ranges="doc_ids"))),
+    *(("ql_attn_mod_bwd", c) for c in (
+        dict(dq="dout"), dict(dk="dout"), dict(dv="out"), dict(dq="q"), dict(dk="k"), dict(dk="v"),
+        dict(dq="dk"), dict(dk="dv"), dict(dv="lse"), dict(workspace="dout"), dict(workspace="dq"),
+        dict(ranges="workspace"), dict(dk=APART["dq"] + 10 * 256 * 2 - 16)))], ids=str)
+def test_outputs_that_share_memory_are_refused(entry, change):
+    f = {**APART, **{x: APART.get(y, y) for x, y in change.items()}}
+    args = fake_args(**f)
+    with pytest.raises(_lib.QLError) as e:
+        _lib.call(entry, ops.ctypes_ref(args), None)
+    assert e.value.status == ops.STATUS_BAD_ARG
+
+
+@pytest.mark.gpu
+def test_shared_memory_is_refused_with_a_reason():
+    q, k, v, dout, cu = batch([40, 9], (2, 2, 64), torch.float16, seed=28)
+    out, lse = ops.attn_mod_fwd(q, k, v, cu, 40, 0.125)
+    place = q.clone()  # out in q's place is no harm
+    got = ops.attn_mod_fwd(place, k, v, cu, 40, 0.125, out=place)
+    assert got[0] is place and torch.equal(place, out) and torch.equal(got[1], lse)
+    wide = torch.empty(49, 3, 64, device="cuda", dtype=q.dtype)
+    for kw in (dict(out=k), dict(out=v), dict(out=wide.view(-1)[:q.numel()].view_as(q))):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.attn_mod_fwd(wide[:, :2], k, v, cu, 40, 0.125, **kw)
+    for kw in (dict(dq=dout), dict(dk=k), dict(dv=out), dict(dq=q, dk=q)):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 40, 0.125, **kw)
+    # neighbours in one buffer do not share
+    want = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 40, 0.125)
+    room = torch.empty(3, *q.shape, device="cuda", dtype=q.dtype)
+    got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 40, 0.125, dq=room[0], dk=room[1], dv=room[2])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # nor do tensors without elements
+    empty = q[:0]
+    ops.attn_mod_fwd(empty, empty, empty, cu[:1], 0, 0.125, out=empty)
