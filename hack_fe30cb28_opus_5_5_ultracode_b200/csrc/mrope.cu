@@ -443,6 +443,10 @@ int mrope_check(const ql_mrope_args& m, MropeArgs& a) {
   return QL_STATUS_OK;
 }
 
+// What both directions read: the tables and positions (by the call's own sizes).
+MemSpan table_span(const ql_mrope_args& m, const float* t) { return {t, (int64_t)m.positions * (m.D / 2) * 4}; }
+MemSpan pos_span(const ql_mrope_args& m) { return {m.pos, ((m.axes - 1) * m.ld_pos + m.n) * 4}; }
+
 bool misaligned(std::initializer_list<const void*> ps, uintptr_t to) {
   uintptr_t bits = 0;
   for (const void* p : ps) bits |= reinterpret_cast<uintptr_t>(p);
@@ -459,6 +463,17 @@ int mrope_fwd(const ql_mrope_args& m, cudaStream_t s) {
   if (m.qkv == nullptr || m.q == nullptr || m.k == nullptr || m.v == nullptr ||
       (m.xq != nullptr && m.Bq == nullptr) || (m.xv != nullptr && m.Bv == nullptr) ||
       misaligned({m.qkv, m.q, m.k, m.v}, 16) || misaligned({m.xq, m.xv, m.Bq, m.Bv}, 8))
+    return QL_STATUS_BAD_ARG;
+  const int64_t qb = (int64_t)m.HQ * m.D * 2, kvb = (int64_t)m.HKV * m.D * 2;  // bytes of a token's heads
+  if (outputs_overlap({{m.q, m.n * qb}, {m.k, m.n * kvb}, {m.v, m.n * kvb}},
+                      {{m.qkv, m.n * (qb + 2 * kvb)},
+                       {m.xq, (int64_t)m.n * MR_RANK * 2},
+                       {m.xv, (int64_t)m.n * MR_RANK * 2},
+                       {m.xq != nullptr ? m.Bq : nullptr, qb * MR_RANK},
+                       {m.xv != nullptr ? m.Bv : nullptr, kvb * MR_RANK},
+                       table_span(m, m.cos),
+                       table_span(m, m.sin),
+                       pos_span(m)}))
     return QL_STATUS_BAD_ARG;
   a.qkv = m.qkv;
   a.xq = m.xq;
@@ -490,6 +505,19 @@ int mrope_bwd(const ql_mrope_args& m, cudaStream_t s) {
   if (m.dq == nullptr || m.dk == nullptr || m.dv == nullptr || m.dqkv == nullptr ||
       (m.dxlo_q != nullptr && m.Bq == nullptr) || (m.dxlo_v != nullptr && m.Bv == nullptr) ||
       misaligned({m.dq, m.dk, m.dv, m.dqkv}, 16) || misaligned({m.Bq, m.Bv}, 8))
+    return QL_STATUS_BAD_ARG;
+  const int64_t qc = (int64_t)m.HQ * m.D, kvc = (int64_t)m.HKV * m.D, size = m.grad_dtype == QL_F32 ? 4 : 2;
+  if (outputs_overlap({{m.dqkv, m.n * (qc + 2 * kvc) * 2},
+                       {m.dxlo_q, (int64_t)m.n * MR_RANK * 4},
+                       {m.dxlo_v, (int64_t)m.n * MR_RANK * 4}},
+                      {{m.dq, m.n * qc * size},
+                       {m.dk, m.n * kvc * size},
+                       {m.dv, m.n * kvc * size},
+                       {m.dxlo_q != nullptr ? m.Bq : nullptr, qc * MR_RANK * 2},
+                       {m.dxlo_v != nullptr ? m.Bv : nullptr, kvc * MR_RANK * 2},
+                       table_span(m, m.cos),
+                       table_span(m, m.sin),
+                       pos_span(m)}))
     return QL_STATUS_BAD_ARG;
   a.dq = m.dq;
   a.dk = m.dk;

@@ -412,7 +412,8 @@ def mrope_fwd(qkv, cos, sin, pos, HQ, HKV, D, sections, interleaved=False, lora_
     sections = how many of the D / 2 frequencies each axis has, in blocks or (interleaved) dealt
     to the axes in turn while an axis has some left; cos / sin the rotary table of one axis.
     xq / Bq, xv / Bv: the LoRA-B products q += lora_scale xq Bq^T, added in fp32. A position outside the
-    table turns nothing (its frequencies give 0) and is recorded for device_status()."""
+    table turns nothing (its frequencies give 0) and is recorded for device_status(). out: (q, k, v) to
+    write; they must not share memory with an input or one another."""
     dev = _index_of(qkv, cos, sin, pos, xq, xv, Bq, Bv)
     if qkv.dim() != 2:
         raise ValueError("qkv must be [tokens, (HQ + 2 HKV) D]")
@@ -443,7 +444,7 @@ def mrope_bwd(dq, dk, dv, cos, sin, pos, HQ, HKV, D, sections, interleaved=False
               dtype=torch.float16, Bq=None, Bv=None, lora_scale=1.0, out=None):
     """(dqkv, dxlo_q, dxlo_v) of mrope_fwd (ql_mrope_bwd): the pre-rotary qkv gradient in `dtype`
     from dq [n, HQ, D], dk / dv [n, HKV, D] (dtype or fp32), and with Bq / Bv the LoRA-A output
-    gradients lora_scale * (g . B), fp32 [n, 16]."""
+    gradients lora_scale * (g . B), fp32 [n, 16]. out: dqkv to write; it must not share memory with an input."""
     dev = _index_of(dq, dk, dv, cos, sin, pos, Bq, Bv)
     if dq.dim() != 3:
         raise ValueError("dq must be [tokens, HQ, D]")

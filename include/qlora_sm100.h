@@ -237,7 +237,8 @@ int ql_rope_bwd(const ql_rope_bwd_args* args, cudaStream_t stream);
  * its table entry at row pos[axis][token]. sec0 .. sec3: how many frequencies each axis has (their
  * sum is D / 2), in blocks, or with `interleaved` dealt to the axes in turn while an axis has some
  * left. D a multiple of 64, at most 256; rank 16; all tensors contiguous and 16-byte aligned
- * (x*, B*: 8-byte). The LoRA-B product is added in fp32 without a rounding of its own, and dxlo is
+ * (x*, B*: 8-byte), outputs sharing no memory with inputs or one another (QL_STATUS_BAD_ARG). The
+ * LoRA-B product is added in fp32 without a rounding of its own, and dxlo is
  * lora_scale * (g . B) of the unrounded gradient g, in fp32. A position outside [0, positions)
  * records QL_STATUS_BAD_ARG in the device status word, where it stays until it is read with clear
  * (or a timeout is recorded over it); its frequencies give 0. Other calls are not affected. */

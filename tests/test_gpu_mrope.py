@@ -311,3 +311,35 @@ def test_dx_lo_of_small_and_large_gradients(size, dtype, n):
     for a, g, B in zip(got, (gq, gv), (c["Bq"].double(), c["Bv"].double())):
         assert ((a.double().cpu() - g @ B).abs() <= 50 * 2.0 ** -23 * (g.abs() @ B.abs())).all()
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("entry,change", [
+    *(("ql_mrope_fwd", c) for c in (dict(q="qkv"), dict(k="qkv"), dict(v="q"), dict(k="v"), dict(q="xq"),
+                                    dict(v="Bv"), dict(k="pos"), dict(q=(1 << 20) + 5 * 512 * 2 - 16))),
+    *(("ql_mrope_bwd", c) for c in (dict(dqkv="dq"), dict(dqkv="dk"), dict(dqkv="dv"), dict(dxlo_q="dqkv"),
+                                    dict(dxlo_v="Bq"), dict(dxlo_q="dxlo_v"), dict(dxlo_v="dv")))],
+    ids=str)
+def test_outputs_that_share_memory_are_refused(entry, change):
+    names = "qkv q k v dq dk dv dqkv cos sin pos xq xv Bq Bv dxlo_q dxlo_v".split()
+    apart = {x: (i + 1) << 20 for i, x in enumerate(names)}
+    f = {**apart, **{x: apart.get(y, y) for x, y in change.items()}}
+    args = fake_args(**f)
+    with pytest.raises(_lib.QLError) as e:
+        _lib.call(entry, ops.ctypes_ref(args), None)
+    assert e.value.status == ops.STATUS_BAD_ARG
+
+
+@pytest.mark.gpu
+def test_shared_memory_is_refused_with_a_reason():
+    heads, n, sections = (4, 2, 64), 30, (8, 12, 12)
+    c = cuda(case(n, heads, torch.bfloat16, sections))
+    tables = (c["cos"], c["sin"], c["pos"], *heads, sections)
+    room = torch.empty(n * 8 * 64, device="cuda", dtype=torch.bfloat16)
+    q, k, v = (t.view(n, h, 64) for t, h in zip(room.split([n * 256, n * 128, n * 128]), (4, 2, 2)))
+    got = ops.mrope_fwd(c["qkv"], *tables, out=(q, k, v))  # neighbours do not share
+    assert all(torch.equal(x, y) for x, y in zip(got, ops.mrope_fwd(c["qkv"], *tables)))
+    for out in ((q, k, k), (q, q.view(-1)[:n * 128].view(n, 2, 64), c["qkv"].view(-1)[:n * 128].view(n, 2, 64))):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.mrope_fwd(c["qkv"], *tables, out=out)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.mrope_bwd(q, k, v, *tables, dtype=torch.bfloat16, out=room.view(n, -1))
