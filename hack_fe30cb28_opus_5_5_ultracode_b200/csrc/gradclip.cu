@@ -17,6 +17,7 @@
 // launch latencies for small ones. 0.9 G bf16 gradients: norm 256 us (7.0 TB/s), norm and rescale into
 // fp32 1,205 us (6.0 TB/s of the bytes both passes move).
 #include <algorithm>
+#include <exception>
 #include <utility>
 #include <vector>
 
@@ -336,11 +337,15 @@ int clip_check(const GradTensors& t, const float* norm, const double* ws, int64_
   return QL_STATUS_OK;
 }
 
-// Whether any two of the tensors written (or read beside one that is) share memory; an output that is
-// its own gradient counts once.
-bool any_overlap(const GradTensors& t) {
+// Refuses a call where any two of the tensors written (or read beside one that is) share memory; an output
+// that is its own gradient counts once.
+int check_overlap(const GradTensors& t) {
   std::vector<std::pair<uint64_t, uint64_t>> spans;  // [first byte, end)
-  spans.reserve(2 * (size_t)t.count);
+  try {
+    spans.reserve(2 * (size_t)t.count);  // all that this function allocates
+  } catch (const std::exception&) {
+    return QL_STATUS_CUDA;  // no memory for it: an exception must not cross the C entry
+  }
   for (int i = 0; i < t.count; ++i) {
     if (t.elements[i] == 0) continue;
     spans.emplace_back(t.grads[i], t.grads[i] + (uint64_t)t.elements[i] * elem_bytes(t.dtypes[i]));
@@ -349,8 +354,8 @@ bool any_overlap(const GradTensors& t) {
   }
   std::sort(spans.begin(), spans.end());
   for (size_t k = 1; k < spans.size(); ++k)
-    if (spans[k].first < spans[k - 1].second) return true;
-  return false;
+    if (spans[k].first < spans[k - 1].second) return QL_STATUS_BAD_ARG;
+  return QL_STATUS_OK;
 }
 
 int all_squares(const GradTensors& t, ClipCall& c, cudaStream_t s) {
@@ -396,7 +401,8 @@ int clip_grads(const GradTensors& t, float max_norm, float inv_scale, const floa
       return QL_STATUS_BAD_ARG;
     in_place &= t.outs[i] == t.grads[i];
   }
-  if (any_overlap(t)) return QL_STATUS_BAD_ARG;
+  st = check_overlap(t);
+  if (st != QL_STATUS_OK) return st;
   ProfScope prof(PK_OTHER, 0, 0, s);
   ClipCall c{max_norm, inv_scale, inv_scale_dev, norm, in_place, 0, ws};
   st = all_squares(t, c, s);

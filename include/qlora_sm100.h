@@ -23,7 +23,7 @@ extern "C" {
 enum {
   QL_STATUS_OK = 0,
   QL_STATUS_BAD_ARG = 1,     /* a size, stride, alignment or dtype the kernel does not take */
-  QL_STATUS_CUDA = 2,        /* a CUDA runtime / driver call failed */
+  QL_STATUS_CUDA = 2,        /* a CUDA runtime / driver call or a host allocation failed */
   QL_STATUS_UNSUPPORTED = 3, /* a valid request this build has no kernel for */
   QL_STATUS_TIMEOUT = 4      /* a kernel gave up a bounded wait (device status word) */
 };

@@ -2,6 +2,8 @@
 refusals (CPU)."""
 
 import math
+import subprocess
+import sys
 from array import array
 
 import pytest
@@ -284,3 +286,30 @@ def test_what_an_infinite_norm_and_a_nan_do(place):
         assert norm.item() == math.inf and math.isnan(got[1][2].item())
         got[1][2] = 0.0
         assert not any(o.any() for o in got)
+
+
+def test_a_list_too_long_for_the_memory_is_an_error_not_an_abort():
+    """The check for shared memory of 4 M tensors wants 128 MB; where the process may have 32 MB more, the entry
+    returns a status."""
+    code = """
+import ctypes, resource, sys
+from array import array
+lib = ctypes.CDLL(sys.argv[1])
+n = 1 << 22
+addr, out = array("Q", range(1 << 20, (1 << 20) + 4 * n, 4)), array("Q", range(1 << 30, (1 << 30) + 4 * n, 4))
+size, kind = array("q", [1]) * n, array("i", [2]) * n
+at = [ctypes.c_void_p(a.buffer_info()[0]) for a in (addr, out, size, kind, kind)]
+one = ctypes.c_float(1.0)
+def call(count):
+    return lib.ql_clip_grads(*at, count, one, one, None, ctypes.c_void_p(16), ctypes.c_void_p(16),
+                             ctypes.c_int64(1 << 40), None)
+out[0] = out[1]
+assert call(2) == 1  # the library runs and refuses shared memory
+out[0] = 1 << 30
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (used + (32 << 20),) * 2)
+sys.exit(40 + call(n))
+"""
+    done = subprocess.run([sys.executable, "-c", code, _lib.LIB_PATH], capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 40 + 2, (done.returncode, done.stderr[-500:])  # QL_STATUS_CUDA
