@@ -613,6 +613,9 @@ int attn_mod_check(const ql_attn_mod_args& m, AttnModArgs& a) {
   if (m.slopes != nullptr && m.scale < 1e-30f) return QL_STATUS_BAD_ARG;  // slope / scale has to stay finite
   // tanh_short's coefficients hold (scale / softcap)^7: finite up to 10^4, a cap that bends every score
   if (m.softcap > 0.f && m.softcap < 1e-4f * m.scale) return QL_STATUS_BAD_ARG;
+  // scale and softcap times log2(e) have to be finite, scale / softcap a normal number
+  if (m.scale > 2.3e38f || m.softcap > 2.3e38f || (m.softcap > 0.f && m.scale / m.softcap < 1.1754944e-38f))
+    return QL_STATUS_BAD_ARG;
   if (m.n > 0 && m.B > 0 && (m.q == nullptr || m.k == nullptr || m.v == nullptr || m.out == nullptr ||
                              m.lse == nullptr || m.cu_seqlens == nullptr))
     return QL_STATUS_BAD_ARG;

@@ -765,6 +765,9 @@ def _attn_mod_inputs(q, k, v, cu_seqlens, max_len, scale, softcap, slopes, windo
         raise ValueError("slopes with a scale below 1e-30 are not supported")
     if 0 < softcap < 1e-4 * scale:
         raise ValueError("a softcap below 1e-4 scale is not supported")
+    if scale > 2.3e38 or softcap > 2.3e38 or 0 < scale < 1.1754944e-38 * softcap:
+        raise ValueError("scale and softcap of at most 2.3e38 and scale / softcap of at least 1.2e-38 "
+                         "are supported")
     return n, HQ, HKV, D, B, strides, _DT[dt], dev, min(window, INT_MAX)
 
 

@@ -491,7 +491,8 @@ int ql_exp2_fma_eval(const float* x, float* y, int64_t n, cudaStream_t stream);
  * q [n, HQ, D], k / v [n, HKV, D] of dtype with row strides ldq / ldk / ldv (elements, multiples of
  * 8; the heads of a row contiguous), D = 64 or 128, 16-byte aligned; out, dout, dq, dk, dv
  * contiguous in dtype; lse fp32 [HQ, n], natural log. scale > 0 (with
- * slopes at least 1e-30); softcap 0 or at least 1e-4 scale; slopes of any sign. max_len: at least the longest
+ * slopes at least 1e-30); softcap 0 or at least 1e-4 scale, scale / softcap a normal number; neither
+ * above 2.3e38; slopes of any sign. max_len: at least the longest
  * sequence. The gradients are summed in a fixed order (bit-identical from run to run). P and dS, the
  * operands of their products, are rounded to dtype, in two parts (the rounding and the rounding of
  * what it left) wherever no row of a 128-row tile sees more than 256 others: there a gradient is off

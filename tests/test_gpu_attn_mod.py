@@ -683,3 +683,34 @@ def test_shared_memory_is_refused_with_a_reason():
     # nor do tensors without elements
     empty = q[:0]
     ops.attn_mod_fwd(empty, empty, empty, cu[:1], 0, 0.125, out=empty)
+
+
+EXTREME = [dict(softcap=3e38), dict(scale=3e38), dict(scale=1e-30, softcap=1e10), dict(scale=2.0, softcap=2e38)]
+
+
+@pytest.mark.parametrize("change", EXTREME, ids=str)
+def test_scales_and_caps_beyond_fp32_are_refused_by_the_library(change):
+    """softcap log2(e) and scale log2(e) have to be finite, scale / softcap a normal number."""
+    for entry in ("ql_attn_mod_fwd", "ql_attn_mod_bwd"):
+        args = fake_args(**change)
+        with pytest.raises(_lib.QLError) as e:
+            _lib.call(entry, ops.ctypes_ref(args), None)
+        assert e.value.status == ops.STATUS_BAD_ARG
+
+
+@pytest.mark.gpu
+def test_caps_far_above_the_scores_change_nothing_and_larger_ones_are_refused():
+    q, k, v, dout, cu = batch([150, 20], (2, 1, 64), torch.float16, seed=30)
+    plain = ops.attn_mod_fwd(q, k, v, cu, 150, 0.125)
+    for cap in (1e6, 1e20, 1e36):
+        out, lse = ops.attn_mod_fwd(q, k, v, cu, 150, 0.125, softcap=cap)
+        # the same scores, off by 1.2e-7 of a few units
+        assert (lse - plain[1]).abs().max() < 2e-5 and rel(out, plain[0].double().cpu()) < 2.0 ** -11
+        got = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, 150, 0.125, softcap=cap)
+        assert all(torch.isfinite(x).all() for x in got)
+    for change in EXTREME:
+        scale, cap = change.get("scale", 0.125), change.get("softcap", 0.0)
+        with pytest.raises(ValueError):
+            ops.attn_mod_fwd(q, k, v, cu, 150, scale, softcap=cap)
+        with pytest.raises(ValueError):
+            ops.attn_mod_bwd(dout, q, k, v, *plain, cu, 150, scale, softcap=cap)
