@@ -7,8 +7,9 @@
 // documents (runs of equal ids; negative ids are padding) - leaves query i an interval
 // [lo_i, hi_i) of keys, and both ends never decrease with i. So the first and last row of a query
 // tile give the key blocks it has to visit (the hull [lo_first, hi_last)) and those it can visit
-// without looking at the mask (inside [lo_last, hi_first)), and for a block of keys the query
-// tiles that see it are found by bisection. Padding rows get the empty interval [i, i).
+// without looking at the mask (inside [lo_last, hi_first)). Read from the key's side the same
+// conditions leave key j an interval of queries, so a block of keys finds its query tiles in the same
+// way. Padding rows get the empty interval [i, i).
 #pragma once
 #include "common.cuh"
 #include "gemm_common.cuh"
@@ -167,7 +168,7 @@ __device__ __forceinline__ void ex2_2(uint64_t* x) {
 }
 
 // tanh(u) = u P(u^2) for |u| <= 0.75, in place: coefficients of this library's own fit (reweighted least
-// squares in relative error; 2.9e-8, 1.6e-7 in fp32 Horner evaluation).
+// squares in relative error; 6.6e-8, 1.6e-7 in fp32 Horner evaluation).
 constexpr float TANH_POLY_MAX = 0.75f;
 template <int N>
 __device__ __forceinline__ void tanh_poly2(uint64_t* u) {
@@ -189,8 +190,8 @@ __device__ __forceinline__ void tanh_poly2(uint64_t* u) {
   for (int i = 0; i < N; ++i) u[i] = mul2(p[i], u[i]);
 }
 // c tanh(u x) = x (k0 + k1 x^2 + k2 x^4 + k3 x^6) for |u x| <= 0.4, in place: the fit with u and c in
-// its coefficients (1.0e-7 relative), five operations a pair where tanh_poly2 with its two
-// scalings takes nine. Scores of a model trained with a cap rarely leave this range.
+// its coefficients (1.2e-7 relative, 2.3e-7 in fp32), five operations a pair where tanh_poly2 with
+// its two scalings takes nine. Scores of a model trained with a cap rarely leave this range.
 constexpr float TANH_SHORT_MAX = 0.4f;
 struct TanhShort {
   float k[4];

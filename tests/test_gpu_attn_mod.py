@@ -714,3 +714,27 @@ def test_caps_far_above_the_scores_change_nothing_and_larger_ones_are_refused():
             ops.attn_mod_fwd(q, k, v, cu, 150, scale, softcap=cap)
         with pytest.raises(ValueError):
             ops.attn_mod_bwd(dout, q, k, v, *plain, cu, 150, scale, softcap=cap)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap,scale", [(30.0, 0.125), (50.0, 0.0883883), (1.5, 0.25), (1e4, 1.0)])
+def test_the_cap_against_tanh_in_64_bits(cap, scale):
+    """A query that sees one key has lse = cap(scale q . k). Scores of one size share a batch, so that each
+    of the three forms is used over its whole range."""
+    dtype = torch.float16
+    for low, high in ((1e-3, 0.1), (0.1, 0.4), (0.4, 0.75), (0.75, 4.0)):  # of the tanh's argument
+        n, g = 4000, torch.Generator().manual_seed(29)
+        x = torch.linspace(low, high, n, dtype=torch.float64) * cap / scale
+        q, k = torch.zeros(n, 1, 64), torch.zeros(n, 1, 64)
+        q[:, 0, 0] = x.sqrt()
+        k[:, 0, 0] = x.sqrt() * torch.where(torch.rand(n, generator=g) < 0.5, -1.0, 1.0)
+        q, k = q.to(dtype), k.to(dtype)
+        cu = torch.arange(n + 1, dtype=torch.int32).cuda()
+        lse = ops.attn_mod_fwd(q.cuda(), k.cuda(), k.cuda(), cu, 1, scale, softcap=cap)[1][0]
+        score = q[:, 0, 0].double() * k[:, 0, 0].double() * scale
+        want = cap * torch.tanh(score / cap)
+        # the fits' 1.2e-7 and 0.7e-7, their evaluation, scale / cap, the two changes of the logarithm's base and the
+        # constants of both: at most ten roundings of 2^-24; the 2^7 of fp16 in the row's sum: two of 2^-24 x 7
+        bound = want.abs() * (1.2e-7 + 10 * 2.0 ** -24) + 14 * 2.0 ** -24
+        assert ((lse.double().cpu() - want).abs() <= bound).all(), (low, high)
+    assert ops.device_status() == 0
