@@ -11,6 +11,8 @@
 // conditions leave key j an interval of queries, so a block of keys finds its query tiles in the same
 // way. Padding rows get the empty interval [i, i).
 #pragma once
+#include <atomic>
+
 #include "common.cuh"
 #include "gemm_common.cuh"
 #include "ops.h"
@@ -435,14 +437,15 @@ __device__ __forceinline__ void stage_flush(uint8_t* stage, uint8_t* dst, int64_
   __syncwarp();
 }
 
-// Host: raises a kernel's dynamic shared-memory limit on the current device, once per device.
-inline int attn_smem_limit(const void* kernel, int bytes, unsigned long long* done) {
+// Host: raises a kernel's dynamic shared-memory limit on the current device, once per device (host threads
+// may race to it: the limit is the same).
+inline int attn_smem_limit(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return QL_STATUS_CUDA;
-  if (dev < 64 && ((*done >> dev) & 1)) return QL_STATUS_OK;
+  if (dev < 64 && ((done.load(std::memory_order_acquire) >> dev) & 1)) return QL_STATUS_OK;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
     return QL_STATUS_CUDA;
-  if (dev < 64) *done |= 1ull << dev;
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
   return QL_STATUS_OK;
 }
 

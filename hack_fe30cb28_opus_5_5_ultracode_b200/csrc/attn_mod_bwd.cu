@@ -755,12 +755,12 @@ int dkv_splits(const AttnModArgs& a) {
 template <typename T, int D, int MODE>
 int launch_bwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mdo,
                const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
-  static unsigned long long done_q = 0, done_kv = 0;
+  static std::atomic<unsigned long long> done_q{0}, done_kv{0};
   auto kq = attn_mod_bwd_kernel<T, D, MODE, false>;
   auto kkv = attn_mod_bwd_kernel<T, D, MODE, true>;
   constexpr int smem = BwdCfg<D>::SMEM;
-  int st = attn_smem_limit(reinterpret_cast<const void*>(kq), smem, &done_q);
-  if (st == QL_STATUS_OK) st = attn_smem_limit(reinterpret_cast<const void*>(kkv), smem, &done_kv);
+  int st = attn_smem_limit(reinterpret_cast<const void*>(kq), smem, done_q);
+  if (st == QL_STATUS_OK) st = attn_smem_limit(reinterpret_cast<const void*>(kkv), smem, done_kv);
   if (st != QL_STATUS_OK) return st;
   const unsigned tiles = (unsigned)cdiv(a.max_len, AM_T);
   int* err = status_word();

@@ -551,9 +551,9 @@ template <typename T, int D, int MODE, bool SPLIT>
 int launch_fwd(const AttnModArgs& a, const CUtensorMap& mq, const CUtensorMap& mk,
                const CUtensorMap& mv, cudaStream_t s) {
   using C = FwdCfg<D, SPLIT>;
-  static unsigned long long done = 0;
+  static std::atomic<unsigned long long> done{0};
   auto kern = attn_mod_fwd_kernel<T, D, MODE, SPLIT>;
-  const int st = attn_smem_limit(reinterpret_cast<const void*>(kern), C::SMEM, &done);
+  const int st = attn_smem_limit(reinterpret_cast<const void*>(kern), C::SMEM, done);
   if (st != QL_STATUS_OK) return st;
   const dim3 grid((unsigned)(a.HQ * a.B), (unsigned)cdiv(a.max_len, C::Q_TILES * AM_T));
   launch_k(kern, grid, dim3(FWD_THREADS), C::SMEM, s, mq, mk, mv, a, status_word());

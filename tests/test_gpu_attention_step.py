@@ -2,6 +2,7 @@
 would: mrope_fwd, attn_mod_fwd, attn_mod_bwd, mrope_bwd, the LoRA gradients, clip_grads."""
 
 import sys
+import threading
 
 import pytest
 import torch
@@ -166,3 +167,49 @@ def test_a_step_of_longer_rows(dtype, monkeypatch):
         assert rel(x, y) < 9 * u, name
     total = torch.stack([y.norm() for y in want]).norm()
     assert abs(norm.item() - total.item()) < 9 * u * total.item()
+
+
+@pytest.mark.gpu
+def test_two_host_threads_at_once():
+    """The same calls from two threads, each on a stream of its own, give what one gives, first calls of a
+    kernel included."""
+    dtype = torch.bfloat16
+    n = sum(LENGTHS)
+    d = {x: t.cuda() for x, t in case(n, (HQ, HKV, D), dtype, SECTIONS, seed=41).items()}
+    cu = torch.tensor([0] + LENGTHS, dtype=torch.int32).cumsum(0, dtype=torch.int32).cuda()
+    rope = (d["cos"], d["sin"], d["pos"], HQ, HKV, D, SECTIONS)
+    dout = torch.randn(n, HQ, D, device="cuda").to(dtype)
+    slopes = torch.linspace(0.1, 0.9, HQ).cuda()
+    mods = [dict(window=50), dict(softcap=20.0), dict(slopes=slopes), dict(softcap=9.0, slopes=slopes)]
+
+    def step(mod):
+        q, k, v = ops.mrope_fwd(d["qkv"], *rope)
+        out, lse = ops.attn_mod_fwd(q, k, v, cu, max(LENGTHS), SCALE, **mod)
+        grads = ops.attn_mod_bwd(dout, q, k, v, out, lse, cu, max(LENGTHS), SCALE, **mod)
+        dqkv = ops.mrope_bwd(*grads, *rope, dtype=dtype)[0]
+        return [out, lse, *grads, ops.clip_grads([dqkv], 0.5), dqkv]
+
+    torch.cuda.synchronize()
+    start, results, errors = threading.Barrier(2), [None, None], []
+
+    def work(at):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                start.wait()
+                results[at] = [step(m) for _ in range(5) for m in mods]
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    want = [step(m) for m in mods]
+    for got in results:
+        for i, one in enumerate(got):
+            assert all(torch.equal(a, b) for a, b in zip(one, want[i % len(mods)]))
+    assert ops.device_status() == 0

@@ -343,3 +343,28 @@ def test_shared_memory_is_refused_with_a_reason():
             ops.mrope_fwd(c["qkv"], *tables, out=out)
     with pytest.raises(ValueError, match="share memory"):
         ops.mrope_bwd(q, k, v, *tables, dtype=torch.bfloat16, out=room.view(n, -1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,sections", [((4, 1, 128), (24, 20, 20)), ((2, 2, 64), (14, 10, 8))], ids=str)
+def test_interleaved_axes_whose_first_keeps_the_remainder(heads, sections):
+    n, dtype = 333, torch.bfloat16
+    HQ, HKV, D = heads
+    c = case(n, heads, dtype, sections, seed=33)
+    d = cuda(c)
+    got = ops.mrope_fwd(d["qkv"], d["cos"], d["sin"], d["pos"], *heads, sections, interleaved=True)
+    back = ops.mrope_bwd(d["dq"], d["dk"], d["dv"], d["cos"], d["sin"], d["pos"], *heads, sections, interleaved=True,
+                         dtype=dtype)[0]
+    # in turn while an axis has some left: 0 1 2 0 1 2 ..., the first axis alone at the end
+    order = [f % 3 if f < 3 * min(sections) else None for f in range(D // 2)]
+    left = [s - min(sections) for s in sections]
+    rest = [a for r in range(max(left)) for a in range(3) if left[a] > r]
+    ax = torch.tensor([a for a in order if a is not None] + rest)
+    row, f = c["pos"].long()[ax].t(), torch.arange(D // 2)
+    cos, sin = c["cos"].double()[row, f][:, None], c["sin"].double()[row, f][:, None]
+    x = c["qkv"].double().view(n, HQ + 2 * HKV, D)
+    for a, b in zip(got, (rotate(x[:, :HQ], cos, sin), rotate(x[:, HQ:HQ + HKV], cos, sin), x[:, HQ + HKV:])):
+        assert rel(a, b) < HALF_STEP[dtype] * 1.01 + 1e-6
+    want = torch.cat([rotate(c["dq"].double(), cos, sin, back=True), rotate(c["dk"].double(), cos, sin, back=True),
+                      c["dv"].double()], 1).view(n, -1)
+    assert rel(back, want) < HALF_STEP[dtype] * 1.01 + 1e-6
