@@ -3,7 +3,7 @@
 // is the table's at row pos[axis(f)][t], so a text token (all positions equal) rotates as in
 // rope.cu and a picture's tokens by their row and column.
 //
-// A tile is 16 tokens (8 in the backward of short batches). The tile's cosines and sines are gathered once into shared memory (a
+// A tile is 16 tokens (8 in the backward of short batches, see mrope_bwd). The tile's cosines and sines are gathered once into shared memory (a
 // gather of single floats where neighbouring frequencies belong to different axes) and serve every
 // head. Then each warp takes units of 32 columns of a head together with their 32 partners
 // D / 2 further on. The LoRA-B product of a unit is formed on the tensor cores in the layout the data
@@ -549,7 +549,10 @@ int mrope_bwd(const ql_mrope_args& m, cudaStream_t s) {
       else QL_MROPEB(__nv_bfloat16, __nv_bfloat16, ROWS);                                         \
     }                                                                                             \
   } while (0)
-  if (m.n > 16 * 2 * sm_count()) QL_MROPEB2(16); else QL_MROPEB2(8);
+  // 8 tokens per CTA while all CTAs are resident at once (3,552 tokens on 148 SMs): B is read twice as
+  // often, but by twice as many CTAs. 8 against 16 tokens, us: 61 tokens of 12 + 2 heads 7.6 / 10.5, 1,090
+  // 9.0 / 11.6, 3,000 13.0 / 16.6, 4,000 20.8 / 18.8, 24 k of 28 + 4 heads 160 / 137.
+  if (m.n > 8 * MR_CTAS * sm_count()) QL_MROPEB2(16); else QL_MROPEB2(8);
 #undef QL_MROPEB2
 #undef QL_MROPEB
   return launched(1);
