@@ -330,6 +330,23 @@ __global__ void __launch_bounds__(MR_THREADS, MR_CTAS) mrope_bwd_kernel(const __
   __syncthreads();
   const bool lq = a.dxlo_q != nullptr, lv = a.dxlo_v != nullptr;
   float cq[2][4] = {}, cv[2][4] = {};
+  // The tensor core cuts its sums off where fp32 addition rounds them: running sums over a token's 56 units
+  // (28 heads of 128) were off by 1.5e-6, sums of one unit each, added up here, by 2.7e-7. fp16's are added
+  // unit by unit for their scales; a bf16 unit's (c) when the next one's loads are on their way
+  // (24 k tokens of 28 + 4 heads: 131 -> 134 us, at once 144).
+  constexpr bool LATER = std::is_same<T, __nv_bfloat16>::value;
+  float c[2][4] = {};
+  bool of_q = true;  // whose unit c is
+  auto add_unit = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (of_q) cq[nt][e] += c[nt][e];
+        else cv[nt][e] += c[nt][e];
+        c[nt][e] = 0.f;
+      }
+  };
   for (int u = blockIdx.y * warps + warp; u < units; u += gridDim.y * warps) {
     const Unit un = unit_of(u, per_head);
     const int d = un.d0 + t * 8;
@@ -345,6 +362,7 @@ __global__ void __launch_bounds__(MR_THREADS, MR_CTAS) mrope_bwd_kernel(const __
       raw[rh][0] = r < ROWS && tok < a.n ? load8<TG>(src + tok * ld + d) : Raw8<TG>{};
       raw[rh][1] = r < ROWS && tok < a.n ? load8<TG>(src + tok * ld + d + half) : Raw8<TG>{};
     }
+    if (LATER && (lq || lv)) add_unit();
     float x1[2][8], x2[2][8];
 #pragma unroll
     for (int rh = 0; rh < 2; ++rh) {
@@ -362,15 +380,18 @@ __global__ void __launch_bounds__(MR_THREADS, MR_CTAS) mrope_bwd_kernel(const __
     }
     if (is_q && lq) {
       const int64_t o = (int64_t)un.head * a.D + un.d0;
-      lora_back<T>(x1, a.Bq, o, cq);
-      lora_back<T>(x2, a.Bq, o + half, cq);
+      lora_back<T>(x1, a.Bq, o, LATER ? c : cq);
+      lora_back<T>(x2, a.Bq, o + half, LATER ? c : cq);
+      of_q = true;
     } else if (is_v && lv) {
       const int64_t o = (int64_t)(un.head - a.HQ - a.HKV) * a.D + un.d0;
-      lora_back<T>(x1, a.Bv, o, cv);
-      lora_back<T>(x2, a.Bv, o + half, cv);
+      lora_back<T>(x1, a.Bv, o, LATER ? c : cv);
+      lora_back<T>(x2, a.Bv, o + half, LATER ? c : cv);
+      of_q = false;
     }
   }
   if (!lq && !lv) return;
+  if (LATER) add_unit();
   // the warps' partial sums, added in warp order
   float* red = angle_smem + 2 * ROWS * pitch;  // [warps][2][16 tokens][16]
 #pragma unroll

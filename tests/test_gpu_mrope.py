@@ -368,3 +368,22 @@ def test_interleaved_axes_whose_first_keeps_the_remainder(heads, sections):
     want = torch.cat([rotate(c["dq"].double(), cos, sin, back=True), rotate(c["dk"].double(), cos, sin, back=True),
                       c["dv"].double()], 1).view(n, -1)
     assert rel(back, want) < HALF_STEP[dtype] * 1.01 + 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 4, 60])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_dx_lo_over_many_heads(n, dtype):
+    """3,584 terms a sum. A unit of 64 terms takes at most six sums on the tensor core, cut off by up to 2^-23
+    each; the units' errors have independent signs, and adding them up rounds by 2^-24."""
+    HQ, HKV, D = heads = (28, 4, 128)
+    sections = (16, 24, 24)
+    c = case(n, heads, dtype, sections, seed=34)
+    d = cuda(c)
+    got = ops.mrope_bwd(d["dq"], d["dk"], d["dv"], d["cos"], d["sin"], d["pos"], *heads, sections, dtype=dtype,
+                        Bq=d["Bq"], Bv=d["Bv"])[1:]
+    cos, sin = angles(c["cos"], c["sin"], c["pos"], sections, False)
+    gq, gv = rotate(c["dq"].double(), cos, sin, back=True).view(n, -1), c["dv"].double().view(n, -1)
+    for a, g, B in zip(got, (gq, gv), (c["Bq"].double(), c["Bv"].double())):
+        assert rel(a, g @ B) < 8 * 2.0 ** -23
+    assert ops.device_status() == 0
