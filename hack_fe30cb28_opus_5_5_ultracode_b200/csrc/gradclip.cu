@@ -5,8 +5,8 @@
 // factor, and rescales its part. A gradient list that fits in L2 is read from HBM once. Squares are
 // summed in fp32 over eight loads of a thread (four sums of 8 to 16 values; over thousands of them the
 // norm was off by 1.5e-6), from there on in fp64; loads whose squares leave fp32's range (gradients above
-// 1.8e19, or all below 1e-15) are looked at once more and squared in fp64 unless they are zeros (0.28 G fp32 zeros, or 5% nonzero values:
-// 157 -> 211 us).
+// 1.8e19, or all below 1e-15) are looked at once more and squared in fp64 unless they are zeros (0.28 G
+// fp32 zeros, or 5% nonzero values: 157 -> 211 us).
 //
 // The tensors' addresses and sizes travel as kernel parameters (up to 1,024 tensors a launch), so a
 // call copies nothing to the device and can be captured. Work is cut into chunks of 32 KB of one

@@ -3,16 +3,17 @@
 // is the table's at row pos[axis(f)][t], so a text token (all positions equal) rotates as in
 // rope.cu and a picture's tokens by their row and column.
 //
-// A tile is 16 tokens (8 in the backward of short batches, see mrope_bwd). The tile's cosines and sines are gathered once into shared memory (a
-// gather of single floats where neighbouring frequencies belong to different axes) and serve every
-// head. Then each warp takes units of 32 columns of a head together with their 32 partners
-// D / 2 further on. The LoRA-B product of a unit is formed on the tensor cores in the layout the data
+// A tile is 16 tokens (8 in the backward of short batches, see mrope_bwd). The tile's cosines and
+// sines are gathered once into shared memory (a gather of single floats where neighbouring
+// frequencies belong to different axes) and serve every head. Then each warp takes units of 32
+// columns of a head together with their 32 partners D / 2 further on. The LoRA-B product of a unit is formed on the tensor cores in the layout the data
 // is moved in: the eight columns of an m16n8k16 step can be any eight outputs, and with output
 // 8 t + 2 j + e in column 2 t + e of step j, thread t of a row ends up with eight consecutive
 // columns after four steps - one 16-byte load and store. The product stays in fp32 (nothing is
 // rounded between the factors and the output). The backward uses the same ordering for the K
 // dimension of dx_lo = s g B, with g split into 16-bit parts (fp16: brought to one size by a power of
-// two per token and unit first), so dx_lo is good to fp32 whatever the gradients' size.
+// two per token and unit first) and the units' sums added up in fp32, so dx_lo is good to fp32 whatever the
+// gradients' size.
 //
 // Bound: HBM for long batches (2 bytes read and 2 written per element in each direction), launch and
 // L2 latency for short ones.
