@@ -313,3 +313,20 @@ sys.exit(40 + call(n))
     done = subprocess.run([sys.executable, "-c", code, _lib.LIB_PATH], capture_output=True, text=True,
                           timeout=300)
     assert done.returncode == 40 + 2, (done.returncode, done.stderr[-500:])  # QL_STATUS_CUDA
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("size", [1e-25, 1e-3, 1e22])
+def test_few_values_among_zeros(dtype, size):
+    """Sparse gradients, zeros of both signs: each value counts, whatever the loads beside it hold."""
+    g = torch.Generator().manual_seed(7)
+    for n, offset in ((100_003, 0), (40_000, 1), (31, 0), (9, 3)):
+        flat = torch.zeros(n + offset)
+        flat[::2] = -0.0
+        at = torch.randint(offset, n + offset, (max(1, n // 997),), generator=g).unique()
+        flat[at] = (torch.rand(len(at), generator=g) + 0.5) * size
+        view = flat.to(dtype).cuda()[offset:]
+        want = norm_of([view])
+        assert want > 0 and abs(ops.grad_norm([view]).item() - want) <= 1e-6 * want
+        assert ops.grad_norm([torch.full_like(view, -0.0)]).item() == 0.0
